@@ -11,7 +11,7 @@ Four operators that one serving step chains:
 
     K codes [16 tokens][4 t][NG groups] u32   dim = group * 32 + t * 8 + nibble (8 nibbles, lowest first)
     K scales [16][NG] f16, K minima [16][NG] f16
-    V codes [8 token pairs][8 g][NG groups][2 tokens] u16   dim = group * 32 + g * 4 + nibble
+    V codes [8 token pairs][8 x][NG groups][2 tokens] u16   dim = group * 32 + g * 4 + nibble, g = x ^ 2 (pair % 4)
     V scales [8][NG][2] f16, V minima [8][NG][2] f16
 
 A value is code * scale + minimum.  Quantization of a group x[32] (clamped to +-65504): minimum = f16(min x),
@@ -141,13 +141,22 @@ def _quant(x):
     x = x.reshape(*x.shape[:-1], -1, 32)
     lo, hi = x.amin(-1, keepdim=True), x.amax(-1, keepdim=True)
     m = lo.half().float()
-    s = ((hi - m) / 15.0).half().float()
+    s = ((hi - m) / torch.full_like(m, 15.0)).half().float()   # (a plain number would be multiplied by its reciprocal)
     code = torch.where(s > 0, torch.round((x - m) / torch.where(s > 0, s, torch.ones_like(s))), torch.zeros_like(x)).clamp(0, 15)
     return code.to(torch.uint8), s.squeeze(-1).half(), m.squeeze(-1).half()
 
 
 def _bytes(t):
     return t.contiguous().view(torch.uint8)
+
+
+def _pairs():
+    return torch.arange(8, device=DEV)[:, None]
+
+
+def _crossed():
+    """[pair, x]: which g stands at x (its own inverse)."""
+    return torch.arange(8, device=DEV)[None, :] ^ (2 * (_pairs() % 4))
 
 
 def _pack(k, v):
@@ -159,7 +168,8 @@ def _pack(k, v):
     kc = (kc[..., 0] | (kc[..., 1] << 4)).transpose(3, 4)
     vc, vs, vm = _quant(v.transpose(1, 2))
     vc = vc.reshape(N, Hkv, 8, 2, G, 8, 2, 2)    # pair, token, group, g, byte, nibble
-    vc = (vc[..., 0] | (vc[..., 1] << 4)).permute(0, 1, 2, 5, 4, 3, 6)
+    vc = (vc[..., 0] | (vc[..., 1] << 4)).permute(0, 1, 2, 5, 4, 3, 6)   # pair, g, group, token, byte
+    vc = vc[:, :, _pairs(), _crossed()]
     pairs = lambda t: t.reshape(N, Hkv, 8, 2, G).transpose(3, 4)  # noqa: E731
     parts = [kc, _bytes(ks), _bytes(km), vc, _bytes(pairs(vs)), _bytes(pairs(vm))]
     return torch.cat([p.reshape(N, Hkv, -1) for p in parts], dim=-1)
@@ -247,8 +257,8 @@ def _unpack(pages, D):
     n = len(lead) + 1
     kc = nib(kc.reshape(*lead, Hkv, 16, 4, G, 4)).transpose(n + 1, n + 2).reshape(*lead, Hkv, 16, G, 32).float()
     k = kc * half(ks).reshape(*lead, Hkv, 16, G, 1) + half(km).reshape(*lead, Hkv, 16, G, 1)
-    vc = nib(vc.reshape(*lead, Hkv, 8, 8, G, 2, 2))             # pair, g, group, token, byte, nibble
-    ax = list(range(n))
+    vc = nib(vc.reshape(-1, 8, 8, G, 2, 2)[:, _pairs(), _crossed()].reshape(*lead, Hkv, 8, 8, G, 2, 2))
+    ax = list(range(n))                                         # then pair, g, group, token, byte, nibble
     vc = vc.permute(*ax, n, n + 3, n + 2, n + 1, n + 4, n + 5).reshape(*lead, Hkv, 16, G, 32).float()
     tok = lambda c: half(c).reshape(*lead, Hkv, 8, G, 2).transpose(-1, -2).reshape(*lead, Hkv, 16, G, 1)  # noqa: E731
     v = vc * tok(vs) + tok(vm)
@@ -372,7 +382,8 @@ def _read64(page, D):
     grp, r = d // 32, d % 32
     k_at = t[:, None] * (D // 2) + ((r // 8) * G + grp) * 4 + (r % 8) // 2
     v0 = 8 * D + 64 * G
-    v_at = v0 + (((t[:, None] // 2) * 8 + r // 4) * G + grp) * 4 + (t[:, None] % 2) * 2 + (r % 4) // 2
+    pair = t[:, None] // 2
+    v_at = v0 + ((pair * 8 + ((r // 4) ^ (2 * (pair % 4)))) * G + grp) * 4 + (t[:, None] % 2) * 2 + (r % 4) // 2
     ks_at = 8 * D + (t[:, None] * G + grp) * 2
     vs_at = v0 + 8 * D + (((t[:, None] // 2) * G + grp) * 2 + t[:, None] % 2) * 2
 
