@@ -113,8 +113,11 @@ void prefill_attention_tc(torch::Tensor q, torch::Tensor k_cache, torch::Tensor 
                           torch::Tensor seq_qlen, torch::Tensor seq_pos0, int64_t n_tiles, torch::Tensor out,
                           c10::optional<torch::Tensor> err);
 
+void bind_serve_ops(pybind11::module& m);   // serve_ops.cpp
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.doc() = "fak_b200 sm_100a kernels";
+  bind_serve_ops(m);
   m.def("quantize_blocks", &quantize_blocks);
   m.def("dequantize_rows", &dequantize_rows);
   m.def("quant_act", &quant_act);

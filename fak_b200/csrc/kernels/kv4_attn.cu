@@ -1,0 +1,641 @@
+// Attention over the 4-bit paged KV cache (layout in kv4.cuh): single tokens, verification blocks and chunks.
+//
+// Sequence b has ctx_b keys, the last n_b of them its new tokens; query i of them sees the keys up to its
+// own position ctx_b - n_b + i (with a window, only the last `window` of those).  The n_b * G query rows
+// of a KV head (G query heads share it) are the columns of the matrix products, 8 NT of them a CTA:
+//
+//   S^T [16 tokens x 8 rows] = K Q^T    m16n8k16, K codes as the A operand, straight from the page words
+//   O^T [D x 8 rows]        += V^T P^T  m16n8k16, V codes as the A operand, P^T from S^T by movmatrix
+//
+// Codes enter the tensor cores as f16 denormals: a nibble in the low bits of a half is code * 2^-24
+// exactly, one in bits 4-7 is 16 times that, so one AND makes two operands and no conversion is needed
+// (products with f16 and their f32 sums are exact for denormals too).  Scales and minima stay outside:
+//   q.k = sum_g s_g (q_g . c_g) + sum_g m_g sum(q_g)      the group's product is scaled in f32; the second
+//                                                         sum is one m16n8k8 with sum(q_g) in two f16 parts
+//   o_d = sum_j (p_j s_jg) c_jd + sum_j p_j m_jg          the scale multiplies P (f16) per group; the second
+//                                                         sum is one m16n8k16 whose fifth row, all ones,
+//                                                         gives the softmax denominator
+// Queries are rounded to f16 after a power-of-two scaling of their row (exact for bf16 and f16 inputs up
+// to 28 binades below the row's largest); P is f16: at most 7.5, so that P s stays below 65504.
+//
+// A warp streams its own pages through a ring of shared memory filled by one bulk copy a page and walks
+// them with an online softmax whose base moves only when a row outgrows it; the CTA's warps, then the
+// splits of a sequence (k_kv4_combine), are merged at the end.
+#include "kv4.cuh"
+#include "mma.cuh"
+#include "tc.cuh"
+
+#include <algorithm>
+#include <stdexcept>
+#include <string>
+
+#include "../serve_ops.h"
+
+namespace fak {
+namespace {
+
+using kv4::Lay;
+using kv4::PAGE;
+
+constexpr int W = 4;          // warps per CTA
+constexpr int STAGES = 4;     // pages in flight per warp
+constexpr float HEADROOM = 0.875f;   // log2 growth of a row's max before its base moves
+constexpr float LIFT = 2.f;          // P = 2^(z - base + LIFT) <= 2^2.875 < 7.5
+constexpr float LOG2E = 1.4426950408889634f;
+
+FAK_DEV void mma_f16_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+FAK_DEV void mma_f16_1688(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t b0) {
+  asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5}, {%6}, {%0,%1,%2,%3};"
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+               : "r"(a0), "r"(a1), "r"(b0));
+}
+FAK_DEV uint32_t movmatrix(uint32_t a) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(a));
+  return r;
+}
+FAK_DEV uint32_t pack_f16(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+FAK_DEV uint32_t mul_h2(uint32_t a, uint32_t b) {
+  const __half2 h = __hmul2(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+FAK_DEV float2 unpack_h2(uint32_t a) { return __half22float2(*reinterpret_cast<__half2*>(&a)); }
+FAK_DEV float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+FAK_DEV void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(dst)),
+      "l"(src), "r"(bytes), "r"(smem_u32(bar))
+      : "memory");
+}
+
+template <int N>
+FAK_DEV void lds(const uint8_t* p, uint32_t (&r)[N]) {
+  if constexpr (N == 4) {
+    const uint4 v = *reinterpret_cast<const uint4*>(p);
+    r[0] = v.x; r[1] = v.y; r[2] = v.z; r[3] = v.w;
+  } else if constexpr (N == 2) {
+    const uint2 v = *reinterpret_cast<const uint2*>(p);
+    r[0] = v.x; r[1] = v.y;
+  } else {
+    r[0] = *reinterpret_cast<const uint32_t*>(p);
+  }
+}
+
+// The pages one CTA column block needs, and how the splits share them: the same arithmetic in the
+// attention kernel and in the combine.
+struct Span {
+  int p0, p1, pps, live;   // pages [p0, p1), pages per split, splits that hold any
+};
+FAK_DEV Span span_of(int ctx, int n, int i_lo, int i_hi, int window, int n_split, int width) {
+  Span s;
+  const int last = min(ctx - n + i_hi, ctx - 1);               // the last key any row of the block sees
+  const int first = window > 0 ? max(0, ctx - n + i_lo + 1 - window) : 0;
+  s.p0 = first / PAGE;
+  s.p1 = min(width, last / PAGE + 1);
+  if (last < 0) s.p1 = s.p0;
+  const int pages = max(0, s.p1 - s.p0);
+  s.pps = max(W, (pages + n_split - 1) / n_split);
+  s.live = (pages + s.pps - 1) / s.pps;
+  return s;
+}
+
+template <typename T>
+FAK_DEV float to_f32(const T* p, int64_t i) { return (float)p[i]; }
+FAK_DEV float load_elt(const void* p, Elt t, int64_t i) {
+  if (t == Elt::F32) return ((const float*)p)[i];
+  if (t == Elt::F16) return __half2float(((const __half*)p)[i]);
+  return __bfloat162float(((const __nv_bfloat16*)p)[i]);
+}
+FAK_DEV void store_elt(void* p, Elt t, int64_t i, float v) {
+  if (t == Elt::F32) ((float*)p)[i] = v;
+  else if (t == Elt::F16) ((__half*)p)[i] = __float2half_rn(v);
+  else ((__nv_bfloat16*)p)[i] = __float2bfloat16_rn(v);
+}
+
+template <int D, int NT>
+struct Smem {
+  static constexpr int COLS = 8 * NT;
+  static constexpr int OSTRIDE = D + 4;   // floats per column of the merge area (keeps its stores on distinct banks)
+  union {
+    uint8_t ring[W][STAGES][Lay<D>::BYTES];
+    float o[W][COLS][OSTRIDE];
+  };
+  uint64_t full[W][STAGES];
+  float base[W][COLS], sum[W][COLS];
+};
+
+template <int D, int NT, bool CAP>
+__global__ void __launch_bounds__(W * 32)
+k_kv4_attn(Kv4Attn a, int n_split) {
+  using L = Lay<D>;
+  constexpr int NG = L::NG;
+  constexpr int COLS = 8 * NT;
+  extern __shared__ __align__(128) uint8_t smem_raw[];
+  Smem<D, NT>& sm = *reinterpret_cast<Smem<D, NT>*>(smem_raw);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int g = lane >> 2, t = lane & 3;
+  const int split = blockIdx.x % n_split, rc = blockIdx.x / n_split, kvh = blockIdx.y, b = blockIdx.z;
+  const int G = a.H / a.Hkv;
+  if (lane < STAGES) tc::mbar_init(&sm.full[warp][lane], 1);
+  tc::fence_mbar_init();
+  __syncwarp();
+  pdl_wait();
+
+  const int ctx = min(a.ctx[b], a.width * PAGE);
+  int tok0 = b, n = 1;
+  if (a.q_off) {
+    tok0 = max(a.q_off[b], 0);
+    n = min(a.q_off[b + 1], a.n_tokens) - tok0;
+    if (n > a.max_new) {
+      report_error(a.err, 3);
+      n = a.max_new;
+    }
+  }
+  const int R = n * G, r0 = rc * COLS;
+  if (R <= r0) return;
+  const Span sp = span_of(ctx, n, r0 / G, min(R - 1, r0 + COLS - 1) / G, a.window, n_split, a.width);
+  const int p_begin = sp.p0 + split * sp.pps, p_end = min(sp.p1, p_begin + sp.pps);
+  if (p_begin >= p_end && !(split == 0 && sp.live == 0)) return;
+
+  // pages of this warp: p_begin + warp, + W, ..; 32 table entries at a time, one a lane
+  const int np = max(0, (p_end - p_begin - warp + W - 1) / W);
+  const int* table = a.table + (int64_t)b * a.table_stride + p_begin + warp;
+  int entry = 0;
+  auto fetch_entries = [&](int i) {   // entries of pages i .. i + 31 of this warp
+    entry = i + lane < np ? table[(int64_t)W * (i + lane)] : 0;
+    if ((unsigned)entry >= (uint64_t)a.n_pages) {
+      report_error(a.err, 2);
+      entry = 0;
+    }
+  };
+  auto issue = [&](int i) {
+    if ((i & 31) == 0) fetch_entries(i);
+    const int pid = __shfl_sync(0xffffffffu, entry, i & 31);
+    if (lane == 0) {
+      uint64_t* bar = &sm.full[warp][i % STAGES];
+      tc::mbar_arrive_expect_tx(bar, L::BYTES);
+      bulk_load(sm.ring[warp][i % STAGES], a.pages + ((int64_t)pid * a.Hkv + kvh) * L::BYTES, L::BYTES, bar);
+    }
+  };
+#pragma unroll
+  for (int i = 0; i < STAGES - 1; i++)
+    if (i < np) issue(i);
+
+  // Queries: lane (g, t) holds column nt * 8 + g, dims group * 32 + 8 t .. + 7
+  uint32_t qf[NT][NG][4], qs[NT];
+  float cf[NT][2];                 // logit factor (log2 units) of columns 2 t, 2 t + 1
+  int lim[NT][2], low[NT][2];      // keys [low, lim) are seen by the column
+  int lim_min = INT_MAX, low_max = 0;
+#pragma unroll
+  for (int nt = 0; nt < NT; nt++) {
+    const int r = r0 + nt * 8 + g;
+    const bool live = r < R;
+    const int i = live ? r / G : 0, h = kvh * G + (live ? r % G : 0);
+    float x[NG][8], amax = 0.f;
+    const int64_t at = (int64_t)(tok0 + i) * a.q_tok + (int64_t)h * a.q_head + 8 * t;
+#pragma unroll
+    for (int gr = 0; gr < NG; gr++)
+#pragma unroll
+      for (int e = 0; e < 8; e++) {
+        x[gr][e] = live ? load_elt(a.q, a.q_type, at + gr * 32 + e) : 0.f;
+        amax = fmaxf(amax, fabsf(x[gr][e]));
+      }
+    amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+    amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+    // power of two that brings the row's largest into [2^13, 2^14)
+    int ex = 0;
+    if (amax > 0.f && amax < INFINITY) frexpf(amax, &ex);
+    ex = amax > 0.f && amax < INFINITY ? 14 - ex : 0;
+    // (a denormal maximum would ask for more than 2^127: two steps)
+    const float f1 = exp2f((float)(ex / 2)), f2 = exp2f((float)(ex - ex / 2));
+    float sum[NG];
+#pragma unroll
+    for (int gr = 0; gr < NG; gr++) {
+      sum[gr] = 0.f;
+      float y[8];
+#pragma unroll
+      for (int e = 0; e < 8; e++) {
+        y[e] = __half2float(__float2half_rn(x[gr][e] * f1 * f2));
+        sum[gr] += y[e];
+      }
+      // nibble pairs (e, e + 4); the odd pairs arrive 16 times too large
+      qf[nt][gr][0] = pack_f16(y[0], y[4]);
+      qf[nt][gr][1] = pack_f16(y[1] * 0.0625f, y[5] * 0.0625f);
+      qf[nt][gr][2] = pack_f16(y[2], y[6]);
+      qf[nt][gr][3] = pack_f16(y[3] * 0.0625f, y[7] * 0.0625f);
+      sum[gr] += __shfl_xor_sync(0xffffffffu, sum[gr], 1);
+      sum[gr] += __shfl_xor_sync(0xffffffffu, sum[gr], 2);
+      sum[gr] *= 0.015625f;   // |sum| <= 32 * 2^14: back into f16's range
+    }
+    // B of the m16n8k8: rows 2 t, 2 t + 1 = the groups' sums, their high parts then the remainders
+    {
+      const int pr = NG == 4 ? (t & 1) : 0;
+      const bool lo_part = NG == 4 ? t >= 2 : t == 1;
+      float s0 = sum[0], s1 = sum[1];
+      if constexpr (NG == 4) {
+        s0 = pr ? sum[2] : sum[0];
+        s1 = pr ? sum[3] : sum[1];
+      }
+      const float h0 = __half2float(__float2half_rn(s0)), h1 = __half2float(__float2half_rn(s1));
+      qs[nt] = lo_part ? pack_f16(s0 - h0, s1 - h1) : pack_f16(h0, h1);
+      if (NG == 2 && t >= 2) qs[nt] = 0;
+    }
+    const int my_lim = live ? min(ctx - n + i + 1, ctx) : 0;
+    const int my_low = live && a.window > 0 ? max(0, my_lim - a.window) : 0;
+    const float my_cf = 64.f / f1 / f2 * a.scale * (CAP ? 1.f : LOG2E);
+#pragma unroll
+    for (int e = 0; e < 2; e++) {
+      lim[nt][e] = __shfl_sync(0xffffffffu, my_lim, (2 * t + e) * 4);
+      low[nt][e] = __shfl_sync(0xffffffffu, my_low, (2 * t + e) * 4);
+      cf[nt][e] = __shfl_sync(0xffffffffu, my_cf, (2 * t + e) * 4);
+    }
+    if (live) {
+      lim_min = min(lim_min, my_lim);
+      low_max = max(low_max, my_low);
+    }
+  }
+  // keys every live row sees: pages inside [low_max, lim_min) need no mask (dead columns are dropped
+  // at the end).  Keys outside [low_any, lim_any) are seen by no row: their V is not touched.
+#pragma unroll
+  for (int d = 4; d < 32; d <<= 1) {
+    lim_min = min(lim_min, __shfl_xor_sync(0xffffffffu, lim_min, d));
+    low_max = max(low_max, __shfl_xor_sync(0xffffffffu, low_max, d));
+  }
+  const int i_first = r0 / G, i_last = min(R - 1, r0 + COLS - 1) / G;
+  const int lim_any = ctx - n + i_last + 1;
+  const int low_any = a.window > 0 ? max(0, ctx - n + i_first + 1 - a.window) : 0;
+
+  float o[NT][NG][2][4], mt[NT][4], base[NT][2];
+#pragma unroll
+  for (int nt = 0; nt < NT; nt++) {
+    base[nt][0] = base[nt][1] = -INFINITY;
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+      mt[nt][e] = 0.f;
+#pragma unroll
+      for (int gr = 0; gr < NG; gr++) o[nt][gr][0][e] = o[nt][gr][1][e] = 0.f;
+    }
+  }
+  constexpr uint32_t M0 = 0x000f000fu, M4 = 0x00f000f0u;
+  const float cap_in = CAP ? 1.f / a.softcap : 0.f, cap_out = CAP ? a.softcap * LOG2E : 0.f;
+  bool ok = true;
+  int done = 0;   // pages waited for
+
+#pragma unroll 1
+  for (int i = 0; i < np; i++) {
+    if (i + STAGES - 1 < np) issue(i + STAGES - 1);
+    ok = ok && tc::mbar_wait(&sm.full[warp][i % STAGES], (uint32_t)((i / STAGES) & 1), a.err);
+    done = i + 1;
+    if (!__all_sync(0xffffffffu, ok)) break;
+    const uint8_t* pg = sm.ring[warp][i % STAGES];
+    const int key0 = (p_begin + warp + W * i) * PAGE;
+    const bool whole = key0 >= low_max && key0 + PAGE <= lim_min;   // warp-uniform
+
+    // S^T: rows = tokens g and g + 8, columns = query rows 2 t, 2 t + 1 of each n-tile
+    float z[NT][4];
+    {
+      uint32_t k0[NG], k1[NG], s0[NG / 2], s1[NG / 2], m0[1], m1[1];
+      lds(pg + L::KC + g * (D / 2) + t * 4 * NG, k0);
+      lds(pg + L::KC + (g + 8) * (D / 2) + t * 4 * NG, k1);
+      lds(pg + L::KS + g * 2 * NG, s0);
+      lds(pg + L::KS + (g + 8) * 2 * NG, s1);
+      lds(pg + L::KM + g * 2 * NG + (NG == 4 ? (t & 1) * 4 : 0), m0);
+      lds(pg + L::KM + (g + 8) * 2 * NG + (NG == 4 ? (t & 1) * 4 : 0), m1);
+      float acc[NT][4];
+#pragma unroll
+      for (int nt = 0; nt < NT; nt++) {
+        acc[nt][0] = acc[nt][1] = acc[nt][2] = acc[nt][3] = 0.f;
+        z[nt][0] = z[nt][1] = z[nt][2] = z[nt][3] = 0.f;
+        mma_f16_1688(z[nt], m0[0], m1[0], qs[nt]);
+      }
+#pragma unroll
+      for (int gr = 0; gr < NG; gr++) {
+        const uint32_t w0 = k0[gr], w1 = k1[gr], u0 = w0 >> 8, u1 = w1 >> 8;
+        const float2 f0 = unpack_h2(s0[gr / 2]), f1 = unpack_h2(s1[gr / 2]);
+        const float sa = gr & 1 ? f0.y : f0.x, sb = gr & 1 ? f1.y : f1.x;
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++) {
+          float d[4] = {0.f, 0.f, 0.f, 0.f};
+          mma_f16_16816(d, w0 & M0, w1 & M0, w0 & M4, w1 & M4, qf[nt][gr][0], qf[nt][gr][1]);
+          mma_f16_16816(d, u0 & M0, u1 & M0, u0 & M4, u1 & M4, qf[nt][gr][2], qf[nt][gr][3]);
+          acc[nt][0] = fmaf(sa, d[0], acc[nt][0]);
+          acc[nt][1] = fmaf(sa, d[1], acc[nt][1]);
+          acc[nt][2] = fmaf(sb, d[2], acc[nt][2]);
+          acc[nt][3] = fmaf(sb, d[3], acc[nt][3]);
+        }
+      }
+      // codes carry 2^-24, the sums 2^-6
+#pragma unroll
+      for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          z[nt][e] = fmaf(acc[nt][e], 262144.f, z[nt][e]) * cf[nt][e & 1];
+          if constexpr (CAP) z[nt][e] = cap_out * tanhf(z[nt][e] * cap_in);
+        }
+    }
+    if (!whole) {
+#pragma unroll
+      for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          const int key = key0 + g + (e >> 1) * 8;
+          if (key < low[nt][e & 1] || key >= lim[nt][e & 1]) z[nt][e] = -INFINITY;
+        }
+    }
+    bool grow = false;
+#pragma unroll
+    for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+      for (int e = 0; e < 4; e++) grow |= z[nt][e] > base[nt][e & 1] + HEADROOM;
+    if (__any_sync(0xffffffffu, grow)) {
+#pragma unroll
+      for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+          float m = fmaxf(z[nt][e], z[nt][e + 2]);
+          m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
+          m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
+          m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
+          m = fmaxf(m, base[nt][e]);
+          const float f = m == -INFINITY ? 1.f : ex2(base[nt][e] - m);
+          base[nt][e] = m;
+          mt[nt][e] *= f;
+#pragma unroll
+          for (int gr = 0; gr < NG; gr++)
+#pragma unroll
+            for (int hf = 0; hf < 2; hf++) {
+              o[nt][gr][hf][e] *= f;
+              o[nt][gr][hf][e + 2] *= f;
+            }
+        }
+    }
+    uint32_t p0[NT], p1[NT];
+#pragma unroll
+    for (int nt = 0; nt < NT; nt++) {
+      float p[4];
+#pragma unroll
+      for (int e = 0; e < 4; e++) {
+        const float bs = base[nt][e & 1] == -INFINITY ? 0.f : base[nt][e & 1];
+        p[e] = ex2(z[nt][e] - bs + LIFT);
+      }
+      p0[nt] = movmatrix(pack_f16(p[0], p[1]));   // tokens 2 t, 2 t + 1 of column g
+      p1[nt] = movmatrix(pack_f16(p[2], p[3]));   // tokens 2 t + 8, 2 t + 9
+    }
+    {
+      uint32_t v0[NG], v1[NG], s0[NG], s1[NG];
+      const int x = g ^ (2 * t);   // pairs t and t + 4 share it
+      lds(pg + L::VC + ((t * 8 + x) * NG) * 4, v0);
+      lds(pg + L::VC + (((t + 4) * 8 + x) * NG) * 4, v1);
+      lds(pg + L::VS + t * NG * 4, s0);
+      lds(pg + L::VS + (t + 4) * NG * 4, s1);
+      uint32_t m0 = 0, m1 = 0;   // rows 0 .. NG - 1: minima of the groups; row 4: ones
+      if (g < NG) {
+        m0 = *reinterpret_cast<const uint32_t*>(pg + L::VM + (t * NG + g) * 4);
+        m1 = *reinterpret_cast<const uint32_t*>(pg + L::VM + ((t + 4) * NG + g) * 4);
+      } else if (g == 4) {
+        m0 = m1 = 0x3c003c00u;
+      }
+      if (key0 < low_any || key0 + PAGE > lim_any) {
+        // tokens no row sees: whatever their bytes hold (memory nobody wrote) must not reach the sums
+        auto keep = [&](int tok) {
+          const bool lo_ok = key0 + tok >= low_any && key0 + tok < lim_any;
+          const bool hi_ok = key0 + tok + 1 >= low_any && key0 + tok + 1 < lim_any;
+          return (lo_ok ? 0x0000ffffu : 0u) | (hi_ok ? 0xffff0000u : 0u);
+        };
+        const uint32_t keep0 = keep(2 * t), keep1 = keep(2 * t + 8);
+#pragma unroll
+        for (int gr = 0; gr < NG; gr++) {
+          s0[gr] &= keep0;
+          s1[gr] &= keep1;
+        }
+        m0 &= keep0;
+        m1 &= keep1;
+      }
+#pragma unroll
+      for (int nt = 0; nt < NT; nt++) mma_f16_16816(mt[nt], m0, 0u, m1, 0u, p0[nt], p1[nt]);
+#pragma unroll
+      for (int gr = 0; gr < NG; gr++) {
+        const uint32_t w0 = v0[gr], w1 = v1[gr], u0 = w0 >> 8, u1 = w1 >> 8;
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++) {
+          const uint32_t b0 = mul_h2(p0[nt], s0[gr]), b1 = mul_h2(p1[nt], s1[gr]);
+          mma_f16_16816(o[nt][gr][0], w0 & M0, w0 & M4, w1 & M0, w1 & M4, b0, b1);   // dims 4 g, 4 g + 1
+          mma_f16_16816(o[nt][gr][1], u0 & M0, u0 & M4, u1 & M0, u1 & M4, b0, b1);   // dims 4 g + 2, 4 g + 3
+        }
+      }
+    }
+    __syncwarp();   // every lane is done with the stage before it is refilled
+  }
+
+  // a wait gave up (the error word says so): the copies still in flight are waited for, again with a limit
+  for (int i = done; i < min(np, done + STAGES - 1); i++)
+    tc::mbar_wait(&sm.full[warp][i % STAGES], (uint32_t)((i / STAGES) & 1), a.err);
+  // merge the CTA's warps; the ring is free once every warp has drained its copies
+  __syncthreads();
+#pragma unroll
+  for (int nt = 0; nt < NT; nt++) {
+    float ml[NG][2];
+#pragma unroll
+    for (int gr = 0; gr < NG; gr++)
+#pragma unroll
+      for (int e = 0; e < 2; e++) ml[gr][e] = __shfl_sync(0xffffffffu, mt[nt][e], gr * 4 + t);
+#pragma unroll
+    for (int e = 0; e < 2; e++) {
+      const int col = nt * 8 + 2 * t + e;
+#pragma unroll
+      for (int gr = 0; gr < NG; gr++)
+        *reinterpret_cast<float4*>(&sm.o[warp][col][gr * 32 + 4 * g]) =
+            make_float4(fmaf(o[nt][gr][0][e], 16777216.f, ml[gr][e]), fmaf(o[nt][gr][0][e + 2], 1048576.f, ml[gr][e]),
+                        fmaf(o[nt][gr][1][e], 16777216.f, ml[gr][e]), fmaf(o[nt][gr][1][e + 2], 1048576.f, ml[gr][e]));
+      if (g == 4) {
+        sm.base[warp][col] = base[nt][e];
+        sm.sum[warp][col] = mt[nt][e];
+      }
+    }
+  }
+  __syncthreads();
+  pdl_launch_dependents();
+  const bool alone = n_split == 1;
+  const int64_t part_col = (((int64_t)b * a.Hkv + kvh) * (gridDim.x / n_split) + rc) * COLS;
+  float* part_ml = a.part + (int64_t)gridDim.z * gridDim.y * (gridDim.x / n_split) * COLS * n_split * D;
+  for (int c = warp; c < COLS; c += W) {
+    const int r = r0 + c;
+    if (r >= R) break;
+    const int h = kvh * G + r % G;
+    float m = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < W; w++) m = fmaxf(m, sm.base[w][c]);
+    const float sink = alone && a.sinks ? a.sinks[h] * LOG2E : -INFINITY;
+    const float mt_ = fmaxf(m, sink), bs = mt_ == -INFINITY ? 0.f : mt_;
+    float f[W], l = 0.f;
+#pragma unroll
+    for (int w = 0; w < W; w++) {
+      f[w] = ex2(sm.base[w][c] - bs);
+      if (sm.base[w][c] == -INFINITY) f[w] = 0.f;
+      l += f[w] * sm.sum[w][c];
+    }
+    if (sink > -INFINITY) l += ex2(sink - bs + LIFT);
+#pragma unroll
+    for (int d0 = 0; d0 < D; d0 += 64) {
+      const int d = d0 + 2 * lane;
+      float2 v = make_float2(0.f, 0.f);
+#pragma unroll
+      for (int w = 0; w < W; w++) {
+        const float2 y = *reinterpret_cast<const float2*>(&sm.o[w][c][d]);
+        v.x += f[w] * y.x;
+        v.y += f[w] * y.y;
+      }
+      if (alone) {
+        const float inv = l != 0.f ? 1.f / l : 0.f;
+        const int64_t at = (int64_t)(tok0 + r / G) * a.o_tok + (int64_t)h * a.o_head + d;
+        store_elt(a.out, a.o_type, at, v.x * inv);
+        store_elt(a.out, a.o_type, at + 1, v.y * inv);
+      } else {
+        *reinterpret_cast<float2*>(a.part + ((part_col + c) * n_split + split) * D + d) = v;
+      }
+    }
+    if (!alone && lane == 0) {
+      float* ml = part_ml + ((part_col + c) * n_split + split) * 2;
+      ml[0] = mt_;
+      ml[1] = l;
+    }
+  }
+}
+
+// One warp merges the live splits of one query row: D / 32 dims a lane.
+template <int D>
+__global__ void __launch_bounds__(128) k_kv4_combine(Kv4Attn a, int n_split, int cols, int row_chunks) {
+  constexpr int V = D / 32;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rc = blockIdx.x, kvh = blockIdx.y, b = blockIdx.z;
+  const int G = a.H / a.Hkv;
+  pdl_wait();
+  const int ctx = min(a.ctx[b], a.width * PAGE);
+  int tok0 = b, n = 1;
+  if (a.q_off) {
+    tok0 = max(a.q_off[b], 0);
+    n = min(min(a.q_off[b + 1], a.n_tokens) - tok0, a.max_new);
+  }
+  const int R = n * G, r0 = rc * cols;
+  if (R <= r0) return;
+  const Span sp = span_of(ctx, n, r0 / G, min(R - 1, r0 + cols - 1) / G, a.window, n_split, a.width);
+  const int live = max(1, sp.live);   // an empty block's split 0 wrote zeros
+  const int64_t part_col = (((int64_t)b * a.Hkv + kvh) * row_chunks + rc) * cols;
+  const float* part_ml = a.part + (int64_t)gridDim.z * gridDim.y * row_chunks * cols * n_split * D;
+  for (int c = warp; c < cols && r0 + c < R; c += 4) {
+    const int r = r0 + c, h = kvh * G + r % G;
+    const float2* ml = reinterpret_cast<const float2*>(part_ml) + (part_col + c) * n_split;
+    const float* po = a.part + (part_col + c) * n_split * D + V * lane;
+    float m = a.sinks ? a.sinks[h] * LOG2E : -INFINITY;
+    const float sink = m;
+    for (int s = lane; s < live; s += 32) m = fmaxf(m, __ldcg(&ml[s].x));
+    m = warp_max(m);
+    const float bs = m == -INFINITY ? 0.f : m;
+    float l = sink > -INFINITY ? ex2(sink - bs + LIFT) : 0.f;
+    float acc[V] = {};
+    for (int s0 = 0; s0 < live; s0 += 32) {
+      float f = 0.f, ls = 0.f;
+      if (s0 + lane < live) {
+        const float2 y = __ldcg(&ml[s0 + lane]);
+        f = y.x == -INFINITY ? 0.f : ex2(y.x - bs);
+        ls = f * y.y;
+      }
+      l += warp_sum(ls);
+      const int e = min(32, live - s0);
+#pragma unroll 8
+      for (int s = 0; s < e; s++) {
+        const float fs = __shfl_sync(0xffffffffu, f, s);
+        const float* p = po + (int64_t)(s0 + s) * D;
+        if constexpr (V == 4) {
+          const float4 y = __ldcg(reinterpret_cast<const float4*>(p));
+          acc[0] += fs * y.x; acc[1] += fs * y.y; acc[2] += fs * y.z; acc[3] += fs * y.w;
+        } else {
+          const float2 y = __ldcg(reinterpret_cast<const float2*>(p));
+          acc[0] += fs * y.x; acc[1] += fs * y.y;
+        }
+      }
+    }
+    const float inv = l != 0.f ? 1.f / l : 0.f;
+    const int64_t at = (int64_t)(tok0 + r / G) * a.o_tok + (int64_t)h * a.o_head + V * lane;
+#pragma unroll
+    for (int i = 0; i < V; i++) store_elt(a.out, a.o_type, at + i, acc[i] * inv);
+  }
+  pdl_launch_dependents();
+}
+
+void pdl(cudaLaunchConfig_t& cfg, cudaLaunchAttribute* attr) {
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = pdl_allowed();
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+}
+
+}  // namespace
+
+Kv4AttnPlan kv4_attn_plan(const Kv4Attn& a, int n_sm) {
+  Kv4AttnPlan p;
+  const int64_t rows = (int64_t)a.max_new * (a.H / a.Hkv);
+  const int nt_most = a.D == 64 ? 4 : 2;
+  p.nt = rows <= 8 ? 1 : (rows <= 16 || nt_most == 2 ? 2 : 4);
+  p.row_chunks = (int)((rows + 8 * p.nt - 1) / (8 * p.nt));
+  // splits: about four CTAs a SM, each warp at least one page
+  const int64_t ctas = (int64_t)a.B * a.Hkv * p.row_chunks;
+  const int most = (a.width + W - 1) / W;
+  int s = a.n_split;
+  if (s <= 0) s = (int)std::min<int64_t>(256, (4 * n_sm + ctas - 1) / std::max<int64_t>(1, ctas));
+  p.n_split = std::max(1, std::min(s, most));
+  p.part_floats = p.n_split > 1 ? ctas * 8 * p.nt * p.n_split * (a.D + 2) : 0;
+  return p;
+}
+
+void kv4_attn_launch(const Kv4Attn& a, const Kv4AttnPlan& p, cudaStream_t stream) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(p.n_split * p.row_chunks), (unsigned)a.Hkv, (unsigned)a.B);
+  cfg.blockDim = dim3(W * 32);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  pdl(cfg, attr);
+  auto go = [&](auto kern, size_t smem) {
+    cfg.dynamicSmemBytes = smem;
+    if (smem > 48 * 1024) FAK_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    FAK_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kern, a, p.n_split));
+  };
+  const bool cap = a.softcap > 0.f;
+#define FAK_KV4(DV, NTV)                                                    \
+  {                                                                         \
+    if (cap) go(k_kv4_attn<DV, NTV, true>, sizeof(Smem<DV, NTV>));          \
+    else go(k_kv4_attn<DV, NTV, false>, sizeof(Smem<DV, NTV>));             \
+  }
+  if (a.D == 128) {
+    if (p.nt == 1) FAK_KV4(128, 1)
+    else FAK_KV4(128, 2)
+  } else {
+    if (p.nt == 1) FAK_KV4(64, 1)
+    else if (p.nt == 2) FAK_KV4(64, 2)
+    else FAK_KV4(64, 4)
+  }
+#undef FAK_KV4
+  if (p.n_split > 1) {
+    cudaLaunchConfig_t c2 = {};
+    c2.gridDim = dim3((unsigned)p.row_chunks, (unsigned)a.Hkv, (unsigned)a.B);
+    c2.blockDim = dim3(128);
+    c2.stream = stream;
+    pdl(c2, attr);
+    if (a.D == 128) FAK_CUDA_CHECK(cudaLaunchKernelEx(&c2, k_kv4_combine<128>, a, p.n_split, 8 * p.nt, p.row_chunks));
+    else FAK_CUDA_CHECK(cudaLaunchKernelEx(&c2, k_kv4_combine<64>, a, p.n_split, 8 * p.nt, p.row_chunks));
+  }
+}
+
+}  // namespace fak

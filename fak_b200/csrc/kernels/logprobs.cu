@@ -1,0 +1,326 @@
+// Log probability, rank, entropy and top alternatives of given tokens, in one pass over the logit rows.
+//
+// Per row x[V], target t, with M = max x and S = sum e^(x - M):
+//   logprob = (x_t - M) - ln S            rank = 1 + #{x_i > x_t} + #{x_i = x_t, i < t}
+//   entropy = ln S - sum e^(x - M) (x - M) / S
+//   the k largest x with their indices, ties to the lowest index.
+// A target outside [0, V) has logprob 0 and rank 0.  A row with only -inf has entropy 0, logprobs -inf.
+//
+// A row is cut into n_seg segments (1 when there are enough rows to fill the machine), one CTA of 8
+// warps each; a warp walks its share of the segment in tiles of 32 lanes x 8 logits.  Each lane keeps its
+// own (M, S, sum) and moves M at most once a tile.  The top list is kept per warp, sorted, one 64-bit key
+// (ordered value, complemented index) a lane; a logit joins the warp's candidate buffer only when it
+// reaches the list's k-th value, which a random row does about k ln(n / 256) times a warp, and 32
+// candidates are sorted and merged at a time.  The first bound comes from the 32 lane maxima of the
+// first tile.  Segments meet in a scratch record per segment; the CTA that takes the row's last ticket
+// merges them in segment order, so results do not depend on the order of arrival.
+#include "common.cuh"
+
+#include <stdexcept>
+#include <string>
+
+#include "../serve_ops.h"
+
+namespace fak {
+namespace {
+
+constexpr int WARPS = 8;
+constexpr int THREADS = WARPS * 32;
+constexpr int PER = 8;                 // logits per lane and tile
+constexpr int TILE = 32 * PER;         // per warp
+constexpr int CAND = TILE + 32;        // candidate keys a warp can hold: < 32 waiting + one tile
+constexpr int MAXK = 32;
+constexpr int REC = 4 + 2 * MAXK;      // words of a segment's record: M, S, T, count, keys
+
+typedef unsigned long long u64;
+
+FAK_DEV u64 key_of(float v, uint32_t i) { return argmax_key(v + 0.f, i); }   // -0 counts as 0
+FAK_DEV float key_value(u64 k) {
+  const uint32_t u = (uint32_t)(k >> 32);
+  return __uint_as_float((u & 0x80000000u) ? (u & 0x7fffffffu) : ~u);
+}
+
+// Keys of a warp, one a lane: exchange towards descending order.
+FAK_DEV void cx(u64& a, int lane, int d, bool down) {
+  const u64 b = __shfl_xor_sync(0xffffffffu, a, d);
+  const bool low = (lane & d) == 0;
+  a = ((a > b) == (low == down)) ? a : b;
+}
+FAK_DEV u64 sort32(u64 a, int lane) {   // descending over lanes (bitonic)
+#pragma unroll
+  for (int n = 2; n <= 32; n <<= 1)
+#pragma unroll
+    for (int d = n >> 1; d > 0; d >>= 1) cx(a, lane, d, n == 32 || (lane & n) == 0);
+  return a;
+}
+FAK_DEV u64 merge32(u64 a, u64 b, int lane) {   // the 32 largest of two descending lists, descending
+  b = __shfl_xor_sync(0xffffffffu, b, 31);
+  a = a > b ? a : b;
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) cx(a, lane, d, true);
+  return a;
+}
+
+struct Stat {
+  float m, s, t;   // max, sum e^(x - m), sum e^(x - m) (x - m)
+};
+FAK_DEV float finite_max(float m) { return m == -INFINITY ? 0.f : m; }
+// (value, scale) of two partial sums against their common max; d = 0 where a side is empty
+FAK_DEV Stat join(const Stat& a, const Stat& b) {
+  Stat r;
+  r.m = fmaxf(a.m, b.m);
+  const float base = finite_max(r.m);
+  // (the clamp keeps 0 * infinity out of t when the maxima are the type's extremes)
+  const float da = a.s == 0.f ? 0.f : fmaxf(a.m - base, -1e30f), db = b.s == 0.f ? 0.f : fmaxf(b.m - base, -1e30f);
+  const float fa = exp2f(da * 1.4426950408889634f), fb = exp2f(db * 1.4426950408889634f);
+  r.s = a.s * fa + b.s * fb;
+  r.t = fa * (a.t + a.s * da) + fb * (b.t + b.s * db);
+  return r;
+}
+
+template <typename T>
+FAK_DEV void load8(const T* __restrict__ p, int i0, int end, bool vec, float (&x)[PER]) {
+  if constexpr (sizeof(T) == 4) {
+    // two float4 a lane, 128 logits apart
+#pragma unroll
+    for (int j = 0; j < 2; j++) {
+      const int i = i0 + j * 128;
+      if (vec && i + 4 <= end) {
+        const float4 f = __ldcs(reinterpret_cast<const float4*>(p + i));
+        x[4 * j] = f.x; x[4 * j + 1] = f.y; x[4 * j + 2] = f.z; x[4 * j + 3] = f.w;
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; e++) x[4 * j + e] = i + e < end ? p[i + e] : -INFINITY;
+      }
+    }
+  } else {
+    if (vec && i0 + 8 <= end) {
+      const uint4 u = __ldcs(reinterpret_cast<const uint4*>(p + i0));
+      T h[8];
+      memcpy(h, &u, 16);
+#pragma unroll
+      for (int e = 0; e < 8; e++) x[e] = (float)h[e];
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; e++) x[e] = i0 + e < end ? (float)p[i0 + e] : -INFINITY;
+    }
+  }
+}
+template <typename T>
+FAK_DEV int lane_first(int lane) { return sizeof(T) == 4 ? 4 * lane : 8 * lane; }
+template <typename T>
+FAK_DEV int elt_at(int e) { return sizeof(T) == 4 ? (e & 3) + (e >> 2) * 128 : e; }
+
+template <typename T, bool TOP, bool CAP>
+__global__ void __launch_bounds__(THREADS) k_logprobs(LogprobArgs a, int seg_len) {
+  __shared__ u64 s_cand[TOP ? WARPS : 1][TOP ? CAND : 1];
+  __shared__ u64 s_list[WARPS][32];
+  __shared__ Stat s_stat[WARPS];
+  __shared__ int s_cnt[WARPS];
+  __shared__ int s_last;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int seg = blockIdx.x;
+  const int64_t r = blockIdx.y + (int64_t)blockIdx.z * 32768;
+  if (r >= a.T) return;
+  pdl_wait();
+  const T* __restrict__ x = (const T*)a.x + r * a.stride;
+  auto cap = [&](float v) { return CAP ? a.softcap * tanhf(v / a.softcap) : v; };
+  const int tgt = a.target[r];
+  const bool given = tgt >= 0 && tgt < a.V;
+  const float xt = given ? cap((float)x[tgt]) : INFINITY;
+  const int i_begin = seg * seg_len, i_end = min(a.V, i_begin + seg_len);
+
+  Stat st = {-INFINITY, 0.f, 0.f};
+  int above = 0;
+  u64 top = 0, kth = 0;          // the warp's list (lane i: i-th largest) and its k-th key
+  float bound = -INFINITY;       // a lower bound of the k-th value over the logits seen so far
+  int waiting = 0;
+  bool first = true;
+  const int k = a.k;
+
+  for (int base = i_begin + warp * TILE; base < i_end; base += WARPS * TILE) {
+    float v[PER];
+    const int i0 = base + lane_first<T>(lane);
+    load8(x, i0, i_end, a.vec, v);
+    float mx = -INFINITY;
+#pragma unroll
+    for (int e = 0; e < PER; e++) {
+      if constexpr (CAP) v[e] = cap(v[e]);
+      mx = fmaxf(mx, v[e]);
+    }
+    if (mx > st.m) {   // move the base of this lane's sums
+      const float d = st.s == 0.f ? 0.f : fmaxf(st.m - mx, -1e30f), f = exp2f(d * 1.4426950408889634f);
+      st.t = f * (st.t + st.s * d);
+      st.s *= f;
+      st.m = mx;
+    }
+    const float mb = finite_max(st.m);
+#pragma unroll
+    for (int e = 0; e < PER; e++) {
+      const float d = v[e] - mb, p = exp2f(d * 1.4426950408889634f);
+      st.s += p;
+      st.t = fmaf(p, fmaxf(d, -1e30f), st.t);   // p is 0 where the clamp acts; a NaN stays in p
+    }
+    const bool past = base > tgt, before = base + TILE <= tgt;   // tile after / before the target
+    if (past) {
+#pragma unroll
+      for (int e = 0; e < PER; e++) above += v[e] > xt;
+    } else if (before) {
+#pragma unroll
+      for (int e = 0; e < PER; e++) above += v[e] >= xt;
+    } else {
+#pragma unroll
+      for (int e = 0; e < PER; e++) above += i0 + elt_at<T>(e) < tgt ? v[e] >= xt : v[e] > xt;
+    }
+    if constexpr (TOP) {
+      if (first) {   // 32 lane maxima: the k-th largest of them bounds the tile's k-th from below
+        first = false;
+        bound = key_value(__shfl_sync(0xffffffffu, sort32(key_of(mx, lane), lane), k - 1));
+      }
+      if (__any_sync(0xffffffffu, mx >= bound)) {
+#pragma unroll
+        for (int e = 0; e < PER; e++) {
+          const int i = i0 + elt_at<T>(e);
+          const u64 key = key_of(v[e], (uint32_t)i);
+          const bool take = v[e] >= bound && i < i_end && key > kth;
+          const uint32_t votes = __ballot_sync(0xffffffffu, take);
+          if (take) s_cand[warp][waiting + __popc(votes & ((1u << lane) - 1))] = key;
+          waiting += __popc(votes);
+        }
+        __syncwarp();
+        while (waiting >= 32) {
+          waiting -= 32;
+          top = merge32(top, sort32(s_cand[warp][waiting + lane], lane), lane);
+        }
+        kth = __shfl_sync(0xffffffffu, top, k - 1);
+        if (kth != 0) bound = fmaxf(bound, key_value(kth));
+        __syncwarp();
+      }
+    }
+  }
+  if constexpr (TOP) {
+    if (waiting > 0) top = merge32(top, sort32(lane < waiting ? s_cand[warp][lane] : 0ull, lane), lane);
+    s_list[warp][lane] = top;
+  }
+  // the lanes' sums, then the warps', always in the same order
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) {
+    Stat o;
+    o.m = __shfl_xor_sync(0xffffffffu, st.m, d);
+    o.s = __shfl_xor_sync(0xffffffffu, st.s, d);
+    o.t = __shfl_xor_sync(0xffffffffu, st.t, d);
+    st = (lane & d) ? join(o, st) : join(st, o);
+    above += __shfl_xor_sync(0xffffffffu, above, d);
+  }
+  if (lane == 0) {
+    s_stat[warp] = st;
+    s_cnt[warp] = above;
+  }
+  __syncthreads();
+  if (warp != 0 && a.n_seg == 1) return;
+  if (warp == 0) {
+    for (int w = 1; w < WARPS; w++) {
+      st = join(st, s_stat[w]);
+      above += s_cnt[w];
+      if constexpr (TOP) top = merge32(top, s_list[w][lane], lane);
+    }
+  }
+  if (a.n_seg > 1) {
+    float* rec = a.part + ((int64_t)r * a.n_seg + seg) * REC;
+    if (warp == 0) {
+      if (lane == 0) {
+        rec[0] = st.m; rec[1] = st.s; rec[2] = st.t;
+        rec[3] = __int_as_float(above);
+      }
+      if constexpr (TOP) reinterpret_cast<u64*>(rec + 4)[lane] = top;
+      __threadfence();
+      __syncwarp();
+      if (lane == 0) s_last = atomicAdd(a.tickets + r, 1) == a.n_seg - 1;
+    }
+    __syncthreads();
+    if (!s_last) {
+      pdl_launch_dependents();
+      return;
+    }
+    __threadfence();
+    // every warp takes the segments w, w + 8, ..; then warp 0 the warps
+    const float* recs = a.part + (int64_t)r * a.n_seg * REC;
+    st = {-INFINITY, 0.f, 0.f};
+    above = 0;
+    top = 0;
+    for (int s = warp; s < a.n_seg; s += WARPS) {
+      const float* q = recs + (int64_t)s * REC;
+      const Stat o = {__ldcg(q), __ldcg(q + 1), __ldcg(q + 2)};
+      st = join(st, o);
+      above += __float_as_int(__ldcg(q + 3));
+      if constexpr (TOP) top = merge32(top, __ldcg(reinterpret_cast<const u64*>(q + 4) + lane), lane);
+    }
+    if (lane == 0) {
+      s_stat[warp] = st;
+      s_cnt[warp] = above;
+    }
+    if constexpr (TOP) s_list[warp][lane] = top;
+    __syncthreads();
+    if (warp != 0) return;
+    for (int w = 1; w < WARPS; w++) {
+      st = join(st, s_stat[w]);
+      above += s_cnt[w];
+      if constexpr (TOP) top = merge32(top, s_list[w][lane], lane);
+    }
+    if (lane == 0) a.tickets[r] = 0;
+  }
+  const float log_s = logf(st.s);   // S >= 1 unless the row is empty
+  if (lane == 0) {
+    const bool none = st.m == -INFINITY && st.s == 0.f;
+    a.logprob[r] = !given ? 0.f : none ? -INFINITY : (xt - st.m) - log_s;
+    a.entropy[r] = none ? 0.f : log_s - st.t / st.s;
+    a.rank[r] = given ? above + 1 : 0;
+  }
+  if constexpr (TOP) {
+    if (lane < k) {
+      const bool has = top != 0;
+      const float tv = key_value(top);
+      a.top_ids[r * k + lane] = has ? argmax_key_index(top) : -1;
+      a.top_logprobs[r * k + lane] = !has || tv == -INFINITY ? (st.s != st.s ? st.s : -INFINITY) : (tv - st.m) - log_s;
+    }
+  }
+}
+
+}  // namespace
+
+// Segments per row: enough CTAs for four a SM, a segment at least two tiles of every warp.
+int logprob_segments(int T, int V, int n_sm) {
+  const int most = (V + 2 * WARPS * TILE - 1) / (2 * WARPS * TILE);
+  const int want = (4 * n_sm + T - 1) / T;
+  const int n = want < most ? want : most;
+  return n < 1 ? 1 : (n > 64 ? 64 : n);
+}
+int64_t logprob_part_words(int T, int n_seg) { return n_seg > 1 ? (int64_t)T * n_seg * REC : 0; }
+
+void logprob_launch(const LogprobArgs& a, cudaStream_t stream) {
+  if (a.T == 0) return;
+  int seg = (a.V + a.n_seg - 1) / a.n_seg;
+  seg = (seg + TILE - 1) / TILE * TILE;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)a.n_seg, (unsigned)(a.T < 32768 ? a.T : 32768), (unsigned)((a.T + 32767) / 32768));
+  cfg.blockDim = dim3(THREADS);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = pdl_allowed();
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  auto go = [&](auto tag) {
+    using E = decltype(tag);
+    const bool top = a.k > 0, cap = a.softcap > 0.f;
+    if (top && cap) FAK_CUDA_CHECK(cudaLaunchKernelEx(&cfg, k_logprobs<E, true, true>, a, seg));
+    else if (top) FAK_CUDA_CHECK(cudaLaunchKernelEx(&cfg, k_logprobs<E, true, false>, a, seg));
+    else if (cap) FAK_CUDA_CHECK(cudaLaunchKernelEx(&cfg, k_logprobs<E, false, true>, a, seg));
+    else FAK_CUDA_CHECK(cudaLaunchKernelEx(&cfg, k_logprobs<E, false, false>, a, seg));
+  };
+  if (a.type == Elt::F32) go(float());
+  else if (a.type == Elt::F16) go(__half());
+  else go(__nv_bfloat16());
+}
+
+}  // namespace fak

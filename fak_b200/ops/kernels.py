@@ -1,6 +1,8 @@
 """Thin typed wrappers over the sm_100a extension, plus the GEMM dispatch used by prefill."""
 from __future__ import annotations
 
+from typing import NamedTuple
+
 import torch
 
 from ._ext import ext
@@ -305,3 +307,133 @@ def gemm(a: torch.Tensor, w, out: torch.Tensor, epi: int = EPI_STORE, bias: torc
     """out (op)= a[M,K] (bf16) . W^T on the tcgen05 tensor cores (W: QuantWeight -> its dense bf16 copy)."""
     ext().gemm_bf16(a, w.dense() if not isinstance(w, torch.Tensor) else w, out, bias, epi, err)
     count()
+
+
+# ------------------------------------------------------------------------------ 4-bit KV cache
+KV4_PAGE = 16
+
+
+def kv4_page_bytes(head_dim: int) -> int:
+    """Bytes of one (16-token page, KV head) of the 4-bit cache: codes of K and V, an f16 scale and
+    minimum per token and 32 dims of each (csrc/kernels/kv4.cuh has the order)."""
+    if head_dim not in (64, 128):
+        raise ValueError(f"the 4-bit KV cache takes head dim 64 or 128, not {head_dim}")
+    return 20 * head_dim
+
+
+def kv4_append(k: torch.Tensor, v: torch.Tensor, slot: torch.Tensor, pages: torch.Tensor) -> None:
+    """Quantize rows into one layer's pages [P, Hkv, kv4_page_bytes(D)] (uint8).
+
+    k, v: [T, Hkv, D] (float32, float16 or bfloat16; token and head strides free, so slices of a fused
+    q|k|v projection do), or the pages [P', Hkv, 16, D] of a 16-bit cache whose tokens 0 .. T - 1 are
+    meant.  slot [T] int32: page * 16 + offset of each row, -1 for rows to skip.  A slot past the pages
+    is skipped and reported as code 2 in the device's error word.  Groups of 32 dims get
+    minimum = f16(min x), scale = f16((max x - minimum) / 15), code = rint((x - minimum) / scale);
+    values are clamped to +-65504, a group with a NaN reads back as NaN."""
+    ext().kv4_append(k, v, slot, pages, _err_word.get(pages.device))
+    count()
+
+
+def kv4_read(pages: torch.Tensor, slot: torch.Tensor, head_dim: int, dtype: torch.dtype = torch.bfloat16
+             ) -> tuple[torch.Tensor, torch.Tensor]:
+    """The values that rows of one layer's 4-bit pages stand for: k, v [T, Hkv, D] of ``dtype`` (rows with
+    slot -1 are zero)."""
+    k, v = ext().kv4_read(pages, slot, head_dim, dtype, _err_word.get(pages.device))
+    count()
+    return k, v
+
+
+def kv4_decode_attention(q: torch.Tensor, pages: torch.Tensor, block_table: torch.Tensor, ctx_len: torch.Tensor,
+                         out: torch.Tensor, *, scale: float = 0.0, softcap: float = 0.0, window: int = 0,
+                         sinks: torch.Tensor | None = None, n_split: int = 0, workspace: torch.Tensor | None = None) -> None:
+    """One query token per sequence over the 4-bit cache: q, out [B, H, D] (float32, float16 or bfloat16,
+    each its own; token and head strides free), pages of one layer, block_table [B, W] int32, ctx_len [B]
+    int32 keys per sequence (the token's own among them; 0 gives a row of zeros).  scale 0 = 1/sqrt(D);
+    softcap > 0: logits cap * tanh(logit / cap); window > 0: the last ``window`` keys; sinks [H] f32.
+    n_split splits of each sequence's pages (0: chosen from B, heads and the table's width; a fixed count
+    makes a sequence's result independent of its batch).  workspace: float32 scratch for the splits
+    (allocated when not given)."""
+    ext().kv4_attention(q, pages, block_table, None, ctx_len, out, 1, scale, softcap, window, sinks, n_split, workspace,
+                        _err_word.get(q.device))
+    count()
+
+
+def kv4_prefill_attention(q: torch.Tensor, pages: torch.Tensor, block_table: torch.Tensor, q_off: torch.Tensor,
+                          ctx_len: torch.Tensor, out: torch.Tensor, max_new: int, *, scale: float = 0.0,
+                          softcap: float = 0.0, window: int = 0, sinks: torch.Tensor | None = None, n_split: int = 0,
+                          workspace: torch.Tensor | None = None) -> None:
+    """Causal attention of packed new tokens (their K / V already appended) over the 4-bit cache: q, out
+    [T, H, D]; q_off [B + 1] int32 packed offsets of the sequences' tokens (``BatchPlan.q_off``), ctx_len
+    [B] int32 keys with the new ones (``BatchPlan.ctx``); max_new: an upper bound of the new tokens of one
+    sequence.  Sequences without new tokens are skipped.  The other arguments as kv4_decode_attention."""
+    ext().kv4_attention(q, pages, block_table, q_off, ctx_len, out, max_new, scale, softcap, window, sinks, n_split,
+                        workspace, _err_word.get(q.device))
+    count()
+
+
+class BatchPlan(NamedTuple):
+    """Plan of a ragged batch (int32 on the device).  Rows past the last new token: slot -1, pos 0, seq -1."""
+    slot: torch.Tensor       # [max_tokens] cache slot (page * 16 + offset) of each packed new token
+    pos: torch.Tensor        # [max_tokens] its position in its sequence
+    seq: torch.Tensor        # [max_tokens] its request
+    q_off: torch.Tensor      # [B + 1] packed offset of each request's first new token
+    ctx: torch.Tensor        # [B] cached + new tokens
+    last: torch.Tensor       # [B] packed index of the request's last new token (-1: none)
+    free_head: torch.Tensor  # [1] free pages consumed so far
+
+    @classmethod
+    def allocate(cls, n_requests: int, max_tokens: int, device) -> "BatchPlan":
+        return cls(*(torch.zeros(n, dtype=torch.int32, device=device)
+                     for n in (max_tokens, max_tokens, max_tokens, n_requests + 1, n_requests, n_requests, 1)))
+
+
+def plan_batch(cached: torch.Tensor, new: torch.Tensor, block_table: torch.Tensor, free_pages: torch.Tensor,
+               free_head: torch.Tensor, max_tokens: int, plan: BatchPlan | None = None) -> BatchPlan:
+    """Block-table entries, slots, positions and offsets of a batch, from lengths on the device, in one
+    launch and without a host synchronisation.
+
+    cached, new [B] int32: tokens each request has in the cache and brings now.  block_table [B, W] int32
+    holds the pages of the cached tokens; the entries of the pages that new tokens open are written from
+    free_pages (int32), consumed in request order from index free_head[0] on.  max_tokens bounds the sum
+    of ``new``.  ``plan``: tensors to fill (BatchPlan.allocate; CUDA graphs), else new ones.  When the
+    table is too narrow, the free pages run out, tokens pass max_tokens or a length is negative, the
+    tokens concerned get slot -1 and code 2 goes to the device's error word."""
+    p = BatchPlan(*ext().plan_batch(cached, new, block_table, free_pages, free_head, max_tokens, plan,
+                                    _err_word.get(cached.device)))
+    count()
+    return p
+
+
+class TokenLogprobs(NamedTuple):
+    logprob: torch.Tensor        # [T] f32 log probability of each row's target (0 without one)
+    entropy: torch.Tensor        # [T] f32 entropy of the row's distribution, nats
+    rank: torch.Tensor           # [T] int32: 1 for the most likely token (0 without a target)
+    top_ids: torch.Tensor        # [T, k] int32, most likely first, ties by the lowest id
+    top_logprobs: torch.Tensor   # [T, k] f32
+
+
+_lp_tickets: dict = {}
+
+
+def _logprob_tickets(device, rows: int) -> torch.Tensor:
+    """Zeroed row counters, left at zero by every launch; one set per stream, so that calls on different
+    streams cannot meet in them.  Inside a graph capture each call gets its own (zeroed by the graph)."""
+    if torch.cuda.is_current_stream_capturing():
+        return torch.zeros(rows, dtype=torch.int32, device=device)
+    key = (device, torch.cuda.current_stream(device).cuda_stream)
+    t = _lp_tickets.get(key)
+    if t is None or t.numel() < rows:
+        t = _lp_tickets[key] = torch.zeros(max(rows, 4096), dtype=torch.int32, device=device)
+    return t
+
+
+def token_logprobs(logits: torch.Tensor, V: int, targets: torch.Tensor, top_k: int = 0, softcap: float = 0.0
+                   ) -> TokenLogprobs:
+    """Log probability, entropy and rank of one given token per row, and the row's ``top_k`` (at most 32)
+    alternatives, over the first V columns of logits [T, >= V] (float32, float16 or bfloat16), each logit
+    read once.  targets [T] int32; a target outside [0, V) means none.  softcap > 0: the logits are
+    cap * tanh(logit / cap).  Masked logits (-inf) have probability 0; rows with a NaN or +inf are NaN."""
+    r = TokenLogprobs(*ext().token_logprobs(logits, V, targets, top_k, softcap,
+                                            _logprob_tickets(logits.device, logits.shape[0]) if logits.is_cuda else None))
+    count()
+    return r

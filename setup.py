@@ -23,7 +23,7 @@ NVCC_FLAGS = [
 ]
 CXX_FLAGS = ["-O3", "-std=c++17"]
 
-cuda_sources = sorted(glob.glob(os.path.join(CSRC, "kernels", "*.cu"))) + [os.path.join(CSRC, "bindings.cpp")]
+cuda_sources = sorted(glob.glob(os.path.join(CSRC, "kernels", "*.cu")) + glob.glob(os.path.join(CSRC, "*.cpp")))
 cpu_sources = sorted(glob.glob(os.path.join(CSRC, "cpu", "*.cpp")))
 
 ext_modules = [
