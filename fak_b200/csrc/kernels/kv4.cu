@@ -5,8 +5,11 @@
 // minimum to 11 bits, more than the bf16 values that come in; the subtraction and the division are done
 // in f32.  A group that holds a not-a-number stores m = NaN and reads back as NaN.
 //
-// Eight lanes hold one group, four consecutive dims each: a warp takes one row at head dim 128, two at
-// 64.  Bound by the bytes read (2 D each of K and V per row against 20 D / 16 written).
+// Four lanes hold one group, eight consecutive dims each: two rows a warp at head dim 128, four at 64, K
+// and V of a row in the same lanes.  The bytes (2 D each of K and V per row in, 20 D / 16 out) are few, so
+// instructions decide: the per-element divide is q = d r corrected by one remainder step with r = 1 / s
+// correctly rounded (Markstein 1990: the result is the correctly rounded quotient), the four codes of a
+// half word are summed as floats (c0 + 16 c1 + 256 c2 + 4096 c3 is exact), and heads are a grid dimension.
 #include "kv4.cuh"
 
 #include <cuda_fp16.h>
@@ -18,163 +21,182 @@
 namespace fak {
 namespace {
 
+constexpr int THREADS = 256;
+
 template <typename T>
-FAK_DEV void load4(const T* p, bool vec, float (&x)[4]) {
-  if constexpr (sizeof(T) == 4) {
-    if (vec) {
-      const float4 f = *reinterpret_cast<const float4*>(p);
+FAK_DEV void load8(const T* p, bool vec, float (&x)[8]) {
+  if (vec) {
+    if constexpr (sizeof(T) == 4) {
+      const float4 f = *reinterpret_cast<const float4*>(p), h = *reinterpret_cast<const float4*>(p + 4);
       x[0] = f.x; x[1] = f.y; x[2] = f.z; x[3] = f.w;
-      return;
+      x[4] = h.x; x[5] = h.y; x[6] = h.z; x[7] = h.w;
+    } else {
+      const uint4 u = *reinterpret_cast<const uint4*>(p);
+      T h[8];
+      memcpy(h, &u, 16);
+#pragma unroll
+      for (int i = 0; i < 8; i++) x[i] = (float)h[i];
     }
   } else {
-    if (vec) {
-      const uint2 u = *reinterpret_cast<const uint2*>(p);
-      T h[4];
-      memcpy(h, &u, 8);
 #pragma unroll
-      for (int i = 0; i < 4; i++) x[i] = (float)h[i];
-      return;
-    }
+    for (int i = 0; i < 8; i++) x[i] = (float)p[i];
   }
-#pragma unroll
-  for (int i = 0; i < 4; i++) x[i] = (float)p[i];
 }
 
-// Four values of a group held by 8 lanes -> their codes (one u16), the group's scale and minimum.
-FAK_DEV uint32_t quant4(float (&x)[4], __half& s16, __half& m16) {
-  constexpr float LIM = 65504.f;
+struct Group {
+  uint32_t lo, hi;   // codes of the lane's dims 0-3 and 4-7, 16 bits each
+  __half s, m;
+};
+
+// Eight values of a group held by 4 lanes.
+FAK_DEV Group quant8(float (&x)[8]) {
+  constexpr float LIM = 65504.f, MAGIC = 12582912.f;   // adding 1.5 * 2^23 rounds to whole numbers, ties to even
   bool nan = false;
+  float lo = INFINITY, hi = -INFINITY;
 #pragma unroll
-  for (int i = 0; i < 4; i++) {
+  for (int i = 0; i < 8; i++) {
     nan |= x[i] != x[i];
     x[i] = fminf(fmaxf(x[i], -LIM), LIM);
+    lo = fminf(lo, x[i]);
+    hi = fmaxf(hi, x[i]);
   }
-  float lo = fminf(fminf(x[0], x[1]), fminf(x[2], x[3]));
-  float hi = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
 #pragma unroll
-  for (int o = 4; o > 0; o >>= 1) {
+  for (int o = 2; o > 0; o >>= 1) {
     lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
     hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
   }
-  const uint32_t votes = __ballot_sync(0xffffffffu, nan) >> (threadIdx.x & 24);
-  m16 = __float2half_rn(lo);
-  const float m = __half2float(m16);
-  s16 = __float2half_rn(__fdiv_rn(hi - m, 15.f));
-  const float s = __half2float(s16);
-  uint32_t c = 0;
-  if (s > 0.f) {
+  Group g;
+  g.m = __float2half_rn(lo);
+  const float m = __half2float(g.m);
+  g.s = __float2half_rn(__fdiv_rn(hi - m, 15.f));
+  const float s = __half2float(g.s);
+  const float r = s > 0.f ? __frcp_rn(s) : 0.f;   // a constant group: all codes 0
+  float c[2] = {0.f, 0.f};
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-      const float q = rintf(__fdiv_rn(x[i] - m, s));
-      c |= (uint32_t)(int)fminf(fmaxf(q, 0.f), 15.f) << (4 * i);
+  for (int i = 7; i >= 0; i--) {
+    const float d = x[i] - m;
+    float q = d * r;
+    q = fmaf(fmaf(-q, s, d), r, q);
+    q = fminf(fmaxf(q, 0.f), 15.f);
+    q = (q + MAGIC) - MAGIC;
+    c[i >> 2] = fmaf(c[i >> 2], 16.f, q);
+  }
+  g.lo = (uint32_t)__float_as_int(c[0] + 8388608.f) & 0xffffu;
+  g.hi = (uint32_t)__float_as_int(c[1] + 8388608.f) & 0xffffu;
+  if (__any_sync(0xffffffffu, nan)) {
+    const uint32_t votes = __ballot_sync(0xffffffffu, nan) >> (threadIdx.x & 28);
+    if (votes & 0xfu) {
+      g.m = __ushort_as_half(0x7fff);
+      g.s = __ushort_as_half(0);
+      g.lo = g.hi = 0;
     }
   }
-  if (votes & 0xffu) {   // a NaN in the group
-    m16 = __ushort_as_half(0x7fff);
-    s16 = __ushort_as_half(0);
-    c = 0;
-  }
-  return c;
+  return g;
 }
 
+// The row (token, head) of a lane: heads along the grid's x, tokens along its y.
+template <int D>
+struct RowOf {
+  static constexpr int LANES = D / 8, PER_CTA = THREADS / LANES;
+  int64_t tok;
+  int h, grp, j;   // head, group, the lane's eighth dims 8 j of the group
+  FAK_DEV RowOf() {
+    const int l = threadIdx.x % LANES;
+    grp = l >> 2;
+    j = l & 3;
+    tok = ((int64_t)blockIdx.z * gridDim.y + blockIdx.y) * PER_CTA + threadIdx.x / LANES;
+    h = blockIdx.x;
+  }
+};
+
 template <typename T, int D>
-__global__ void __launch_bounds__(256)
-k_kv4_append(Kv4Rows r, const int* __restrict__ slot, int64_t n_rows, int Hkv, uint8_t* __restrict__ pages,
+__global__ void __launch_bounds__(THREADS)
+k_kv4_append(const __grid_constant__ Kv4Rows r, const int* __restrict__ slot, int n_tok, int Hkv, uint8_t* __restrict__ pages,
              int64_t n_pages, int* __restrict__ err) {
   using L = kv4::Lay<D>;
-  constexpr int RPW = 4 / L::NG;   // rows per warp
   pdl_wait();
-  const int lane = threadIdx.x & 31, u = lane >> 3, j = lane & 7;
-  const int grp = u % L::NG;
-  const int64_t warp = (int64_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
-  const int64_t row = warp * RPW + u / L::NG;
-  const bool live = row < n_rows;
-  const int64_t tok = live ? row / Hkv : 0;
-  const int h = live ? (int)(row % Hkv) : 0;
-  const int sl = live ? slot[tok] : -1;
-  const bool in = sl >= 0 && sl / kv4::PAGE < n_pages;
+  const RowOf<D> w;
+  const int sl = w.tok < n_tok ? slot[w.tok] : -1;
+  const bool in = sl >= 0 && (sl >> 4) < n_pages;
   if (sl >= 0 && !in) report_error(err, 2);
-  float k[4] = {0.f, 0.f, 0.f, 0.f}, v[4] = {0.f, 0.f, 0.f, 0.f};
+  float k[8] = {}, v[8] = {};
   if (in) {
-    const int d = grp * 32 + 4 * j;
-    load4((const T*)r.k + (tok >> 4) * r.ks_page + (tok & 15) * r.ks_row + h * r.ks_head + d, r.vec, k);
-    load4((const T*)r.v + (tok >> 4) * r.vs_page + (tok & 15) * r.vs_row + h * r.vs_head + d, r.vec, v);
+    const int d = w.grp * 32 + 8 * w.j;
+    const int64_t pg = w.tok >> 4, row = w.tok & 15;
+    load8((const T*)r.k + pg * r.ks_page + row * r.ks_row + w.h * r.ks_head + d, r.vec, k);
+    load8((const T*)r.v + pg * r.vs_page + row * r.vs_row + w.h * r.vs_head + d, r.vec, v);
   }
-  __half ks, km, vs, vm;
-  const uint32_t kc = quant4(k, ks, km), vc = quant4(v, vs, vm);
+  const Group gk = quant8(k), gv = quant8(v);
   if (in) {
-    uint8_t* pg = pages + ((int64_t)(sl >> 4) * Hkv + h) * L::BYTES;
+    uint8_t* pg = pages + ((int64_t)(sl >> 4) * Hkv + w.h) * L::BYTES;
     const int t = sl & 15;
-    *reinterpret_cast<uint16_t*>(pg + L::k_u16(t, grp, j)) = (uint16_t)kc;
-    *reinterpret_cast<uint16_t*>(pg + L::v_u16(t, grp, j)) = (uint16_t)vc;
-    if (j == 0) *reinterpret_cast<__half*>(pg + L::KS + L::k_meta(t, grp)) = ks;
-    if (j == 1) *reinterpret_cast<__half*>(pg + L::KM + L::k_meta(t, grp)) = km;
-    if (j == 2) *reinterpret_cast<__half*>(pg + L::VS + L::v_meta(t, grp)) = vs;
-    if (j == 3) *reinterpret_cast<__half*>(pg + L::VM + L::v_meta(t, grp)) = vm;
+    *reinterpret_cast<uint32_t*>(pg + L::k_u16(t, w.grp, 2 * w.j)) = gk.lo | gk.hi << 16;
+    *reinterpret_cast<uint16_t*>(pg + L::v_u16(t, w.grp, 2 * w.j)) = (uint16_t)gv.lo;
+    *reinterpret_cast<uint16_t*>(pg + L::v_u16(t, w.grp, 2 * w.j + 1)) = (uint16_t)gv.hi;
+    // lane j of the group stores one of its four halves
+    const __half x = w.j == 0 ? gk.s : w.j == 1 ? gk.m : w.j == 2 ? gv.s : gv.m;
+    const int at = w.j < 2 ? L::KS + 32 * L::NG * w.j + L::k_meta(t, w.grp) : L::VS + 32 * L::NG * (w.j - 2) + L::v_meta(t, w.grp);
+    *reinterpret_cast<__half*>(pg + at) = x;
   }
   pdl_launch_dependents();
 }
 
 template <typename T>
-FAK_DEV void store4(T* p, const float (&x)[4]) {
+FAK_DEV void store8(T* p, const float (&x)[8]) {
   if constexpr (sizeof(T) == 4) {
     *reinterpret_cast<float4*>(p) = make_float4(x[0], x[1], x[2], x[3]);
+    *reinterpret_cast<float4*>(p + 4) = make_float4(x[4], x[5], x[6], x[7]);
   } else {
-    T h[4];
+    T h[8];
 #pragma unroll
-    for (int i = 0; i < 4; i++) h[i] = (T)x[i];
-    uint2 u;
-    memcpy(&u, h, 8);
-    *reinterpret_cast<uint2*>(p) = u;
+    for (int i = 0; i < 8; i++) h[i] = (T)x[i];
+    uint4 u;
+    memcpy(&u, h, 16);
+    *reinterpret_cast<uint4*>(p) = u;
   }
 }
 
 template <typename T, int D>
-__global__ void __launch_bounds__(256)
-k_kv4_read(const uint8_t* __restrict__ pages, int64_t n_pages, const int* __restrict__ slot, int64_t n_rows, int Hkv,
+__global__ void __launch_bounds__(THREADS)
+k_kv4_read(const uint8_t* __restrict__ pages, int64_t n_pages, const int* __restrict__ slot, int n_tok, int Hkv,
            T* __restrict__ ko, T* __restrict__ vo, int* __restrict__ err) {
   using L = kv4::Lay<D>;
-  constexpr int RPW = 4 / L::NG;
   pdl_wait();
-  const int lane = threadIdx.x & 31, u = lane >> 3, j = lane & 7;
-  const int grp = u % L::NG;
-  const int64_t warp = (int64_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
-  const int64_t row = warp * RPW + u / L::NG;
-  if (row < n_rows) {
-    const int64_t tok = row / Hkv;
-    const int h = (int)(row % Hkv);
-    const int sl = slot[tok];
-    const bool in = sl >= 0 && sl / kv4::PAGE < n_pages;
+  const RowOf<D> w;
+  if (w.tok < n_tok) {
+    const int sl = slot[w.tok];
+    const bool in = sl >= 0 && (sl >> 4) < n_pages;
     if (sl >= 0 && !in) report_error(err, 2);
-    float k[4] = {0.f, 0.f, 0.f, 0.f}, v[4] = {0.f, 0.f, 0.f, 0.f};
+    float k[8] = {}, v[8] = {};
     if (in) {
-      const uint8_t* pg = pages + ((int64_t)(sl >> 4) * Hkv + h) * L::BYTES;
+      const uint8_t* pg = pages + ((int64_t)(sl >> 4) * Hkv + w.h) * L::BYTES;
       const int t = sl & 15;
-      const uint32_t kc = *reinterpret_cast<const uint16_t*>(pg + L::k_u16(t, grp, j));
-      const uint32_t vc = *reinterpret_cast<const uint16_t*>(pg + L::v_u16(t, grp, j));
+      const uint32_t kc = *reinterpret_cast<const uint32_t*>(pg + L::k_u16(t, w.grp, 2 * w.j));
+      const uint32_t vc = *reinterpret_cast<const uint16_t*>(pg + L::v_u16(t, w.grp, 2 * w.j)) |
+                          (uint32_t)*reinterpret_cast<const uint16_t*>(pg + L::v_u16(t, w.grp, 2 * w.j + 1)) << 16;
       auto h16 = [&](int at) { return __half2float(*reinterpret_cast<const __half*>(pg + at)); };
-      const float ks = h16(L::KS + L::k_meta(t, grp)), km = h16(L::KM + L::k_meta(t, grp));
-      const float vs = h16(L::VS + L::v_meta(t, grp)), vm = h16(L::VM + L::v_meta(t, grp));
+      const float ks = h16(L::KS + L::k_meta(t, w.grp)), km = h16(L::KM + L::k_meta(t, w.grp));
+      const float vs = h16(L::VS + L::v_meta(t, w.grp)), vm = h16(L::VM + L::v_meta(t, w.grp));
 #pragma unroll
-      for (int i = 0; i < 4; i++) {
-        // separate roundings of the product (exact: 4 x 11 bits) and the sum
-        k[i] = __fadd_rn(__fmul_rn((float)((kc >> (4 * i)) & 15u), ks), km);
-        v[i] = __fadd_rn(__fmul_rn((float)((vc >> (4 * i)) & 15u), vs), vm);
+      for (int i = 0; i < 8; i++) {   // the code as a float from its bits; the product (15 bits) is exact in the fma
+        k[i] = fmaf(__int_as_float(0x4b000000 | (kc >> (4 * i) & 15u)) - 8388608.f, ks, km);
+        v[i] = fmaf(__int_as_float(0x4b000000 | (vc >> (4 * i) & 15u)) - 8388608.f, vs, vm);
       }
     }
-    const int64_t at = row * D + grp * 32 + 4 * j;
-    store4(ko + at, k);
-    store4(vo + at, v);
+    const int64_t at = (w.tok * Hkv + w.h) * D + w.grp * 32 + 8 * w.j;
+    store8(ko + at, k);
+    store8(vo + at, v);
   }
   pdl_launch_dependents();
 }
 
 template <typename... P, typename... A>
-void launch_rows(void (*kern)(P...), int64_t n_rows, int D, cudaStream_t stream, A... args) {
-  const int64_t per_block = 8 * (D == 64 ? 2 : 1);
+void launch_rows(void (*kern)(P...), int T, int Hkv, int D, cudaStream_t stream, A... args) {
+  const int per_cta = THREADS / (D / 8);
+  const int n = (T + per_cta - 1) / per_cta, y = n < 32768 ? n : 32768;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)((n_rows + per_block - 1) / per_block));
-  cfg.blockDim = dim3(256);
+  cfg.gridDim = dim3((unsigned)Hkv, (unsigned)y, (unsigned)((n + y - 1) / y));
+  cfg.blockDim = dim3(THREADS);
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -188,12 +210,11 @@ void launch_rows(void (*kern)(P...), int64_t n_rows, int D, cudaStream_t stream,
 
 void kv4_append_launch(const Kv4Rows& r, const int* slot, int T, int Hkv, int D, uint8_t* pages, int64_t n_pages,
                        int* err, cudaStream_t stream) {
-  const int64_t n = (int64_t)T * Hkv;
-  if (n == 0) return;
+  if (T == 0) return;
   auto go = [&](auto tag) {
     using E = decltype(tag);
-    if (D == 128) launch_rows(k_kv4_append<E, 128>, n, D, stream, r, slot, n, Hkv, pages, n_pages, err);
-    else launch_rows(k_kv4_append<E, 64>, n, D, stream, r, slot, n, Hkv, pages, n_pages, err);
+    if (D == 128) launch_rows(k_kv4_append<E, 128>, T, Hkv, D, stream, r, slot, T, Hkv, pages, n_pages, err);
+    else launch_rows(k_kv4_append<E, 64>, T, Hkv, D, stream, r, slot, T, Hkv, pages, n_pages, err);
   };
   if (r.type == Elt::F32) go(float());
   else if (r.type == Elt::F16) go(__half());
@@ -202,12 +223,11 @@ void kv4_append_launch(const Kv4Rows& r, const int* slot, int T, int Hkv, int D,
 
 void kv4_read_launch(const uint8_t* pages, int64_t n_pages, const int* slot, int T, int Hkv, int D, void* k, void* v,
                      Elt type, int* err, cudaStream_t stream) {
-  const int64_t n = (int64_t)T * Hkv;
-  if (n == 0) return;
+  if (T == 0) return;
   auto go = [&](auto tag) {
     using E = decltype(tag);
-    if (D == 128) launch_rows(k_kv4_read<E, 128>, n, D, stream, pages, n_pages, slot, n, Hkv, (E*)k, (E*)v, err);
-    else launch_rows(k_kv4_read<E, 64>, n, D, stream, pages, n_pages, slot, n, Hkv, (E*)k, (E*)v, err);
+    if (D == 128) launch_rows(k_kv4_read<E, 128>, T, Hkv, D, stream, pages, n_pages, slot, T, Hkv, (E*)k, (E*)v, err);
+    else launch_rows(k_kv4_read<E, 64>, T, Hkv, D, stream, pages, n_pages, slot, T, Hkv, (E*)k, (E*)v, err);
   };
   if (type == Elt::F32) go(float());
   else if (type == Elt::F16) go(__half());

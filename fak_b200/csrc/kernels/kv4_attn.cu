@@ -49,10 +49,17 @@ FAK_DEV void mma_f16_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2,
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-FAK_DEV void mma_f16_1688(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t b0) {
-  asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5}, {%6}, {%0,%1,%2,%3};"
-               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-               : "r"(a0), "r"(a1), "r"(b0));
+// the same with a zero accumulator
+FAK_DEV void mma_f16_16816_z(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+}
+FAK_DEV void mma_f16_1688_z(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t b0) {
+  asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5}, {%6}, {%7,%7,%7,%7};"
+               : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+               : "r"(a0), "r"(a1), "r"(b0), "f"(0.f));
 }
 FAK_DEV uint32_t movmatrix(uint32_t a) {
   uint32_t r;
@@ -96,23 +103,19 @@ FAK_DEV void lds(const uint8_t* p, uint32_t (&r)[N]) {
 // The pages one CTA column block needs, and how the splits share them: the same arithmetic in the
 // attention kernel and in the combine.
 struct Span {
-  int p0, p1, pps, live;   // pages [p0, p1), pages per split, splits that hold any
+  int p0, p1, live;   // pages [p0, p1), splits of pps pages that hold any
 };
-FAK_DEV Span span_of(int ctx, int n, int i_lo, int i_hi, int window, int n_split, int width) {
+FAK_DEV Span span_of(int ctx, int n, int i_lo, int i_hi, int window, int pps, int width) {
   Span s;
   const int last = min(ctx - n + i_hi, ctx - 1);               // the last key any row of the block sees
   const int first = window > 0 ? max(0, ctx - n + i_lo + 1 - window) : 0;
   s.p0 = first / PAGE;
   s.p1 = min(width, last / PAGE + 1);
   if (last < 0) s.p1 = s.p0;
-  const int pages = max(0, s.p1 - s.p0);
-  s.pps = max(W, (pages + n_split - 1) / n_split);
-  s.live = (pages + s.pps - 1) / s.pps;
+  s.live = (max(0, s.p1 - s.p0) + pps - 1) / pps;
   return s;
 }
 
-template <typename T>
-FAK_DEV float to_f32(const T* p, int64_t i) { return (float)p[i]; }
 FAK_DEV float load_elt(const void* p, Elt t, int64_t i) {
   if (t == Elt::F32) return ((const float*)p)[i];
   if (t == Elt::F16) return __half2float(((const __half*)p)[i]);
@@ -138,7 +141,7 @@ struct Smem {
 
 template <int D, int NT, bool CAP>
 __global__ void __launch_bounds__(W * 32)
-k_kv4_attn(Kv4Attn a, int n_split) {
+k_kv4_attn(const __grid_constant__ Kv4Attn a, int n_split, int pps) {
   using L = Lay<D>;
   constexpr int NG = L::NG;
   constexpr int COLS = 8 * NT;
@@ -165,28 +168,27 @@ k_kv4_attn(Kv4Attn a, int n_split) {
   }
   const int R = n * G, r0 = rc * COLS;
   if (R <= r0) return;
-  const Span sp = span_of(ctx, n, r0 / G, min(R - 1, r0 + COLS - 1) / G, a.window, n_split, a.width);
-  const int p_begin = sp.p0 + split * sp.pps, p_end = min(sp.p1, p_begin + sp.pps);
+  const Span sp = span_of(ctx, n, r0 / G, min(R - 1, r0 + COLS - 1) / G, a.window, pps, a.width);
+  const int p_begin = sp.p0 + split * pps, p_end = min(sp.p1, p_begin + pps);
   if (p_begin >= p_end && !(split == 0 && sp.live == 0)) return;
 
   // pages of this warp: p_begin + warp, + W, ..; 32 table entries at a time, one a lane
   const int np = max(0, (p_end - p_begin - warp + W - 1) / W);
   const int* table = a.table + (int64_t)b * a.table_stride + p_begin + warp;
-  int entry = 0;
-  auto fetch_entries = [&](int i) {   // entries of pages i .. i + 31 of this warp
-    entry = i + lane < np ? table[(int64_t)W * (i + lane)] : 0;
-    if ((unsigned)entry >= (uint64_t)a.n_pages) {
-      report_error(a.err, 2);
-      entry = 0;
-    }
-  };
+  const uint8_t* page = nullptr;   // lane l: address of page 32 j + l, refreshed every 32 pages
   auto issue = [&](int i) {
-    if ((i & 31) == 0) fetch_entries(i);
-    const int pid = __shfl_sync(0xffffffffu, entry, i & 31);
-    if (lane == 0) {
+    if ((i & 31) == 0 && i + lane < np) {
+      int pid = table[(int64_t)W * (i + lane)];
+      if ((unsigned)pid >= (uint64_t)a.n_pages) {
+        report_error(a.err, 2);
+        pid = 0;
+      }
+      page = a.pages + ((int64_t)pid * a.Hkv + kvh) * L::BYTES;
+    }
+    if (lane == (i & 31)) {
       uint64_t* bar = &sm.full[warp][i % STAGES];
       tc::mbar_arrive_expect_tx(bar, L::BYTES);
-      bulk_load(sm.ring[warp][i % STAGES], a.pages + ((int64_t)pid * a.Hkv + kvh) * L::BYTES, L::BYTES, bar);
+      bulk_load(sm.ring[warp][i % STAGES], page, L::BYTES, bar);
     }
   };
 #pragma unroll
@@ -205,13 +207,35 @@ k_kv4_attn(Kv4Attn a, int n_split) {
     const int i = live ? r / G : 0, h = kvh * G + (live ? r % G : 0);
     float x[NG][8], amax = 0.f;
     const int64_t at = (int64_t)(tok0 + i) * a.q_tok + (int64_t)h * a.q_head + 8 * t;
+    if (!live) {
+#pragma unroll
+      for (int gr = 0; gr < NG; gr++)
+#pragma unroll
+        for (int e = 0; e < 8; e++) x[gr][e] = 0.f;
+    } else if (a.q_vec && a.q_type != Elt::F32) {
+      uint4 u[NG];
+#pragma unroll
+      for (int gr = 0; gr < NG; gr++) u[gr] = *reinterpret_cast<const uint4*>((const uint16_t*)a.q + at + gr * 32);
+#pragma unroll
+      for (int gr = 0; gr < NG; gr++) {
+        const uint32_t w[4] = {u[gr].x, u[gr].y, u[gr].z, u[gr].w};
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          const float2 f = unpack_h2(w[e]);
+          x[gr][2 * e] = a.q_type == Elt::F16 ? f.x : bf16_bits_lo(w[e]);
+          x[gr][2 * e + 1] = a.q_type == Elt::F16 ? f.y : bf16_bits_hi(w[e]);
+        }
+      }
+    } else {
+#pragma unroll
+      for (int gr = 0; gr < NG; gr++)
+#pragma unroll
+        for (int e = 0; e < 8; e++) x[gr][e] = load_elt(a.q, a.q_type, at + gr * 32 + e);
+    }
 #pragma unroll
     for (int gr = 0; gr < NG; gr++)
 #pragma unroll
-      for (int e = 0; e < 8; e++) {
-        x[gr][e] = live ? load_elt(a.q, a.q_type, at + gr * 32 + e) : 0.f;
-        amax = fmaxf(amax, fabsf(x[gr][e]));
-      }
+      for (int e = 0; e < 8; e++) amax = fmaxf(amax, fabsf(x[gr][e]));
     amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
     amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
     // power of two that brings the row's largest into [2^13, 2^14)
@@ -278,9 +302,11 @@ k_kv4_attn(Kv4Attn a, int n_split) {
   const int low_any = a.window > 0 ? max(0, ctx - n + i_first + 1 - a.window) : 0;
 
   float o[NT][NG][2][4], mt[NT][4], base[NT][2];
+  float lift[NT][2];   // LIFT - base (0 while the base is -inf: then every z is -inf too)
 #pragma unroll
   for (int nt = 0; nt < NT; nt++) {
     base[nt][0] = base[nt][1] = -INFINITY;
+    lift[nt][0] = lift[nt][1] = 0.f;
 #pragma unroll
     for (int e = 0; e < 4; e++) {
       mt[nt][e] = 0.f;
@@ -290,15 +316,11 @@ k_kv4_attn(Kv4Attn a, int n_split) {
   }
   constexpr uint32_t M0 = 0x000f000fu, M4 = 0x00f000f0u;
   const float cap_in = CAP ? 1.f / a.softcap : 0.f, cap_out = CAP ? a.softcap * LOG2E : 0.f;
-  bool ok = true;
-  int done = 0;   // pages waited for
-
 #pragma unroll 1
   for (int i = 0; i < np; i++) {
     if (i + STAGES - 1 < np) issue(i + STAGES - 1);
-    ok = ok && tc::mbar_wait(&sm.full[warp][i % STAGES], (uint32_t)((i / STAGES) & 1), a.err);
-    done = i + 1;
-    if (!__all_sync(0xffffffffu, ok)) break;
+    // (a wait that gives up has set the error word; the loop goes on, so that every copy is waited for)
+    tc::mbar_wait(&sm.full[warp][i % STAGES], (uint32_t)((i / STAGES) & 1), a.err);
     const uint8_t* pg = sm.ring[warp][i % STAGES];
     const int key0 = (p_begin + warp + W * i) * PAGE;
     const bool whole = key0 >= low_max && key0 + PAGE <= lim_min;   // warp-uniform
@@ -316,9 +338,7 @@ k_kv4_attn(Kv4Attn a, int n_split) {
       float acc[NT][4];
 #pragma unroll
       for (int nt = 0; nt < NT; nt++) {
-        acc[nt][0] = acc[nt][1] = acc[nt][2] = acc[nt][3] = 0.f;
-        z[nt][0] = z[nt][1] = z[nt][2] = z[nt][3] = 0.f;
-        mma_f16_1688(z[nt], m0[0], m1[0], qs[nt]);
+        mma_f16_1688_z(z[nt], m0[0], m1[0], qs[nt]);
       }
 #pragma unroll
       for (int gr = 0; gr < NG; gr++) {
@@ -327,13 +347,11 @@ k_kv4_attn(Kv4Attn a, int n_split) {
         const float sa = gr & 1 ? f0.y : f0.x, sb = gr & 1 ? f1.y : f1.x;
 #pragma unroll
         for (int nt = 0; nt < NT; nt++) {
-          float d[4] = {0.f, 0.f, 0.f, 0.f};
-          mma_f16_16816(d, w0 & M0, w1 & M0, w0 & M4, w1 & M4, qf[nt][gr][0], qf[nt][gr][1]);
+          float d[4];
+          mma_f16_16816_z(d, w0 & M0, w1 & M0, w0 & M4, w1 & M4, qf[nt][gr][0], qf[nt][gr][1]);
           mma_f16_16816(d, u0 & M0, u1 & M0, u0 & M4, u1 & M4, qf[nt][gr][2], qf[nt][gr][3]);
-          acc[nt][0] = fmaf(sa, d[0], acc[nt][0]);
-          acc[nt][1] = fmaf(sa, d[1], acc[nt][1]);
-          acc[nt][2] = fmaf(sb, d[2], acc[nt][2]);
-          acc[nt][3] = fmaf(sb, d[3], acc[nt][3]);
+#pragma unroll
+          for (int e = 0; e < 4; e++) acc[nt][e] = gr == 0 ? (e < 2 ? sa : sb) * d[e] : fmaf(e < 2 ? sa : sb, d[e], acc[nt][e]);
         }
       }
       // codes carry 2^-24, the sums 2^-6
@@ -371,6 +389,7 @@ k_kv4_attn(Kv4Attn a, int n_split) {
           m = fmaxf(m, base[nt][e]);
           const float f = m == -INFINITY ? 1.f : ex2(base[nt][e] - m);
           base[nt][e] = m;
+          lift[nt][e] = m == -INFINITY ? 0.f : LIFT - m;
           mt[nt][e] *= f;
 #pragma unroll
           for (int gr = 0; gr < NG; gr++)
@@ -386,10 +405,7 @@ k_kv4_attn(Kv4Attn a, int n_split) {
     for (int nt = 0; nt < NT; nt++) {
       float p[4];
 #pragma unroll
-      for (int e = 0; e < 4; e++) {
-        const float bs = base[nt][e & 1] == -INFINITY ? 0.f : base[nt][e & 1];
-        p[e] = ex2(z[nt][e] - bs + LIFT);
-      }
+      for (int e = 0; e < 4; e++) p[e] = ex2(z[nt][e] + lift[nt][e & 1]);
       p0[nt] = movmatrix(pack_f16(p[0], p[1]));   // tokens 2 t, 2 t + 1 of column g
       p1[nt] = movmatrix(pack_f16(p[2], p[3]));   // tokens 2 t + 8, 2 t + 9
     }
@@ -407,7 +423,7 @@ k_kv4_attn(Kv4Attn a, int n_split) {
       } else if (g == 4) {
         m0 = m1 = 0x3c003c00u;
       }
-      if (key0 < low_any || key0 + PAGE > lim_any) {
+      if (!whole) {
         // tokens no row sees: whatever their bytes hold (memory nobody wrote) must not reach the sums
         auto keep = [&](int tok) {
           const bool lo_ok = key0 + tok >= low_any && key0 + tok < lim_any;
@@ -439,9 +455,6 @@ k_kv4_attn(Kv4Attn a, int n_split) {
     __syncwarp();   // every lane is done with the stage before it is refilled
   }
 
-  // a wait gave up (the error word says so): the copies still in flight are waited for, again with a limit
-  for (int i = done; i < min(np, done + STAGES - 1); i++)
-    tc::mbar_wait(&sm.full[warp][i % STAGES], (uint32_t)((i / STAGES) & 1), a.err);
   // merge the CTA's warps; the ring is free once every warp has drained its copies
   __syncthreads();
 #pragma unroll
@@ -514,9 +527,9 @@ k_kv4_attn(Kv4Attn a, int n_split) {
   }
 }
 
-// One warp merges the live splits of one query row: D / 32 dims a lane.
+// One warp merges the live splits of one query row: D / 32 dims a lane, up to 16 splits' loads in flight.
 template <int D>
-__global__ void __launch_bounds__(128) k_kv4_combine(Kv4Attn a, int n_split, int cols, int row_chunks) {
+__global__ void __launch_bounds__(256) k_kv4_combine(const __grid_constant__ Kv4Attn a, int n_split, int pps, int cols, int row_chunks) {
   constexpr int V = D / 32;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rc = blockIdx.x, kvh = blockIdx.y, b = blockIdx.z;
@@ -530,11 +543,11 @@ __global__ void __launch_bounds__(128) k_kv4_combine(Kv4Attn a, int n_split, int
   }
   const int R = n * G, r0 = rc * cols;
   if (R <= r0) return;
-  const Span sp = span_of(ctx, n, r0 / G, min(R - 1, r0 + cols - 1) / G, a.window, n_split, a.width);
+  const Span sp = span_of(ctx, n, r0 / G, min(R - 1, r0 + cols - 1) / G, a.window, pps, a.width);
   const int live = max(1, sp.live);   // an empty block's split 0 wrote zeros
   const int64_t part_col = (((int64_t)b * a.Hkv + kvh) * row_chunks + rc) * cols;
   const float* part_ml = a.part + (int64_t)gridDim.z * gridDim.y * row_chunks * cols * n_split * D;
-  for (int c = warp; c < cols && r0 + c < R; c += 4) {
+  for (int c = warp; c < cols && r0 + c < R; c += 8) {
     const int r = r0 + c, h = kvh * G + r % G;
     const float2* ml = reinterpret_cast<const float2*>(part_ml) + (part_col + c) * n_split;
     const float* po = a.part + (part_col + c) * n_split * D + V * lane;
@@ -554,7 +567,7 @@ __global__ void __launch_bounds__(128) k_kv4_combine(Kv4Attn a, int n_split, int
       }
       l += warp_sum(ls);
       const int e = min(32, live - s0);
-#pragma unroll 8
+#pragma unroll 16
       for (int s = 0; s < e; s++) {
         const float fs = __shfl_sync(0xffffffffu, f, s);
         const float* p = po + (int64_t)(s0 + s) * D;
@@ -590,12 +603,14 @@ Kv4AttnPlan kv4_attn_plan(const Kv4Attn& a, int n_sm) {
   const int nt_most = a.D == 64 ? 4 : 2;
   p.nt = rows <= 8 ? 1 : (rows <= 16 || nt_most == 2 ? 2 : 4);
   p.row_chunks = (int)((rows + 8 * p.nt - 1) / (8 * p.nt));
-  // splits: about four CTAs a SM, each warp at least one page
+  // Splits of pps pages each, the same for every sequence, so that CTAs are alike whatever the lengths:
+  // one wave of four CTAs a SM if every sequence filled its table, between W and 128 pages a split.
   const int64_t ctas = (int64_t)a.B * a.Hkv * p.row_chunks;
-  const int most = (a.width + W - 1) / W;
-  int s = a.n_split;
-  if (s <= 0) s = (int)std::min<int64_t>(256, (4 * n_sm + ctas - 1) / std::max<int64_t>(1, ctas));
-  p.n_split = std::max(1, std::min(s, most));
+  int64_t pps = a.n_split > 0 ? (a.width + a.n_split - 1) / a.n_split
+                              : std::min<int64_t>(128, (a.width * ctas + 4 * n_sm - 1) / (4 * n_sm));
+  pps = std::max<int64_t>((pps + W - 1) / W * W, W);
+  p.pps = (int)pps;
+  p.n_split = std::max(1, (int)((a.width + pps - 1) / pps));
   p.part_floats = p.n_split > 1 ? ctas * 8 * p.nt * p.n_split * (a.D + 2) : 0;
   return p;
 }
@@ -609,8 +624,8 @@ void kv4_attn_launch(const Kv4Attn& a, const Kv4AttnPlan& p, cudaStream_t stream
   pdl(cfg, attr);
   auto go = [&](auto kern, size_t smem) {
     cfg.dynamicSmemBytes = smem;
-    if (smem > 48 * 1024) FAK_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-    FAK_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kern, a, p.n_split));
+    FAK_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    FAK_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kern, a, p.n_split, p.pps));
   };
   const bool cap = a.softcap > 0.f;
 #define FAK_KV4(DV, NTV)                                                    \
@@ -630,11 +645,11 @@ void kv4_attn_launch(const Kv4Attn& a, const Kv4AttnPlan& p, cudaStream_t stream
   if (p.n_split > 1) {
     cudaLaunchConfig_t c2 = {};
     c2.gridDim = dim3((unsigned)p.row_chunks, (unsigned)a.Hkv, (unsigned)a.B);
-    c2.blockDim = dim3(128);
+    c2.blockDim = dim3(256);
     c2.stream = stream;
     pdl(c2, attr);
-    if (a.D == 128) FAK_CUDA_CHECK(cudaLaunchKernelEx(&c2, k_kv4_combine<128>, a, p.n_split, 8 * p.nt, p.row_chunks));
-    else FAK_CUDA_CHECK(cudaLaunchKernelEx(&c2, k_kv4_combine<64>, a, p.n_split, 8 * p.nt, p.row_chunks));
+    if (a.D == 128) FAK_CUDA_CHECK(cudaLaunchKernelEx(&c2, k_kv4_combine<128>, a, p.n_split, p.pps, 8 * p.nt, p.row_chunks));
+    else FAK_CUDA_CHECK(cudaLaunchKernelEx(&c2, k_kv4_combine<64>, a, p.n_split, p.pps, 8 * p.nt, p.row_chunks));
   }
 }
 

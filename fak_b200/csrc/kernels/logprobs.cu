@@ -7,12 +7,12 @@
 // A target outside [0, V) has logprob 0 and rank 0.  A row with only -inf has entropy 0, logprobs -inf.
 //
 // A row is cut into n_seg segments (1 when there are enough rows to fill the machine), one CTA of 8
-// warps each; a warp walks its share of the segment in tiles of 32 lanes x 8 logits.  Each lane keeps its
+// warps each; a warp walks its share of the segment in tiles of 32 lanes x 16 logits.  Each lane keeps its
 // own (M, S, sum) and moves M at most once a tile.  The top list is kept per warp, sorted, one 64-bit key
 // (ordered value, complemented index) a lane; a logit joins the warp's candidate buffer only when it
-// reaches the list's k-th value, which a random row does about k ln(n / 256) times a warp, and 32
-// candidates are sorted and merged at a time.  The first bound comes from the 32 lane maxima of the
-// first tile.  Segments meet in a scratch record per segment; the CTA that takes the row's last ticket
+// reaches the bound: the largest k-th value that any warp of the CTA has (32 candidates are sorted and
+// merged at a time; a random row adds about k ln(V / 512) in all).  The first bound comes from the 32
+// lane maxima of the first tile.  Segments meet in a scratch record per segment; the CTA that takes the row's last ticket
 // merges them in segment order, so results do not depend on the order of arrival.
 #include "common.cuh"
 
@@ -26,9 +26,9 @@ namespace {
 
 constexpr int WARPS = 8;
 constexpr int THREADS = WARPS * 32;
-constexpr int PER = 8;                 // logits per lane and tile
+constexpr int PER = 16;                // logits per lane and tile
 constexpr int TILE = 32 * PER;         // per warp
-constexpr int CAND = TILE + 32;        // candidate keys a warp can hold: < 32 waiting + one tile
+constexpr int CAND = 64;               // candidate keys a warp can hold: < 32 waiting + one per lane
 constexpr int MAXK = 32;
 constexpr int REC = 4 + 2 * MAXK;      // words of a segment's record: M, S, T, count, keys
 
@@ -78,38 +78,40 @@ FAK_DEV Stat join(const Stat& a, const Stat& b) {
   return r;
 }
 
+// 16 logits a lane: 16-byte loads, neighbouring lanes side by side.
 template <typename T>
-FAK_DEV void load8(const T* __restrict__ p, int i0, int end, bool vec, float (&x)[PER]) {
-  if constexpr (sizeof(T) == 4) {
-    // two float4 a lane, 128 logits apart
+constexpr int VEC = 16 / sizeof(T);
+template <typename T>
+FAK_DEV void load16(const T* __restrict__ p, int i0, int end, bool vec, float (&x)[PER]) {
+  constexpr int E = VEC<T>;
 #pragma unroll
-    for (int j = 0; j < 2; j++) {
-      const int i = i0 + j * 128;
-      if (vec && i + 4 <= end) {
-        const float4 f = __ldcs(reinterpret_cast<const float4*>(p + i));
-        x[4 * j] = f.x; x[4 * j + 1] = f.y; x[4 * j + 2] = f.z; x[4 * j + 3] = f.w;
-      } else {
-#pragma unroll
-        for (int e = 0; e < 4; e++) x[4 * j + e] = i + e < end ? p[i + e] : -INFINITY;
-      }
-    }
-  } else {
-    if (vec && i0 + 8 <= end) {
-      const uint4 u = __ldcs(reinterpret_cast<const uint4*>(p + i0));
-      T h[8];
+  for (int j = 0; j < PER / E; j++) {
+    const int i = i0 + j * 32 * E;
+    if (vec && i + E <= end) {
+      const uint4 u = __ldcs(reinterpret_cast<const uint4*>(p + i));
+      T h[E];
       memcpy(h, &u, 16);
 #pragma unroll
-      for (int e = 0; e < 8; e++) x[e] = (float)h[e];
+      for (int e = 0; e < E; e++) x[j * E + e] = (float)h[e];
     } else {
 #pragma unroll
-      for (int e = 0; e < 8; e++) x[e] = i0 + e < end ? (float)p[i0 + e] : -INFINITY;
+      for (int e = 0; e < E; e++) x[j * E + e] = i + e < end ? (float)p[i + e] : -INFINITY;
     }
   }
 }
 template <typename T>
-FAK_DEV int lane_first(int lane) { return sizeof(T) == 4 ? 4 * lane : 8 * lane; }
-template <typename T>
-FAK_DEV int elt_at(int e) { return sizeof(T) == 4 ? (e & 3) + (e >> 2) * 128 : e; }
+FAK_DEV int elt_at(int e) { return e % VEC<T> + e / VEC<T> * 32 * VEC<T>; }
+FAK_DEV float ex2(float x) {   // 2^x, results below 2^-126 are zero
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __noinline__ u64 merge_batch(u64 top, u64 cand, int lane) { return merge32(top, sort32(cand, lane), lane); }
+// order-preserving integer form of a float, for an integer maximum in shared memory
+FAK_DEV int ordered(float v) {
+  const int b = __float_as_int(v);
+  return b >= 0 ? b : b ^ 0x7fffffff;
+}
 
 template <typename T, bool TOP, bool CAP>
 __global__ void __launch_bounds__(THREADS) k_logprobs(LogprobArgs a, int seg_len) {
@@ -117,11 +119,14 @@ __global__ void __launch_bounds__(THREADS) k_logprobs(LogprobArgs a, int seg_len
   __shared__ u64 s_list[WARPS][32];
   __shared__ Stat s_stat[WARPS];
   __shared__ int s_cnt[WARPS];
-  __shared__ int s_last;
+  __shared__ int s_last, s_bound;
+  constexpr float LOG2E = 1.4426950408889634f;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int seg = blockIdx.x;
   const int64_t r = blockIdx.y + (int64_t)blockIdx.z * 32768;
   if (r >= a.T) return;
+  if (TOP && tid == 0) s_bound = ordered(-INFINITY);
+  if (TOP) __syncthreads();
   pdl_wait();
   const T* __restrict__ x = (const T*)a.x + r * a.stride;
   auto cap = [&](float v) { return CAP ? a.softcap * tanhf(v / a.softcap) : v; };
@@ -133,15 +138,15 @@ __global__ void __launch_bounds__(THREADS) k_logprobs(LogprobArgs a, int seg_len
   Stat st = {-INFINITY, 0.f, 0.f};
   int above = 0;
   u64 top = 0, kth = 0;          // the warp's list (lane i: i-th largest) and its k-th key
-  float bound = -INFINITY;       // a lower bound of the k-th value over the logits seen so far
+  float bound = -INFINITY;       // a lower bound of the row's k-th value
   int waiting = 0;
   bool first = true;
   const int k = a.k;
 
   for (int base = i_begin + warp * TILE; base < i_end; base += WARPS * TILE) {
     float v[PER];
-    const int i0 = base + lane_first<T>(lane);
-    load8(x, i0, i_end, a.vec, v);
+    const int i0 = base + VEC<T> * lane;
+    load16(x, i0, i_end, a.vec, v);
     float mx = -INFINITY;
 #pragma unroll
     for (int e = 0; e < PER; e++) {
@@ -149,7 +154,7 @@ __global__ void __launch_bounds__(THREADS) k_logprobs(LogprobArgs a, int seg_len
       mx = fmaxf(mx, v[e]);
     }
     if (mx > st.m) {   // move the base of this lane's sums
-      const float d = st.s == 0.f ? 0.f : fmaxf(st.m - mx, -1e30f), f = exp2f(d * 1.4426950408889634f);
+      const float d = st.s == 0.f ? 0.f : fmaxf(st.m - mx, -1e30f), f = ex2(d * LOG2E);
       st.t = f * (st.t + st.s * d);
       st.s *= f;
       st.m = mx;
@@ -157,7 +162,7 @@ __global__ void __launch_bounds__(THREADS) k_logprobs(LogprobArgs a, int seg_len
     const float mb = finite_max(st.m);
 #pragma unroll
     for (int e = 0; e < PER; e++) {
-      const float d = v[e] - mb, p = exp2f(d * 1.4426950408889634f);
+      const float d = v[e] - mb, p = ex2(d * LOG2E);
       st.s += p;
       st.t = fmaf(p, fmaxf(d, -1e30f), st.t);   // p is 0 where the clamp acts; a NaN stays in p
     }
@@ -173,28 +178,38 @@ __global__ void __launch_bounds__(THREADS) k_logprobs(LogprobArgs a, int seg_len
       for (int e = 0; e < PER; e++) above += i0 + elt_at<T>(e) < tgt ? v[e] >= xt : v[e] > xt;
     }
     if constexpr (TOP) {
+      const int sb = *reinterpret_cast<volatile int*>(&s_bound);
+      bound = fmaxf(bound, __int_as_float(sb >= 0 ? sb : sb ^ 0x7fffffff));
       if (first) {   // 32 lane maxima: the k-th largest of them bounds the tile's k-th from below
         first = false;
-        bound = key_value(__shfl_sync(0xffffffffu, sort32(key_of(mx, lane), lane), k - 1));
+        bound = fmaxf(bound, key_value(__shfl_sync(0xffffffffu, sort32(key_of(mx, lane), lane), k - 1)));
+        if (lane == 0) atomicMax(&s_bound, ordered(bound));
       }
       if (__any_sync(0xffffffffu, mx >= bound)) {
 #pragma unroll
         for (int e = 0; e < PER; e++) {
-          const int i = i0 + elt_at<T>(e);
-          const u64 key = key_of(v[e], (uint32_t)i);
-          const bool take = v[e] >= bound && i < i_end && key > kth;
-          const uint32_t votes = __ballot_sync(0xffffffffu, take);
-          if (take) s_cand[warp][waiting + __popc(votes & ((1u << lane) - 1))] = key;
-          waiting += __popc(votes);
+          uint32_t votes = __ballot_sync(0xffffffffu, v[e] >= bound);
+          if (votes) {
+            const int i = i0 + elt_at<T>(e);
+            const u64 key = key_of(v[e], (uint32_t)i);
+            const bool take = v[e] >= bound && i < i_end && key > kth;
+            votes = __ballot_sync(0xffffffffu, take);
+            if (take) s_cand[warp][waiting + __popc(votes & ((1u << lane) - 1))] = key;
+            waiting += __popc(votes);
+            __syncwarp();
+            if (waiting >= 32) {
+              waiting -= 32;
+              const u64 cand = s_cand[warp][waiting + lane];
+              top = merge_batch(top, cand, lane);
+              kth = __shfl_sync(0xffffffffu, top, k - 1);
+              if (kth != 0) {
+                bound = fmaxf(bound, key_value(kth));
+                if (lane == 0) atomicMax(&s_bound, ordered(bound));
+              }
+              __syncwarp();
+            }
+          }
         }
-        __syncwarp();
-        while (waiting >= 32) {
-          waiting -= 32;
-          top = merge32(top, sort32(s_cand[warp][waiting + lane], lane), lane);
-        }
-        kth = __shfl_sync(0xffffffffu, top, k - 1);
-        if (kth != 0) bound = fmaxf(bound, key_value(kth));
-        __syncwarp();
       }
     }
   }
@@ -288,9 +303,9 @@ __global__ void __launch_bounds__(THREADS) k_logprobs(LogprobArgs a, int seg_len
 
 }  // namespace
 
-// Segments per row: enough CTAs for four a SM, a segment at least two tiles of every warp.
+// Segments per row: enough CTAs for four a SM, a segment at least a tile of every warp.
 int logprob_segments(int T, int V, int n_sm) {
-  const int most = (V + 2 * WARPS * TILE - 1) / (2 * WARPS * TILE);
+  const int most = (V + WARPS * TILE - 1) / (WARPS * TILE);
   const int want = (4 * n_sm + T - 1) / T;
   const int n = want < most ? want : most;
   return n < 1 ? 1 : (n > 64 ? 64 : n);

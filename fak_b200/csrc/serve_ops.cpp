@@ -4,6 +4,10 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <ATen/cuda/CUDAContext.h>
+#include <c10/cuda/CUDAGraphsC10Utils.h>
+
+#include <map>
+#include <mutex>
 
 #include "serve_ops.h"
 
@@ -45,6 +49,27 @@ int check_pages(const Tensor& pages, const char* what) {
   TORCH_CHECK(pages.size(0) > 0 && pages.size(1) > 0, what, ": no pages");
   TORCH_CHECK(reinterpret_cast<uintptr_t>(pages.data_ptr()) % 16 == 0, what, ": pages must start on a 16-byte boundary");
   return (int)pages.size(2) / 20;
+}
+// A tensor of 4-byte elements inside one buffer of them: an operator's outputs share one allocation.
+Tensor carve(const Tensor& buf, int64_t at, at::IntArrayRef sizes, c10::ScalarType type) {
+  Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(buf.storage()), buf.key_set(),
+                                                      c10::scalarTypeToTypeMeta(type));
+  t.unsafeGetTensorImpl()->set_storage_offset(at);
+  t.unsafeGetTensorImpl()->set_sizes_contiguous(sizes);
+  return t;
+}
+int64_t up4(int64_t n) { return (n + 3) / 4 * 4; }
+// Zeroed counters, left at zero by every launch: one set per stream, so that calls on different streams
+// cannot meet in them.  A captured call gets its own, which the graph zeroes.
+Tensor tickets_for(const Tensor& like, int64_t n) {
+  auto opt = like.options().dtype(torch::kInt32);
+  if (c10::cuda::currentStreamCaptureStatusMayInitCtx() != c10::cuda::CaptureStatus::None) return torch::zeros({n}, opt);
+  static std::mutex mu;
+  static auto* held = new std::map<std::pair<int, cudaStream_t>, Tensor>();   // (lives as long as the process)
+  std::lock_guard<std::mutex> lock(mu);
+  Tensor& t = (*held)[{like.get_device(), stream_of(like)}];
+  if (!t.defined() || t.numel() < n) t = torch::zeros({std::max<int64_t>(n, 4096)}, opt);
+  return t;
 }
 bool aligned(const Tensor& t, int64_t elems) {
   return reinterpret_cast<uintptr_t>(t.data_ptr()) % (elems * t.element_size()) == 0;
@@ -121,6 +146,7 @@ void kv4_attention(Tensor q, Tensor pages, Tensor table, OptTensor q_off, Tensor
   a.q_type = elt(q, "kv4_attention: q");
   a.q_tok = q.stride(0);
   a.q_head = q.stride(1);
+  a.q_vec = reinterpret_cast<uintptr_t>(a.q) % 16 == 0 && a.q_tok * q.element_size() % 16 == 0 && a.q_head * q.element_size() % 16 == 0;
   a.out = out.data_ptr();
   a.o_type = elt(out, "kv4_attention: out");
   a.o_tok = out.stride(0);
@@ -202,15 +228,14 @@ std::vector<Tensor> plan_batch(Tensor old_len, Tensor new_len, Tensor table, Ten
     for (int i = 0; i < 7; i++) i32(o[i], n[i], old_len, "plan_batch: plan tensor");
     TORCH_CHECK(o[6].data_ptr() != free_head.data_ptr(), "plan_batch: the new free head needs a word of its own");
   } else {
-    // one allocation; every part starts on 16 bytes
-    auto up = [](int64_t n) { return (n + 3) / 4 * 4; };
     const int64_t n[7] = {max_tokens, max_tokens, max_tokens, B + 1, B, B, 1};
     int64_t at = 0, all = 0;
-    for (int64_t k : n) all += up(k);
+    for (int64_t k : n) all += up4(k);
     Tensor buf = torch::empty({all}, old_len.options());
+    o.reserve(7);
     for (int64_t k : n) {
-      o.push_back(buf.narrow(0, at, k));
-      at += up(k);
+      o.push_back(carve(buf, at, {k}, torch::kInt32));
+      at += up4(k);
     }
   }
   a.slot = o[0].data_ptr<int>();
@@ -224,7 +249,7 @@ std::vector<Tensor> plan_batch(Tensor old_len, Tensor new_len, Tensor table, Ten
   return o;
 }
 
-std::vector<Tensor> token_logprobs(Tensor logits, int64_t V, Tensor target, int64_t k, double softcap, OptTensor tickets) {
+std::vector<Tensor> token_logprobs(Tensor logits, int64_t V, Tensor target, int64_t k, double softcap) {
   TORCH_CHECK(logits.is_cuda() && logits.dim() == 2 && (logits.stride(1) == 1 || logits.size(1) <= 1),
               "token_logprobs: logits [T, >= V] on the GPU, last dimension contiguous");
   TORCH_CHECK(V > 0 && V <= logits.size(1) && V < (int64_t(1) << 30), "token_logprobs: V ", S(V), " of ", S(logits.size(1)), " columns");
@@ -242,20 +267,22 @@ std::vector<Tensor> token_logprobs(Tensor logits, int64_t V, Tensor target, int6
   const int64_t per = a.type == fak::Elt::F32 ? 4 : 8;
   a.vec = aligned(logits, per) && (a.stride % per == 0 || a.T <= 1);
   c10::cuda::CUDAGuard guard(logits.device());
-  auto f32 = logits.options().dtype(torch::kFloat32), i = logits.options().dtype(torch::kInt32);
-  Tensor lp = torch::empty({a.T}, f32), en = torch::empty({a.T}, f32), rank = torch::empty({a.T}, i);
-  Tensor ids = torch::empty({a.T, k}, i), top = torch::empty({a.T, k}, f32);
+  const int64_t T = a.T, rows = up4(T);
+  Tensor buf = torch::empty({3 * rows + 2 * up4(T * k)}, logits.options().dtype(torch::kFloat32));
+  Tensor lp = carve(buf, 0, {T}, torch::kFloat32), en = carve(buf, rows, {T}, torch::kFloat32);
+  Tensor rank = carve(buf, 2 * rows, {T}, torch::kInt32), ids = carve(buf, 3 * rows, {T, k}, torch::kInt32);
+  Tensor top = carve(buf, 3 * rows + up4(T * k), {T, k}, torch::kFloat32);
   a.logprob = lp.data_ptr<float>();
   a.entropy = en.data_ptr<float>();
   a.rank = rank.data_ptr<int>();
   a.top_ids = ids.data_ptr<int>();
   a.top_logprobs = top.data_ptr<float>();
   a.n_seg = fak::logprob_segments(a.T, a.V, sms(logits));
-  Tensor part;
+  Tensor part, tickets;
   if (a.n_seg > 1) {
-    TORCH_CHECK(tickets.has_value(), "token_logprobs: tickets");
-    a.tickets = const_cast<int*>(i32(*tickets, a.T, logits, "token_logprobs: tickets"));
-    part = torch::empty({fak::logprob_part_words(a.T, a.n_seg)}, f32);
+    tickets = tickets_for(logits, T);
+    a.tickets = tickets.data_ptr<int>();
+    part = torch::empty({fak::logprob_part_words(a.T, a.n_seg)}, buf.options());
     a.part = part.data_ptr<float>();
   }
   fak::logprob_launch(a, stream_of(logits));
@@ -274,5 +301,5 @@ void bind_serve_ops(pybind11::module& m) {
   m.def("plan_batch", &plan_batch, py::arg("old_len"), py::arg("new_len"), py::arg("table"), py::arg("free_pages"),
         py::arg("free_head"), py::arg("max_tokens"), py::arg("outs") = py::none(), py::arg("err") = py::none());
   m.def("token_logprobs", &token_logprobs, py::arg("logits"), py::arg("V"), py::arg("target"), py::arg("k"),
-        py::arg("softcap") = 0.0, py::arg("tickets") = py::none());
+        py::arg("softcap") = 0.0);
 }

@@ -24,6 +24,7 @@ struct Kv4Attn {
   const void* q;             // [T, H, D], row strides q_tok, q_head (elements)
   int64_t q_tok, q_head;
   Elt q_type;
+  bool q_vec;                // rows start on 16 bytes
   const uint8_t* pages;      // [n_pages, Hkv, 20 D]
   int64_t n_pages;
   const int* table;          // [B, >= width]
@@ -44,7 +45,7 @@ struct Kv4Attn {
   int* err;
 };
 struct Kv4AttnPlan {
-  int nt, row_chunks, n_split;
+  int nt, row_chunks, n_split, pps;
   int64_t part_floats;
 };
 Kv4AttnPlan kv4_attn_plan(const Kv4Attn& a, int n_sm);

@@ -412,28 +412,12 @@ class TokenLogprobs(NamedTuple):
     top_logprobs: torch.Tensor   # [T, k] f32
 
 
-_lp_tickets: dict = {}
-
-
-def _logprob_tickets(device, rows: int) -> torch.Tensor:
-    """Zeroed row counters, left at zero by every launch; one set per stream, so that calls on different
-    streams cannot meet in them.  Inside a graph capture each call gets its own (zeroed by the graph)."""
-    if torch.cuda.is_current_stream_capturing():
-        return torch.zeros(rows, dtype=torch.int32, device=device)
-    key = (device, torch.cuda.current_stream(device).cuda_stream)
-    t = _lp_tickets.get(key)
-    if t is None or t.numel() < rows:
-        t = _lp_tickets[key] = torch.zeros(max(rows, 4096), dtype=torch.int32, device=device)
-    return t
-
-
 def token_logprobs(logits: torch.Tensor, V: int, targets: torch.Tensor, top_k: int = 0, softcap: float = 0.0
                    ) -> TokenLogprobs:
     """Log probability, entropy and rank of one given token per row, and the row's ``top_k`` (at most 32)
     alternatives, over the first V columns of logits [T, >= V] (float32, float16 or bfloat16), each logit
     read once.  targets [T] int32; a target outside [0, V) means none.  softcap > 0: the logits are
     cap * tanh(logit / cap).  Masked logits (-inf) have probability 0; rows with a NaN or +inf are NaN."""
-    r = TokenLogprobs(*ext().token_logprobs(logits, V, targets, top_k, softcap,
-                                            _logprob_tickets(logits.device, logits.shape[0]) if logits.is_cuda else None))
+    r = TokenLogprobs(*ext().token_logprobs(logits, V, targets, top_k, softcap))
     count()
     return r
