@@ -21,27 +21,24 @@
 // A warp streams its own pages through a ring of shared memory filled by one bulk copy a page and walks
 // them with an online softmax whose base moves only when a row outgrows it; the CTA's warps, then the
 // splits of a sequence (k_kv4_combine), are merged at the end.
-#include "kv4.cuh"
-#include "mma.cuh"
-#include "tc.cuh"
+#include "kv4_common.cuh"
 
 #include <algorithm>
 #include <stdexcept>
 #include <string>
 
-#include "../serve_ops.h"
-
 namespace fak {
 namespace {
 
-using kv4::Lay;
-using kv4::PAGE;
+using namespace kv4;
 
 constexpr int W = 4;          // warps per CTA
 constexpr int STAGES = 4;     // pages in flight per warp
 constexpr float HEADROOM = 0.875f;   // log2 growth of a row's max before its base moves
 constexpr float LIFT = 2.f;          // P = 2^(z - base + LIFT) <= 2^2.875 < 7.5
 constexpr float LOG2E = 1.4426950408889634f;
+constexpr int kPrefillRows = 64;     // more query rows than this per (sequence, KV head): kv4_prefill.cu
+constexpr float kPrefillLift = 4.f;   // LIFT of that kernel
 
 FAK_DEV void mma_f16_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm volatile(
@@ -66,67 +63,10 @@ FAK_DEV uint32_t movmatrix(uint32_t a) {
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(a));
   return r;
 }
-FAK_DEV uint32_t pack_f16(float lo, float hi) {
-  const __half2 h = __floats2half2_rn(lo, hi);
-  return *reinterpret_cast<const uint32_t*>(&h);
-}
 FAK_DEV uint32_t mul_h2(uint32_t a, uint32_t b) {
   const __half2 h = __hmul2(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b));
   return *reinterpret_cast<const uint32_t*>(&h);
 }
-FAK_DEV float2 unpack_h2(uint32_t a) { return __half22float2(*reinterpret_cast<__half2*>(&a)); }
-FAK_DEV float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-FAK_DEV void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
-  asm volatile(
-      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(dst)),
-      "l"(src), "r"(bytes), "r"(smem_u32(bar))
-      : "memory");
-}
-
-template <int N>
-FAK_DEV void lds(const uint8_t* p, uint32_t (&r)[N]) {
-  if constexpr (N == 4) {
-    const uint4 v = *reinterpret_cast<const uint4*>(p);
-    r[0] = v.x; r[1] = v.y; r[2] = v.z; r[3] = v.w;
-  } else if constexpr (N == 2) {
-    const uint2 v = *reinterpret_cast<const uint2*>(p);
-    r[0] = v.x; r[1] = v.y;
-  } else {
-    r[0] = *reinterpret_cast<const uint32_t*>(p);
-  }
-}
-
-// The pages one CTA column block needs, and how the splits share them: the same arithmetic in the
-// attention kernel and in the combine.
-struct Span {
-  int p0, p1, live;   // pages [p0, p1), splits of pps pages that hold any
-};
-FAK_DEV Span span_of(int ctx, int n, int i_lo, int i_hi, int window, int pps, int width) {
-  Span s;
-  const int last = min(ctx - n + i_hi, ctx - 1);               // the last key any row of the block sees
-  const int first = window > 0 ? max(0, ctx - n + i_lo + 1 - window) : 0;
-  s.p0 = first / PAGE;
-  s.p1 = min(width, last / PAGE + 1);
-  if (last < 0) s.p1 = s.p0;
-  s.live = (max(0, s.p1 - s.p0) + pps - 1) / pps;
-  return s;
-}
-
-FAK_DEV float load_elt(const void* p, Elt t, int64_t i) {
-  if (t == Elt::F32) return ((const float*)p)[i];
-  if (t == Elt::F16) return __half2float(((const __half*)p)[i]);
-  return __bfloat162float(((const __nv_bfloat16*)p)[i]);
-}
-FAK_DEV void store_elt(void* p, Elt t, int64_t i, float v) {
-  if (t == Elt::F32) ((float*)p)[i] = v;
-  else if (t == Elt::F16) ((__half*)p)[i] = __float2half_rn(v);
-  else ((__nv_bfloat16*)p)[i] = __float2bfloat16_rn(v);
-}
-
 template <int D, int NT>
 struct Smem {
   static constexpr int COLS = 8 * NT;
@@ -137,10 +77,14 @@ struct Smem {
   };
   uint64_t full[W][STAGES];
   float base[W][COLS], sum[W][COLS];
+  float qmax[COLS][Lay<D>::NG];
+  alignas(16) float qsum[COLS][Lay<D>::NG];
+  uint4 qf[NT][Lay<D>::NG][32];
+  int fail;   // a wait gave up
 };
 
 template <int D, int NT, bool CAP>
-__global__ void __launch_bounds__(W * 32)
+__global__ void __launch_bounds__(W * 32, NT == 1 ? 4 : 2)
 k_kv4_attn(const __grid_constant__ Kv4Attn a, int n_split, int pps) {
   using L = Lay<D>;
   constexpr int NG = L::NG;
@@ -152,8 +96,9 @@ k_kv4_attn(const __grid_constant__ Kv4Attn a, int n_split, int pps) {
   const int split = blockIdx.x % n_split, rc = blockIdx.x / n_split, kvh = blockIdx.y, b = blockIdx.z;
   const int G = a.H / a.Hkv;
   if (lane < STAGES) tc::mbar_init(&sm.full[warp][lane], 1);
+  if (tid == 0) sm.fail = 0;
   tc::fence_mbar_init();
-  __syncwarp();
+  __syncthreads();
   pdl_wait();
 
   const int ctx = min(a.ctx[b], a.width * PAGE);
@@ -195,111 +140,97 @@ k_kv4_attn(const __grid_constant__ Kv4Attn a, int n_split, int pps) {
   for (int i = 0; i < STAGES - 1; i++)
     if (i < np) issue(i);
 
-  // Queries: lane (g, t) holds column nt * 8 + g, dims group * 32 + 8 t .. + 7
-  uint32_t qf[NT][NG][4], qs[NT];
-  float cf[NT][2];                 // logit factor (log2 units) of columns 2 t, 2 t + 1
-  int lim[NT][2], low[NT][2];      // keys [low, lim) are seen by the column
-  int lim_min = INT_MAX, low_max = 0;
+  // Queries.  Lane (g, t) of the fragments holds column nt * 8 + g, dims group * 32 + 8 t .. + 7; the CTA's
+  // warps share the (n-tile, group) pairs out, and every warp then reads all of them.
+  constexpr int PAIRS = NT * NG, MINE = (PAIRS + W - 1) / W;
+  float x[MINE][8];
 #pragma unroll
-  for (int nt = 0; nt < NT; nt++) {
+  for (int m = 0; m < MINE; m++) {
+    const int pr = warp + m * W, nt = pr / NG, gr = pr % NG;
     const int r = r0 + nt * 8 + g;
-    const bool live = r < R;
-    const int i = live ? r / G : 0, h = kvh * G + (live ? r % G : 0);
-    float x[NG][8], amax = 0.f;
-    const int64_t at = (int64_t)(tok0 + i) * a.q_tok + (int64_t)h * a.q_head + 8 * t;
-    if (!live) {
 #pragma unroll
-      for (int gr = 0; gr < NG; gr++)
-#pragma unroll
-        for (int e = 0; e < 8; e++) x[gr][e] = 0.f;
-    } else if (a.q_vec && a.q_type != Elt::F32) {
-      uint4 u[NG];
-#pragma unroll
-      for (int gr = 0; gr < NG; gr++) u[gr] = *reinterpret_cast<const uint4*>((const uint16_t*)a.q + at + gr * 32);
-#pragma unroll
-      for (int gr = 0; gr < NG; gr++) {
-        const uint32_t w[4] = {u[gr].x, u[gr].y, u[gr].z, u[gr].w};
+    for (int e = 0; e < 8; e++) x[m][e] = 0.f;
+    if (pr < PAIRS && r < R) {
+      const int64_t at = (int64_t)(tok0 + r / G) * a.q_tok + (int64_t)(kvh * G + r % G) * a.q_head + gr * 32 + 8 * t;
+      if (a.q_vec && a.q_type != Elt::F32) {
+        const uint4 u = *reinterpret_cast<const uint4*>((const uint16_t*)a.q + at);
+        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
         for (int e = 0; e < 4; e++) {
           const float2 f = unpack_h2(w[e]);
-          x[gr][2 * e] = a.q_type == Elt::F16 ? f.x : bf16_bits_lo(w[e]);
-          x[gr][2 * e + 1] = a.q_type == Elt::F16 ? f.y : bf16_bits_hi(w[e]);
+          x[m][2 * e] = a.q_type == Elt::F16 ? f.x : bf16_bits_lo(w[e]);
+          x[m][2 * e + 1] = a.q_type == Elt::F16 ? f.y : bf16_bits_hi(w[e]);
         }
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; e++) x[m][e] = load_elt(a.q, a.q_type, at + e);
       }
-    } else {
-#pragma unroll
-      for (int gr = 0; gr < NG; gr++)
-#pragma unroll
-        for (int e = 0; e < 8; e++) x[gr][e] = load_elt(a.q, a.q_type, at + gr * 32 + e);
     }
+    float amax = 0.f;
 #pragma unroll
-    for (int gr = 0; gr < NG; gr++)
-#pragma unroll
-      for (int e = 0; e < 8; e++) amax = fmaxf(amax, fabsf(x[gr][e]));
+    for (int e = 0; e < 8; e++) amax = fmaxf(amax, fabsf(x[m][e]));
     amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
     amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-    // power of two that brings the row's largest into [2^13, 2^14)
-    int ex = 0;
-    if (amax > 0.f && amax < INFINITY) frexpf(amax, &ex);
-    ex = amax > 0.f && amax < INFINITY ? 14 - ex : 0;
-    // (a denormal maximum would ask for more than 2^127: two steps)
-    const float f1 = exp2f((float)(ex / 2)), f2 = exp2f((float)(ex - ex / 2));
-    float sum[NG];
+    if (pr < PAIRS && t == 0) sm.qmax[nt * 8 + g][gr] = amax;
+  }
+  __syncthreads();
+  // a power of two brings the row's largest into [2^13, 2^14)
+  auto factor = [&](int col) {
+    float amax = 0.f;
 #pragma unroll
-    for (int gr = 0; gr < NG; gr++) {
-      sum[gr] = 0.f;
-      float y[8];
+    for (int gr = 0; gr < NG; gr++) amax = fmaxf(amax, sm.qmax[col][gr]);
+    const int ex = (int)(__float_as_uint(amax) >> 23);           // biased exponent; 255: infinity
+    return __uint_as_float((uint32_t)(ex == 255 ? 127 : min(127 + 126, 127 + 13 + 127 - ex)) << 23);
+  };
+#pragma unroll
+  for (int m = 0; m < MINE; m++) {
+    const int pr = warp + m * W, nt = pr / NG, gr = pr % NG;
+    if (pr < PAIRS) {
+      const float f = factor(nt * 8 + g);
+      float y[8], sum = 0.f;
 #pragma unroll
       for (int e = 0; e < 8; e++) {
-        y[e] = __half2float(__float2half_rn(x[gr][e] * f1 * f2));
-        sum[gr] += y[e];
+        y[e] = __half2float(__float2half_rn(x[m][e] * f));
+        sum += y[e];
       }
       // nibble pairs (e, e + 4); the odd pairs arrive 16 times too large
-      qf[nt][gr][0] = pack_f16(y[0], y[4]);
-      qf[nt][gr][1] = pack_f16(y[1] * 0.0625f, y[5] * 0.0625f);
-      qf[nt][gr][2] = pack_f16(y[2], y[6]);
-      qf[nt][gr][3] = pack_f16(y[3] * 0.0625f, y[7] * 0.0625f);
-      sum[gr] += __shfl_xor_sync(0xffffffffu, sum[gr], 1);
-      sum[gr] += __shfl_xor_sync(0xffffffffu, sum[gr], 2);
-      sum[gr] *= 0.015625f;   // |sum| <= 32 * 2^14: back into f16's range
+      sm.qf[nt][gr][lane] = make_uint4(pack_f16(y[0], y[4]), pack_f16(y[1] * 0.0625f, y[5] * 0.0625f), pack_f16(y[2], y[6]),
+                                       pack_f16(y[3] * 0.0625f, y[7] * 0.0625f));
+      sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+      sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+      if (t == 0) sm.qsum[nt * 8 + g][gr] = sum * 0.015625f;   // |sum| <= 32 * 2^14: back into f16's range
+    }
+  }
+  __syncthreads();
+  uint32_t qf[NT][NG][4], qs[NT];
+  float cf[NT][2];                 // logit factor (log2 units) of columns 2 t, 2 t + 1
+  int lim[NT][2], low[NT][2];      // keys [low, lim) are seen by the column
+#pragma unroll
+  for (int nt = 0; nt < NT; nt++) {
+#pragma unroll
+    for (int gr = 0; gr < NG; gr++) {
+      const uint4 u = sm.qf[nt][gr][lane];
+      qf[nt][gr][0] = u.x; qf[nt][gr][1] = u.y; qf[nt][gr][2] = u.z; qf[nt][gr][3] = u.w;
     }
     // B of the m16n8k8: rows 2 t, 2 t + 1 = the groups' sums, their high parts then the remainders
-    {
-      const int pr = NG == 4 ? (t & 1) : 0;
-      const bool lo_part = NG == 4 ? t >= 2 : t == 1;
-      float s0 = sum[0], s1 = sum[1];
-      if constexpr (NG == 4) {
-        s0 = pr ? sum[2] : sum[0];
-        s1 = pr ? sum[3] : sum[1];
-      }
-      const float h0 = __half2float(__float2half_rn(s0)), h1 = __half2float(__float2half_rn(s1));
-      qs[nt] = lo_part ? pack_f16(s0 - h0, s1 - h1) : pack_f16(h0, h1);
-      if (NG == 2 && t >= 2) qs[nt] = 0;
-    }
-    const int my_lim = live ? min(ctx - n + i + 1, ctx) : 0;
-    const int my_low = live && a.window > 0 ? max(0, my_lim - a.window) : 0;
-    const float my_cf = 64.f / f1 / f2 * a.scale * (CAP ? 1.f : LOG2E);
+    const float2 s = *reinterpret_cast<const float2*>(&sm.qsum[nt * 8 + g][NG == 4 ? 2 * (t & 1) : 0]);
+    const float h0 = __half2float(__float2half_rn(s.x)), h1 = __half2float(__float2half_rn(s.y));
+    qs[nt] = (NG == 4 ? t >= 2 : t == 1) ? pack_f16(s.x - h0, s.y - h1) : pack_f16(h0, h1);
+    if (NG == 2 && t >= 2) qs[nt] = 0;
 #pragma unroll
     for (int e = 0; e < 2; e++) {
-      lim[nt][e] = __shfl_sync(0xffffffffu, my_lim, (2 * t + e) * 4);
-      low[nt][e] = __shfl_sync(0xffffffffu, my_low, (2 * t + e) * 4);
-      cf[nt][e] = __shfl_sync(0xffffffffu, my_cf, (2 * t + e) * 4);
-    }
-    if (live) {
-      lim_min = min(lim_min, my_lim);
-      low_max = max(low_max, my_low);
+      const int r = r0 + nt * 8 + 2 * t + e;
+      cf[nt][e] = 64.f / factor(nt * 8 + 2 * t + e) * a.scale * (CAP ? 1.f : LOG2E);
+      lim[nt][e] = r < R ? min(ctx - n + r / G + 1, ctx) : 0;
+      low[nt][e] = a.window > 0 ? max(0, lim[nt][e] - a.window) : 0;
     }
   }
-  // keys every live row sees: pages inside [low_max, lim_min) need no mask (dead columns are dropped
-  // at the end).  Keys outside [low_any, lim_any) are seen by no row: their V is not touched.
-#pragma unroll
-  for (int d = 4; d < 32; d <<= 1) {
-    lim_min = min(lim_min, __shfl_xor_sync(0xffffffffu, lim_min, d));
-    low_max = max(low_max, __shfl_xor_sync(0xffffffffu, low_max, d));
-  }
+  // Keys every live row sees, [low_max, lim_min): pages inside need no mask (dead columns are dropped at
+  // the end).  Keys outside [low_any, lim_any) are seen by no row: their V is not touched.
   const int i_first = r0 / G, i_last = min(R - 1, r0 + COLS - 1) / G;
-  const int lim_any = ctx - n + i_last + 1;
-  const int low_any = a.window > 0 ? max(0, ctx - n + i_first + 1 - a.window) : 0;
+  const int lim_any = ctx - n + i_last + 1, lim_min = ctx - n + i_first + 1;
+  const int low_any = a.window > 0 ? max(0, lim_min - a.window) : 0;
+  const int low_max = a.window > 0 ? max(0, lim_any - a.window) : 0;
 
   float o[NT][NG][2][4], mt[NT][4], base[NT][2];
   float lift[NT][2];   // LIFT - base (0 while the base is -inf: then every z is -inf too)
@@ -319,8 +250,8 @@ k_kv4_attn(const __grid_constant__ Kv4Attn a, int n_split, int pps) {
 #pragma unroll 1
   for (int i = 0; i < np; i++) {
     if (i + STAGES - 1 < np) issue(i + STAGES - 1);
-    // (a wait that gives up has set the error word; the loop goes on, so that every copy is waited for)
-    tc::mbar_wait(&sm.full[warp][i % STAGES], (uint32_t)((i / STAGES) & 1), a.err);
+    // (a wait that gives up is reported at the end; the loop goes on, so that every copy is waited for)
+    tc::mbar_wait(&sm.full[warp][i % STAGES], (uint32_t)((i / STAGES) & 1), &sm.fail);
     const uint8_t* pg = sm.ring[warp][i % STAGES];
     const int key0 = (p_begin + warp + W * i) * PAGE;
     const bool whole = key0 >= low_max && key0 + PAGE <= lim_min;   // warp-uniform
@@ -457,6 +388,7 @@ k_kv4_attn(const __grid_constant__ Kv4Attn a, int n_split, int pps) {
 
   // merge the CTA's warps; the ring is free once every warp has drained its copies
   __syncthreads();
+  if (tid == 0 && sm.fail) report_error(a.err, 1);
 #pragma unroll
   for (int nt = 0; nt < NT; nt++) {
     float ml[NG][2];
@@ -529,10 +461,11 @@ k_kv4_attn(const __grid_constant__ Kv4Attn a, int n_split, int pps) {
 
 // One warp merges the live splits of one query row: D / 32 dims a lane, up to 16 splits' loads in flight.
 template <int D>
-__global__ void __launch_bounds__(256) k_kv4_combine(const __grid_constant__ Kv4Attn a, int n_split, int pps, int cols, int row_chunks) {
+__global__ void __launch_bounds__(256) k_kv4_combine(const __grid_constant__ Kv4Attn a, int n_split, int pps, int cols, int row_chunks, float lift) {
   constexpr int V = D / 32;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int rc = blockIdx.x, kvh = blockIdx.y, b = blockIdx.z;
+  const int rc = blockIdx.x / (cols / 8), kvh = blockIdx.y, b = blockIdx.z;
+  const int c = blockIdx.x % (cols / 8) * 8 + warp;
   const int G = a.H / a.Hkv;
   pdl_wait();
   const int ctx = min(a.ctx[b], a.width * PAGE);
@@ -547,7 +480,7 @@ __global__ void __launch_bounds__(256) k_kv4_combine(const __grid_constant__ Kv4
   const int live = max(1, sp.live);   // an empty block's split 0 wrote zeros
   const int64_t part_col = (((int64_t)b * a.Hkv + kvh) * row_chunks + rc) * cols;
   const float* part_ml = a.part + (int64_t)gridDim.z * gridDim.y * row_chunks * cols * n_split * D;
-  for (int c = warp; c < cols && r0 + c < R; c += 8) {
+  if (r0 + c < R) {
     const int r = r0 + c, h = kvh * G + r % G;
     const float2* ml = reinterpret_cast<const float2*>(part_ml) + (part_col + c) * n_split;
     const float* po = a.part + (part_col + c) * n_split * D + V * lane;
@@ -556,7 +489,7 @@ __global__ void __launch_bounds__(256) k_kv4_combine(const __grid_constant__ Kv4
     for (int s = lane; s < live; s += 32) m = fmaxf(m, __ldcg(&ml[s].x));
     m = warp_max(m);
     const float bs = m == -INFINITY ? 0.f : m;
-    float l = sink > -INFINITY ? ex2(sink - bs + LIFT) : 0.f;
+    float l = sink > -INFINITY ? ex2(sink - bs + lift) : 0.f;
     float acc[V] = {};
     for (int s0 = 0; s0 < live; s0 += 32) {
       float f = 0.f, ls = 0.f;
@@ -598,9 +531,21 @@ void pdl(cudaLaunchConfig_t& cfg, cudaLaunchAttribute* attr) {
 }  // namespace
 
 Kv4AttnPlan kv4_attn_plan(const Kv4Attn& a, int n_sm) {
-  Kv4AttnPlan p;
+  Kv4AttnPlan p{};
   const int64_t rows = (int64_t)a.max_new * (a.H / a.Hkv);
   const int nt_most = a.D == 64 ? 4 : 2;
+  p.tc = rows > kPrefillRows;
+  if (p.tc) {
+    // 256 rows a CTA, one CTA a SM: keys are split until every SM has one, eight steps a split at least
+    p.row_chunks = (int)((rows + 255) / 256);
+    const int64_t ctas = (int64_t)a.B * a.Hkv * p.row_chunks;
+    int64_t pps = a.n_split > 0 ? (a.width + a.n_split - 1) / a.n_split : std::max<int64_t>(64, (a.width * ctas + n_sm - 1) / n_sm);
+    pps = std::min<int64_t>((pps + 7) / 8 * 8, (a.width + 7) / 8 * 8);
+    p.pps = (int)pps;
+    p.n_split = (int)((a.width + pps - 1) / pps);
+    p.part_floats = p.n_split > 1 ? ctas * 256 * p.n_split * (a.D + 2) : 0;
+    return p;
+  }
   p.nt = rows <= 8 ? 1 : (rows <= 16 || nt_most == 2 ? 2 : 4);
   p.row_chunks = (int)((rows + 8 * p.nt - 1) / (8 * p.nt));
   // Splits of pps pages each, the same for every sequence, so that CTAs are alike whatever the lengths:
@@ -615,7 +560,7 @@ Kv4AttnPlan kv4_attn_plan(const Kv4Attn& a, int n_sm) {
   return p;
 }
 
-void kv4_attn_launch(const Kv4Attn& a, const Kv4AttnPlan& p, cudaStream_t stream) {
+static void split_launch(const Kv4Attn& a, const Kv4AttnPlan& p, cudaStream_t stream) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(p.n_split * p.row_chunks), (unsigned)a.Hkv, (unsigned)a.B);
   cfg.blockDim = dim3(W * 32);
@@ -642,14 +587,21 @@ void kv4_attn_launch(const Kv4Attn& a, const Kv4AttnPlan& p, cudaStream_t stream
     else FAK_KV4(64, 4)
   }
 #undef FAK_KV4
+}
+
+void kv4_attn_launch(const Kv4Attn& a, const Kv4AttnPlan& p, cudaStream_t stream) {
+  if (p.tc) kv4_prefill_launch(a, p, stream);
+  else split_launch(a, p, stream);
+  cudaLaunchAttribute attr[1];
   if (p.n_split > 1) {
     cudaLaunchConfig_t c2 = {};
-    c2.gridDim = dim3((unsigned)p.row_chunks, (unsigned)a.Hkv, (unsigned)a.B);
+    const int cols = p.tc ? 256 : 8 * p.nt;
+    c2.gridDim = dim3((unsigned)(p.row_chunks * cols / 8), (unsigned)a.Hkv, (unsigned)a.B);
     c2.blockDim = dim3(256);
     c2.stream = stream;
     pdl(c2, attr);
-    if (a.D == 128) FAK_CUDA_CHECK(cudaLaunchKernelEx(&c2, k_kv4_combine<128>, a, p.n_split, p.pps, 8 * p.nt, p.row_chunks));
-    else FAK_CUDA_CHECK(cudaLaunchKernelEx(&c2, k_kv4_combine<64>, a, p.n_split, p.pps, 8 * p.nt, p.row_chunks));
+    if (a.D == 128) FAK_CUDA_CHECK(cudaLaunchKernelEx(&c2, k_kv4_combine<128>, a, p.n_split, p.pps, cols, p.row_chunks, p.tc ? kPrefillLift : LIFT));
+    else FAK_CUDA_CHECK(cudaLaunchKernelEx(&c2, k_kv4_combine<64>, a, p.n_split, p.pps, cols, p.row_chunks, p.tc ? kPrefillLift : LIFT));
   }
 }
 

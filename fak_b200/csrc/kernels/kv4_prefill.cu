@@ -1,0 +1,552 @@
+// Chunk attention over the 4-bit paged KV cache on the 5th-generation tensor cores (tcgen05 + TMEM).
+//
+// The n * G query rows of a (sequence, KV head) -- row r is query r / G, head r % G of the group -- are
+// packed into tiles of 128 rows, two tiles a CTA, so that one pass of dequantized keys and values serves
+// 256 rows whatever the group size.  Warp roles:
+//   warps 0-3, 4-7  softmax of tile 0 / 1, one row a thread: S from TMEM, P = 2^(S c - base) back into
+//                   TMEM as f16 over the first half of S's columns (the A operand of P V is read there);
+//   warps 8-11      dequantization: codes of 128 keys to f16 K [keys][dims] and V^T [dims][keys] in the
+//                   128-byte swizzle, two buffers each;
+//   warp 12         one thread issues the matrix products: S = Q K^T and O += P V per tile, alternating
+//                   between the tiles so that one tile's softmax runs under the other's products;
+//   warp 13         bulk copies of the pages' K and V halves into rings of 12 slots.
+// A row's maximum is found in a first pass over S; its exponent base moves (O rescaled in TMEM) only when
+// the maximum outgrows it by 2^8, so P <= 2^12.  Each 16 columns' P is stored as soon as it is computed:
+// it covers columns of S that have been read (keeping the row's P in registers instead, to read S once,
+// spilled at 160 registers a thread).
+// Orders: a K chunk of 8 dims keeps its nibble pairs (0,4) (1,5) (2,6) (3,7) and Q is stored in the same
+// order; within a page's upper half the pairs of keys are swapped (key ^ 2), which keeps the V reads of a
+// warp on distinct banks, and the masks follow.
+// Rounding: Q to f16 after a power-of-two scaling of its row (exact for f16, and for bf16 down to 2^-21
+// of the row's largest), K and V to f16, P to f16; sums in f32.
+// Every wait is bounded (tc::mbar_wait); no load uses multicast.
+#include "kv4_common.cuh"
+
+#include <algorithm>
+#include <stdexcept>
+#include <string>
+
+namespace fak {
+namespace {
+
+using kv4::Lay;
+using kv4::PAGE;
+using kv4::Span;
+
+constexpr int ROWS = 128;          // query rows per tile, two tiles a CTA
+constexpr int KEYS = 128;          // keys per step
+constexpr int PPT = KEYS / PAGE;   // pages per step
+constexpr int SLOTS = 12;          // ring slots of page halves
+constexpr int THREADS = 448;
+constexpr float LIFT = 4.f, HEADROOM = 8.f;
+constexpr float LOG2E = 1.4426950408889634f;
+
+template <int D>
+struct Smem {
+  static constexpr int HALF = Lay<D>::VC;          // bytes of a page's K part, and of its V part
+  static constexpr int SLOT_V = HALF + 64;         // (an odd multiple of 64 spreads two pages over the banks)
+  alignas(1024) __half q[2][D / 64][ROWS * 64];    // [tile][64-dim half][row][64]
+  alignas(1024) __half k[2][D / 64][KEYS * 64];    // [buffer][64-dim half][key][64]
+  alignas(1024) __half v[2][2][D * 64];            // [buffer][64-key half][dim][64]
+  alignas(128) uint8_t raw_k[SLOTS][HALF];
+  alignas(128) uint8_t raw_v[SLOTS][SLOT_V];
+  uint64_t q_full, k_full[2], k_empty[2], v_full[2], v_empty[2];
+  uint64_t s_full[2], p_full[2], pv_done[2];
+  uint64_t rk_full[SLOTS], rk_empty[SLOTS], rv_full[SLOTS], rv_empty[SLOTS];
+  uint32_t tmem;
+  int fail;
+};
+
+// f16 operands, f32 accumulator, both K-major
+constexpr uint32_t idesc_f16(int M, int N) { return (1u << 4) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24); }
+
+FAK_DEV void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) { tc::mma_bf16(d, a, b, idesc, acc); }
+FAK_DEV void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(acc)
+      : "memory");
+}
+// waits for this thread's TMEM loads; the operands tie their uses to the wait
+FAK_DEV void ld_wait(uint32_t (&r)[16]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]),
+                 "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])::"memory");
+}
+FAK_DEV void st8(uint32_t taddr, const uint32_t (&r)[8]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr), "r"(r[0]), "r"(r[1]),
+               "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+               : "memory");
+}
+FAK_DEV uint32_t h2_fma(uint32_t a, uint32_t b, uint32_t c) {
+  const __half2 r = __hfma2(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b), *reinterpret_cast<__half2*>(&c));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+FAK_DEV uint32_t h2_add(uint32_t a, uint32_t b) {
+  const __half2 r = __hadd2(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+// The four half2 of a code word, times s plus m.  1024 + c and 1024 + 16 c come from one AND-OR; the
+// subtraction (and the product with 1/16) is exact.
+FAK_DEV void dequant_word(uint32_t w, uint32_t s, uint32_t m, uint32_t (&o)[4]) {
+  constexpr uint32_t BIAS = 0x64006400u;
+  const uint32_t u = w >> 8;
+  o[0] = h2_fma(h2_add((w & 0x000f000fu) | BIAS, 0xe400e400u), s, m);              // - 1024
+  o[1] = h2_fma(h2_fma((w & 0x00f000f0u) | BIAS, 0x2c002c00u, 0xd400d400u), s, m); // / 16 - 64
+  o[2] = h2_fma(h2_add((u & 0x000f000fu) | BIAS, 0xe400e400u), s, m);
+  o[3] = h2_fma(h2_fma((u & 0x00f000f0u) | BIAS, 0x2c002c00u, 0xd400d400u), s, m);
+}
+FAK_DEV uint32_t dup_lo(uint32_t x) { return __byte_perm(x, x, 0x1010); }
+FAK_DEV uint32_t dup_hi(uint32_t x) { return __byte_perm(x, x, 0x3232); }
+
+template <int D, bool CAP>
+__global__ void __launch_bounds__(THREADS, 1)
+k_kv4_prefill(const __grid_constant__ Kv4Attn a, int n_split, int pps) {
+  using L = Lay<D>;
+  constexpr int NG = L::NG;
+  extern __shared__ uint8_t smem_raw[];
+  Smem<D>& sm = *reinterpret_cast<Smem<D>*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int n_blk = gridDim.x / n_split;
+  // blocks with the longest causal range first
+  const int split = blockIdx.x % n_split, blk = n_blk - 1 - (int)(blockIdx.x / n_split), kvh = blockIdx.y, b = blockIdx.z;
+  const int G = a.H / a.Hkv;
+  pdl_wait();
+  const int ctx = min(a.ctx[b], a.width * PAGE);
+  int tok0 = b, n = 1;
+  if (a.q_off) {
+    tok0 = max(a.q_off[b], 0);
+    n = min(a.q_off[b + 1], a.n_tokens) - tok0;
+    if (n > a.max_new) {
+      report_error(a.err, 3);
+      n = a.max_new;
+    }
+  }
+  const int R = n * G, r0 = blk * 2 * ROWS;
+  if (R <= r0) return;
+  const int i_first = r0 / G, i_last = min(R - 1, r0 + 2 * ROWS - 1) / G;
+  const Span sp = kv4::span_of(ctx, n, i_first, i_last, a.window, pps, a.width);
+  const int p_begin = sp.p0 + split * pps, p_end = min(sp.p1, p_begin + pps);
+  if (p_begin >= p_end && !(split == 0 && sp.live == 0)) return;
+  const int n_pages = max(0, p_end - p_begin);
+  const int NJ = (n_pages + PPT - 1) / PPT;
+  const int tiles = R - r0 > ROWS ? 2 : 1;
+  const int lim_any = ctx - n + i_last + 1;                                            // keys some row sees: below
+  const int low_any = a.window > 0 ? max(0, ctx - n + i_first + 1 - a.window) : 0;     // and from here
+
+  if (threadIdx.x == 0) {
+    tc::mbar_init(&sm.q_full, 4 * tiles);
+    for (int i = 0; i < 2; i++) {
+      tc::mbar_init(&sm.k_full[i], 4);
+      tc::mbar_init(&sm.k_empty[i], 1);
+      tc::mbar_init(&sm.v_full[i], 4);
+      tc::mbar_init(&sm.v_empty[i], 1);
+      tc::mbar_init(&sm.s_full[i], 1);
+      tc::mbar_init(&sm.p_full[i], 4);
+      tc::mbar_init(&sm.pv_done[i], 1);
+    }
+    for (int i = 0; i < SLOTS; i++) {
+      tc::mbar_init(&sm.rk_full[i], 1);
+      tc::mbar_init(&sm.rk_empty[i], 1);
+      tc::mbar_init(&sm.rv_full[i], 1);
+      tc::mbar_init(&sm.rv_empty[i], 1);
+    }
+    sm.fail = 0;
+    tc::fence_mbar_init();
+  }
+  if (warp == 12) {
+    tc::tmem_alloc(&sm.tmem, 512);   // S0 [0, 128) S1 [128, 256) O0 [256, 256 + D) O1 [256 + D, 256 + 2 D)
+    tc::tmem_relinquish();
+  }
+  tc::tc_fence_before();
+  __syncthreads();
+  tc::tc_fence_after();
+  const uint32_t tmem = sm.tmem;
+  int* fail = &sm.fail;
+
+  if (warp >= 12) {
+    if (warp == 13) {
+      // ---- page loader: lane l holds the address of page 32 i + l
+      const int* table = a.table + (int64_t)b * a.table_stride + p_begin;
+      const uint8_t* src = nullptr;
+      for (int i = 0; i < n_pages; i++) {
+        if ((i & 31) == 0 && i + lane < n_pages) {
+          int pid = table[i + lane];
+          if ((unsigned)pid >= (uint64_t)a.n_pages) {
+            report_error(a.err, 2);
+            pid = 0;
+          }
+          src = a.pages + ((int64_t)pid * a.Hkv + kvh) * L::BYTES;
+        }
+        const int s = i % SLOTS;
+        const uint32_t free_parity = (uint32_t)((i / SLOTS) & 1) ^ 1u;
+        if (lane == (i & 31)) {
+          tc::mbar_wait(&sm.rk_empty[s], free_parity, fail);
+          tc::mbar_arrive_expect_tx(&sm.rk_full[s], Smem<D>::HALF);
+          kv4::bulk_load(sm.raw_k[s], src, Smem<D>::HALF, &sm.rk_full[s]);
+          tc::mbar_wait(&sm.rv_empty[s], free_parity, fail);
+          tc::mbar_arrive_expect_tx(&sm.rv_full[s], Smem<D>::HALF);
+          kv4::bulk_load(sm.raw_v[s], src + L::VC, Smem<D>::HALF, &sm.rv_full[s]);
+        }
+        __syncwarp();
+      }
+    } else if (warp == 12) {
+      // ---- matrix products
+      if (lane == 0 && NJ > 0) {
+        constexpr uint32_t id_s = idesc_f16(ROWS, KEYS), id_o = idesc_f16(ROWS, D);
+        auto issue_s = [&](int t, int j) {
+          const int kb = j & 1;
+          if (t == 0) tc::mbar_wait(&sm.k_full[kb], (uint32_t)((j >> 1) & 1), fail);
+          // P of the step before sits in S's columns until its product is done
+          if (j > 0) tc::mbar_wait(&sm.pv_done[t], (uint32_t)((j - 1) & 1), fail);
+          tc::tc_fence_after();
+#pragma unroll
+          for (int hd = 0; hd < D / 64; hd++) {
+            const uint64_t ad = tc::smem_desc_sw128(sm.q[t][hd]), bd = tc::smem_desc_sw128(sm.k[kb][hd]);
+#pragma unroll
+            for (int kk = 0; kk < 4; kk++) mma_ss(tmem + t * 128, ad + 2 * kk, bd + 2 * kk, id_s, (hd | kk) != 0);
+          }
+          tc::mma_commit(&sm.s_full[t]);
+          if (t == tiles - 1) tc::mma_commit(&sm.k_empty[kb]);
+        };
+        tc::mbar_wait(&sm.q_full, 0, fail);
+        for (int t = 0; t < tiles; t++) issue_s(t, 0);
+        for (int j = 0; j < NJ; j++) {
+          const int vb = j & 1;
+          for (int t = 0; t < tiles; t++) {
+            if (t == 0) tc::mbar_wait(&sm.v_full[vb], (uint32_t)((j >> 1) & 1), fail);
+            tc::mbar_wait(&sm.p_full[t], (uint32_t)(j & 1), fail);
+            tc::tc_fence_after();
+#pragma unroll
+            for (int ks = 0; ks < KEYS / 16; ks++) {
+              const uint64_t bd = tc::smem_desc_sw128(sm.v[vb][ks >> 2]) + 2 * (ks & 3);
+              mma_ts(tmem + 256 + t * D, tmem + t * 128 + ks * 8, bd, id_o, (j > 0 || ks > 0) ? 1u : 0u);
+            }
+            tc::mma_commit(&sm.pv_done[t]);
+            if (t == tiles - 1) tc::mma_commit(&sm.v_empty[vb]);
+            if (j + 1 < NJ) issue_s(t, j + 1);
+          }
+        }
+    }
+    }
+  } else if (warp >= 8) {
+    // ---- dequantization: this warp's two pages of every step
+    const int w = warp - 8;
+    // K lanes: (token bits 0, 1, 2; t); V lanes: (g, half of the page, page of the pair)
+    const int kt = lane & 3, ktok = ((lane >> 2) & 1) * 4 + (lane >> 3);
+    const int vg = (lane & 1) | (lane >> 3) << 1, vh = (lane >> 1) & 1, vp = (lane >> 2) & 1;
+    for (int j = 0; j < NJ; j++) {
+      const int buf = j & 1;
+      const uint32_t free_parity = (uint32_t)((j >> 1) & 1) ^ 1u;
+      tc::mbar_wait(&sm.k_empty[buf], free_parity, fail);
+#pragma unroll
+      for (int u = 0; u < 2; u++) {
+        const int i = j * PPT + 2 * w + u, s = i % SLOTS;
+        if (i < n_pages) {   // (rows of pages that do not exist are masked in S)
+          tc::mbar_wait(&sm.rk_full[s], (uint32_t)((i / SLOTS) & 1), fail);
+          const uint8_t* pg = sm.raw_k[s];
+#pragma unroll
+          for (int hf = 0; hf < 2; hf++) {
+            const int tok = hf * 8 + ktok;
+            uint32_t c[NG], sc[NG / 2], mn[NG / 2];
+            kv4::lds(pg + L::KC + tok * (D / 2) + kt * 4 * NG, c);
+            kv4::lds(pg + L::KS + tok * 2 * NG, sc);
+            kv4::lds(pg + L::KM + tok * 2 * NG, mn);
+            const int row = (2 * w + u) * PAGE + (tok ^ (hf * 2));
+#pragma unroll
+            for (int gr = 0; gr < NG; gr++) {
+              uint32_t o[4];
+              dequant_word(c[gr], gr & 1 ? dup_hi(sc[gr / 2]) : dup_lo(sc[gr / 2]), gr & 1 ? dup_hi(mn[gr / 2]) : dup_lo(mn[gr / 2]), o);
+              uint8_t* dst = reinterpret_cast<uint8_t*>(sm.k[buf][gr >> 1]) + row * 128 + ((((gr & 1) * 4 + kt) ^ (row & 7)) << 4);
+              *reinterpret_cast<uint4*>(dst) = make_uint4(o[0], o[1], o[2], o[3]);
+            }
+          }
+          __syncwarp();
+          if (lane == 0) tc::mbar_arrive(&sm.rk_empty[s]);
+        }
+      }
+      tc::fence_proxy_async();
+      __syncwarp();
+      if (lane == 0) tc::mbar_arrive(&sm.k_full[buf]);
+
+      tc::mbar_wait(&sm.v_empty[buf], free_parity, fail);
+      const int i0 = j * PPT + 2 * w, i = i0 + vp, s = i % SLOTS;
+      if (i0 < n_pages) tc::mbar_wait(&sm.rv_full[i0 % SLOTS], (uint32_t)((i0 / SLOTS) & 1), fail);
+      if (i0 + 1 < n_pages) tc::mbar_wait(&sm.rv_full[(i0 + 1) % SLOTS], (uint32_t)(((i0 + 1) / SLOTS) & 1), fail);
+      uint32_t c[4][NG], sc[4][NG], mn[4][NG];
+      const uint8_t* pg = sm.raw_v[s];   // (offsets of the layout count from the page's start)
+      const int key0 = (p_begin + i) * PAGE;
+#pragma unroll
+      for (int e = 0; e < 4; e++) {
+        const int p = vh * 4 + (e ^ vh);
+        kv4::lds(pg + ((p * 8 + (vg ^ (2 * (p & 3)))) * NG) * 4, c[e]);
+        kv4::lds(pg + L::VS - L::VC + p * NG * 4, sc[e]);
+        kv4::lds(pg + L::VM - L::VC + p * NG * 4, mn[e]);
+      }
+      const int step0 = (p_begin + j * PPT) * PAGE;
+      if (step0 < low_any || step0 + KEYS > min(lim_any, p_end * PAGE)) {
+        // tokens no row sees (memory nobody wrote, pages that do not exist): zero
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          const int key = key0 + 2 * (vh * 4 + (e ^ vh));
+          const uint32_t keep = (i < n_pages && key >= low_any && key < lim_any ? 0x0000ffffu : 0u) |
+                                (i < n_pages && key + 1 >= low_any && key + 1 < lim_any ? 0xffff0000u : 0u);
+#pragma unroll
+          for (int gr = 0; gr < NG; gr++) {
+            sc[e][gr] &= keep;
+            mn[e][gr] &= keep;
+          }
+        }
+      }
+      const int pos = 2 * w + vp, chunk = (pos & 3) * 2 + vh;
+#pragma unroll
+      for (int gr = 0; gr < NG; gr++) {
+        uint32_t o[4][4];
+#pragma unroll
+        for (int e = 0; e < 4; e++) dequant_word(c[e][gr], sc[e][gr], mn[e][gr], o[e]);
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          const int d = gr * 32 + 4 * vg + e;
+          uint8_t* dst = reinterpret_cast<uint8_t*>(sm.v[buf][pos >> 2]) + d * 128 + ((chunk ^ (d & 7)) << 4);
+          *reinterpret_cast<uint4*>(dst) = make_uint4(o[0][e], o[1][e], o[2][e], o[3][e]);
+        }
+      }
+      tc::fence_proxy_async();
+      __syncwarp();
+      if (lane == 0) {
+        if (i0 < n_pages) tc::mbar_arrive(&sm.rv_empty[i0 % SLOTS]);
+        if (i0 + 1 < n_pages) tc::mbar_arrive(&sm.rv_empty[(i0 + 1) % SLOTS]);
+        tc::mbar_arrive(&sm.v_full[buf]);
+      }
+    }
+  } else if ((warp >> 2) < tiles) {
+    // ---- softmax of tile t, one row a thread
+    const int t = warp >> 2, quarter = warp & 3, row = quarter * 32 + lane;
+    const int rr = r0 + t * ROWS + row;
+    const bool live = rr < R;
+    const int qi = live ? rr / G : 0, h = kvh * G + (live ? rr % G : 0);
+    float cf;
+    {
+      // the row to f16, its largest value scaled into [2^7, 2^8)
+      const int64_t at = (int64_t)(tok0 + qi) * a.q_tok + (int64_t)h * a.q_head;
+      const bool packed = a.q_vec && a.q_type != Elt::F32;
+      auto load8 = [&](int c, float (&x)[8]) {
+        if (!live) {
+#pragma unroll
+          for (int e = 0; e < 8; e++) x[e] = 0.f;
+        } else if (packed) {
+          const uint4 u = *reinterpret_cast<const uint4*>((const uint16_t*)a.q + at + 8 * c);
+          const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+          for (int e = 0; e < 4; e++) {
+            const float2 y = kv4::unpack_h2(w[e]);
+            x[2 * e] = a.q_type == Elt::F16 ? y.x : bf16_bits_lo(w[e]);
+            x[2 * e + 1] = a.q_type == Elt::F16 ? y.y : bf16_bits_hi(w[e]);
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; e++) x[e] = kv4::load_elt(a.q, a.q_type, at + 8 * c + e);
+        }
+      };
+      float amax = 0.f;   // (the row is read twice, the second time out of L1)
+#pragma unroll 4
+      for (int c = 0; c < D / 8; c++) {
+        float x[8];
+        load8(c, x);
+#pragma unroll
+        for (int e = 0; e < 8; e++) amax = fmaxf(amax, fabsf(x[e]));
+      }
+      const int ex = (int)(__float_as_uint(amax) >> 23);
+      const float f = __uint_as_float((uint32_t)(ex == 255 ? 127 : max(1, min(127 + 126, 127 + 7 + 127 - ex))) << 23);
+#pragma unroll 4
+      for (int c = 0; c < D / 8; c++) {
+        float x[8];
+        load8(c, x);
+        uint8_t* dst = reinterpret_cast<uint8_t*>(sm.q[t][c >> 3]) + row * 128 + (((c & 7) ^ (row & 7)) << 4);
+        *reinterpret_cast<uint4*>(dst) = make_uint4(kv4::pack_f16(x[0] * f, x[4] * f), kv4::pack_f16(x[1] * f, x[5] * f),
+                                                    kv4::pack_f16(x[2] * f, x[6] * f), kv4::pack_f16(x[3] * f, x[7] * f));
+      }
+      cf = a.scale / f * (CAP ? 1.f : LOG2E);
+      tc::fence_proxy_async();
+      __syncwarp();
+      if (lane == 0) tc::mbar_arrive(&sm.q_full);
+    }
+    const float cap_in = CAP ? 1.f / a.softcap : 0.f, cap_out = CAP ? a.softcap * LOG2E : 0.f;
+    const int lim = live ? min(ctx - n + qi + 1, ctx) : 0;
+    const int low = a.window > 0 ? max(0, lim - a.window) : 0;
+    // keys every live row of the warp sees
+    int lim_min = live ? lim : INT_MAX, low_max = low;
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) {
+      lim_min = min(lim_min, __shfl_xor_sync(0xffffffffu, lim_min, d));
+      low_max = max(low_max, __shfl_xor_sync(0xffffffffu, low_max, d));
+    }
+    const uint32_t ts = tmem + ((uint32_t)(quarter * 32) << 16) + t * 128;
+    const uint32_t to = tmem + ((uint32_t)(quarter * 32) << 16) + 256 + t * D;
+    float base = -INFINITY, l = 0.f;
+    for (int j = 0; j < NJ; j++) {
+      const int key0 = (p_begin + j * PPT) * PAGE;
+      const bool whole = key0 >= low_max && key0 + KEYS <= lim_min;
+      tc::mbar_wait(&sm.s_full[t], (uint32_t)(j & 1), fail);
+      tc::tc_fence_after();
+      // 16 logits of the row: scaled (CAP: final log2 logits, scale 1), masked
+      auto logits = [&](const uint32_t (&r)[16], int c, float (&x)[16]) {
+#pragma unroll
+        for (int e = 0; e < 16; e++) {
+          x[e] = __uint_as_float(r[e]);
+          if constexpr (CAP) x[e] = cap_out * tanhf(x[e] * cf * cap_in);
+          if (!whole) {
+            const int key = key0 + c * 16 + (e ^ ((e & 8) >> 2));
+            if (key < low || key >= lim) x[e] = -INFINITY;
+          }
+        }
+      };
+      const float mul = CAP ? 1.f : cf;
+      uint32_t r[2][16];
+      float m4[2] = {-INFINITY, -INFINITY};
+      tc::tmem_ld16(ts, r[0]);
+#pragma unroll
+      for (int c = 0; c < 8; c++) {
+        ld_wait(r[c & 1]);
+        if (c < 7) tc::tmem_ld16(ts + (c + 1) * 16, r[(c + 1) & 1]);
+        float x[16];
+        logits(r[c & 1], c, x);
+#pragma unroll
+        for (int e = 0; e < 16; e += 2) m4[(e >> 1) & 1] = fmaxf(m4[(e >> 1) & 1], fmaxf(x[e], x[e + 1]));
+      }
+      const float mx = fmaxf(m4[0], m4[1]) * mul;
+      tc::tmem_ld16(ts, r[0]);
+      if (__any_sync(0xffffffffu, mx > base + HEADROOM)) {
+        // some row outgrew its base: every row of the warp moves to its maximum and O is rescaled (the
+        // product of the step before is done: S of this one was issued after it)
+        const float nw = fmaxf(base, mx), f = nw == -INFINITY ? 1.f : kv4::ex2(base - nw);
+        if (j > 0) {
+#pragma unroll 1
+          for (int c = 0; c < D / 16; c++) {
+            uint32_t o[16];
+            tc::tmem_ld16(to + c * 16, o);
+            ld_wait(o);
+#pragma unroll
+            for (int e = 0; e < 16; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+            tc::tmem_st16(to + c * 16, o);
+          }
+          tc::tmem_st_wait();
+        }
+        l *= f;
+        base = nw;
+      }
+      const float nb = base == -INFINITY ? 0.f : LIFT - base;
+      float s4[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int c = 0; c < 8; c++) {
+        ld_wait(r[c & 1]);
+        if (c < 7) tc::tmem_ld16(ts + (c + 1) * 16, r[(c + 1) & 1]);
+        float x[16];
+        logits(r[c & 1], c, x);
+        uint32_t pk[8];
+#pragma unroll
+        for (int e = 0; e < 16; e += 2) {
+          const float p0 = kv4::ex2(fmaf(x[e], mul, nb)), p1 = kv4::ex2(fmaf(x[e + 1], mul, nb));
+          s4[(e >> 1) & 3] += p0 + p1;
+          pk[e >> 1] = kv4::pack_f16(p0, p1);
+        }
+        st8(ts + c * 8, pk);
+      }
+      l += (s4[0] + s4[1]) + (s4[2] + s4[3]);
+      tc::tmem_st_wait();
+      tc::tc_fence_before();
+      __syncwarp();
+      if (lane == 0) tc::mbar_arrive(&sm.p_full[t]);
+    }
+    // ---- output
+    const bool alone = n_split == 1;
+    if (NJ > 0) {
+      tc::mbar_wait(&sm.pv_done[t], (uint32_t)((NJ - 1) & 1), fail);
+      tc::tc_fence_after();
+    }
+    const float sink = alone && a.sinks ? a.sinks[h] * LOG2E : -INFINITY;
+    float f = 1.f;
+    if (alone) {
+      const float top = fmaxf(base, sink);
+      if (sink > -INFINITY) {
+        f = base == -INFINITY ? 0.f : kv4::ex2(base - top);
+        l = l * f + kv4::ex2(sink - top + LIFT);
+      }
+      f = l != 0.f ? f / l : 0.f;
+    }
+    const int64_t part_row = ((((int64_t)b * a.Hkv + kvh) * n_blk + blk) * (2 * ROWS) + t * ROWS + row) * n_split + split;
+    const int64_t at = (int64_t)(tok0 + qi) * a.o_tok + (int64_t)h * a.o_head;
+#pragma unroll 1
+    for (int c = 0; c < D / 16; c++) {
+      uint32_t o[16];
+      if (NJ > 0) {
+        tc::tmem_ld16(to + c * 16, o);
+        ld_wait(o);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 16; e++) o[e] = 0;
+      }
+      if (live && alone) {
+        if (a.o_vec) {
+          uint32_t y[8];
+#pragma unroll
+          for (int e = 0; e < 8; e++) {
+            const float y0 = __uint_as_float(o[2 * e]) * f, y1 = __uint_as_float(o[2 * e + 1]) * f;
+            y[e] = a.o_type == Elt::F16 ? kv4::pack_f16(y0, y1) : kv4::pack_bf16x2(y0, y1);
+          }
+          uint4* dst = reinterpret_cast<uint4*>((uint16_t*)a.out + at + c * 16);
+          dst[0] = make_uint4(y[0], y[1], y[2], y[3]);
+          dst[1] = make_uint4(y[4], y[5], y[6], y[7]);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 16; e++) kv4::store_elt(a.out, a.o_type, at + c * 16 + e, __uint_as_float(o[e]) * f);
+        }
+      } else if (live) {
+        float4* dst = reinterpret_cast<float4*>(a.part + part_row * D + c * 16);
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+          dst[e] = make_float4(__uint_as_float(o[4 * e]), __uint_as_float(o[4 * e + 1]), __uint_as_float(o[4 * e + 2]), __uint_as_float(o[4 * e + 3]));
+      }
+      __syncwarp();
+    }
+    if (!alone && live) {
+      float* ml = a.part + (int64_t)gridDim.z * gridDim.y * n_blk * (2 * ROWS) * n_split * D + part_row * 2;
+      ml[0] = base;
+      ml[1] = l;
+    }
+    tc::tc_fence_before();
+  }
+  pdl_launch_dependents();
+  __syncthreads();
+  if (threadIdx.x == 0 && sm.fail) report_error(a.err, 1);
+  if (warp == 12) {
+    tc::tc_fence_after();
+    tc::tmem_dealloc(tmem, 512);
+  }
+}
+
+}  // namespace
+
+void kv4_prefill_launch(const Kv4Attn& a, const Kv4AttnPlan& p, cudaStream_t stream) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(p.n_split * p.row_chunks), (unsigned)a.Hkv, (unsigned)a.B);
+  cfg.blockDim = dim3(THREADS);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = pdl_allowed();
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  auto go = [&](auto kern, size_t smem) {
+    cfg.dynamicSmemBytes = smem + 1024;
+    FAK_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)cfg.dynamicSmemBytes));
+    FAK_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kern, a, p.n_split, p.pps));
+  };
+  const bool cap = a.softcap > 0.f;
+  if (a.D == 128 && cap) go(k_kv4_prefill<128, true>, sizeof(Smem<128>));
+  else if (a.D == 128) go(k_kv4_prefill<128, false>, sizeof(Smem<128>));
+  else if (cap) go(k_kv4_prefill<64, true>, sizeof(Smem<64>));
+  else go(k_kv4_prefill<64, false>, sizeof(Smem<64>));
+}
+
+}  // namespace fak

@@ -16,6 +16,7 @@
 // merges them in segment order, so results do not depend on the order of arrival.
 #include "common.cuh"
 
+#include <algorithm>
 #include <stdexcept>
 #include <string>
 
@@ -82,23 +83,34 @@ FAK_DEV Stat join(const Stat& a, const Stat& b) {
 template <typename T>
 constexpr int VEC = 16 / sizeof(T);
 template <typename T>
-FAK_DEV void load16(const T* __restrict__ p, int i0, int end, bool vec, float (&x)[PER]) {
-  constexpr int E = VEC<T>;
+struct Tile16 {
+  static constexpr int E = VEC<T>;
+  uint4 u[PER / E];
+  // logits past `end` read as -inf
+  FAK_DEV void load(const T* __restrict__ p, int i0, int end, bool vec) {
 #pragma unroll
-  for (int j = 0; j < PER / E; j++) {
-    const int i = i0 + j * 32 * E;
-    if (vec && i + E <= end) {
-      const uint4 u = __ldcs(reinterpret_cast<const uint4*>(p + i));
-      T h[E];
-      memcpy(h, &u, 16);
+    for (int j = 0; j < PER / E; j++) {
+      const int i = i0 + j * 32 * E;
+      if (vec && i + E <= end) {
+        u[j] = __ldcs(reinterpret_cast<const uint4*>(p + i));
+      } else {
+        T h[E];
 #pragma unroll
-      for (int e = 0; e < E; e++) x[j * E + e] = (float)h[e];
-    } else {
-#pragma unroll
-      for (int e = 0; e < E; e++) x[j * E + e] = i + e < end ? (float)p[i + e] : -INFINITY;
+        for (int e = 0; e < E; e++) h[e] = i + e < end ? p[i + e] : (T)-INFINITY;
+        memcpy(&u[j], h, 16);
+      }
     }
   }
-}
+  FAK_DEV void values(float (&x)[PER]) const {
+#pragma unroll
+    for (int j = 0; j < PER / E; j++) {
+      T h[E];
+      memcpy(h, &u[j], 16);
+#pragma unroll
+      for (int e = 0; e < E; e++) x[j * E + e] = (float)h[e];
+    }
+  }
+};
 template <typename T>
 FAK_DEV int elt_at(int e) { return e % VEC<T> + e / VEC<T> * 32 * VEC<T>; }
 FAK_DEV float ex2(float x) {   // 2^x, results below 2^-126 are zero
@@ -132,7 +144,6 @@ __global__ void __launch_bounds__(THREADS) k_logprobs(LogprobArgs a, int seg_len
   auto cap = [&](float v) { return CAP ? a.softcap * tanhf(v / a.softcap) : v; };
   const int tgt = a.target[r];
   const bool given = tgt >= 0 && tgt < a.V;
-  const float xt = given ? cap((float)x[tgt]) : INFINITY;
   const int i_begin = seg * seg_len, i_end = min(a.V, i_begin + seg_len);
 
   Stat st = {-INFINITY, 0.f, 0.f};
@@ -143,10 +154,14 @@ __global__ void __launch_bounds__(THREADS) k_logprobs(LogprobArgs a, int seg_len
   bool first = true;
   const int k = a.k;
 
+  Tile16<T> next;   // the loads of the following tile are in flight while one is worked on
+  if (i_begin + warp * TILE < i_end) next.load(x, i_begin + warp * TILE + VEC<T> * lane, i_end, a.vec);
+  const float xt = given ? cap((float)x[tgt]) : INFINITY;
   for (int base = i_begin + warp * TILE; base < i_end; base += WARPS * TILE) {
     float v[PER];
     const int i0 = base + VEC<T> * lane;
-    load16(x, i0, i_end, a.vec, v);
+    next.values(v);
+    if (base + WARPS * TILE < i_end) next.load(x, i0 + WARPS * TILE, i_end, a.vec);
     float mx = -INFINITY;
 #pragma unroll
     for (int e = 0; e < PER; e++) {

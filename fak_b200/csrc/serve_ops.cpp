@@ -151,6 +151,7 @@ void kv4_attention(Tensor q, Tensor pages, Tensor table, OptTensor q_off, Tensor
   a.o_type = elt(out, "kv4_attention: out");
   a.o_tok = out.stride(0);
   a.o_head = out.stride(1);
+  a.o_vec = out.element_size() == 2 && reinterpret_cast<uintptr_t>(a.out) % 16 == 0 && a.o_tok % 8 == 0 && a.o_head % 8 == 0;
   a.pages = pages.data_ptr<uint8_t>();
   a.n_pages = pages.size(0);
   a.table = table.data_ptr<int>();

@@ -37,6 +37,7 @@ struct Kv4Attn {
   void* out;                 // [T, H, D], row strides o_tok, o_head
   int64_t o_tok, o_head;
   Elt o_type;
+  bool o_vec;                // 16-bit rows that start on 16 bytes
   float scale, softcap;
   int window;
   const float* sinks;        // [H] or null
@@ -45,10 +46,12 @@ struct Kv4Attn {
   int* err;
 };
 struct Kv4AttnPlan {
+  bool tc;
   int nt, row_chunks, n_split, pps;
   int64_t part_floats;
 };
 Kv4AttnPlan kv4_attn_plan(const Kv4Attn& a, int n_sm);
+void kv4_prefill_launch(const Kv4Attn& a, const Kv4AttnPlan& p, cudaStream_t stream);
 void kv4_attn_launch(const Kv4Attn& a, const Kv4AttnPlan& p, cudaStream_t stream);
 
 struct BatchPlanArgs {
