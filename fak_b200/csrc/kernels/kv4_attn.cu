@@ -63,10 +63,6 @@ FAK_DEV uint32_t movmatrix(uint32_t a) {
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(a));
   return r;
 }
-FAK_DEV uint32_t mul_h2(uint32_t a, uint32_t b) {
-  const __half2 h = __hmul2(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b));
-  return *reinterpret_cast<const uint32_t*>(&h);
-}
 template <int D, int NT>
 struct Smem {
   static constexpr int COLS = 8 * NT;
@@ -295,6 +291,7 @@ k_kv4_attn(const __grid_constant__ Kv4Attn a, int n_split, int pps) {
         }
     }
     if (!whole) {
+      asm volatile("");   // a branch, not predicated work on every page
 #pragma unroll
       for (int nt = 0; nt < NT; nt++)
 #pragma unroll
@@ -309,6 +306,7 @@ k_kv4_attn(const __grid_constant__ Kv4Attn a, int n_split, int pps) {
 #pragma unroll
       for (int e = 0; e < 4; e++) grow |= z[nt][e] > base[nt][e & 1] + HEADROOM;
     if (__any_sync(0xffffffffu, grow)) {
+      asm volatile("");
 #pragma unroll
       for (int nt = 0; nt < NT; nt++)
 #pragma unroll
@@ -355,6 +353,7 @@ k_kv4_attn(const __grid_constant__ Kv4Attn a, int n_split, int pps) {
         m0 = m1 = 0x3c003c00u;
       }
       if (!whole) {
+        asm volatile("");
         // tokens no row sees: whatever their bytes hold (memory nobody wrote) must not reach the sums
         auto keep = [&](int tok) {
           const bool lo_ok = key0 + tok >= low_any && key0 + tok < lim_any;
@@ -536,11 +535,12 @@ Kv4AttnPlan kv4_attn_plan(const Kv4Attn& a, int n_sm) {
   const int nt_most = a.D == 64 ? 4 : 2;
   p.tc = rows > kPrefillRows;
   if (p.tc) {
-    // 256 rows a CTA, one CTA a SM: keys are split until every SM has one, eight steps a split at least
+    // 256 rows a CTA, one CTA a SM: with fewer CTAs than SMs the keys are split, eight steps a split at least
     p.row_chunks = (int)((rows + 255) / 256);
     const int64_t ctas = (int64_t)a.B * a.Hkv * p.row_chunks;
-    int64_t pps = a.n_split > 0 ? (a.width + a.n_split - 1) / a.n_split : std::max<int64_t>(64, (a.width * ctas + n_sm - 1) / n_sm);
-    pps = std::min<int64_t>((pps + 7) / 8 * 8, (a.width + 7) / 8 * 8);
+    const int64_t want = a.n_split > 0 ? a.n_split : std::min<int64_t>(n_sm / ctas, a.width / 64);
+    int64_t pps = (a.width + std::max<int64_t>(want, 1) - 1) / std::max<int64_t>(want, 1);
+    pps = (pps + 7) / 8 * 8;
     p.pps = (int)pps;
     p.n_split = (int)((a.width + pps - 1) / pps);
     p.part_floats = p.n_split > 1 ? ctas * 256 * p.n_split * (a.D + 2) : 0;

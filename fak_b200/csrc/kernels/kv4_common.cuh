@@ -16,6 +16,10 @@ FAK_DEV uint32_t pack_bf16x2(float lo, float hi) {
   const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&v);
 }
+FAK_DEV uint32_t mul_h2(uint32_t a, uint32_t b) {
+  const __half2 h = __hmul2(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
 FAK_DEV float2 unpack_h2(uint32_t a) { return __half22float2(*reinterpret_cast<__half2*>(&a)); }
 FAK_DEV float ex2(float x) {
   float y;

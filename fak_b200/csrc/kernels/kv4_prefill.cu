@@ -10,10 +10,11 @@
 //   warp 12         one thread issues the matrix products: S = Q K^T and O += P V per tile, alternating
 //                   between the tiles so that one tile's softmax runs under the other's products;
 //   warp 13         bulk copies of the pages' K and V halves into rings of 12 slots.
-// A row's maximum is found in a first pass over S; its exponent base moves (O rescaled in TMEM) only when
-// the maximum outgrows it by 2^8, so P <= 2^12.  Each 16 columns' P is stored as soon as it is computed:
-// it covers columns of S that have been read (keeping the row's P in registers instead, to read S once,
-// spilled at 160 registers a thread).
+// A row's exponent base is a whole number that moves only when 32 columns' maximum outgrows it by 2^8 (then
+// O, and what P of the step is stored already, are scaled by an exact power of two), so P <= 2^12 and S is
+// read once.  Steps that need a mask or a soft-cap are rewritten in TMEM by a small loop first: the main
+// loop then has one form, which matters because four roles' code shares the instruction caches (with the
+// mask inside the unrolled loops, waits for instructions were the first stall and a step took 12.6k cycles).
 // Orders: a K chunk of 8 dims keeps its nibble pairs (0,4) (1,5) (2,6) (3,7) and Q is stored in the same
 // order; within a page's upper half the pairs of keys are swapped (key ^ 2), which keeps the V reads of a
 // warp on distinct banks, and the masks follow.
@@ -73,10 +74,23 @@ FAK_DEV void ld_wait(uint32_t (&r)[16]) {
                : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]),
                  "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])::"memory");
 }
-FAK_DEV void st8(uint32_t taddr, const uint32_t (&r)[8]) {
-  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr), "r"(r[0]), "r"(r[1]),
-               "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
-               : "memory");
+FAK_DEV void ld32(uint32_t taddr, uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,"
+      "%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]),
+        "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]),
+        "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr));
+}
+FAK_DEV void ld_wait(uint32_t (&r)[32]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]),
+                 "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]),
+                 "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]), "+r"(r[24]),
+                 "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28])::"memory");
+  asm volatile("" : "+r"(r[29]), "+r"(r[30]), "+r"(r[31]));
 }
 FAK_DEV uint32_t h2_fma(uint32_t a, uint32_t b, uint32_t c) {
   const __half2 r = __hfma2(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b), *reinterpret_cast<__half2*>(&c));
@@ -107,9 +121,9 @@ k_kv4_prefill(const __grid_constant__ Kv4Attn a, int n_split, int pps) {
   extern __shared__ uint8_t smem_raw[];
   Smem<D>& sm = *reinterpret_cast<Smem<D>*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int n_blk = gridDim.x / n_split;
+  const int n_blk = gridDim.y;
   // blocks with the longest causal range first
-  const int split = blockIdx.x % n_split, blk = n_blk - 1 - (int)(blockIdx.x / n_split), kvh = blockIdx.y, b = blockIdx.z;
+  const int split = blockIdx.x % n_split, kvh = blockIdx.x / n_split, blk = n_blk - 1 - (int)blockIdx.y, b = blockIdx.z;
   const int G = a.H / a.Hkv;
   pdl_wait();
   const int ctx = min(a.ctx[b], a.width * PAGE);
@@ -239,13 +253,13 @@ k_kv4_prefill(const __grid_constant__ Kv4Attn a, int n_split, int pps) {
       const int buf = j & 1;
       const uint32_t free_parity = (uint32_t)((j >> 1) & 1) ^ 1u;
       tc::mbar_wait(&sm.k_empty[buf], free_parity, fail);
-#pragma unroll
+#pragma unroll 1
       for (int u = 0; u < 2; u++) {
         const int i = j * PPT + 2 * w + u, s = i % SLOTS;
         if (i < n_pages) {   // (rows of pages that do not exist are masked in S)
           tc::mbar_wait(&sm.rk_full[s], (uint32_t)((i / SLOTS) & 1), fail);
           const uint8_t* pg = sm.raw_k[s];
-#pragma unroll
+#pragma unroll 1
           for (int hf = 0; hf < 2; hf++) {
             const int tok = hf * 8 + ktok;
             uint32_t c[NG], sc[NG / 2], mn[NG / 2];
@@ -386,71 +400,75 @@ k_kv4_prefill(const __grid_constant__ Kv4Attn a, int n_split, int pps) {
     float base = -INFINITY, l = 0.f;
     for (int j = 0; j < NJ; j++) {
       const int key0 = (p_begin + j * PPT) * PAGE;
-      const bool whole = key0 >= low_max && key0 + KEYS <= lim_min;
       tc::mbar_wait(&sm.s_full[t], (uint32_t)(j & 1), fail);
       tc::tc_fence_after();
-      // 16 logits of the row: scaled (CAP: final log2 logits, scale 1), masked
-      auto logits = [&](const uint32_t (&r)[16], int c, float (&x)[16]) {
-#pragma unroll
-        for (int e = 0; e < 16; e++) {
-          x[e] = __uint_as_float(r[e]);
-          if constexpr (CAP) x[e] = cap_out * tanhf(x[e] * cf * cap_in);
-          if (!whole) {
-            const int key = key0 + c * 16 + (e ^ ((e & 8) >> 2));
-            if (key < low || key >= lim) x[e] = -INFINITY;
-          }
-        }
-      };
-      const float mul = CAP ? 1.f : cf;
-      uint32_t r[2][16];
-      float m4[2] = {-INFINITY, -INFINITY};
-      tc::tmem_ld16(ts, r[0]);
-#pragma unroll
-      for (int c = 0; c < 8; c++) {
-        ld_wait(r[c & 1]);
-        if (c < 7) tc::tmem_ld16(ts + (c + 1) * 16, r[(c + 1) & 1]);
-        float x[16];
-        logits(r[c & 1], c, x);
-#pragma unroll
-        for (int e = 0; e < 16; e += 2) m4[(e >> 1) & 1] = fmaxf(m4[(e >> 1) & 1], fmaxf(x[e], x[e + 1]));
-      }
-      const float mx = fmaxf(m4[0], m4[1]) * mul;
-      tc::tmem_ld16(ts, r[0]);
-      if (__any_sync(0xffffffffu, mx > base + HEADROOM)) {
-        // some row outgrew its base: every row of the warp moves to its maximum and O is rescaled (the
-        // product of the step before is done: S of this one was issued after it)
-        const float nw = fmaxf(base, mx), f = nw == -INFINITY ? 1.f : kv4::ex2(base - nw);
-        if (j > 0) {
+      if (CAP || key0 < low_max || key0 + KEYS > lim_min) {
 #pragma unroll 1
-          for (int c = 0; c < D / 16; c++) {
-            uint32_t o[16];
-            tc::tmem_ld16(to + c * 16, o);
-            ld_wait(o);
+        for (int c = 0; c < 8; c++) {
+          uint32_t x[16];
+          tc::tmem_ld16(ts + c * 16, x);
+          ld_wait(x);
 #pragma unroll
-            for (int e = 0; e < 16; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-            tc::tmem_st16(to + c * 16, o);
+          for (int e = 0; e < 16; e++) {
+            const int key = key0 + c * 16 + (e ^ ((e & 8) >> 2));
+            float y = __uint_as_float(x[e]);
+            if constexpr (CAP) y = cap_out * tanhf(y * cf * cap_in);
+            x[e] = __float_as_uint(key >= low && key < lim ? y : -INFINITY);
+          }
+          tc::tmem_st16(ts + c * 16, x);
+        }
+        tc::tmem_st_wait();
+      }
+      const float mul = CAP ? 1.f : cf;
+      float s4[4] = {0.f, 0.f, 0.f, 0.f};
+      auto part = [&](int c, uint32_t (&cur)[32], uint32_t (&nxt)[32]) {   // 32 columns
+        ld_wait(cur);
+        if (c < 3) ld32(ts + (c + 1) * 32, nxt);
+        float m4[4];
+#pragma unroll
+        for (int e = 0; e < 4; e++) m4[e] = fmaxf(__uint_as_float(cur[2 * e]), __uint_as_float(cur[2 * e + 1]));
+#pragma unroll
+        for (int e = 8; e < 32; e += 2)
+          m4[(e >> 1) & 3] = fmaxf(m4[(e >> 1) & 3], fmaxf(__uint_as_float(cur[e]), __uint_as_float(cur[e + 1])));
+        const float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * mul;
+        if (__any_sync(0xffffffffu, mx > base + HEADROOM)) {
+          // some row outgrew its base: every row of the warp moves to its maximum (the product of the step
+          // before is done: S of this one was issued after it)
+          const float nw = ceilf(fmaxf(base, mx)), f = nw == -INFINITY ? 1.f : kv4::ex2(base - nw);
+          const uint32_t f2 = kv4::pack_f16(f, f);
+#pragma unroll 1
+          for (int i = 0; i < c + (j > 0 ? D / 16 : 0); i++) {
+            const uint32_t at = i < c ? ts + i * 16 : to + (i - c) * 16;
+            uint32_t y[16];
+            tc::tmem_ld16(at, y);
+            ld_wait(y);
+#pragma unroll
+            for (int e = 0; e < 16; e++)
+              y[e] = i < c ? kv4::mul_h2(y[e], f2) : __float_as_uint(__uint_as_float(y[e]) * f);
+            tc::tmem_st16(at, y);
           }
           tc::tmem_st_wait();
+          l *= f;
+#pragma unroll
+          for (int e = 0; e < 4; e++) s4[e] *= f;
+          base = nw;
         }
-        l *= f;
-        base = nw;
-      }
-      const float nb = base == -INFINITY ? 0.f : LIFT - base;
-      float s4[4] = {0.f, 0.f, 0.f, 0.f};
+        const float nb = base == -INFINITY ? 0.f : LIFT - base;
+        uint32_t pk[16];
 #pragma unroll
-      for (int c = 0; c < 8; c++) {
-        ld_wait(r[c & 1]);
-        if (c < 7) tc::tmem_ld16(ts + (c + 1) * 16, r[(c + 1) & 1]);
-        float x[16];
-        logits(r[c & 1], c, x);
-        uint32_t pk[8];
-#pragma unroll
-        for (int e = 0; e < 16; e += 2) {
-          const float p0 = kv4::ex2(fmaf(x[e], mul, nb)), p1 = kv4::ex2(fmaf(x[e + 1], mul, nb));
+        for (int e = 0; e < 32; e += 2) {
+          const float p0 = kv4::ex2(fmaf(__uint_as_float(cur[e]), mul, nb)), p1 = kv4::ex2(fmaf(__uint_as_float(cur[e + 1]), mul, nb));
           s4[(e >> 1) & 3] += p0 + p1;
           pk[e >> 1] = kv4::pack_f16(p0, p1);
         }
-        st8(ts + c * 8, pk);
+        tc::tmem_st16(ts + c * 16, pk);   // (columns of S that have been read)
+      };
+      uint32_t ra[32], rb[32];
+      ld32(ts, ra);
+#pragma unroll 1
+      for (int c = 0; c < 4; c += 2) {
+        part(c, ra, rb);
+        part(c + 1, rb, ra);
       }
       l += (s4[0] + s4[1]) + (s4[2] + s4[3]);
       tc::tmem_st_wait();
@@ -510,7 +528,7 @@ k_kv4_prefill(const __grid_constant__ Kv4Attn a, int n_split, int pps) {
       __syncwarp();
     }
     if (!alone && live) {
-      float* ml = a.part + (int64_t)gridDim.z * gridDim.y * n_blk * (2 * ROWS) * n_split * D + part_row * 2;
+      float* ml = a.part + (int64_t)gridDim.z * a.Hkv * n_blk * (2 * ROWS) * n_split * D + part_row * 2;
       ml[0] = base;
       ml[1] = l;
     }
@@ -529,7 +547,7 @@ k_kv4_prefill(const __grid_constant__ Kv4Attn a, int n_split, int pps) {
 
 void kv4_prefill_launch(const Kv4Attn& a, const Kv4AttnPlan& p, cudaStream_t stream) {
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(p.n_split * p.row_chunks), (unsigned)a.Hkv, (unsigned)a.B);
+  cfg.gridDim = dim3((unsigned)(p.n_split * a.Hkv), (unsigned)p.row_chunks, (unsigned)a.B);
   cfg.blockDim = dim3(THREADS);
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];

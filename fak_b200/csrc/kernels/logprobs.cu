@@ -118,6 +118,7 @@ FAK_DEV float ex2(float x) {   // 2^x, results below 2^-126 are zero
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+// (out of line: the main loop shares the instruction caches with nothing larger than itself)
 __device__ __noinline__ u64 merge_batch(u64 top, u64 cand, int lane) { return merge32(top, sort32(cand, lane), lane); }
 // order-preserving integer form of a float, for an integer maximum in shared memory
 FAK_DEV int ordered(float v) {
@@ -157,6 +158,7 @@ __global__ void __launch_bounds__(THREADS) k_logprobs(LogprobArgs a, int seg_len
   Tile16<T> next;   // the loads of the following tile are in flight while one is worked on
   if (i_begin + warp * TILE < i_end) next.load(x, i_begin + warp * TILE + VEC<T> * lane, i_end, a.vec);
   const float xt = given ? cap((float)x[tgt]) : INFINITY;
+  const float xt_above = nextafterf(xt, INFINITY);
   for (int base = i_begin + warp * TILE; base < i_end; base += WARPS * TILE) {
     float v[PER];
     const int i0 = base + VEC<T> * lane;
@@ -169,6 +171,7 @@ __global__ void __launch_bounds__(THREADS) k_logprobs(LogprobArgs a, int seg_len
       mx = fmaxf(mx, v[e]);
     }
     if (mx > st.m) {   // move the base of this lane's sums
+      asm volatile("");
       const float d = st.s == 0.f ? 0.f : fmaxf(st.m - mx, -1e30f), f = ex2(d * LOG2E);
       st.t = f * (st.t + st.s * d);
       st.s *= f;
@@ -181,55 +184,65 @@ __global__ void __launch_bounds__(THREADS) k_logprobs(LogprobArgs a, int seg_len
       st.s += p;
       st.t = fmaf(p, fmaxf(d, -1e30f), st.t);   // p is 0 where the clamp acts; a NaN stays in p
     }
-    const bool past = base > tgt, before = base + TILE <= tgt;   // tile after / before the target
-    if (past) {
+    // #{x >= x_t} in tiles before the target, #{x > x_t} = #{x >= the float above x_t} in those after it
+    if (base > tgt || base + TILE <= tgt) {
+      const float bar = base > tgt ? xt_above : xt;
 #pragma unroll
-      for (int e = 0; e < PER; e++) above += v[e] > xt;
-    } else if (before) {
-#pragma unroll
-      for (int e = 0; e < PER; e++) above += v[e] >= xt;
+      for (int e = 0; e < PER; e++) above += v[e] >= bar;
     } else {
-#pragma unroll
-      for (int e = 0; e < PER; e++) above += i0 + elt_at<T>(e) < tgt ? v[e] >= xt : v[e] > xt;
+      asm volatile("");   // a branch, not predicated work in every tile
+#pragma unroll 1
+      for (int e = 0; e < PER; e++) {
+        const int i = i0 + elt_at<T>(e);
+        if (i < i_end) {
+          const float y = cap((float)x[i]);
+          above += i < tgt ? y >= xt : y > xt;
+        }
+      }
     }
     if constexpr (TOP) {
       const int sb = *reinterpret_cast<volatile int*>(&s_bound);
       bound = fmaxf(bound, __int_as_float(sb >= 0 ? sb : sb ^ 0x7fffffff));
       if (first) {   // 32 lane maxima: the k-th largest of them bounds the tile's k-th from below
         first = false;
-        bound = fmaxf(bound, key_value(__shfl_sync(0xffffffffu, sort32(key_of(mx, lane), lane), k - 1)));
+        bound = fmaxf(bound, key_value(__shfl_sync(0xffffffffu, merge_batch(0, key_of(mx, lane), lane), k - 1)));
         if (lane == 0) atomicMax(&s_bound, ordered(bound));
       }
       if (__any_sync(0xffffffffu, mx >= bound)) {
+        uint32_t cand = 0;   // this lane's logits that reach the bound
 #pragma unroll
-        for (int e = 0; e < PER; e++) {
-          uint32_t votes = __ballot_sync(0xffffffffu, v[e] >= bound);
-          if (votes) {
-            const int i = i0 + elt_at<T>(e);
-            const u64 key = key_of(v[e], (uint32_t)i);
-            const bool take = v[e] >= bound && i < i_end && key > kth;
-            votes = __ballot_sync(0xffffffffu, take);
-            if (take) s_cand[warp][waiting + __popc(votes & ((1u << lane) - 1))] = key;
-            waiting += __popc(votes);
-            __syncwarp();
-            if (waiting >= 32) {
-              waiting -= 32;
-              const u64 cand = s_cand[warp][waiting + lane];
-              top = merge_batch(top, cand, lane);
-              kth = __shfl_sync(0xffffffffu, top, k - 1);
-              if (kth != 0) {
-                bound = fmaxf(bound, key_value(kth));
-                if (lane == 0) atomicMax(&s_bound, ordered(bound));
-              }
-              __syncwarp();
+        for (int e = 0; e < PER; e++) cand |= v[e] >= bound ? 1u << e : 0u;
+        while (__any_sync(0xffffffffu, cand != 0)) {   // one a lane at a time, read again (they are few)
+          bool take = false;
+          u64 key = 0;
+          if (cand) {
+            const int e = __ffs(cand) - 1, i = i0 + elt_at<T>(e);
+            cand &= cand - 1;
+            if (i < i_end) {
+              key = key_of(cap((float)x[i]), (uint32_t)i);
+              take = key > kth;
             }
+          }
+          const uint32_t votes = __ballot_sync(0xffffffffu, take);
+          if (take) s_cand[warp][waiting + __popc(votes & ((1u << lane) - 1))] = key;
+          waiting += __popc(votes);
+          __syncwarp();
+          if (waiting >= 32) {
+            waiting -= 32;
+            top = merge_batch(top, s_cand[warp][waiting + lane], lane);
+            kth = __shfl_sync(0xffffffffu, top, k - 1);
+            if (kth != 0) {
+              bound = fmaxf(bound, key_value(kth));
+              if (lane == 0) atomicMax(&s_bound, ordered(bound));
+            }
+            __syncwarp();
           }
         }
       }
     }
   }
   if constexpr (TOP) {
-    if (waiting > 0) top = merge32(top, sort32(lane < waiting ? s_cand[warp][lane] : 0ull, lane), lane);
+    if (waiting > 0) top = merge_batch(top, lane < waiting ? s_cand[warp][lane] : 0ull, lane);
     s_list[warp][lane] = top;
   }
   // the lanes' sums, then the warps', always in the same order
