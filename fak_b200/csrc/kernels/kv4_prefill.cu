@@ -7,12 +7,13 @@
 //                   TMEM as f16 over the first half of S's columns (the A operand of P V is read there);
 //   warps 8-11      dequantization: codes of 128 keys to f16 K [keys][dims] and V^T [dims][keys] in the
 //                   128-byte swizzle, two buffers each;
-//   warp 12         one thread issues the matrix products: S = Q K^T and O += P V per tile, alternating
-//                   between the tiles so that one tile's softmax runs under the other's products;
-//   warp 13         bulk copies of the pages' K and V halves into rings of 12 slots.
-// A row's exponent base is a whole number that moves only when 32 columns' maximum outgrows it by 2^8 (then
-// O, and what P of the step is stored already, are scaled by an exact power of two), so P <= 2^12 and S is
-// read once.  Steps that need a mask or a soft-cap are rewritten in TMEM by a small loop first: the main
+//   warps 12, 15    issue the matrix products of tile 0 / 1, S = Q K^T and O += P V, so that one tile's softmax
+//                   runs under the other's products (one warp for both, polling, took 0.7k cycles to notice);
+//   warps 13, 14    bulk copies of the pages' K and V halves into rings of 12 slots (one warp for both made
+//                   K wait for V's slots: 7.3k cycles a step even without softmax and dequantization).
+// A step's 128 keys are taken in halves: P of the first 64 is multiplied while the softmax of the others
+// runs.  A row's exponent base moves only when a half's maximum outgrows it by 2^8 (then O is scaled, after
+// the first half's product where there is one), so P <= 2^12 and S is read once.  Steps that need a mask or a soft-cap are rewritten in TMEM by a small loop first: the main
 // loop then has one form, which matters because four roles' code shares the instruction caches (with the
 // mask inside the unrolled loops, waits for instructions were the first stall and a step took 12.6k cycles).
 // Orders: a K chunk of 8 dims keeps its nibble pairs (0,4) (1,5) (2,6) (3,7) and Q is stored in the same
@@ -38,7 +39,7 @@ constexpr int ROWS = 128;          // query rows per tile, two tiles a CTA
 constexpr int KEYS = 128;          // keys per step
 constexpr int PPT = KEYS / PAGE;   // pages per step
 constexpr int SLOTS = 12;          // ring slots of page halves
-constexpr int THREADS = 448;
+constexpr int THREADS = 512;
 constexpr float LIFT = 4.f, HEADROOM = 8.f;
 constexpr float LOG2E = 1.4426950408889634f;
 
@@ -52,7 +53,7 @@ struct Smem {
   alignas(128) uint8_t raw_k[SLOTS][HALF];
   alignas(128) uint8_t raw_v[SLOTS][SLOT_V];
   uint64_t q_full, k_full[2], k_empty[2], v_full[2], v_empty[2];
-  uint64_t s_full[2], p_full[2], pv_done[2];
+  uint64_t s_full[2], p_full[2][2], pv_half[2], pv_done[2], turn[2];   // p_full: [tile][64-key half]
   uint64_t rk_full[SLOTS], rk_empty[SLOTS], rv_full[SLOTS], rv_empty[SLOTS];
   uint32_t tmem;
   int fail;
@@ -61,11 +62,31 @@ struct Smem {
 // f16 operands, f32 accumulator, both K-major
 constexpr uint32_t idesc_f16(int M, int N) { return (1u << 4) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24); }
 
-FAK_DEV void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) { tc::mma_bf16(d, a, b, idesc, acc); }
-FAK_DEV void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+FAK_DEV uint32_t elect_one() {
+  uint32_t r;
+  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}" : "=r"(r));
+  return r;
+}
+// D (+)= A B by the lane with `lead` set; operands by the low words of their descriptors (high word `hi`)
+FAK_DEV void mma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t hi, uint32_t idesc, uint32_t acc, uint32_t lead) {
   asm volatile(
-      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}" ::"r"(d),
-      "r"(a), "l"(b), "r"(idesc), "r"(acc)
+      "{\n .reg .pred p, q;\n .reg .b64 x, y;\n setp.ne.b32 p, %5, 0;\n setp.ne.b32 q, %6, 0;\n mov.b64 x, {%1, %3};\n"
+      " mov.b64 y, {%2, %3};\n @q tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %4, p;\n}" ::"r"(d),
+      "r"(a), "r"(b), "r"(hi), "r"(idesc), "r"(acc), "r"(lead)
+      : "memory");
+}
+FAK_DEV void mma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t hi, uint32_t idesc, uint32_t acc, uint32_t lead) {
+  asm volatile(
+      "{\n .reg .pred p, q;\n .reg .b64 y;\n setp.ne.b32 p, %5, 0;\n setp.ne.b32 q, %6, 0;\n mov.b64 y, {%2, %3};\n"
+      " @q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], y, %4, p;\n}" ::"r"(d),
+      "r"(a), "r"(b), "r"(hi), "r"(idesc), "r"(acc), "r"(lead)
+      : "memory");
+}
+FAK_DEV void commit(uint64_t* bar, uint32_t lead) {
+  asm volatile(
+      "{\n .reg .pred q;\n setp.ne.b32 q, %1, 0;\n"
+      " @q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}" ::"r"(tc::smem_addr(bar)),
+      "r"(lead)
       : "memory");
 }
 // waits for this thread's TMEM loads; the operands tie their uses to the wait
@@ -152,11 +173,14 @@ k_kv4_prefill(const __grid_constant__ Kv4Attn a, int n_split, int pps) {
     tc::mbar_init(&sm.q_full, 4 * tiles);
     for (int i = 0; i < 2; i++) {
       tc::mbar_init(&sm.k_full[i], 4);
-      tc::mbar_init(&sm.k_empty[i], 1);
+      tc::mbar_init(&sm.k_empty[i], tiles);
       tc::mbar_init(&sm.v_full[i], 4);
-      tc::mbar_init(&sm.v_empty[i], 1);
+      tc::mbar_init(&sm.v_empty[i], tiles);
       tc::mbar_init(&sm.s_full[i], 1);
-      tc::mbar_init(&sm.p_full[i], 4);
+      tc::mbar_init(&sm.p_full[i][0], 4);
+      tc::mbar_init(&sm.p_full[i][1], 4);
+      tc::mbar_init(&sm.pv_half[i], 1);
+      tc::mbar_init(&sm.turn[i], 4);
       tc::mbar_init(&sm.pv_done[i], 1);
     }
     for (int i = 0; i < SLOTS; i++) {
@@ -179,10 +203,16 @@ k_kv4_prefill(const __grid_constant__ Kv4Attn a, int n_split, int pps) {
   int* fail = &sm.fail;
 
   if (warp >= 12) {
-    if (warp == 13) {
-      // ---- page loader: lane l holds the address of page 32 i + l
+    if (warp == 13 || warp == 14) {
+      // ---- page loaders: lane l holds the address of page 32 i + l
+      const bool is_v = warp == 14;
       const int* table = a.table + (int64_t)b * a.table_stride + p_begin;
+      uint64_t* full = is_v ? sm.rv_full : sm.rk_full;
+      uint64_t* empty = is_v ? sm.rv_empty : sm.rk_empty;
+      uint8_t* ring = is_v ? sm.raw_v[0] : sm.raw_k[0];
+      const int pitch = is_v ? Smem<D>::SLOT_V : Smem<D>::HALF;
       const uint8_t* src = nullptr;
+#pragma unroll 1
       for (int i = 0; i < n_pages; i++) {
         if ((i & 31) == 0 && i + lane < n_pages) {
           int pid = table[i + lane];
@@ -190,58 +220,56 @@ k_kv4_prefill(const __grid_constant__ Kv4Attn a, int n_split, int pps) {
             report_error(a.err, 2);
             pid = 0;
           }
-          src = a.pages + ((int64_t)pid * a.Hkv + kvh) * L::BYTES;
+          src = a.pages + ((int64_t)pid * a.Hkv + kvh) * L::BYTES + (is_v ? L::VC : 0);
         }
         const int s = i % SLOTS;
-        const uint32_t free_parity = (uint32_t)((i / SLOTS) & 1) ^ 1u;
         if (lane == (i & 31)) {
-          tc::mbar_wait(&sm.rk_empty[s], free_parity, fail);
-          tc::mbar_arrive_expect_tx(&sm.rk_full[s], Smem<D>::HALF);
-          kv4::bulk_load(sm.raw_k[s], src, Smem<D>::HALF, &sm.rk_full[s]);
-          tc::mbar_wait(&sm.rv_empty[s], free_parity, fail);
-          tc::mbar_arrive_expect_tx(&sm.rv_full[s], Smem<D>::HALF);
-          kv4::bulk_load(sm.raw_v[s], src + L::VC, Smem<D>::HALF, &sm.rv_full[s]);
+          tc::mbar_wait(&empty[s], (uint32_t)((i / SLOTS) & 1) ^ 1u, fail);
+          tc::mbar_arrive_expect_tx(&full[s], Smem<D>::HALF);
+          kv4::bulk_load(ring + s * pitch, src, Smem<D>::HALF, &full[s]);
         }
         __syncwarp();
       }
-    } else if (warp == 12) {
-      // ---- matrix products
-      if (lane == 0 && NJ > 0) {
-        constexpr uint32_t id_s = idesc_f16(ROWS, KEYS), id_o = idesc_f16(ROWS, D);
-        auto issue_s = [&](int t, int j) {
-          const int kb = j & 1;
-          if (t == 0) tc::mbar_wait(&sm.k_full[kb], (uint32_t)((j >> 1) & 1), fail);
-          // P of the step before sits in S's columns until its product is done
-          if (j > 0) tc::mbar_wait(&sm.pv_done[t], (uint32_t)((j - 1) & 1), fail);
+    } else if (const int t = warp == 12 ? 0 : 1; t < tiles && NJ > 0) {
+      // ---- matrix products of tile t.  The whole warp walks the loop, so that descriptors stay warp-uniform; one
+      // lane's instructions take effect.
+      constexpr uint32_t id_s = idesc_f16(ROWS, KEYS), id_o = idesc_f16(ROWS, D);
+      constexpr uint32_t HALF_Q = ROWS * 128 / 16, HALF_V = D * 128 / 16;   // 64-dim / 64-key halves, 16-byte units
+      const uint32_t leader = elect_one();
+      const uint32_t hi = (uint32_t)(tc::smem_desc_sw128(sm.q) >> 32);      // (the same for every operand)
+      const uint32_t lq = (uint32_t)tc::smem_desc_sw128(sm.q) + t * (D / 64) * HALF_Q;
+      const uint32_t lk = (uint32_t)tc::smem_desc_sw128(sm.k), lv = (uint32_t)tc::smem_desc_sw128(sm.v);
+      const uint32_t ts = tmem + t * 128, to = tmem + 256 + t * D;
+      tc::mbar_wait(&sm.q_full, 0, fail);
+#pragma unroll 1
+      for (int j = 0; j < NJ; j++) {
+        const uint32_t buf = j & 1, par = j & 1, par2 = (j >> 1) & 1;
+        tc::mbar_wait(&sm.k_full[buf], par2, fail);
+        if (j > 0) tc::mbar_wait(&sm.pv_done[t], par ^ 1u, fail);   // P sits in S's columns until its product is done
+        // the tiles keep half a step apart: each waits until a quarter of the other's softmax is through
+        if (t == 1) tc::mbar_wait(&sm.turn[0], par, fail);
+        else if (j > 0 && tiles == 2) tc::mbar_wait(&sm.turn[1], par ^ 1u, fail);
+        __syncwarp();
+        tc::tc_fence_after();
+        const uint32_t k = lk + buf * (D / 64) * HALF_Q;
+#pragma unroll
+        for (int kk = 0; kk < D / 16; kk++)
+          mma_ss(ts, lq + (kk >> 2) * HALF_Q + 2 * (kk & 3), k + (kk >> 2) * HALF_Q + 2 * (kk & 3), hi, id_s, kk != 0, leader);
+        commit(&sm.s_full[t], leader);
+        commit(&sm.k_empty[buf], leader);
+        tc::mbar_wait(&sm.v_full[buf], par2, fail);
+#pragma unroll
+        for (int h = 0; h < 2; h++) {   // each half of P V once that half of P is there
+          tc::mbar_wait(&sm.p_full[t][h], par, fail);
+          __syncwarp();
           tc::tc_fence_after();
+          const uint32_t v = lv + (buf * 2 + h) * HALF_V;
 #pragma unroll
-          for (int hd = 0; hd < D / 64; hd++) {
-            const uint64_t ad = tc::smem_desc_sw128(sm.q[t][hd]), bd = tc::smem_desc_sw128(sm.k[kb][hd]);
-#pragma unroll
-            for (int kk = 0; kk < 4; kk++) mma_ss(tmem + t * 128, ad + 2 * kk, bd + 2 * kk, id_s, (hd | kk) != 0);
-          }
-          tc::mma_commit(&sm.s_full[t]);
-          if (t == tiles - 1) tc::mma_commit(&sm.k_empty[kb]);
-        };
-        tc::mbar_wait(&sm.q_full, 0, fail);
-        for (int t = 0; t < tiles; t++) issue_s(t, 0);
-        for (int j = 0; j < NJ; j++) {
-          const int vb = j & 1;
-          for (int t = 0; t < tiles; t++) {
-            if (t == 0) tc::mbar_wait(&sm.v_full[vb], (uint32_t)((j >> 1) & 1), fail);
-            tc::mbar_wait(&sm.p_full[t], (uint32_t)(j & 1), fail);
-            tc::tc_fence_after();
-#pragma unroll
-            for (int ks = 0; ks < KEYS / 16; ks++) {
-              const uint64_t bd = tc::smem_desc_sw128(sm.v[vb][ks >> 2]) + 2 * (ks & 3);
-              mma_ts(tmem + 256 + t * D, tmem + t * 128 + ks * 8, bd, id_o, (j > 0 || ks > 0) ? 1u : 0u);
-            }
-            tc::mma_commit(&sm.pv_done[t]);
-            if (t == tiles - 1) tc::mma_commit(&sm.v_empty[vb]);
-            if (j + 1 < NJ) issue_s(t, j + 1);
-          }
+          for (int ks = 0; ks < 4; ks++) mma_ts(to, ts + h * 32 + ks * 8, v + 2 * ks, hi, id_o, ks != 0 || h > 0 || j > 0, leader);
+          commit(h == 0 ? &sm.pv_half[t] : &sm.pv_done[t], leader);
         }
-    }
+        commit(&sm.v_empty[buf], leader);
+      }
     }
   } else if (warp >= 8) {
     // ---- dequantization: this warp's two pages of every step
@@ -420,61 +448,63 @@ k_kv4_prefill(const __grid_constant__ Kv4Attn a, int n_split, int pps) {
         tc::tmem_st_wait();
       }
       const float mul = CAP ? 1.f : cf;
-      float s4[4] = {0.f, 0.f, 0.f, 0.f};
-      auto part = [&](int c, uint32_t (&cur)[32], uint32_t (&nxt)[32]) {   // 32 columns
-        ld_wait(cur);
-        if (c < 3) ld32(ts + (c + 1) * 32, nxt);
-        float m4[4];
+#pragma unroll 1
+      for (int hf = 0; hf < 2; hf++) {   // 64 keys
+        uint32_t x[2][32];
+        ld32(ts + hf * 64, x[0]);
+        ld32(ts + hf * 64 + 32, x[1]);
+        ld_wait(x[0]);
+        ld_wait(x[1]);
+        float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-        for (int e = 0; e < 4; e++) m4[e] = fmaxf(__uint_as_float(cur[2 * e]), __uint_as_float(cur[2 * e + 1]));
-#pragma unroll
-        for (int e = 8; e < 32; e += 2)
-          m4[(e >> 1) & 3] = fmaxf(m4[(e >> 1) & 3], fmaxf(__uint_as_float(cur[e]), __uint_as_float(cur[e + 1])));
+        for (int e = 0; e < 64; e += 2)
+          m4[(e >> 1) & 3] = fmaxf(m4[(e >> 1) & 3], fmaxf(__uint_as_float(x[e >> 5][e & 31]), __uint_as_float(x[e >> 5][(e & 31) + 1])));
         const float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * mul;
         if (__any_sync(0xffffffffu, mx > base + HEADROOM)) {
-          // some row outgrew its base: every row of the warp moves to its maximum (the product of the step
-          // before is done: S of this one was issued after it)
-          const float nw = ceilf(fmaxf(base, mx)), f = nw == -INFINITY ? 1.f : kv4::ex2(base - nw);
-          const uint32_t f2 = kv4::pack_f16(f, f);
-#pragma unroll 1
-          for (int i = 0; i < c + (j > 0 ? D / 16 : 0); i++) {
-            const uint32_t at = i < c ? ts + i * 16 : to + (i - c) * 16;
-            uint32_t y[16];
-            tc::tmem_ld16(at, y);
-            ld_wait(y);
-#pragma unroll
-            for (int e = 0; e < 16; e++)
-              y[e] = i < c ? kv4::mul_h2(y[e], f2) : __float_as_uint(__uint_as_float(y[e]) * f);
-            tc::tmem_st16(at, y);
+          // some row outgrew its base: every row of the warp moves to its maximum.  The product of the step
+          // before is done (S of this one was issued after it); the first half's is waited for.
+          const float nw = fmaxf(base, mx), f = nw == -INFINITY ? 1.f : kv4::ex2(base - nw);
+          if (hf == 1) {
+            tc::mbar_wait(&sm.pv_half[t], (uint32_t)(j & 1), fail);
+            tc::tc_fence_after();
           }
-          tc::tmem_st_wait();
-          l *= f;
+          if (j > 0 || hf == 1) {
+#pragma unroll 1
+            for (int c = 0; c < D / 16; c++) {
+              uint32_t y[16];
+              tc::tmem_ld16(to + c * 16, y);
+              ld_wait(y);
 #pragma unroll
-          for (int e = 0; e < 4; e++) s4[e] *= f;
+              for (int e = 0; e < 16; e++) y[e] = __float_as_uint(__uint_as_float(y[e]) * f);
+              tc::tmem_st16(to + c * 16, y);
+            }
+          }
+          l *= f;
           base = nw;
         }
         const float nb = base == -INFINITY ? 0.f : LIFT - base;
-        uint32_t pk[16];
+        float s4[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int e = 0; e < 32; e += 2) {
-          const float p0 = kv4::ex2(fmaf(__uint_as_float(cur[e]), mul, nb)), p1 = kv4::ex2(fmaf(__uint_as_float(cur[e + 1]), mul, nb));
-          s4[(e >> 1) & 3] += p0 + p1;
-          pk[e >> 1] = kv4::pack_f16(p0, p1);
+        for (int c = 0; c < 2; c++) {
+          uint32_t pk[16];
+#pragma unroll
+          for (int e = 0; e < 32; e += 2) {
+            const float p0 = kv4::ex2(fmaf(__uint_as_float(x[c][e]), mul, nb)), p1 = kv4::ex2(fmaf(__uint_as_float(x[c][e + 1]), mul, nb));
+            s4[(e >> 1) & 3] += p0 + p1;
+            pk[e >> 1] = kv4::pack_f16(p0, p1);
+          }
+          tc::tmem_st16(ts + hf * 32 + c * 16, pk);   // (columns of S that have been read)
+          if (c == 0 && hf == 0) {
+            __syncwarp();
+            if (lane == 0) tc::mbar_arrive(&sm.turn[t]);
+          }
         }
-        tc::tmem_st16(ts + c * 16, pk);   // (columns of S that have been read)
-      };
-      uint32_t ra[32], rb[32];
-      ld32(ts, ra);
-#pragma unroll 1
-      for (int c = 0; c < 4; c += 2) {
-        part(c, ra, rb);
-        part(c + 1, rb, ra);
+        l += (s4[0] + s4[1]) + (s4[2] + s4[3]);
+        tc::tmem_st_wait();
+        tc::tc_fence_before();
+        __syncwarp();
+        if (lane == 0) tc::mbar_arrive(&sm.p_full[t][hf]);
       }
-      l += (s4[0] + s4[1]) + (s4[2] + s4[3]);
-      tc::tmem_st_wait();
-      tc::tc_fence_before();
-      __syncwarp();
-      if (lane == 0) tc::mbar_arrive(&sm.p_full[t]);
     }
     // ---- output
     const bool alone = n_split == 1;
