@@ -48,49 +48,76 @@ struct Group {
   __half s, m;
 };
 
-// Eight values of a group held by 4 lanes.
+FAK_DEV float min_nan(float a, float b) {   // as fminf, but a NaN stays
+  float r;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+FAK_DEV float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
+// Eight values of a group held by 4 lanes.  In ordinary groups no clamp can act: all values are within
+// +-65504, the rounding of the minimum moves no quotient below -1/2 (s > 2^-10 |m|) nor that of a normal
+// scale one above 15 1/2.  Other groups send their warp through the clamping loop.
 FAK_DEV Group quant8(float (&x)[8]) {
   constexpr float LIM = 65504.f, MAGIC = 12582912.f;   // adding 1.5 * 2^23 rounds to whole numbers, ties to even
-  bool nan = false;
-  float lo = INFINITY, hi = -INFINITY;
+  float lo = x[0], hi = x[0];
 #pragma unroll
-  for (int i = 0; i < 8; i++) {
-    nan |= x[i] != x[i];
-    x[i] = fminf(fmaxf(x[i], -LIM), LIM);
-    lo = fminf(lo, x[i]);
-    hi = fmaxf(hi, x[i]);
+  for (int i = 1; i < 8; i++) {
+    lo = min_nan(lo, x[i]);
+    hi = max_nan(hi, x[i]);
   }
 #pragma unroll
   for (int o = 2; o > 0; o >>= 1) {
-    lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-    hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+    lo = min_nan(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+    hi = max_nan(hi, __shfl_xor_sync(0xffffffffu, hi, o));
   }
+  const bool nan = hi != hi;
+  lo = fminf(fmaxf(lo, -LIM), LIM);
+  hi = fminf(fmaxf(hi, -LIM), LIM);
   Group g;
   g.m = __float2half_rn(lo);
   const float m = __half2float(g.m);
   g.s = __float2half_rn(__fdiv_rn(hi - m, 15.f));
+  // code 15 of the largest values may round past f16's range, where the readers compute in f16
+  if (m + 15.f * __half2float(g.s) > LIM) g.s = __ushort_as_half(__half_as_ushort(g.s) - 1);
   const float s = __half2float(g.s);
   const float r = s > 0.f ? __frcp_rn(s) : 0.f;   // a constant group: all codes 0
+  const bool plain = s > fabsf(m) * 0.0009765625f && s >= 6.103515625e-5f && lo > -LIM && hi < LIM && !nan;
   float c[2] = {0.f, 0.f};
+  if (__all_sync(0xffffffffu, plain)) {
+    asm volatile("");
 #pragma unroll
-  for (int i = 7; i >= 0; i--) {
-    const float d = x[i] - m;
-    float q = d * r;
-    q = fmaf(fmaf(-q, s, d), r, q);
-    q = fminf(fmaxf(q, 0.f), 15.f);
-    q = (q + MAGIC) - MAGIC;
-    c[i >> 2] = fmaf(c[i >> 2], 16.f, q);
+    for (int i = 7; i >= 0; i--) {
+      const float d = x[i] - m;
+      float q = d * r;
+      q = (fmaf(fmaf(-q, s, d), r, q) + MAGIC) - MAGIC;
+      c[i >> 2] = fmaf(c[i >> 2], 16.f, q);
+    }
+  } else {
+    asm volatile("");
+#pragma unroll 1
+    for (int i = 7; i >= 0; i--) {
+      const float d = fminf(fmaxf(x[7], -LIM), LIM) - m;   // (rotated below: no indexed registers)
+      float q = d * r;
+      q = fmaf(fmaf(-q, s, d), r, q);
+      q = (fminf(fmaxf(q, 0.f), 15.f) + MAGIC) - MAGIC;
+      if (i >= 4) c[1] = fmaf(c[1], 16.f, q);
+      else c[0] = fmaf(c[0], 16.f, q);
+#pragma unroll
+      for (int e = 7; e > 0; e--) x[e] = x[e - 1];
+    }
+    if (nan) {
+      g.m = __ushort_as_half(0x7fff);
+      g.s = __ushort_as_half(0);
+      c[0] = c[1] = 0.f;
+    }
   }
   g.lo = (uint32_t)__float_as_int(c[0] + 8388608.f) & 0xffffu;
   g.hi = (uint32_t)__float_as_int(c[1] + 8388608.f) & 0xffffu;
-  if (__any_sync(0xffffffffu, nan)) {
-    const uint32_t votes = __ballot_sync(0xffffffffu, nan) >> (threadIdx.x & 28);
-    if (votes & 0xfu) {
-      g.m = __ushort_as_half(0x7fff);
-      g.s = __ushort_as_half(0);
-      g.lo = g.hi = 0;
-    }
-  }
   return g;
 }
 

@@ -97,6 +97,9 @@ k_kv4_attn(const __grid_constant__ Kv4Attn a, int n_split, int pps) {
   __syncthreads();
   pdl_wait();
 
+  const int* row = a.table + (int64_t)b * a.table_stride;
+  const int ahead = split * pps + warp + W * lane;   // without a window a split's first page is known: its table
+  const int early = a.window <= 0 && lane * W < pps && ahead < a.width ? row[ahead] : -1;   // entries travel with ctx
   const int ctx = min(a.ctx[b], a.width * PAGE);
   int tok0 = b, n = 1;
   if (a.q_off) {
@@ -115,11 +118,11 @@ k_kv4_attn(const __grid_constant__ Kv4Attn a, int n_split, int pps) {
 
   // pages of this warp: p_begin + warp, + W, ..; 32 table entries at a time, one a lane
   const int np = max(0, (p_end - p_begin - warp + W - 1) / W);
-  const int* table = a.table + (int64_t)b * a.table_stride + p_begin + warp;
+  const int* table = row + p_begin + warp;
   const uint8_t* page = nullptr;   // lane l: address of page 32 j + l, refreshed every 32 pages
   auto issue = [&](int i) {
     if ((i & 31) == 0 && i + lane < np) {
-      int pid = table[(int64_t)W * (i + lane)];
+      int pid = i == 0 && a.window <= 0 ? early : table[(int64_t)W * (i + lane)];
       if ((unsigned)pid >= (uint64_t)a.n_pages) {
         report_error(a.err, 2);
         pid = 0;
@@ -467,6 +470,10 @@ __global__ void __launch_bounds__(256) k_kv4_combine(const __grid_constant__ Kv4
   const int c = blockIdx.x % (cols / 8) * 8 + warp;
   const int G = a.H / a.Hkv;
   pdl_wait();
+  const int64_t part_col = (((int64_t)b * a.Hkv + kvh) * row_chunks + rc) * cols;
+  const float* part_ml = a.part + (int64_t)gridDim.z * gridDim.y * row_chunks * cols * n_split * D;
+  const float2* ml = reinterpret_cast<const float2*>(part_ml) + (part_col + c) * n_split;
+  const float2 first = lane < n_split ? __ldcg(&ml[lane]) : make_float2(-INFINITY, 0.f);   // (travels with ctx)
   const int ctx = min(a.ctx[b], a.width * PAGE);
   int tok0 = b, n = 1;
   if (a.q_off) {
@@ -477,41 +484,36 @@ __global__ void __launch_bounds__(256) k_kv4_combine(const __grid_constant__ Kv4
   if (R <= r0) return;
   const Span sp = span_of(ctx, n, r0 / G, min(R - 1, r0 + cols - 1) / G, a.window, pps, a.width);
   const int live = max(1, sp.live);   // an empty block's split 0 wrote zeros
-  const int64_t part_col = (((int64_t)b * a.Hkv + kvh) * row_chunks + rc) * cols;
-  const float* part_ml = a.part + (int64_t)gridDim.z * gridDim.y * row_chunks * cols * n_split * D;
   if (r0 + c < R) {
     const int r = r0 + c, h = kvh * G + r % G;
-    const float2* ml = reinterpret_cast<const float2*>(part_ml) + (part_col + c) * n_split;
+    const float sink = a.sinks ? a.sinks[h] * LOG2E : -INFINITY;
     const float* po = a.part + (part_col + c) * n_split * D + V * lane;
-    float m = a.sinks ? a.sinks[h] * LOG2E : -INFINITY;
-    const float sink = m;
-    for (int s = lane; s < live; s += 32) m = fmaxf(m, __ldcg(&ml[s].x));
-    m = warp_max(m);
-    const float bs = m == -INFINITY ? 0.f : m;
-    float l = sink > -INFINITY ? ex2(sink - bs + lift) : 0.f;
-    float acc[V] = {};
+    // (base, sum) of 32 splits a lane each; the partial rows' loads do not wait for them
+    float m = sink, l = 0.f, acc[V] = {};
     for (int s0 = 0; s0 < live; s0 += 32) {
-      float f = 0.f, ls = 0.f;
-      if (s0 + lane < live) {
-        const float2 y = __ldcg(&ml[s0 + lane]);
-        f = y.x == -INFINITY ? 0.f : ex2(y.x - bs);
-        ls = f * y.y;
-      }
-      l += warp_sum(ls);
+      const float2 y = s0 == 0 ? first : s0 + lane < live ? __ldcg(&ml[s0 + lane]) : make_float2(-INFINITY, 0.f);
+      const float yb = s0 + lane < live ? y.x : -INFINITY;
+      const float mn = fmaxf(m, warp_max(yb));
+      const float keep = m == -INFINITY ? 0.f : ex2(m - mn), f = yb == -INFINITY ? 0.f : ex2(yb - mn);
+      m = mn;
+      l = l * keep + warp_sum(f == 0.f ? 0.f : f * y.y);
+#pragma unroll
+      for (int i = 0; i < V; i++) acc[i] *= keep;
       const int e = min(32, live - s0);
 #pragma unroll 16
       for (int s = 0; s < e; s++) {
         const float fs = __shfl_sync(0xffffffffu, f, s);
         const float* p = po + (int64_t)(s0 + s) * D;
         if constexpr (V == 4) {
-          const float4 y = __ldcg(reinterpret_cast<const float4*>(p));
-          acc[0] += fs * y.x; acc[1] += fs * y.y; acc[2] += fs * y.z; acc[3] += fs * y.w;
+          const float4 z = __ldcg(reinterpret_cast<const float4*>(p));
+          acc[0] += fs * z.x; acc[1] += fs * z.y; acc[2] += fs * z.z; acc[3] += fs * z.w;
         } else {
-          const float2 y = __ldcg(reinterpret_cast<const float2*>(p));
-          acc[0] += fs * y.x; acc[1] += fs * y.y;
+          const float2 z = __ldcg(reinterpret_cast<const float2*>(p));
+          acc[0] += fs * z.x; acc[1] += fs * z.y;
         }
       }
     }
+    if (sink > -INFINITY) l += ex2(sink - m + lift);
     const float inv = l != 0.f ? 1.f / l : 0.f;
     const int64_t at = (int64_t)(tok0 + r / G) * a.o_tok + (int64_t)h * a.o_head + V * lane;
 #pragma unroll

@@ -7,13 +7,16 @@
 // A target outside [0, V) has logprob 0 and rank 0.  A row with only -inf has entropy 0, logprobs -inf.
 //
 // A row is cut into n_seg segments (1 when there are enough rows to fill the machine), one CTA of 8
-// warps each; a warp walks its share of the segment in tiles of 32 lanes x 16 logits.  Each lane keeps its
-// own (M, S, sum) and moves M at most once a tile.  The top list is kept per warp, sorted, one 64-bit key
-// (ordered value, complemented index) a lane; a logit joins the warp's candidate buffer only when it
-// reaches the bound: the largest k-th value that any warp of the CTA has (32 candidates are sorted and
-// merged at a time; a random row adds about k ln(V / 512) in all).  The first bound comes from the 32
-// lane maxima of the first tile.  Segments meet in a scratch record per segment; the CTA that takes the row's last ticket
-// merges them in segment order, so results do not depend on the order of arrival.
+// warps each; the warps walk the segment in tiles of 32 lanes x 16 logits.  Each lane keeps its own
+// (M, S, sum) and moves M at most once a tile.  For the top list a logit has to reach a bound: a value that
+// at least k logits seen by the CTA reach.  Those that do (64-bit keys: ordered value, complemented index)
+// go to a pool of the CTA, which warp 0 merges, 32 sorted keys at a time, after tiles 1, 2, 4, 8, ..; the
+// bound is then the k-th value so far, so that a random row adds about k logits between two merges.  (A list
+// per warp, merged when it had 32, left the bound at the 8 k-th value: half of the tiles had candidates to
+// the end and a row cost 24 instructions a logit.)  The first bound comes from the 32 lane maxima of each
+// warp's first tile.  A full pool (rising rows) sends a warp's candidates to a list of its own instead.
+// Segments meet in a scratch record per segment; the CTA that takes the row's last ticket merges them in
+// segment order, so results do not depend on the order of arrival.
 #include "common.cuh"
 
 #include <algorithm>
@@ -29,7 +32,8 @@ constexpr int WARPS = 8;
 constexpr int THREADS = WARPS * 32;
 constexpr int PER = 16;                // logits per lane and tile
 constexpr int TILE = 32 * PER;         // per warp
-constexpr int CAND = 64;               // candidate keys a warp can hold: < 32 waiting + one per lane
+constexpr int POOL = 512;              // candidate keys of the CTA between two merges
+constexpr int CAND = 64;               // a warp's own, when the pool is full: < 32 waiting + one per lane
 constexpr int MAXK = 32;
 constexpr int REC = 4 + 2 * MAXK;      // words of a segment's record: M, S, T, count, keys
 
@@ -120,6 +124,11 @@ FAK_DEV float ex2(float x) {   // 2^x, results below 2^-126 are zero
 }
 // (out of line: the main loop shares the instruction caches with nothing larger than itself)
 __device__ __noinline__ u64 merge_batch(u64 top, u64 cand, int lane) { return merge32(top, sort32(cand, lane), lane); }
+FAK_DEV float ge_one(float a, float b) {   // a >= b ? 1 : 0
+  float r;
+  asm("set.ge.f32.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
 // order-preserving integer form of a float, for an integer maximum in shared memory
 FAK_DEV int ordered(float v) {
   const int b = __float_as_int(v);
@@ -132,13 +141,17 @@ __global__ void __launch_bounds__(THREADS) k_logprobs(LogprobArgs a, int seg_len
   __shared__ u64 s_list[WARPS][32];
   __shared__ Stat s_stat[WARPS];
   __shared__ int s_cnt[WARPS];
-  __shared__ int s_last, s_bound;
+  __shared__ u64 s_pool[TOP ? POOL : 1];
+  __shared__ int s_last, s_bound, s_n;
   constexpr float LOG2E = 1.4426950408889634f;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int seg = blockIdx.x;
   const int64_t r = blockIdx.y + (int64_t)blockIdx.z * 32768;
   if (r >= a.T) return;
-  if (TOP && tid == 0) s_bound = ordered(-INFINITY);
+  if (TOP && tid == 0) {
+    s_bound = ordered(-INFINITY);
+    s_n = 0;
+  }
   if (TOP) __syncthreads();
   pdl_wait();
   const T* __restrict__ x = (const T*)a.x + r * a.stride;
@@ -148,7 +161,7 @@ __global__ void __launch_bounds__(THREADS) k_logprobs(LogprobArgs a, int seg_len
   const int i_begin = seg * seg_len, i_end = min(a.V, i_begin + seg_len);
 
   Stat st = {-INFINITY, 0.f, 0.f};
-  int above = 0;
+  float above_f = 0.f;           // (a lane's count stays far below 2^24)
   u64 top = 0, kth = 0;          // the warp's list (lane i: i-th largest) and its k-th key
   float bound = -INFINITY;       // a lower bound of the row's k-th value
   int waiting = 0;
@@ -159,89 +172,124 @@ __global__ void __launch_bounds__(THREADS) k_logprobs(LogprobArgs a, int seg_len
   if (i_begin + warp * TILE < i_end) next.load(x, i_begin + warp * TILE + VEC<T> * lane, i_end, a.vec);
   const float xt = given ? cap((float)x[tgt]) : INFINITY;
   const float xt_above = nextafterf(xt, INFINITY);
-  for (int base = i_begin + warp * TILE; base < i_end; base += WARPS * TILE) {
-    float v[PER];
-    const int i0 = base + VEC<T> * lane;
-    next.values(v);
-    if (base + WARPS * TILE < i_end) next.load(x, i0 + WARPS * TILE, i_end, a.vec);
-    float mx = -INFINITY;
+  int round = 0, merge_at = 1;
+  for (int base0 = i_begin; base0 < i_end; base0 += WARPS * TILE) {   // (the same rounds for every warp)
+    const int base = base0 + warp * TILE;
+    if (base < i_end) {
+      float v[PER];
+      const int i0 = base + VEC<T> * lane;
+      next.values(v);
+      if (base + WARPS * TILE < i_end) next.load(x, i0 + WARPS * TILE, i_end, a.vec);
+      float mx = -INFINITY;
 #pragma unroll
-    for (int e = 0; e < PER; e++) {
-      if constexpr (CAP) v[e] = cap(v[e]);
-      mx = fmaxf(mx, v[e]);
-    }
-    if (mx > st.m) {   // move the base of this lane's sums
-      asm volatile("");
-      const float d = st.s == 0.f ? 0.f : fmaxf(st.m - mx, -1e30f), f = ex2(d * LOG2E);
-      st.t = f * (st.t + st.s * d);
-      st.s *= f;
-      st.m = mx;
-    }
-    const float mb = finite_max(st.m);
-#pragma unroll
-    for (int e = 0; e < PER; e++) {
-      const float d = v[e] - mb, p = ex2(d * LOG2E);
-      st.s += p;
-      st.t = fmaf(p, fmaxf(d, -1e30f), st.t);   // p is 0 where the clamp acts; a NaN stays in p
-    }
-    // #{x >= x_t} in tiles before the target, #{x > x_t} = #{x >= the float above x_t} in those after it
-    if (base > tgt || base + TILE <= tgt) {
-      const float bar = base > tgt ? xt_above : xt;
-#pragma unroll
-      for (int e = 0; e < PER; e++) above += v[e] >= bar;
-    } else {
-      asm volatile("");   // a branch, not predicated work in every tile
-#pragma unroll 1
       for (int e = 0; e < PER; e++) {
-        const int i = i0 + elt_at<T>(e);
-        if (i < i_end) {
-          const float y = cap((float)x[i]);
-          above += i < tgt ? y >= xt : y > xt;
+        if constexpr (CAP) v[e] = cap(v[e]);
+        mx = fmaxf(mx, v[e]);
+      }
+      if (mx > st.m) {   // move the base of this lane's sums
+        asm volatile("");
+        const float d = st.s == 0.f ? 0.f : fmaxf(st.m - mx, -1e30f), f = ex2(d * LOG2E);
+        st.t = f * (st.t + st.s * d);
+        st.s *= f;
+        st.m = mx;
+      }
+      const float mb = finite_max(st.m);
+#pragma unroll
+      for (int e = 0; e < PER; e++) {
+        const float d = v[e] - mb, p = ex2(d * LOG2E);
+        st.s += p;
+        st.t = fmaf(p, fmaxf(d, -1e30f), st.t);   // p is 0 where the clamp acts; a NaN stays in p
+      }
+      // #{x >= x_t} in tiles before the target, #{x > x_t} = #{x >= the float above x_t} in those after it
+      if (base > tgt || base + TILE <= tgt) {
+        const float bar = base > tgt ? xt_above : xt;
+#pragma unroll
+        for (int e = 0; e < PER; e++) above_f += ge_one(v[e], bar);
+      } else {
+        asm volatile("");   // a branch, not predicated work in every tile
+#pragma unroll 1
+        for (int e = 0; e < PER; e++) {
+          const int i = i0 + elt_at<T>(e);
+          if (i < i_end) {
+            const float y = cap((float)x[i]);
+            above_f += (i < tgt ? y >= xt : y > xt) ? 1.f : 0.f;
+          }
+        }
+      }
+      if constexpr (TOP) {
+        const int sb = *reinterpret_cast<volatile int*>(&s_bound);
+        bound = fmaxf(bound, __int_as_float(sb >= 0 ? sb : sb ^ 0x7fffffff));
+        if (first) {   // 32 lane maxima: the k-th largest of them bounds the tile's k-th from below
+          first = false;
+          bound = fmaxf(bound, key_value(__shfl_sync(0xffffffffu, merge_batch(0, key_of(mx, lane), lane), k - 1)));
+          if (lane == 0) atomicMax(&s_bound, ordered(bound));
+        }
+        if (__any_sync(0xffffffffu, mx >= bound)) {
+          uint32_t cand = 0;   // this lane's logits that reach the bound
+#pragma unroll
+          for (int e = 0; e < PER; e++) cand |= v[e] >= bound ? 1u << e : 0u;
+          while (__any_sync(0xffffffffu, cand != 0)) {   // one a lane at a time, read again (they are few)
+            bool take = false;
+            u64 key = 0;
+            if (cand) {
+              const int e = __ffs(cand) - 1, i = i0 + elt_at<T>(e);
+              cand &= cand - 1;
+              if (i < i_end) {
+                key = key_of(cap((float)x[i]), (uint32_t)i);
+                take = key > kth;
+              }
+            }
+            const uint32_t votes = __ballot_sync(0xffffffffu, take);
+            const int n = __popc(votes), my = __popc(votes & ((1u << lane) - 1));
+            int at = 0;
+            if (lane == 0 && n) at = atomicAdd(&s_n, n);
+            at = __shfl_sync(0xffffffffu, at, 0);
+            if (at + n <= POOL) {
+              if (take) s_pool[at + my] = key;
+            } else {   // no room: this warp's own list (s_n stays past the end until the next merge)
+              if (take && at + my < POOL) s_pool[at + my] = 0;
+              if (take) s_cand[warp][waiting + my] = key;
+              waiting += n;
+              __syncwarp();
+              if (waiting >= 32) {
+                waiting -= 32;
+                top = merge_batch(top, s_cand[warp][waiting + lane], lane);
+                kth = __shfl_sync(0xffffffffu, top, k - 1);
+                if (kth != 0) {
+                  bound = fmaxf(bound, key_value(kth));
+                  if (lane == 0) atomicMax(&s_bound, ordered(bound));
+                }
+                __syncwarp();
+              }
+            }
+          }
         }
       }
     }
     if constexpr (TOP) {
-      const int sb = *reinterpret_cast<volatile int*>(&s_bound);
-      bound = fmaxf(bound, __int_as_float(sb >= 0 ? sb : sb ^ 0x7fffffff));
-      if (first) {   // 32 lane maxima: the k-th largest of them bounds the tile's k-th from below
-        first = false;
-        bound = fmaxf(bound, key_value(__shfl_sync(0xffffffffu, merge_batch(0, key_of(mx, lane), lane), k - 1)));
-        if (lane == 0) atomicMax(&s_bound, ordered(bound));
-      }
-      if (__any_sync(0xffffffffu, mx >= bound)) {
-        uint32_t cand = 0;   // this lane's logits that reach the bound
-#pragma unroll
-        for (int e = 0; e < PER; e++) cand |= v[e] >= bound ? 1u << e : 0u;
-        while (__any_sync(0xffffffffu, cand != 0)) {   // one a lane at a time, read again (they are few)
-          bool take = false;
-          u64 key = 0;
-          if (cand) {
-            const int e = __ffs(cand) - 1, i = i0 + elt_at<T>(e);
-            cand &= cand - 1;
-            if (i < i_end) {
-              key = key_of(cap((float)x[i]), (uint32_t)i);
-              take = key > kth;
-            }
-          }
-          const uint32_t votes = __ballot_sync(0xffffffffu, take);
-          if (take) s_cand[warp][waiting + __popc(votes & ((1u << lane) - 1))] = key;
-          waiting += __popc(votes);
-          __syncwarp();
-          if (waiting >= 32) {
-            waiting -= 32;
-            top = merge_batch(top, s_cand[warp][waiting + lane], lane);
-            kth = __shfl_sync(0xffffffffu, top, k - 1);
-            if (kth != 0) {
-              bound = fmaxf(bound, key_value(kth));
-              if (lane == 0) atomicMax(&s_bound, ordered(bound));
-            }
-            __syncwarp();
+      if (++round == merge_at) {
+        merge_at *= 2;
+        __syncthreads();
+        if (warp == 0) {
+          const int n = min(s_n, POOL);
+          for (int b = 0; b < n; b += 32) top = merge_batch(top, b + lane < n ? s_pool[b + lane] : 0ull, lane);
+          kth = __shfl_sync(0xffffffffu, top, k - 1);
+          if (lane == 0) {
+            s_n = 0;
+            if (kth != 0) atomicMax(&s_bound, ordered(key_value(kth)));
           }
         }
+        __syncthreads();
       }
     }
   }
+  int above = (int)above_f;
   if constexpr (TOP) {
+    __syncthreads();
+    if (warp == 0) {
+      const int n = min(s_n, POOL);
+      for (int b = 0; b < n; b += 32) top = merge_batch(top, b + lane < n ? s_pool[b + lane] : 0ull, lane);
+    }
     if (waiting > 0) top = merge_batch(top, lane < waiting ? s_cand[warp][lane] : 0ull, lane);
     s_list[warp][lane] = top;
   }
