@@ -8,13 +8,14 @@
 //
 // A row is cut into n_seg segments (1 when there are enough rows to fill the machine), one CTA of 8
 // warps each; the warps walk the segment in tiles of 32 lanes x 16 logits.  Each lane keeps its own
-// (M, S, sum) and moves M at most once a tile.  For the top list a logit has to reach a bound: a value that
-// at least k logits seen by the CTA reach.  Those that do (64-bit keys: ordered value, complemented index)
-// go to a pool of the CTA, which warp 0 merges, 32 sorted keys at a time, after tiles 1, 2, 4, 8, ..; the
-// bound is then the k-th value so far, so that a random row adds about k logits between two merges.  (A list
-// per warp, merged when it had 32, left the bound at the 8 k-th value: half of the tiles had candidates to
-// the end and a row cost 24 instructions a logit.)  The first bound comes from the 32 lane maxima of each
-// warp's first tile.  A full pool (rising rows) sends a warp's candidates to a list of its own instead.
+// (M, S, sum) and moves M at most once a tile.  For the top list the walk only stores the maximum of every
+// lane's 32 logits of two tiles in shared memory.  Afterwards the k-th largest of the 256 lanes' maxima M bounds the k-th
+// logit from below, the few groups that reach it are read again (about k of V / 32), and their logits
+// that reach it are merged as 64-bit keys (ordered value, complemented index), 32 sorted ones at a time.  So
+// selecting costs one store a tile: at 2048 x 152064 f32, k = 20, candidates sorted out during the walk cost
+// 100 us on top of 191 us without alternatives, this way see the table of measurements below.
+// Where the bound is -inf (a mask left fewer than k lanes a token) only larger logits and the first k indices
+// can be in the list.  More candidates than the pool holds (equal logits) go to a list of each warp's own.
 // Segments meet in a scratch record per segment; the CTA that takes the row's last ticket merges them in
 // segment order, so results do not depend on the order of arrival.
 #include "common.cuh"
@@ -32,7 +33,8 @@ constexpr int WARPS = 8;
 constexpr int THREADS = WARPS * 32;
 constexpr int PER = 16;                // logits per lane and tile
 constexpr int TILE = 32 * PER;         // per warp
-constexpr int POOL = 512;              // candidate keys of the CTA between two merges
+constexpr int POOL = 512;              // candidate keys of the CTA
+constexpr int MOST_TILES = 96;         // per warp and segment (their maxima take 0.5 KB of shared memory each)
 constexpr int CAND = 64;               // a warp's own, when the pool is full: < 32 waiting + one per lane
 constexpr int MAXK = 32;
 constexpr int REC = 4 + 2 * MAXK;      // words of a segment's record: M, S, T, count, keys
@@ -129,30 +131,23 @@ FAK_DEV float ge_one(float a, float b) {   // a >= b ? 1 : 0
   asm("set.ge.f32.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
   return r;
 }
-// order-preserving integer form of a float, for an integer maximum in shared memory
-FAK_DEV int ordered(float v) {
-  const int b = __float_as_int(v);
-  return b >= 0 ? b : b ^ 0x7fffffff;
-}
 
 template <typename T, bool TOP, bool CAP>
-__global__ void __launch_bounds__(THREADS) k_logprobs(LogprobArgs a, int seg_len) {
+__global__ void __launch_bounds__(THREADS, 5) k_logprobs(LogprobArgs a, int seg_len) {
   __shared__ u64 s_cand[TOP ? WARPS : 1][TOP ? CAND : 1];
   __shared__ u64 s_list[WARPS][32];
   __shared__ Stat s_stat[WARPS];
   __shared__ int s_cnt[WARPS];
   __shared__ u64 s_pool[TOP ? POOL : 1];
-  __shared__ int s_last, s_bound, s_n;
+  __shared__ int s_last, s_n, s_own;   // s_own: some warp has a list of its own
+  __shared__ float s_bound;
+  extern __shared__ float s_mx[];   // TOP: [two tiles of the warp][thread] maxima of 32 logits
   constexpr float LOG2E = 1.4426950408889634f;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int seg = blockIdx.x;
   const int64_t r = blockIdx.y + (int64_t)blockIdx.z * 32768;
   if (r >= a.T) return;
-  if (TOP && tid == 0) {
-    s_bound = ordered(-INFINITY);
-    s_n = 0;
-  }
-  if (TOP) __syncthreads();
+  if (TOP && tid == 0) s_n = s_own = 0;   // (a barrier comes before their use)
   pdl_wait();
   const T* __restrict__ x = (const T*)a.x + r * a.stride;
   auto cap = [&](float v) { return CAP ? a.softcap * tanhf(v / a.softcap) : v; };
@@ -162,17 +157,14 @@ __global__ void __launch_bounds__(THREADS) k_logprobs(LogprobArgs a, int seg_len
 
   Stat st = {-INFINITY, 0.f, 0.f};
   float above_f = 0.f;           // (a lane's count stays far below 2^24)
-  u64 top = 0, kth = 0;          // the warp's list (lane i: i-th largest) and its k-th key
-  float bound = -INFINITY;       // a lower bound of the row's k-th value
-  int waiting = 0;
-  bool first = true;
   const int k = a.k;
 
   Tile16<T> next;   // the loads of the following tile are in flight while one is worked on
   if (i_begin + warp * TILE < i_end) next.load(x, i_begin + warp * TILE + VEC<T> * lane, i_end, a.vec);
   const float xt = given ? cap((float)x[tgt]) : INFINITY;
   const float xt_above = nextafterf(xt, INFINITY);
-  int round = 0, merge_at = 1;
+  int round = 0;
+  float pair = -INFINITY;
   for (int base0 = i_begin; base0 < i_end; base0 += WARPS * TILE) {   // (the same rounds for every warp)
     const int base = base0 + warp * TILE;
     if (base < i_end) {
@@ -207,84 +199,83 @@ __global__ void __launch_bounds__(THREADS) k_logprobs(LogprobArgs a, int seg_len
         for (int e = 0; e < PER; e++) above_f += ge_one(v[e], bar);
       } else {
         asm volatile("");   // a branch, not predicated work in every tile
-#pragma unroll 1
+#pragma unroll
         for (int e = 0; e < PER; e++) {
           const int i = i0 + elt_at<T>(e);
-          if (i < i_end) {
-            const float y = cap((float)x[i]);
-            above_f += (i < tgt ? y >= xt : y > xt) ? 1.f : 0.f;
-          }
+          above_f += i < tgt ? ge_one(v[e], xt) : i < i_end ? ge_one(v[e], xt_above) : 0.f;
         }
       }
-      if constexpr (TOP) {
-        const int sb = *reinterpret_cast<volatile int*>(&s_bound);
-        bound = fmaxf(bound, __int_as_float(sb >= 0 ? sb : sb ^ 0x7fffffff));
-        if (first) {   // 32 lane maxima: the k-th largest of them bounds the tile's k-th from below
-          first = false;
-          bound = fmaxf(bound, key_value(__shfl_sync(0xffffffffu, merge_batch(0, key_of(mx, lane), lane), k - 1)));
-          if (lane == 0) atomicMax(&s_bound, ordered(bound));
-        }
-        if (__any_sync(0xffffffffu, mx >= bound)) {
-          uint32_t cand = 0;   // this lane's logits that reach the bound
-#pragma unroll
-          for (int e = 0; e < PER; e++) cand |= v[e] >= bound ? 1u << e : 0u;
-          while (__any_sync(0xffffffffu, cand != 0)) {   // one a lane at a time, read again (they are few)
-            bool take = false;
-            u64 key = 0;
-            if (cand) {
-              const int e = __ffs(cand) - 1, i = i0 + elt_at<T>(e);
-              cand &= cand - 1;
-              if (i < i_end) {
-                key = key_of(cap((float)x[i]), (uint32_t)i);
-                take = key > kth;
-              }
-            }
-            const uint32_t votes = __ballot_sync(0xffffffffu, take);
-            const int n = __popc(votes), my = __popc(votes & ((1u << lane) - 1));
-            int at = 0;
-            if (lane == 0 && n) at = atomicAdd(&s_n, n);
-            at = __shfl_sync(0xffffffffu, at, 0);
-            if (at + n <= POOL) {
-              if (take) s_pool[at + my] = key;
-            } else {   // no room: this warp's own list (s_n stays past the end until the next merge)
-              if (take && at + my < POOL) s_pool[at + my] = 0;
-              if (take) s_cand[warp][waiting + my] = key;
-              waiting += n;
-              __syncwarp();
-              if (waiting >= 32) {
-                waiting -= 32;
-                top = merge_batch(top, s_cand[warp][waiting + lane], lane);
-                kth = __shfl_sync(0xffffffffu, top, k - 1);
-                if (kth != 0) {
-                  bound = fmaxf(bound, key_value(kth));
-                  if (lane == 0) atomicMax(&s_bound, ordered(bound));
-                }
-                __syncwarp();
-              }
-            }
-          }
-        }
+      if constexpr (TOP) {   // one maximum for two tiles
+        pair = (round & 1) ? fmaxf(pair, mx) : mx;
+        s_mx[(round >> 1) * THREADS + tid] = pair;
       }
     }
-    if constexpr (TOP) {
-      if (++round == merge_at) {
-        merge_at *= 2;
-        __syncthreads();
-        if (warp == 0) {
-          const int n = min(s_n, POOL);
-          for (int b = 0; b < n; b += 32) top = merge_batch(top, b + lane < n ? s_pool[b + lane] : 0ull, lane);
-          kth = __shfl_sync(0xffffffffu, top, k - 1);
-          if (lane == 0) {
-            s_n = 0;
-            if (kth != 0) atomicMax(&s_bound, ordered(key_value(kth)));
-          }
-        }
-        __syncthreads();
-      }
-    }
+    round++;
   }
   int above = (int)above_f;
+  u64 top = 0;   // the warp's list: lane i holds the i-th largest key
   if constexpr (TOP) {
+    // lane maxima as (value, lane) keys: the k-th largest of the CTA's 256
+    s_list[warp][lane] = merge_batch(0, key_of(st.m, lane), lane);
+    __syncthreads();
+    if (warp == 0) {
+      u64 m = s_list[0][lane];
+      for (int w = 1; w < WARPS; w++) m = merge32(m, s_list[w][lane], lane);
+      if (lane == k - 1) s_bound = key_value(m);
+    }
+    __syncthreads();
+    const float bound = s_bound;
+    u64 kth = 0;
+    int waiting = 0;
+    for (int t = 0; t < round; t++) {
+      const int i0 = i_begin + (t * WARPS + warp) * TILE + VEC<T> * lane;
+      const float mx = s_mx[(t >> 1) * THREADS + tid];
+      const bool look = i0 < i_end && (mx > -INFINITY ? mx >= bound : bound == -INFINITY && i0 < k);
+      if (!__any_sync(0xffffffffu, look)) continue;
+      uint32_t cand = 0;   // the lane's logits that may be in the list
+      if (look) {
+        Tile16<T> g;
+        g.load(x, i0, i_end, a.vec);
+        float v[PER];
+        g.values(v);
+#pragma unroll
+        for (int e = 0; e < PER; e++) {
+          const int i = i0 + elt_at<T>(e);
+          const float y = cap(v[e]);
+          if (i < i_end && (y > -INFINITY ? y >= bound : y == -INFINITY && bound == -INFINITY && i < k)) cand |= 1u << e;
+        }
+      }
+      while (__any_sync(0xffffffffu, cand != 0)) {   // one a lane at a time, read again (they are few)
+        u64 key = 0;
+        if (cand) {
+          const int i = i0 + elt_at<T>(__ffs(cand) - 1);
+          cand &= cand - 1;
+          key = key_of(cap((float)x[i]), (uint32_t)i);
+        }
+        const bool take = key > kth;
+        const uint32_t votes = __ballot_sync(0xffffffffu, take);
+        if (votes == 0) continue;
+        const int n = __popc(votes), my = __popc(votes & ((1u << lane) - 1));
+        int at = 0;
+        if (lane == 0) at = atomicAdd(&s_n, n);
+        at = __shfl_sync(0xffffffffu, at, 0);
+        if (at + n <= POOL) {
+          if (take) s_pool[at + my] = key;
+        } else {   // no room: this warp's own list
+          if (take && at + my < POOL) s_pool[at + my] = 0;
+          if (take) s_cand[warp][waiting + my] = key;
+          waiting += n;
+          s_own = 1;
+          __syncwarp();
+          if (waiting >= 32) {
+            waiting -= 32;
+            top = merge_batch(top, s_cand[warp][waiting + lane], lane);
+            kth = __shfl_sync(0xffffffffu, top, k - 1);
+            __syncwarp();
+          }
+        }
+      }
+    }
     __syncthreads();
     if (warp == 0) {
       const int n = min(s_n, POOL);
@@ -313,7 +304,7 @@ __global__ void __launch_bounds__(THREADS) k_logprobs(LogprobArgs a, int seg_len
     for (int w = 1; w < WARPS; w++) {
       st = join(st, s_stat[w]);
       above += s_cnt[w];
-      if constexpr (TOP) top = merge32(top, s_list[w][lane], lane);
+      if (TOP && s_own) top = merge32(top, s_list[w][lane], lane);
     }
   }
   if (a.n_seg > 1) {
@@ -379,12 +370,11 @@ __global__ void __launch_bounds__(THREADS) k_logprobs(LogprobArgs a, int seg_len
 
 }  // namespace
 
-// Segments per row: enough CTAs for four a SM, a segment at least a tile of every warp.
+// Segments per row: enough CTAs for four a SM, a segment at least a tile of every warp and at most 96.
 int logprob_segments(int T, int V, int n_sm) {
-  const int most = (V + WARPS * TILE - 1) / (WARPS * TILE);
-  const int want = (4 * n_sm + T - 1) / T;
-  const int n = want < most ? want : most;
-  return n < 1 ? 1 : (n > 64 ? 64 : n);
+  const int tiles = (V + WARPS * TILE - 1) / (WARPS * TILE);
+  const int want = std::min((4 * n_sm + T - 1) / T, std::min(tiles, 64));
+  return std::max(want, (tiles + MOST_TILES - 1) / MOST_TILES);
 }
 int64_t logprob_part_words(int T, int n_seg) { return n_seg > 1 ? (int64_t)T * n_seg * REC : 0; }
 
@@ -392,6 +382,7 @@ void logprob_launch(const LogprobArgs& a, cudaStream_t stream) {
   if (a.T == 0) return;
   int seg = (a.V + a.n_seg - 1) / a.n_seg;
   seg = (seg + TILE - 1) / TILE * TILE;
+  const int tiles = (seg + WARPS * TILE - 1) / (WARPS * TILE);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)a.n_seg, (unsigned)(a.T < 32768 ? a.T : 32768), (unsigned)((a.T + 32767) / 32768));
   cfg.blockDim = dim3(THREADS);
@@ -404,10 +395,16 @@ void logprob_launch(const LogprobArgs& a, cudaStream_t stream) {
   auto go = [&](auto tag) {
     using E = decltype(tag);
     const bool top = a.k > 0, cap = a.softcap > 0.f;
-    if (top && cap) FAK_CUDA_CHECK(cudaLaunchKernelEx(&cfg, k_logprobs<E, true, true>, a, seg));
-    else if (top) FAK_CUDA_CHECK(cudaLaunchKernelEx(&cfg, k_logprobs<E, true, false>, a, seg));
-    else if (cap) FAK_CUDA_CHECK(cudaLaunchKernelEx(&cfg, k_logprobs<E, false, true>, a, seg));
-    else FAK_CUDA_CHECK(cudaLaunchKernelEx(&cfg, k_logprobs<E, false, false>, a, seg));
+    auto launch = [&](auto kern, size_t smem) {
+      cfg.dynamicSmemBytes = smem;
+      FAK_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+      FAK_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kern, a, seg));
+    };
+    const size_t maxima = (size_t)((tiles + 1) / 2) * THREADS * sizeof(float);
+    if (top && cap) launch(k_logprobs<E, true, true>, maxima);
+    else if (top) launch(k_logprobs<E, true, false>, maxima);
+    else if (cap) launch(k_logprobs<E, false, true>, 0);
+    else launch(k_logprobs<E, false, false>, 0);
   };
   if (a.type == Elt::F32) go(float());
   else if (a.type == Elt::F16) go(__half());
