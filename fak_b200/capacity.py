@@ -63,6 +63,7 @@ KV_PRECISION_BYTES = {
     "bf16": 2.0,          # the engine's resident layout
     "fp8": 1.0 + 4 / 128,  # e4m3 codes + one f32 scale per (token, KV head) of 128 elements
     "q8": 34 / 32,         # q8_0 blocks: int8 codes + one f16 scale per 32 elements
+    "q4": 20 / 32,         # the engine's 4-bit layout: 16 bytes of codes + f16 scale and minimum per 32 elements
 }
 
 

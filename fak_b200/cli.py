@@ -83,6 +83,8 @@ def build_model_backend(args):
     from .engine import Engine
     from .serve import EngineBackend
     ecfg = EngineConfig.from_env(max_batch=args.max_batch)
+    if getattr(args, "kv_precision", None):
+        ecfg.kv_precision = args.kv_precision
     if getattr(args, "cpu_offload_experts", False):
         ecfg.cpu_offload_experts = True
     dev = torch.device("cuda", int(os.environ.get("LOCAL_RANK", "0")))
@@ -126,6 +128,8 @@ def _add_model_args(ap):
                     help="plan each chat prompt as a view of at most this many tokens (0: whole transcript)")
     ap.add_argument("--max-batch", type=int, default=32)
     ap.add_argument("--max-context", type=int, default=8192)
+    ap.add_argument("--kv-precision", choices=("bf16", "q4"), default=None,
+                    help="KV cache of the GPU engine: bf16, or 4-bit codes with scales (3.2x the tokens)")
     ap.add_argument("--cpu-offload-experts", action="store_true",
                     help="keep MoE expert weights in host memory and run their FFNs on the CPU")
 
@@ -189,6 +193,23 @@ def cmd_inspect(args) -> int:
     return 0
 
 
+def cmd_score(args) -> int:
+    """Log probabilities of a text's own tokens: one JSON line per text."""
+    import json
+    import math
+    if args.cpu or args.upstream:
+        raise SystemExit("score runs on the GPU engine")
+    be = build_model_backend(args)
+    ids = [be.tok.encode(t) for t in args.text]
+    if any(len(i) < 2 for i in ids):
+        raise SystemExit("score needs texts of at least two tokens")
+    for t, i, r in zip(args.text, ids, be.score(ids, args.top)):
+        n = len(r["logprob"])
+        mean = sum(r["logprob"]) / n
+        print(json.dumps({"text": t, "tokens": i, "mean_logprob": mean, "perplexity": math.exp(min(-mean, 700.0)), **r}))
+    return 0
+
+
 def cmd_adjudicate(args) -> int:
     from .agentkernel import Adjudicator, ToolCall, default_policy, load_policy
     a = Adjudicator(load_policy(args.policy) if args.policy else default_policy())
@@ -221,6 +242,11 @@ def main(argv=None) -> int:
     i = sub.add_parser("inspect", help="describe a GGUF file")
     i.add_argument("path")
     i.set_defaults(fn=cmd_inspect)
+    c = sub.add_parser("score", help="log probability, rank and entropy of a text's tokens, with alternatives")
+    _add_model_args(c)
+    c.add_argument("text", nargs="+")
+    c.add_argument("--top", type=int, default=0, help="alternatives per position (at most 32)")
+    c.set_defaults(fn=cmd_score)
     d = sub.add_parser("adjudicate", help="adjudicate one tool call")
     d.add_argument("call", help='JSON, e.g. {"tool": "Bash", "args": {"command": "ls"}}')
     d.add_argument("--policy")

@@ -328,6 +328,8 @@ class EngineConfig:
     swap_space_gb: float = 16.0         # pinned host memory for swapped-out KV pages
     async_decode: bool = True           # device-resident lane state; tokens read back one step behind
     p2p_spin_limit: int = 0             # polls before a cross-rank wait gives up (0: kernel default, ~1 s)
+    kv_precision: str = "bf16"          # paged KV cache: "bf16", or "q4" (4-bit codes, f16 scale and minimum per 32
+                                        # dims; 3.2x the tokens; one GPU, no span eviction / swap / hand-off / tree)
     cpu_offload_experts: bool = False   # MoE experts in host memory, their FFNs on the CPU (no CUDA graphs)
 
     ENV_KEYS = {
@@ -357,6 +359,7 @@ class EngineConfig:
         "swap_space_gb": ("FAK_SWAP_SPACE_GB", float),
         "async_decode": ("FAK_ASYNC_DECODE", bool),
         "p2p_spin_limit": ("FAK_P2P_SPIN_LIMIT", int),
+        "kv_precision": ("FAK_KV_PRECISION", str),
         "cpu_offload_experts": ("FAK_CPU_OFFLOAD_EXPERTS", bool),
     }
 

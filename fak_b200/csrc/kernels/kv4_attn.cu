@@ -37,7 +37,10 @@ constexpr int STAGES = 4;     // pages in flight per warp
 constexpr float HEADROOM = 0.875f;   // log2 growth of a row's max before its base moves
 constexpr float LIFT = 2.f;          // P = 2^(z - base + LIFT) <= 2^2.875 < 7.5
 constexpr float LOG2E = 1.4426950408889634f;
-constexpr int kPrefillRows = 64;     // more query rows than this per (sequence, KV head): kv4_prefill.cu
+// More query rows than this per (sequence, KV head) go to kv4_prefill.cu.  Measured (us, here / there): 63 rows
+// 8 x 8000 61.5 / 57.3, 1 x 16000 25.7 / 41.0; 128 rows 8 x 8000 124.8 / 60.2, 1 x 32000 64.0 / 45.7 (head dim
+// 128); 64 rows 4 x 8000 38.3 / 48.7 (head dim 64).
+constexpr int kPrefillRows = 64;
 constexpr float kPrefillLift = 4.f;   // LIFT of that kernel
 
 FAK_DEV void mma_f16_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -534,8 +537,7 @@ void pdl(cudaLaunchConfig_t& cfg, cudaLaunchAttribute* attr) {
 Kv4AttnPlan kv4_attn_plan(const Kv4Attn& a, int n_sm) {
   Kv4AttnPlan p{};
   const int64_t rows = (int64_t)a.max_new * (a.H / a.Hkv);
-  const int nt_most = a.D == 64 ? 4 : 2;
-  p.tc = rows > kPrefillRows;
+  p.tc = a.tiles < 0 ? rows > kPrefillRows : a.tiles > 0;
   if (p.tc) {
     // 256 rows a CTA, one CTA a SM: with fewer CTAs than SMs the keys are split, eight steps a split at least
     p.row_chunks = (int)((rows + 255) / 256);
@@ -548,13 +550,19 @@ Kv4AttnPlan kv4_attn_plan(const Kv4Attn& a, int n_sm) {
     p.part_floats = p.n_split > 1 ? ctas * 256 * p.n_split * (a.D + 2) : 0;
     return p;
   }
-  p.nt = rows <= 8 ? 1 : (rows <= 16 || nt_most == 2 ? 2 : 4);
+  // Columns a CTA: 16 at head dim 64 where there are that many rows, else 8.  More columns save unpacking but
+  // cost registers and so warps: at head dim 128 two n-tiles (16 warps a SM become 8) took 29.5 us against
+  // 24.0 at 16 x 2 tokens x 7 rows over 4097, 50.2 against 40.9 at 8 x 35 rows over 8000; at head dim 64 four
+  // (8 warps) took 68.4 us against 56.5 with two at 16 x 40 rows over 4097, and one 48.3 against 38.3 with two
+  // at 4 x 64 rows over 8000.
+  p.nt = a.D == 64 && rows > 8 ? 2 : 1;
   p.row_chunks = (int)((rows + 8 * p.nt - 1) / (8 * p.nt));
-  // Splits of pps pages each, the same for every sequence, so that CTAs are alike whatever the lengths:
-  // one wave of four CTAs a SM if every sequence filled its table, between W and 128 pages a split.
-  const int64_t ctas = (int64_t)a.B * a.Hkv * p.row_chunks;
-  int64_t pps = a.n_split > 0 ? (a.width + a.n_split - 1) / a.n_split
-                              : std::min<int64_t>(128, (a.width * ctas + 4 * n_sm - 1) / (4 * n_sm));
+  // Splits of pps pages each, the same for every sequence, so that CTAs are alike whatever the lengths: if
+  // every sequence filled its table, 2 1/4 CTAs a SM, between W and 128 pages a split.  (5 x 9000 tokens over 4
+  // KV heads: 16 splits, 320 CTAs, 16.4 us; 29 splits, 580 CTAs, one wave of four a SM, 19.4; 8 splits 21.4.
+  // 32 lanes up to 32768 over 8: 128 pages a split 164 us, 64 184, 256 164.)
+  const int64_t ctas = (int64_t)a.B * a.Hkv * p.row_chunks, room = 9 * (int64_t)n_sm / 4;
+  int64_t pps = a.n_split > 0 ? (a.width + a.n_split - 1) / a.n_split : std::min<int64_t>(128, (a.width * ctas + room - 1) / room);
   pps = std::max<int64_t>((pps + W - 1) / W * W, W);
   p.pps = (int)pps;
   p.n_split = std::max(1, (int)((a.width + pps - 1) / pps));
@@ -580,14 +588,9 @@ static void split_launch(const Kv4Attn& a, const Kv4AttnPlan& p, cudaStream_t st
     if (cap) go(k_kv4_attn<DV, NTV, true>, sizeof(Smem<DV, NTV>));          \
     else go(k_kv4_attn<DV, NTV, false>, sizeof(Smem<DV, NTV>));             \
   }
-  if (a.D == 128) {
-    if (p.nt == 1) FAK_KV4(128, 1)
-    else FAK_KV4(128, 2)
-  } else {
-    if (p.nt == 1) FAK_KV4(64, 1)
-    else if (p.nt == 2) FAK_KV4(64, 2)
-    else FAK_KV4(64, 4)
-  }
+  if (a.D == 128) FAK_KV4(128, 1)
+  else if (p.nt == 1) FAK_KV4(64, 1)
+  else FAK_KV4(64, 2)
 #undef FAK_KV4
 }
 

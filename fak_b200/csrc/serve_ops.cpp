@@ -131,7 +131,7 @@ std::vector<Tensor> kv4_read(Tensor pages, Tensor slot, int64_t head_dim, c10::S
 
 void kv4_attention(Tensor q, Tensor pages, Tensor table, OptTensor q_off, Tensor ctx, Tensor out, int64_t max_new,
                    double scale, double softcap, int64_t window, OptTensor sinks, int64_t n_split, OptTensor workspace,
-                   OptTensor err) {
+                   OptTensor err, int64_t tiles) {
   fak::Kv4Attn a{};
   a.D = check_pages(pages, "kv4_attention");
   a.Hkv = (int)pages.size(1);
@@ -179,6 +179,7 @@ void kv4_attention(Tensor q, Tensor pages, Tensor table, OptTensor q_off, Tensor
   a.softcap = (float)softcap;
   a.window = (int)window;
   a.n_split = (int)n_split;
+  a.tiles = (int)tiles;
   a.err = err_ptr(err, q);
   TORCH_CHECK(a.B <= 65535 && a.Hkv <= 65535, "kv4_attention: at most 65535 sequences and kv heads");
   if (a.B == 0 || a.n_tokens == 0 || a.max_new == 0) return;
@@ -298,7 +299,7 @@ void bind_serve_ops(pybind11::module& m) {
   m.def("kv4_attention", &kv4_attention, py::arg("q"), py::arg("pages"), py::arg("table"), py::arg("q_off"), py::arg("ctx"),
         py::arg("out"), py::arg("max_new"), py::arg("scale") = 0.0, py::arg("softcap") = 0.0, py::arg("window") = 0,
         py::arg("sinks") = py::none(), py::arg("n_split") = 0, py::arg("workspace") = py::none(),
-        py::arg("err") = py::none());
+        py::arg("err") = py::none(), py::arg("tiles") = -1);
   m.def("plan_batch", &plan_batch, py::arg("old_len"), py::arg("new_len"), py::arg("table"), py::arg("free_pages"),
         py::arg("free_head"), py::arg("max_tokens"), py::arg("outs") = py::none(), py::arg("err") = py::none());
   m.def("token_logprobs", &token_logprobs, py::arg("logits"), py::arg("V"), py::arg("target"), py::arg("k"),

@@ -42,6 +42,7 @@ struct Kv4Attn {
   int window;
   const float* sinks;        // [H] or null
   int n_split;               // 0: chosen by the rule in kv4_attn.cu
+  int tiles;                 // kernel: -1 by the rows, 0 warps over pages, 1 tiles of query rows
   float* part;               // split partials (kv4_attn_plan)
   int* err;
 };

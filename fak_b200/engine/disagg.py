@@ -49,6 +49,7 @@ def prefill_handoffs(engine, prompts: list[list[int]], sampling: SamplingParams 
                      to_host: bool = False) -> list[KVHandoff]:
     """Prefill ``prompts`` on ``engine`` and export each one's K/V (kept on its device unless
     ``to_host``: then in pinned host memory)."""
+    engine._bf16_cache("a K/V hand-off")
     t0 = time.perf_counter()
     reqs = [engine.add_request(p, 1, sampling) for p in prompts]
     for r in reqs:
@@ -79,6 +80,7 @@ def adopt(engine, h: KVHandoff, max_new_tokens: int, sampling: SamplingParams | 
     """Continue a handed-over request on ``engine``; returns its Request (output starts with the
     handoff's first token)."""
     from .engine import Request
+    engine._bf16_cache("a K/V hand-off")
     if h.page_size != engine.ecfg.page_size:
         raise ValueError(f"handoff page size {h.page_size} != engine page size {engine.ecfg.page_size}")
     if tuple(h.k.shape[0:1] + h.k.shape[2:]) != (engine.kv.k.shape[0],) + tuple(engine.kv.k.shape[2:]):

@@ -33,7 +33,7 @@ import torch
 from ..config import EngineConfig, ModelConfig
 from ..kv import OutOfPages, PagePool, RadixCache
 from ..ops import kernels as K
-from ..models.runner import KVCache, ModelRunner, PrefillMeta
+from ..models.runner import KV4Cache, KVCache, ModelRunner, PrefillMeta
 from ..models.weights import ModelWeights, gguf_source, load_weights, synthetic_source
 from .constraints import guided_decode_enabled
 from .sampling import SamplingParams, device_sample, needs_counts, pack_params, request_seed, sample
@@ -87,9 +87,17 @@ class Engine:
         if ps != 16:
             raise ValueError("the attention kernels are built for 16-token pages")
         self.max_context = max_context or self.cfg.max_context
+        if self.ecfg.kv_precision not in ("bf16", "q4"):
+            raise ValueError(f"kv_precision {self.ecfg.kv_precision!r}: the engine keeps its cache in bf16 or q4")
+        self._kv_type = KV4Cache if self.ecfg.kv_precision == "q4" else KVCache
+        if self._kv_type is KV4Cache:
+            if self.ecfg.preempt_mode == "swap":
+                raise NotImplementedError("swap preemption copies a bf16 cache (kv_precision='q4': use 'recompute')")
+            if self.ecfg.spec_k > 0 and self.ecfg.spec_drafter == "tree":
+                raise NotImplementedError("tree speculation copies rows of a bf16 cache (kv_precision='q4')")
         if n_pages is None:
             n_pages = self.ecfg.kv_pages or self._pages_from_memory()
-        self.kv = KVCache.allocate(self.cfg.n_layers, n_pages, weights.n_kv_local, self.cfg.head_dim, self.device)
+        self.kv = self._kv_type.allocate(self.cfg.n_layers, n_pages, weights.n_kv_local, self.cfg.head_dim, self.device)
         self.pool = PagePool(n_pages, reserve=1)
         self.radix = RadixCache(self.pool, ps) if self.ecfg.radix_cache else None
         if collectives is None and tp_group is not None and weights.tp_size > 1:
@@ -218,7 +226,7 @@ class Engine:
         even one sequence of max_context tokens would fit."""
         from ..capacity import FitError, MemoryPlan
         free, _ = torch.cuda.mem_get_info(self.device)
-        per = KVCache.bytes_per_page(self.cfg.n_layers, self.weights.n_kv_local, self.cfg.head_dim)
+        per = self._kv_type.bytes_per_page(self.cfg.n_layers, self.weights.n_kv_local, self.cfg.head_dim)
         pages = int(free * self.ecfg.kv_mem_fraction) // per
         need = -(-self.max_context // self.ecfg.page_size) + 1
         if pages < need:
@@ -252,6 +260,77 @@ class Engine:
         r.tokens = list(prompt)
         self.waiting.append(r)
         return r
+
+    def _bf16_cache(self, what: str) -> None:
+        """Refuse features that rewrite or export cached rows when the cache is quantized."""
+        if self._kv_type is not KVCache:
+            raise NotImplementedError(f"{what} needs the bf16 KV cache (kv_precision={self.ecfg.kv_precision!r})")
+
+    def score(self, prompts: list[list[int]], top_k: int = 0) -> list[dict]:
+        """Log probabilities of every prompt's own tokens, in one pass per ``max_prefill_tokens`` of them.
+
+        Per prompt: ``logprob`` / ``rank`` of tokens 1 .. n - 1 given those before them, ``entropy`` of the
+        distribution at each position 0 .. n - 1, and with ``top_k`` the ``top_ids`` / ``top_logprobs`` at each.
+        The chunks' block tables, slots and positions are planned on the device (``ops.kernels.plan_batch``)
+        from the lengths; the pages go back to the pool afterwards (nothing enters the radix cache)."""
+        from ..ops import kernels as K
+        if not prompts or any(not p for p in prompts):
+            raise ValueError("score: empty prompt")
+        if max(map(len, prompts)) > self.max_context:
+            raise ValueError(f"score: a prompt exceeds context {self.max_context}")
+        if not 0 <= top_k <= 32:
+            raise ValueError("score: 0 to 32 alternatives")
+        self._drain()
+        ps, dev, cap = self.ecfg.page_size, self.device, self.ecfg.max_prefill_tokens
+        done = [0] * len(prompts)
+        out: list[list] = [[] for _ in prompts]
+        to = lambda a: torch.tensor(a, dtype=torch.int32).pin_memory().to(dev, non_blocking=True)
+        queue = list(range(len(prompts)))
+        while queue:
+            need, active = 0, []     # the group's pages are held until all of it is scored
+            while queue and len(active) < 4096:   # prompts whose pages fit together (one at least)
+                n = -(-len(prompts[queue[0]]) // ps)
+                if active and need + n > self.pool.n_free():
+                    break
+                need += n
+                active.append(queue.pop(0))
+            pages = self._alloc(need)
+            try:
+                free, head = to(pages), to([0])
+                bt = torch.zeros(len(active), max(-(-len(prompts[i]) // ps) for i in active), dtype=torch.int32, device=dev)
+                cached = to([0] * len(active))
+                while any(done[i] < len(prompts[i]) for i in active):
+                    left, new, ids, tgt = cap, [], [], []
+                    for i in active:
+                        n = min(left, len(prompts[i]) - done[i])
+                        left -= n
+                        new.append(n)
+                        ids += prompts[i][done[i]:done[i] + n]
+                        tgt += prompts[i][done[i] + 1:done[i] + n + 1] + ([-1] if done[i] + n == len(prompts[i]) and n else [])
+                    plan = K.plan_batch(cached, to(new), bt, free, head, len(ids))
+                    meta = PrefillMeta.build(new, [done[i] for i in active], dev) if self._kv_type is KVCache else None
+                    r = self.runner.score(to(ids), plan, bt, meta, max(new), to(tgt), top_k)
+                    cached, head = plan.ctx, plan.free_head
+                    lp, ent, rank, tid, tlp = (t.cpu() for t in r)
+                    kerr = int(self.runner.err.item())
+                    if kerr:
+                        self._device_error(kerr, 0)
+                    t0 = 0
+                    for i, n in zip(active, new):
+                        if n:
+                            out[i].append((lp[t0:t0 + n], ent[t0:t0 + n], rank[t0:t0 + n], tid[t0:t0 + n], tlp[t0:t0 + n]))
+                        done[i] += n
+                        t0 += n
+            finally:
+                self.pool.release(pages)
+        res = []
+        for parts in out:
+            lp, ent, rank, tid, tlp = (torch.cat(c) for c in zip(*parts))
+            d = {"logprob": lp[:-1].tolist(), "rank": rank[:-1].tolist(), "entropy": ent.tolist()}
+            if top_k:
+                d.update(top_ids=tid.tolist(), top_logprobs=tlp.tolist())
+            res.append(d)
+        return res
 
     def has_work(self) -> bool:
         return bool(self.waiting or self.prefilling or self.running or self.swapped or self._pending)
@@ -394,8 +473,12 @@ class Engine:
             t.fill_(nan)
         part, _ = K.tgemv_workspace(self.device)
         part.fill_(nan)
-        self.kv.k.fill_(3.0e4)
-        self.kv.v.fill_(3.0e4)
+        if self._kv_type is KV4Cache:
+            # code 15 with scale 2048 and minimum 0: the largest finite values of the layout's f16 parts
+            self.kv.pages.fill_(0x68)
+        else:
+            self.kv.k.fill_(3.0e4)
+            self.kv.v.fill_(3.0e4)
 
     @staticmethod
     def _masked(r: Request) -> bool:
@@ -432,6 +515,7 @@ class Engine:
         only the tokens before the span may enter the radix cache."""
         from ..models.rope import inv_freq
         from ..ops import kernels as K
+        self._bf16_cache("span eviction")
         self._drain()
         self._lanes_valid = False   # pages and positions change under the resident lanes
         if r.finished or r.swap is not None or r in self.waiting or r in self.prefilling:

@@ -29,6 +29,7 @@ def save_session(engine, path: str, include_kv: bool = False) -> dict:
     seqs = engine.radix.sequences() if engine.radix is not None else []
     kv = None
     if include_kv and seqs:
+        engine._bf16_cache("a checkpoint with K/V")
         kv = []
         for toks, pages in seqs:
             idx = torch.tensor(pages, dtype=torch.long, device=engine.kv.k.device)
@@ -57,6 +58,7 @@ def load_session(engine, path: str) -> list:
     ps = engine.ecfg.page_size
     if engine.radix is not None:
         if state["kv"] is not None:
+            engine._bf16_cache("a checkpoint with K/V")
             for toks, (k, v) in zip(state["cache"], state["kv"]):
                 pages = engine._alloc(len(toks) // ps)
                 idx = torch.tensor(pages, dtype=torch.long, device=engine.kv.k.device)

@@ -54,9 +54,41 @@ class KVCache:
     def n_pages(self) -> int:
         return self.k.shape[1]
 
+    @property
+    def device(self) -> torch.device:
+        return self.k.device
+
     @staticmethod
     def bytes_per_page(n_layers: int, n_kv: int, head_dim: int, page_size: int = 16) -> int:
         return 2 * n_layers * n_kv * page_size * head_dim * 2
+
+
+@dataclasses.dataclass
+class KV4Cache:
+    """Paged cache in 4 bits: K and V of one (16-token page, KV head) in one block of 20 * head_dim bytes
+    (``ops.kernels.kv4_page_bytes``; the order inside is csrc/kernels/kv4.cuh's)."""
+    pages: torch.Tensor  # [L, P, Hkv_local, 20 * D] uint8
+    head_dim: int
+
+    @classmethod
+    def allocate(cls, n_layers: int, n_pages: int, n_kv: int, head_dim: int, device, page_size: int = 16
+                 ) -> "KV4Cache":
+        if page_size != K.KV4_PAGE:
+            raise ValueError(f"the 4-bit KV cache has {K.KV4_PAGE}-token pages")
+        return cls(torch.zeros(n_layers, n_pages, n_kv, K.kv4_page_bytes(head_dim), dtype=torch.uint8, device=device),
+                   head_dim)
+
+    @property
+    def n_pages(self) -> int:
+        return self.pages.shape[1]
+
+    @property
+    def device(self) -> torch.device:
+        return self.pages.device
+
+    @staticmethod
+    def bytes_per_page(n_layers: int, n_kv: int, head_dim: int, page_size: int = 16) -> int:
+        return n_layers * n_kv * K.kv4_page_bytes(head_dim)
 
 
 @dataclasses.dataclass
@@ -72,6 +104,12 @@ class PrefillMeta:
     tile128_seq: torch.Tensor | None = None
     tile128_q0: torch.Tensor | None = None
     n_tiles128: int = 0
+    max_qlen: int = 0
+
+    def spans(self) -> tuple[torch.Tensor, torch.Tensor, int]:
+        """(q_off [S + 1], ctx [S], max new tokens): the chunk as ``ops.kernels.kv4_prefill_attention`` takes it."""
+        end = self.seq_qoff[-1:] + self.seq_qlen[-1:]
+        return torch.cat([self.seq_qoff, end]), self.seq_pos0 + self.seq_qlen, self.max_qlen
 
     @classmethod
     def build(cls, qlens: list[int], pos0s: list[int], device) -> "PrefillMeta":
@@ -88,11 +126,11 @@ class PrefillMeta:
             off += ql
         mk = lambda a: torch.tensor(a, dtype=torch.int32).to(device, non_blocking=True)
         return cls(mk(tile_seq), mk(tile_q0), mk(offs), mk(qlens), mk(pos0s), len(tile_seq),
-                   mk(t128_seq), mk(t128_q0), len(t128_seq))
+                   mk(t128_seq), mk(t128_q0), len(t128_seq), max(qlens, default=0))
 
 
 class ModelRunner:
-    def __init__(self, weights: ModelWeights, kv: KVCache, max_batch: int = 64, max_prefill_tokens: int = 4096,
+    def __init__(self, weights: ModelWeights, kv: KVCache | KV4Cache, max_batch: int = 64, max_prefill_tokens: int = 4096,
                  max_context: int | None = None, collectives=None, fused_activations: bool = False,
                  attention_merge: bool = False, l2_prefetch: bool = False, cascade_attention: bool = True,
                  expert_offload=None):
@@ -103,7 +141,7 @@ class ModelRunner:
         self.kv = kv
         self.coll = collectives
         cfg = self.cfg
-        dev = kv.k.device
+        dev = kv.device
         self.device = dev
         self.max_batch = max_batch
         self.max_prefill = max_prefill_tokens
@@ -205,6 +243,20 @@ class ModelRunner:
         self.min_shared_pages = 32     # below this many shared pages the plain path is faster
         self.shared_pages = torch.zeros(1, dtype=torch.int32, device=dev)
 
+        # 4-bit cache: rotated K / V rows pass through 16-bit staging pages (row t of a step at slot t), the
+        # decode attention's output through an fp32 buffer; the split scratch is sized for every bucket
+        self.kv4 = isinstance(kv, KV4Cache)
+        if self.kv4:
+            if collectives is not None or expert_offload is not None:
+                raise NotImplementedError("the 4-bit KV cache runs on one GPU per replica, experts on the device")
+            if self.D not in (64, 128):
+                raise NotImplementedError(f"the 4-bit KV cache has no head dim {self.D}")
+            rows = max(B, max_prefill_tokens)
+            self.stage = KVCache.allocate(1, -(-rows // 16), self.Hkv, self.D, dev)
+            self.stage_slot = torch.arange(rows, dtype=torch.int32, device=dev)
+            self.attn_out = torch.zeros(B, self.Hq, self.D, dtype=torch.float32, device=dev)
+            cols = -(-(self.Hq // self.Hkv) // 16) * 16
+            self.kv4_ws = torch.zeros(B * self.Hkv * cols * self.n_split * (self.D + 2), dtype=torch.float32, device=dev)
         # per-device kernel scratch, allocated here so no graph capture allocates it
         mats = [weights.lm_head] + [m for L in weights.layers
                                     for m in [s for s, _ in L.qkv] + [L.o, L.gate_up, L.down]]
@@ -232,7 +284,7 @@ class ModelRunner:
 
     def cascade_ok(self, B: int) -> bool:
         """Cascade attention can run for a B-lane step (its prefix kernel holds <= 64 query rows)."""
-        return self.cascade and B >= 2 and B * (self.Hq // max(1, self.Hkv)) <= 64
+        return self.cascade and not self.kv4 and B >= 2 and B * (self.Hq // max(1, self.Hkv)) <= 64
 
     def cascade_args(self, B: int, window: int = 0) -> dict:
         """Arguments that turn on cascade attention in the step being run or captured (none when
@@ -268,15 +320,27 @@ class ModelRunner:
                 bias = L.qkv_bias[off:off + seg.rows] if L.qkv_bias is not None else None
                 pf = segs[j + 1][0] if j + 1 < len(segs) else None
                 K.gemv(seg, xin, B, self.qkv[:B, off:off + seg.rows], bias, K.EPI_STORE, prefetch=self._pf(pf))
-        K.rope_kv(self.qkv[:B], pos, slot, self.cos, self.sin, self.Hq, self.Hkv, L.q_norm, L.k_norm, cfg.rms_eps,
-                  self.q[:B], None, kv.k[i], kv.v[i])
+        if self.kv4:
+            K.rope_kv(self.qkv[:B], pos, self.stage_slot[:B], self.cos, self.sin, self.Hq, self.Hkv, L.q_norm, L.k_norm,
+                      cfg.rms_eps, self.q[:B], None, self.stage.k[0], self.stage.v[0])
+            K.kv4_append(self.stage.k[0], self.stage.v[0], slot, kv.pages[i])
+        else:
+            K.rope_kv(self.qkv[:B], pos, slot, self.cos, self.sin, self.Hq, self.Hkv, L.q_norm, L.k_norm, cfg.rms_eps,
+                      self.q[:B], None, kv.k[i], kv.v[i])
         if self.coll is None:
-            K.decode_attention(self.q[:B], kv.k[i], kv.v[i], bt, ctx, n_split, pages_per_split=max(1, self.dec_pps),
-                               act=self.act_attn,
-                               workspace=self.attn_ws, tickets=self.attn_tickets if self.attn_merge else None,
-                               prefetch=self._pf(L.o), window=cfg.layer_window(i),
-                               scale=cfg.attn_scale, softcap=cfg.attn_softcap, sinks=L.attn_sinks,
-                               **self.cascade_args(B, cfg.layer_window(i)))
+            if self.kv4:
+                # a fixed number of splits: a sequence's result does not depend on its batch
+                K.kv4_decode_attention(self.q[:B], kv.pages[i], bt, ctx, self.attn_out[:B], scale=cfg.attn_scale,
+                                       softcap=cfg.attn_softcap, window=cfg.layer_window(i), sinks=L.attn_sinks,
+                                       n_split=n_split, workspace=self.kv4_ws)
+                K.quant_act(self.attn_out[:B].view(B, -1), self.act_attn, prefetch=self._pf(L.o))
+            else:
+                K.decode_attention(self.q[:B], kv.k[i], kv.v[i], bt, ctx, n_split, pages_per_split=max(1, self.dec_pps),
+                                   act=self.act_attn,
+                                   workspace=self.attn_ws, tickets=self.attn_tickets if self.attn_merge else None,
+                                   prefetch=self._pf(L.o), window=cfg.layer_window(i),
+                                   scale=cfg.attn_scale, softcap=cfg.attn_softcap, sinks=L.attn_sinks,
+                                   **self.cascade_args(B, cfg.layer_window(i)))
             if L.post_attn_norm is not None:   # sandwich norm: x += rmsnorm(o_proj(a))
                 K.gemv(L.o, self.act_attn, B, self.tmp[:B], L.o_bias, K.EPI_STORE, prefetch=self._pf(L.gate_up))
                 K.rmsnorm_add(self.tmp[:B], L.post_attn_norm, cfg.rms_eps, x)
@@ -465,11 +529,17 @@ class ModelRunner:
     # ------------------------------------------------------------------------------------
     def prefill(self, ids, pos, slot, bt, meta: PrefillMeta, last_idx: torch.Tensor) -> torch.Tensor:
         """Run a packed chunk; returns logits [S, V] for each sequence's last token (and next ids)."""
+        if self.coll is not None and getattr(self.coll, "sp_ok", lambda *_: False)(ids.numel()):
+            return self._prefill_sp(ids, pos, slot, bt, meta, last_idx)
+        x = self._prefill_hidden(ids, pos, slot, bt, meta, meta.spans() if self.kv4 else None)
+        return self._prefill_logits(x.index_select(0, last_idx.long()))
+
+    def _prefill_hidden(self, ids, pos, slot, bt, meta: PrefillMeta | None, spans=None) -> torch.Tensor:
+        """The layers over a packed chunk: residual rows [T, d] before the final norm.  ``meta`` describes the
+        chunk for the 16-bit cache, ``spans`` (q_off, ctx, max new tokens) for the 4-bit one."""
         cfg, dev = self.cfg, self.device
         T = ids.numel()
         d = cfg.d_model
-        if self.coll is not None and getattr(self.coll, "sp_ok", lambda *_: False)(T):
-            return self._prefill_sp(ids, pos, slot, bt, meta, last_idx)
         # under fused tensor parallelism the residual lives in the peer buffer (the prefill all-reduce
         # stores reduced rows into every rank's copy)
         x = self.coll.prefill_x(T) if self.coll is not None and hasattr(self.coll, "prefill_x") else None
@@ -487,13 +557,21 @@ class ModelRunner:
             for seg, off in L.qkv:
                 bias = L.qkv_bias[off:off + seg.rows] if L.qkv_bias is not None else None
                 K.gemm(hb, seg, qkv[:, off:off + seg.rows], K.EPI_STORE, bias)
-            K.rope_kv(qkv, pos, slot, self.cos, self.sin, self.Hq, self.Hkv, L.q_norm, L.k_norm, cfg.rms_eps,
-                      None, qb, self.kv.k[i], self.kv.v[i])
-            if self.tc_prefill_attn and cfg.layer_window(i) <= 0:
-                K.prefill_attention_tc(qb, self.kv.k, self.kv.v, i, bt, meta, ab, self.err)
+            if self.kv4:
+                K.rope_kv(qkv, pos, self.stage_slot[:T], self.cos, self.sin, self.Hq, self.Hkv, L.q_norm, L.k_norm,
+                          cfg.rms_eps, None, qb, self.stage.k[0], self.stage.v[0])
+                K.kv4_append(self.stage.k[0], self.stage.v[0], slot, self.kv.pages[i])
+                K.kv4_prefill_attention(qb, self.kv.pages[i], bt, spans[0], spans[1], ab.view(T, self.Hq, self.D), spans[2],
+                                        scale=cfg.attn_scale, softcap=cfg.attn_softcap, window=cfg.layer_window(i),
+                                        sinks=L.attn_sinks, n_split=1, tiles=True)   # (independent of the batch)
             else:
-                K.prefill_attention(qb, self.kv.k[i], self.kv.v[i], bt, meta, ab, cfg.layer_window(i),
-                                    cfg.attn_scale, cfg.attn_softcap, L.attn_sinks)
+                K.rope_kv(qkv, pos, slot, self.cos, self.sin, self.Hq, self.Hkv, L.q_norm, L.k_norm, cfg.rms_eps,
+                          None, qb, self.kv.k[i], self.kv.v[i])
+                if self.tc_prefill_attn and cfg.layer_window(i) <= 0:
+                    K.prefill_attention_tc(qb, self.kv.k, self.kv.v, i, bt, meta, ab, self.err)
+                else:
+                    K.prefill_attention(qb, self.kv.k[i], self.kv.v[i], bt, meta, ab, cfg.layer_window(i),
+                                        cfg.attn_scale, cfg.attn_softcap, L.attn_sinks)
             if self.coll is None and L.post_attn_norm is not None:
                 K.gemm(ab, L.o, tmp, K.EPI_STORE, L.o_bias)
                 K.rmsnorm_add(tmp, L.post_attn_norm, cfg.rms_eps, x)
@@ -515,7 +593,27 @@ class ModelRunner:
                 K.gemm(hb2, L.down, x, K.EPI_ADD)
             else:
                 self.coll.prefill_down(self, i, hb2, x)
-        return self._prefill_logits(x.index_select(0, last_idx.long()))
+        return x
+
+    def score(self, ids, plan, bt, meta: PrefillMeta | None, max_new: int, targets, top_k: int = 0,
+              rows: int = 1024) -> "K.TokenLogprobs":
+        """Run a packed chunk laid out by ``ops.kernels.plan_batch`` and score its tokens: log probability, rank,
+        entropy of targets [T] (the token that follows each position; negative: none) and ``top_k`` alternatives.
+        ``meta`` describes the chunk for the 16-bit cache.  Logits exist for ``rows`` positions at a time."""
+        if self.coll is not None:
+            raise NotImplementedError("scoring runs on one GPU per replica")
+        cfg = self.cfg
+        x = self._prefill_hidden(ids, plan.pos, plan.slot, bt, meta, (plan.q_off, plan.ctx, max_new))
+        T = x.shape[0]
+        hb = torch.empty(T, cfg.d_model, dtype=torch.bfloat16, device=self.device)
+        K.rmsnorm_bf16(x, self.w.final_norm, cfg.rms_eps, hb)
+        logits = torch.empty(min(rows, T), cfg.vocab_size, dtype=torch.float32, device=self.device)
+        parts = []
+        for t0 in range(0, T, rows):
+            n = min(rows, T - t0)
+            K.gemm(hb[t0:t0 + n], self.w.lm_head, logits[:n], K.EPI_STORE)
+            parts.append(K.token_logprobs(logits[:n], cfg.vocab_size, targets[t0:t0 + n], top_k, cfg.final_softcap))
+        return parts[0] if len(parts) == 1 else K.TokenLogprobs(*(torch.cat(c) for c in zip(*parts)))
 
     def _prefill_logits(self, xl: torch.Tensor) -> torch.Tensor:
         """LM-head logits [S, V] of the chunk's last rows xl [S, d] (final norm inside the GEMV)."""

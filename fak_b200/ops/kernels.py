@@ -354,20 +354,22 @@ def kv4_decode_attention(q: torch.Tensor, pages: torch.Tensor, block_table: torc
     makes a sequence's result independent of its batch).  workspace: float32 scratch for the splits
     (allocated when not given)."""
     ext().kv4_attention(q, pages, block_table, None, ctx_len, out, 1, scale, softcap, window, sinks, n_split, workspace,
-                        _err_word.get(q.device))
+                        _err_word.get(q.device), 0)
     count()
 
 
 def kv4_prefill_attention(q: torch.Tensor, pages: torch.Tensor, block_table: torch.Tensor, q_off: torch.Tensor,
                           ctx_len: torch.Tensor, out: torch.Tensor, max_new: int, *, scale: float = 0.0,
                           softcap: float = 0.0, window: int = 0, sinks: torch.Tensor | None = None, n_split: int = 0,
-                          workspace: torch.Tensor | None = None) -> None:
+                          workspace: torch.Tensor | None = None, tiles: bool | None = None) -> None:
     """Causal attention of packed new tokens (their K / V already appended) over the 4-bit cache: q, out
     [T, H, D]; q_off [B + 1] int32 packed offsets of the sequences' tokens (``BatchPlan.q_off``), ctx_len
     [B] int32 keys with the new ones (``BatchPlan.ctx``); max_new: an upper bound of the new tokens of one
-    sequence.  Sequences without new tokens are skipped.  The other arguments as kv4_decode_attention."""
+    sequence.  Sequences without new tokens are skipped.  tiles: True takes the tensor-core kernel over tiles of 256
+    query rows, False the one whose warps stream pages, None the faster one for max_new (a fixed choice with
+    n_split = 1 makes a sequence's result independent of its batch).  The other arguments as kv4_decode_attention."""
     ext().kv4_attention(q, pages, block_table, q_off, ctx_len, out, max_new, scale, softcap, window, sinks, n_split,
-                        workspace, _err_word.get(q.device))
+                        workspace, _err_word.get(q.device), -1 if tiles is None else int(tiles))
     count()
 
 

@@ -41,6 +41,11 @@ class EngineBackend:
                 self._wake.wait(0.05)
                 self._wake.clear()
 
+    def score(self, prompts: list[list[int]], top_k: int = 0) -> list[dict]:
+        """``Engine.score`` between two steps of the serving loop."""
+        with self._lock:
+            return self.engine.score(prompts, top_k)
+
     def generate(self, prompt_ids: list[int], max_tokens: int, sampling: SamplingParams,
                  stop_ids=()) -> Iterator[int]:
         q: queue.Queue = queue.Queue()
