@@ -83,7 +83,7 @@ struct Smem {
 };
 
 template <int D, int NT, bool CAP>
-__global__ void __launch_bounds__(W * 32, NT == 1 ? 4 : 2)
+__global__ void __launch_bounds__(W * 32, 4)
 k_kv4_attn(const __grid_constant__ Kv4Attn a, int n_split, int pps) {
   using L = Lay<D>;
   constexpr int NG = L::NG;
@@ -92,8 +92,12 @@ k_kv4_attn(const __grid_constant__ Kv4Attn a, int n_split, int pps) {
   Smem<D, NT>& sm = *reinterpret_cast<Smem<D, NT>*>(smem_raw);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int g = lane >> 2, t = lane & 3;
-  const int split = blockIdx.x % n_split, rc = blockIdx.x / n_split, kvh = blockIdx.y, b = blockIdx.z;
-  const int G = a.H / a.Hkv;
+  const int kvh = blockIdx.y, b = blockIdx.z, G = a.G;
+  int split = blockIdx.x, rc = 0;
+  if (gridDim.x > n_split) {
+    rc = blockIdx.x / n_split;
+    split = blockIdx.x - rc * n_split;
+  }
   if (lane < STAGES) tc::mbar_init(&sm.full[warp][lane], 1);
   if (tid == 0) sm.fail = 0;
   tc::fence_mbar_init();
@@ -115,7 +119,7 @@ k_kv4_attn(const __grid_constant__ Kv4Attn a, int n_split, int pps) {
   }
   const int R = n * G, r0 = rc * COLS;
   if (R <= r0) return;
-  const Span sp = span_of(ctx, n, r0 / G, min(R - 1, r0 + COLS - 1) / G, a.window, pps, a.width);
+  const Span sp = span_of(ctx, n, a.query_of(r0), a.query_of(min(R - 1, r0 + COLS - 1)), a.window, pps, a.width);
   const int p_begin = sp.p0 + split * pps, p_end = min(sp.p1, p_begin + pps);
   if (p_begin >= p_end && !(split == 0 && sp.live == 0)) return;
 
@@ -153,7 +157,8 @@ k_kv4_attn(const __grid_constant__ Kv4Attn a, int n_split, int pps) {
 #pragma unroll
     for (int e = 0; e < 8; e++) x[m][e] = 0.f;
     if (pr < PAIRS && r < R) {
-      const int64_t at = (int64_t)(tok0 + r / G) * a.q_tok + (int64_t)(kvh * G + r % G) * a.q_head + gr * 32 + 8 * t;
+      const int qi = a.query_of(r);
+      const int64_t at = (int64_t)(tok0 + qi) * a.q_tok + (int64_t)(kvh * G + r - qi * G) * a.q_head + gr * 32 + 8 * t;
       if (a.q_vec && a.q_type != Elt::F32) {
         const uint4 u = *reinterpret_cast<const uint4*>((const uint16_t*)a.q + at);
         const uint32_t w[4] = {u.x, u.y, u.z, u.w};
@@ -223,13 +228,13 @@ k_kv4_attn(const __grid_constant__ Kv4Attn a, int n_split, int pps) {
     for (int e = 0; e < 2; e++) {
       const int r = r0 + nt * 8 + 2 * t + e;
       cf[nt][e] = 64.f / factor(nt * 8 + 2 * t + e) * a.scale * (CAP ? 1.f : LOG2E);
-      lim[nt][e] = r < R ? min(ctx - n + r / G + 1, ctx) : 0;
+      lim[nt][e] = r < R ? min(ctx - n + a.query_of(r) + 1, ctx) : 0;
       low[nt][e] = a.window > 0 ? max(0, lim[nt][e] - a.window) : 0;
     }
   }
   // Keys every live row sees, [low_max, lim_min): pages inside need no mask (dead columns are dropped at
   // the end).  Keys outside [low_any, lim_any) are seen by no row: their V is not touched.
-  const int i_first = r0 / G, i_last = min(R - 1, r0 + COLS - 1) / G;
+  const int i_first = a.query_of(r0), i_last = a.query_of(min(R - 1, r0 + COLS - 1));
   const int lim_any = ctx - n + i_last + 1, lim_min = ctx - n + i_first + 1;
   const int low_any = a.window > 0 ? max(0, lim_min - a.window) : 0;
   const int low_max = a.window > 0 ? max(0, lim_any - a.window) : 0;
@@ -423,7 +428,7 @@ k_kv4_attn(const __grid_constant__ Kv4Attn a, int n_split, int pps) {
   for (int c = warp; c < COLS; c += W) {
     const int r = r0 + c;
     if (r >= R) break;
-    const int h = kvh * G + r % G;
+    const int qi = a.query_of(r), h = kvh * G + r - qi * G;
     float m = -INFINITY;
 #pragma unroll
     for (int w = 0; w < W; w++) m = fmaxf(m, sm.base[w][c]);
@@ -449,7 +454,7 @@ k_kv4_attn(const __grid_constant__ Kv4Attn a, int n_split, int pps) {
       }
       if (alone) {
         const float inv = l != 0.f ? 1.f / l : 0.f;
-        const int64_t at = (int64_t)(tok0 + r / G) * a.o_tok + (int64_t)h * a.o_head + d;
+        const int64_t at = (int64_t)(tok0 + qi) * a.o_tok + (int64_t)h * a.o_head + d;
         store_elt(a.out, a.o_type, at, v.x * inv);
         store_elt(a.out, a.o_type, at + 1, v.y * inv);
       } else {
@@ -471,7 +476,7 @@ __global__ void __launch_bounds__(256) k_kv4_combine(const __grid_constant__ Kv4
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rc = blockIdx.x / (cols / 8), kvh = blockIdx.y, b = blockIdx.z;
   const int c = blockIdx.x % (cols / 8) * 8 + warp;
-  const int G = a.H / a.Hkv;
+  const int G = a.G;
   pdl_wait();
   const int64_t part_col = (((int64_t)b * a.Hkv + kvh) * row_chunks + rc) * cols;
   const float* part_ml = a.part + (int64_t)gridDim.z * gridDim.y * row_chunks * cols * n_split * D;
@@ -485,10 +490,10 @@ __global__ void __launch_bounds__(256) k_kv4_combine(const __grid_constant__ Kv4
   }
   const int R = n * G, r0 = rc * cols;
   if (R <= r0) return;
-  const Span sp = span_of(ctx, n, r0 / G, min(R - 1, r0 + cols - 1) / G, a.window, pps, a.width);
+  const Span sp = span_of(ctx, n, a.query_of(r0), a.query_of(min(R - 1, r0 + cols - 1)), a.window, pps, a.width);
   const int live = max(1, sp.live);   // an empty block's split 0 wrote zeros
   if (r0 + c < R) {
-    const int r = r0 + c, h = kvh * G + r % G;
+    const int r = r0 + c, qi = a.query_of(r), h = kvh * G + r - qi * G;
     const float sink = a.sinks ? a.sinks[h] * LOG2E : -INFINITY;
     const float* po = a.part + (part_col + c) * n_split * D + V * lane;
     // (base, sum) of 32 splits a lane each; the partial rows' loads do not wait for them
@@ -518,7 +523,7 @@ __global__ void __launch_bounds__(256) k_kv4_combine(const __grid_constant__ Kv4
     }
     if (sink > -INFINITY) l += ex2(sink - m + lift);
     const float inv = l != 0.f ? 1.f / l : 0.f;
-    const int64_t at = (int64_t)(tok0 + r / G) * a.o_tok + (int64_t)h * a.o_head + V * lane;
+    const int64_t at = (int64_t)(tok0 + qi) * a.o_tok + (int64_t)h * a.o_head + V * lane;
 #pragma unroll
     for (int i = 0; i < V; i++) store_elt(a.out, a.o_type, at + i, acc[i] * inv);
   }

@@ -145,7 +145,7 @@ k_kv4_prefill(const __grid_constant__ Kv4Attn a, int n_split, int pps) {
   const int n_blk = gridDim.y;
   // blocks with the longest causal range first
   const int split = blockIdx.x % n_split, kvh = blockIdx.x / n_split, blk = n_blk - 1 - (int)blockIdx.y, b = blockIdx.z;
-  const int G = a.H / a.Hkv;
+  const int G = a.G;
   pdl_wait();
   const int ctx = min(a.ctx[b], a.width * PAGE);
   int tok0 = b, n = 1;
@@ -159,7 +159,7 @@ k_kv4_prefill(const __grid_constant__ Kv4Attn a, int n_split, int pps) {
   }
   const int R = n * G, r0 = blk * 2 * ROWS;
   if (R <= r0) return;
-  const int i_first = r0 / G, i_last = min(R - 1, r0 + 2 * ROWS - 1) / G;
+  const int i_first = a.query_of(r0), i_last = a.query_of(min(R - 1, r0 + 2 * ROWS - 1));
   const Span sp = kv4::span_of(ctx, n, i_first, i_last, a.window, pps, a.width);
   const int p_begin = sp.p0 + split * pps, p_end = min(sp.p1, p_begin + pps);
   if (p_begin >= p_end && !(split == 0 && sp.live == 0)) return;
@@ -366,7 +366,7 @@ k_kv4_prefill(const __grid_constant__ Kv4Attn a, int n_split, int pps) {
     const int t = warp >> 2, quarter = warp & 3, row = quarter * 32 + lane;
     const int rr = r0 + t * ROWS + row;
     const bool live = rr < R;
-    const int qi = live ? rr / G : 0, h = kvh * G + (live ? rr % G : 0);
+    const int qi = live ? a.query_of(rr) : 0, h = kvh * G + (live ? rr - qi * G : 0);
     float cf;
     {
       // the row to f16, its largest value scaled into [2^7, 2^8)

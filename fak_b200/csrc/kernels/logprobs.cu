@@ -92,14 +92,17 @@ template <typename T>
 struct Tile16 {
   static constexpr int E = VEC<T>;
   uint4 u[PER / E];
-  // logits past `end` read as -inf
-  FAK_DEV void load(const T* __restrict__ p, int i0, int end, bool vec) {
+  // the lane's logits from i0 on; those past `end` read as -inf.  fast: the warp's tile is whole and aligned.
+  FAK_DEV void load(const T* __restrict__ p, int i0, int end, bool fast) {
+    if (fast) {
+      const uint4* q = reinterpret_cast<const uint4*>(p + i0);
 #pragma unroll
-    for (int j = 0; j < PER / E; j++) {
-      const int i = i0 + j * 32 * E;
-      if (vec && i + E <= end) {
-        u[j] = __ldcs(reinterpret_cast<const uint4*>(p + i));
-      } else {
+      for (int j = 0; j < PER / E; j++) u[j] = __ldcs(q + j * 32);
+    } else {
+      asm volatile("");   // a branch
+#pragma unroll
+      for (int j = 0; j < PER / E; j++) {
+        const int i = i0 + j * 32 * E;
         T h[E];
 #pragma unroll
         for (int e = 0; e < E; e++) h[e] = i + e < end ? p[i + e] : (T)-INFINITY;
@@ -133,7 +136,7 @@ FAK_DEV float ge_one(float a, float b) {   // a >= b ? 1 : 0
 }
 
 template <typename T, bool TOP, bool CAP>
-__global__ void __launch_bounds__(THREADS, 5) k_logprobs(LogprobArgs a, int seg_len) {
+__global__ void __launch_bounds__(THREADS, 4) k_logprobs(LogprobArgs a, int seg_len) {
   __shared__ u64 s_cand[TOP ? WARPS : 1][TOP ? CAND : 1];
   __shared__ u64 s_list[WARPS][32];
   __shared__ Stat s_stat[WARPS];
@@ -159,58 +162,65 @@ __global__ void __launch_bounds__(THREADS, 5) k_logprobs(LogprobArgs a, int seg_
   float above_f = 0.f;           // (a lane's count stays far below 2^24)
   const int k = a.k;
 
-  Tile16<T> next;   // the loads of the following tile are in flight while one is worked on
-  if (i_begin + warp * TILE < i_end) next.load(x, i_begin + warp * TILE + VEC<T> * lane, i_end, a.vec);
   const float xt = given ? cap((float)x[tgt]) : INFINITY;
   const float xt_above = nextafterf(xt, INFINITY);
-  int round = 0;
+  auto whole = [&](int base) { return a.vec && base + TILE <= i_end; };
   float pair = -INFINITY;
-  for (int base0 = i_begin; base0 < i_end; base0 += WARPS * TILE) {   // (the same rounds for every warp)
-    const int base = base0 + warp * TILE;
-    if (base < i_end) {
-      float v[PER];
-      const int i0 = base + VEC<T> * lane;
-      next.values(v);
-      if (base + WARPS * TILE < i_end) next.load(x, i0 + WARPS * TILE, i_end, a.vec);
-      float mx = -INFINITY;
+  // one tile of the warp from logit `base` on, the round-th; i0: the lane's first logit
+  auto walk = [&](const Tile16<T>& tile, int base, int round) {
+    float v[PER];
+    const int i0 = base + VEC<T> * lane;
+    tile.values(v);
+    float mx = -INFINITY;
+#pragma unroll
+    for (int e = 0; e < PER; e++) {
+      if constexpr (CAP) v[e] = cap(v[e]);
+      mx = fmaxf(mx, v[e]);
+    }
+    if (mx > st.m) {   // move the base of this lane's sums
+      asm volatile("");
+      const float d = st.s == 0.f ? 0.f : fmaxf(st.m - mx, -1e30f), f = ex2(d * LOG2E);
+      st.t = f * (st.t + st.s * d);
+      st.s *= f;
+      st.m = mx;
+    }
+    const float mb = finite_max(st.m);
+#pragma unroll
+    for (int e = 0; e < PER; e++) {
+      const float d = v[e] - mb, p = ex2(d * LOG2E);
+      st.s += p;
+      st.t = fmaf(p, fmaxf(d, -1e30f), st.t);   // p is 0 where the clamp acts; a NaN stays in p
+    }
+    // #{x >= x_t} in tiles before the target, #{x > x_t} = #{x >= the float above x_t} in those after it
+    if (base > tgt || base + TILE <= tgt) {
+      const float bar = base > tgt ? xt_above : xt;
+#pragma unroll
+      for (int e = 0; e < PER; e++) above_f += ge_one(v[e], bar);
+    } else {
+      asm volatile("");   // a branch, not predicated work in every tile
 #pragma unroll
       for (int e = 0; e < PER; e++) {
-        if constexpr (CAP) v[e] = cap(v[e]);
-        mx = fmaxf(mx, v[e]);
-      }
-      if (mx > st.m) {   // move the base of this lane's sums
-        asm volatile("");
-        const float d = st.s == 0.f ? 0.f : fmaxf(st.m - mx, -1e30f), f = ex2(d * LOG2E);
-        st.t = f * (st.t + st.s * d);
-        st.s *= f;
-        st.m = mx;
-      }
-      const float mb = finite_max(st.m);
-#pragma unroll
-      for (int e = 0; e < PER; e++) {
-        const float d = v[e] - mb, p = ex2(d * LOG2E);
-        st.s += p;
-        st.t = fmaf(p, fmaxf(d, -1e30f), st.t);   // p is 0 where the clamp acts; a NaN stays in p
-      }
-      // #{x >= x_t} in tiles before the target, #{x > x_t} = #{x >= the float above x_t} in those after it
-      if (base > tgt || base + TILE <= tgt) {
-        const float bar = base > tgt ? xt_above : xt;
-#pragma unroll
-        for (int e = 0; e < PER; e++) above_f += ge_one(v[e], bar);
-      } else {
-        asm volatile("");   // a branch, not predicated work in every tile
-#pragma unroll
-        for (int e = 0; e < PER; e++) {
-          const int i = i0 + elt_at<T>(e);
-          above_f += i < tgt ? ge_one(v[e], xt) : i < i_end ? ge_one(v[e], xt_above) : 0.f;
-        }
-      }
-      if constexpr (TOP) {   // one maximum for two tiles
-        pair = (round & 1) ? fmaxf(pair, mx) : mx;
-        s_mx[(round >> 1) * THREADS + tid] = pair;
+        const int i = i0 + elt_at<T>(e);
+        above_f += i < tgt ? ge_one(v[e], xt) : i < i_end ? ge_one(v[e], xt_above) : 0.f;
       }
     }
-    round++;
+    if constexpr (TOP) {   // one maximum for two tiles
+      pair = (round & 1) ? fmaxf(pair, mx) : mx;
+      s_mx[(round >> 1) * THREADS + tid] = pair;
+    }
+  };
+  // two tiles in registers: the loads of one are in flight while the other is worked on
+  constexpr int STEP = WARPS * TILE;
+  Tile16<T> even, odd;
+  const int rounds = (i_end - i_begin + STEP - 1) / STEP, first = i_begin + warp * TILE, lane0 = VEC<T> * lane;
+  if (first < i_end) even.load(x, first + lane0, i_end, whole(first));
+#pragma unroll 1
+  for (int r2 = 0, base = first; base < i_end; r2 += 2, base += 2 * STEP) {
+    const bool more = base + STEP < i_end;
+    if (more) odd.load(x, base + STEP + lane0, i_end, whole(base + STEP));
+    walk(even, base, r2);
+    if (base + 2 * STEP < i_end) even.load(x, base + 2 * STEP + lane0, i_end, whole(base + 2 * STEP));
+    if (more) walk(odd, base + STEP, r2 + 1);
   }
   int above = (int)above_f;
   u64 top = 0;   // the warp's list: lane i holds the i-th largest key
@@ -227,7 +237,7 @@ __global__ void __launch_bounds__(THREADS, 5) k_logprobs(LogprobArgs a, int seg_
     const float bound = s_bound;
     u64 kth = 0;
     int waiting = 0;
-    for (int t = 0; t < round; t++) {
+    for (int t = 0; t < rounds; t++) {
       const int i0 = i_begin + (t * WARPS + warp) * TILE + VEC<T> * lane;
       const float mx = s_mx[(t >> 1) * THREADS + tid];
       const bool look = i0 < i_end && (mx > -INFINITY ? mx >= bound : bound == -INFINITY && i0 < k);
@@ -235,7 +245,7 @@ __global__ void __launch_bounds__(THREADS, 5) k_logprobs(LogprobArgs a, int seg_
       uint32_t cand = 0;   // the lane's logits that may be in the list
       if (look) {
         Tile16<T> g;
-        g.load(x, i0, i_end, a.vec);
+        g.load(x, i0, i_end, a.vec && i0 - VEC<T> * lane + TILE <= i_end);
         float v[PER];
         g.values(v);
 #pragma unroll

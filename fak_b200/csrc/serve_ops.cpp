@@ -160,6 +160,8 @@ void kv4_attention(Tensor q, Tensor pages, Tensor table, OptTensor q_off, Tensor
   a.ctx = i32(ctx, 0, q, "kv4_attention: ctx_len");
   a.n_tokens = (int)q.size(0);
   a.H = (int)q.size(1);
+  a.G = a.H / a.Hkv;
+  a.g_inv = a.G > 1 ? (uint32_t)(((uint64_t(1) << 32) + a.G - 1) / a.G) : 0;
   a.B = (int)ctx.numel();
   a.max_new = (int)max_new;
   TORCH_CHECK(table.size(0) >= a.B, "kv4_attention: block table has ", S(table.size(0)), " rows for ", S(a.B), " sequences");
@@ -182,6 +184,7 @@ void kv4_attention(Tensor q, Tensor pages, Tensor table, OptTensor q_off, Tensor
   a.tiles = (int)tiles;
   a.err = err_ptr(err, q);
   TORCH_CHECK(a.B <= 65535 && a.Hkv <= 65535, "kv4_attention: at most 65535 sequences and kv heads");
+  TORCH_CHECK((int64_t)a.max_new * a.G < (int64_t(1) << 32) / a.G, "kv4_attention: too many query rows");
   if (a.B == 0 || a.n_tokens == 0 || a.max_new == 0) return;
   c10::cuda::CUDAGuard guard(q.device());
   const fak::Kv4AttnPlan p = fak::kv4_attn_plan(a, sms(q));

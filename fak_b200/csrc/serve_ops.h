@@ -34,6 +34,8 @@ struct Kv4Attn {
   const int* ctx;            // [B]
   int n_tokens;              // rows of q
   int B, H, Hkv, D, max_new;
+  int G;                     // query heads per KV head; row r of a (sequence, KV head) is query r / G, head r % G
+  uint32_t g_inv;            // ceil(2^32 / G) for G > 1: r / G = (r g_inv) / 2^32 while r G < 2^32
   void* out;                 // [T, H, D], row strides o_tok, o_head
   int64_t o_tok, o_head;
   Elt o_type;
@@ -43,6 +45,9 @@ struct Kv4Attn {
   const float* sinks;        // [H] or null
   int n_split;               // 0: chosen by the rule in kv4_attn.cu
   int tiles;                 // kernel: -1 by the rows, 0 warps over pages, 1 tiles of query rows
+#ifdef __CUDACC__
+  __device__ __forceinline__ int query_of(int r) const { return G == 1 ? r : (int)__umulhi((uint32_t)r, g_inv); }
+#endif
   float* part;               // split partials (kv4_attn_plan)
   int* err;
 };
