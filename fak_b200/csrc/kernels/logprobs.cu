@@ -12,8 +12,10 @@
 // lane's 32 logits of two tiles in shared memory.  Afterwards the k-th largest of the 256 lanes' maxima M bounds the k-th
 // logit from below, the few groups that reach it are read again (about k of V / 32), and their logits
 // that reach it are merged as 64-bit keys (ordered value, complemented index), 32 sorted ones at a time.  So
-// selecting costs one store a tile: at 2048 x 152064 f32, k = 20, candidates sorted out during the walk cost
-// 100 us on top of 191 us without alternatives, this way see the table of measurements below.
+// selecting costs one store for two tiles and a few microseconds at the end of a row.
+// Measured at 2048 x 152064: f32 without alternatives 183 us (6.8 TB/s, above the copy rate it is compared
+// with), with 20 218 us (5.7 TB/s); bf16 138 and 175 us, bound by instructions.  Candidates sorted out during
+// the walk instead cost 293 us, groups read again one after another 256 us.
 // Where the bound is -inf (a mask left fewer than k lanes a token) only larger logits and the first k indices
 // can be in the list.  More candidates than the pool holds (equal logits) go to a list of each warp's own.
 // Segments meet in a scratch record per segment; the CTA that takes the row's last ticket merges them in
@@ -21,6 +23,7 @@
 #include "common.cuh"
 
 #include <algorithm>
+#include <climits>
 #include <stdexcept>
 #include <string>
 
@@ -34,7 +37,7 @@ constexpr int THREADS = WARPS * 32;
 constexpr int PER = 16;                // logits per lane and tile
 constexpr int TILE = 32 * PER;         // per warp
 constexpr int POOL = 512;              // candidate keys of the CTA
-constexpr int MOST_TILES = 96;         // per warp and segment (their maxima take 0.5 KB of shared memory each)
+constexpr int MOST_TILES = 128;        // per warp and segment (their maxima take 0.5 KB of shared memory each)
 constexpr int CAND = 64;               // a warp's own, when the pool is full: < 32 waiting + one per lane
 constexpr int MAXK = 32;
 constexpr int REC = 4 + 2 * MAXK;      // words of a segment's record: M, S, T, count, keys
@@ -72,17 +75,11 @@ struct Stat {
   float m, s, t;   // max, sum e^(x - m), sum e^(x - m) (x - m)
 };
 FAK_DEV float finite_max(float m) { return m == -INFINITY ? 0.f : m; }
-// (value, scale) of two partial sums against their common max; d = 0 where a side is empty
-FAK_DEV Stat join(const Stat& a, const Stat& b) {
-  Stat r;
-  r.m = fmaxf(a.m, b.m);
-  const float base = finite_max(r.m);
-  // (the clamp keeps 0 * infinity out of t when the maxima are the type's extremes)
-  const float da = a.s == 0.f ? 0.f : fmaxf(a.m - base, -1e30f), db = b.s == 0.f ? 0.f : fmaxf(b.m - base, -1e30f);
-  const float fa = exp2f(da * 1.4426950408889634f), fb = exp2f(db * 1.4426950408889634f);
-  r.s = a.s * fa + b.s * fb;
-  r.t = fa * (a.t + a.s * da) + fb * (b.t + b.s * db);
-  return r;
+// Sums against a maximum m that is at least their own (the clamp keeps 0 * infinity out of t when the maxima
+// are the type's extremes; empty sums stay 0).
+FAK_DEV Stat against(const Stat& a, float m) {
+  const float d = a.s == 0.f ? 0.f : fmaxf(a.m - finite_max(m), -1e30f), f = exp2f(d * 1.4426950408889634f);
+  return {m, a.s * f, f * (a.t + a.s * d)};
 }
 
 // 16 logits a lane: 16-byte loads, neighbouring lanes side by side.
@@ -135,6 +132,17 @@ FAK_DEV float ge_one(float a, float b) {   // a >= b ? 1 : 0
   return r;
 }
 
+FAK_DEV float gt_one(float a, float b) {   // a > b ? 1 : 0
+  float r;
+  asm("set.gt.f32.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+// order-preserving integer form of a float (its own inverse on the bits)
+FAK_DEV int ordered(float v) {
+  const int b = __float_as_int(v);
+  return b >= 0 ? b : b ^ 0x7fffffff;
+}
+
 template <typename T, bool TOP, bool CAP>
 __global__ void __launch_bounds__(THREADS, 4) k_logprobs(LogprobArgs a, int seg_len) {
   __shared__ u64 s_cand[TOP ? WARPS : 1][TOP ? CAND : 1];
@@ -143,14 +151,19 @@ __global__ void __launch_bounds__(THREADS, 4) k_logprobs(LogprobArgs a, int seg_
   __shared__ int s_cnt[WARPS];
   __shared__ u64 s_pool[TOP ? POOL : 1];
   __shared__ int s_last, s_n, s_own;   // s_own: some warp has a list of its own
-  __shared__ float s_bound;
+  __shared__ int s_bound;                            // (an ordered float)
+  __shared__ float s_wmax[WARPS];
+  __shared__ __align__(16) float s_max[TOP ? THREADS : 4];
   extern __shared__ float s_mx[];   // TOP: [two tiles of the warp][thread] maxima of 32 logits
   constexpr float LOG2E = 1.4426950408889634f;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int seg = blockIdx.x;
   const int64_t r = blockIdx.y + (int64_t)blockIdx.z * 32768;
   if (r >= a.T) return;
-  if (TOP && tid == 0) s_n = s_own = 0;   // (a barrier comes before their use)
+  if (TOP && tid == 0) {   // (a barrier comes before their use)
+    s_n = s_own = 0;
+    s_bound = INT_MAX;
+  }
   pdl_wait();
   const T* __restrict__ x = (const T*)a.x + r * a.stride;
   auto cap = [&](float v) { return CAP ? a.softcap * tanhf(v / a.softcap) : v; };
@@ -162,8 +175,7 @@ __global__ void __launch_bounds__(THREADS, 4) k_logprobs(LogprobArgs a, int seg_
   float above_f = 0.f;           // (a lane's count stays far below 2^24)
   const int k = a.k;
 
-  const float xt = given ? cap((float)x[tgt]) : INFINITY;
-  const float xt_above = nextafterf(xt, INFINITY);
+  float xt = INFINITY, xt_above = INFINITY;   // (loaded behind the first tile)
   auto whole = [&](int base) { return a.vec && base + TILE <= i_end; };
   float pair = -INFINITY;
   // one tile of the warp from logit `base` on, the round-th; i0: the lane's first logit
@@ -214,6 +226,8 @@ __global__ void __launch_bounds__(THREADS, 4) k_logprobs(LogprobArgs a, int seg_
   Tile16<T> even, odd;
   const int rounds = (i_end - i_begin + STEP - 1) / STEP, first = i_begin + warp * TILE, lane0 = VEC<T> * lane;
   if (first < i_end) even.load(x, first + lane0, i_end, whole(first));
+  if (given) xt = cap((float)x[tgt]);
+  xt_above = nextafterf(xt, INFINITY);
 #pragma unroll 1
   for (int r2 = 0, base = first; base < i_end; r2 += 2, base += 2 * STEP) {
     const bool more = base + STEP < i_end;
@@ -223,42 +237,73 @@ __global__ void __launch_bounds__(THREADS, 4) k_logprobs(LogprobArgs a, int seg_
     if (more) walk(odd, base + STEP, r2 + 1);
   }
   int above = (int)above_f;
+  // the CTA's maximum; every lane's sums against it, added in a fixed order
+  {
+    const float wm = warp_max(st.m);
+    if (lane == 0) s_wmax[warp] = wm;
+    if (TOP) s_max[tid] = st.m;
+  }
+  __syncthreads();
+  float m_cta = s_wmax[0];
+#pragma unroll
+  for (int w = 1; w < WARPS; w++) m_cta = fmaxf(m_cta, s_wmax[w]);
+  {
+    const Stat y = against(st, m_cta);
+    const float ws = warp_sum(y.s), wt = warp_sum(y.t);
+    const int wc = __reduce_add_sync(0xffffffffu, above);
+    if (lane == 0) {
+      s_stat[warp] = {m_cta, ws, wt};
+      s_cnt[warp] = wc;
+    }
+  }
   u64 top = 0;   // the warp's list: lane i holds the i-th largest key
   if constexpr (TOP) {
-    // lane maxima as (value, lane) keys: the k-th largest of the CTA's 256
-    s_list[warp][lane] = merge_batch(0, key_of(st.m, lane), lane);
-    __syncthreads();
-    if (warp == 0) {
-      u64 m = s_list[0][lane];
-      for (int w = 1; w < WARPS; w++) m = merge32(m, s_list[w][lane], lane);
-      if (lane == k - 1) s_bound = key_value(m);
+    // the k-th largest of the 256 lanes' maxima: the smallest that fewer than k others exceed
+    float larger = 0.f;
+#pragma unroll 8
+    for (int e = 0; e < THREADS / 4; e++) {
+      const float4 y = reinterpret_cast<const float4*>(s_max)[e];
+      larger += (gt_one(y.x, st.m) + gt_one(y.y, st.m)) + (gt_one(y.z, st.m) + gt_one(y.w, st.m));
     }
+    const int cut = __reduce_min_sync(0xffffffffu, larger < (float)k ? ordered(st.m) : INT_MAX);
+    if (lane == 0) atomicMin(&s_bound, cut);
     __syncthreads();
-    const float bound = s_bound;
+    const int sb = s_bound;
+    const float bound = __int_as_float(sb >= 0 ? sb : sb ^ 0x7fffffff);
     u64 kth = 0;
     int waiting = 0;
-    for (int t = 0; t < rounds; t++) {
-      const int i0 = i_begin + (t * WARPS + warp) * TILE + VEC<T> * lane;
-      const float mx = s_mx[(t >> 1) * THREADS + tid];
-      const bool look = i0 < i_end && (mx > -INFINITY ? mx >= bound : bound == -INFINITY && i0 < k);
-      if (!__any_sync(0xffffffffu, look)) continue;
+    // pairs of tiles whose maximum reaches the bound, a bit each; then every lane takes its next one
+    u64 pairs = 0;
+    for (int p = 0; p < (rounds + 1) / 2; p++) {
+      const int i0 = first + 2 * p * STEP + lane0;
+      const float mx = i0 < i_end ? s_mx[p * THREADS + tid] : -INFINITY;
+      if (i0 < i_end && (mx > -INFINITY ? mx >= bound : bound == -INFINITY && i0 < k)) pairs |= 1ull << p;
+    }
+    while (__any_sync(0xffffffffu, pairs != 0)) {
       uint32_t cand = 0;   // the lane's logits that may be in the list
-      if (look) {
-        Tile16<T> g;
-        g.load(x, i0, i_end, a.vec && i0 - VEC<T> * lane + TILE <= i_end);
-        float v[PER];
-        g.values(v);
+      int i0 = 0;
+      if (pairs) {
+        i0 = first + 2 * (__ffsll(pairs) - 1) * STEP + lane0;
+        pairs &= pairs - 1;
 #pragma unroll
-        for (int e = 0; e < PER; e++) {
-          const int i = i0 + elt_at<T>(e);
-          const float y = cap(v[e]);
-          if (i < i_end && (y > -INFINITY ? y >= bound : y == -INFINITY && bound == -INFINITY && i < k)) cand |= 1u << e;
+        for (int h = 0; h < 2; h++) {
+          Tile16<T> g;
+          const int b = i0 + h * STEP;
+          g.load(x, b, i_end, a.vec && b - lane0 + TILE <= i_end);
+          float v[PER];
+          g.values(v);
+#pragma unroll
+          for (int e = 0; e < PER; e++) {
+            const int i = b + elt_at<T>(e);
+            const float y = cap(v[e]);
+            if (i < i_end && (y > -INFINITY ? y >= bound : y == -INFINITY && bound == -INFINITY && i < k)) cand |= 1u << (16 * h + e);
+          }
         }
       }
       while (__any_sync(0xffffffffu, cand != 0)) {   // one a lane at a time, read again (they are few)
         u64 key = 0;
         if (cand) {
-          const int i = i0 + elt_at<T>(__ffs(cand) - 1);
+          const int e = __ffs(cand) - 1, i = i0 + (e >> 4) * STEP + elt_at<T>(e & 15);
           cand &= cand - 1;
           key = key_of(cap((float)x[i]), (uint32_t)i);
         }
@@ -287,34 +332,34 @@ __global__ void __launch_bounds__(THREADS, 4) k_logprobs(LogprobArgs a, int seg_
       }
     }
     __syncthreads();
-    if (warp == 0) {
-      const int n = min(s_n, POOL);
-      for (int b = 0; b < n; b += 32) top = merge_batch(top, b + lane < n ? s_pool[b + lane] : 0ull, lane);
+    const int n = min(s_n, POOL);
+    if (!s_own && n <= THREADS) {   // few candidates: each finds its rank
+      if (tid < n) {
+        const u64 key = s_pool[tid];
+        int rank = 0;
+        for (int e = 0; e < n; e++) rank += s_pool[e] > key;
+        if (rank < 32) s_list[0][rank] = key;
+      } else if (tid < 32) {
+        s_list[0][tid] = 0;
+      }
+    } else {
+      if (warp == 0)
+        for (int b = 0; b < n; b += 32) top = merge_batch(top, b + lane < n ? s_pool[b + lane] : 0ull, lane);
+      if (waiting > 0) top = merge_batch(top, lane < waiting ? s_cand[warp][lane] : 0ull, lane);
+      s_list[warp][lane] = top;
     }
-    if (waiting > 0) top = merge_batch(top, lane < waiting ? s_cand[warp][lane] : 0ull, lane);
-    s_list[warp][lane] = top;
-  }
-  // the lanes' sums, then the warps', always in the same order
-#pragma unroll
-  for (int d = 16; d > 0; d >>= 1) {
-    Stat o;
-    o.m = __shfl_xor_sync(0xffffffffu, st.m, d);
-    o.s = __shfl_xor_sync(0xffffffffu, st.s, d);
-    o.t = __shfl_xor_sync(0xffffffffu, st.t, d);
-    st = (lane & d) ? join(o, st) : join(st, o);
-    above += __shfl_xor_sync(0xffffffffu, above, d);
-  }
-  if (lane == 0) {
-    s_stat[warp] = st;
-    s_cnt[warp] = above;
   }
   __syncthreads();
   if (warp != 0 && a.n_seg == 1) return;
   if (warp == 0) {
+    st = s_stat[0];
+    above = s_cnt[0];
+    if (TOP) top = s_list[0][lane];
     for (int w = 1; w < WARPS; w++) {
-      st = join(st, s_stat[w]);
+      st.s += s_stat[w].s;
+      st.t += s_stat[w].t;
       above += s_cnt[w];
-      if (TOP && s_own) top = merge32(top, s_list[w][lane], lane);
+      if (TOP && (s_own || s_n > THREADS)) top = merge32(top, s_list[w][lane], lane);
     }
   }
   if (a.n_seg > 1) {
@@ -335,30 +380,46 @@ __global__ void __launch_bounds__(THREADS, 4) k_logprobs(LogprobArgs a, int seg_
       return;
     }
     __threadfence();
-    // every warp takes the segments w, w + 8, ..; then warp 0 the warps
+    // lists: every warp takes the segments w, w + 8, .. (eight loads in flight), then warp 0 the warps
     const float* recs = a.part + (int64_t)r * a.n_seg * REC;
-    st = {-INFINITY, 0.f, 0.f};
-    above = 0;
-    top = 0;
-    for (int s = warp; s < a.n_seg; s += WARPS) {
-      const float* q = recs + (int64_t)s * REC;
-      const Stat o = {__ldcg(q), __ldcg(q + 1), __ldcg(q + 2)};
-      st = join(st, o);
-      above += __float_as_int(__ldcg(q + 3));
-      if constexpr (TOP) top = merge32(top, __ldcg(reinterpret_cast<const u64*>(q + 4) + lane), lane);
+    if constexpr (TOP) {
+      top = 0;
+      for (int s0 = warp; s0 < a.n_seg; s0 += 8 * WARPS) {
+        u64 y[8];
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+          const int s = s0 + e * WARPS;
+          y[e] = s < a.n_seg ? __ldcg(reinterpret_cast<const u64*>(recs + (int64_t)s * REC + 4) + lane) : 0ull;
+        }
+#pragma unroll
+        for (int e = 0; e < 8; e++)
+          if (s0 + e * WARPS < a.n_seg) top = merge32(top, y[e], lane);
+      }
+      s_list[warp][lane] = top;
+      __syncthreads();
+      if (warp < 4) s_list[warp][lane] = top = merge32(top, s_list[warp + 4][lane], lane);
+      __syncthreads();
     }
-    if (lane == 0) {
-      s_stat[warp] = st;
-      s_cnt[warp] = above;
-    }
-    if constexpr (TOP) s_list[warp][lane] = top;
-    __syncthreads();
     if (warp != 0) return;
-    for (int w = 1; w < WARPS; w++) {
-      st = join(st, s_stat[w]);
-      above += s_cnt[w];
-      if constexpr (TOP) top = merge32(top, s_list[w][lane], lane);
+    if constexpr (TOP) {
+      for (int w = 1; w < 4; w++) top = merge32(top, s_list[w][lane], lane);
     }
+    // sums: lane l the segments l, l + 32, .., against the largest maximum
+    float m = -INFINITY;
+    for (int s = lane; s < a.n_seg; s += 32) m = fmaxf(m, __ldcg(recs + (int64_t)s * REC));
+    m = warp_max(m);
+    st = {m, 0.f, 0.f};
+    above = 0;
+    for (int s = lane; s < a.n_seg; s += 32) {
+      const float4 q = __ldcg(reinterpret_cast<const float4*>(recs + (int64_t)s * REC));
+      const Stat y = against({q.x, q.y, q.z}, m);
+      st.s += y.s;
+      st.t += y.t;
+      above += __float_as_int(q.w);
+    }
+    st.s = warp_sum(st.s);
+    st.t = warp_sum(st.t);
+    above = __reduce_add_sync(0xffffffffu, above);
     if (lane == 0) a.tickets[r] = 0;
   }
   const float log_s = logf(st.s);   // S >= 1 unless the row is empty
@@ -380,10 +441,12 @@ __global__ void __launch_bounds__(THREADS, 4) k_logprobs(LogprobArgs a, int seg_
 
 }  // namespace
 
-// Segments per row: enough CTAs for four a SM, a segment at least a tile of every warp and at most 96.
+// Segments per row: 2 1/4 CTAs a SM where the rows are fewer, a segment at least a tile of every warp and at
+// most 128.  (A CTA costs about as much as four tiles beside its tiles: 40 rows of 152064 in 8 segments took
+// 20.7 us, in 16 26.5; 148 rows in 1 / 2 / 4 52.4 / 42.2 / 38.8; 300 rows in 1 58.5, in 2 73.8.)
 int logprob_segments(int T, int V, int n_sm) {
   const int tiles = (V + WARPS * TILE - 1) / (WARPS * TILE);
-  const int want = std::min((4 * n_sm + T - 1) / T, std::min(tiles, 64));
+  const int want = std::max(1, std::min(9 * n_sm / (4 * T), std::min(tiles, 64)));
   return std::max(want, (tiles + MOST_TILES - 1) / MOST_TILES);
 }
 int64_t logprob_part_words(int T, int n_seg) { return n_seg > 1 ? (int64_t)T * n_seg * REC : 0; }
