@@ -32,7 +32,7 @@ namespace {
 
 using namespace kv4;
 
-constexpr int W = 4;          // warps per CTA
+constexpr int W = kRowsGrain;   // warps per CTA
 constexpr int STAGES = 4;     // pages in flight per warp
 constexpr float HEADROOM = 0.875f;   // log2 growth of a row's max before its base moves
 constexpr float LIFT = 2.f;          // P = 2^(z - base + LIFT) <= 2^2.875 < 7.5
@@ -76,15 +76,43 @@ struct Smem {
   };
   uint64_t full[W][STAGES];
   float base[W][COLS], sum[W][COLS];
+  alignas(16) float ml[COLS][2];   // (base, sum) of the CTA, for its cluster
   float qmax[COLS][Lay<D>::NG];
   alignas(16) float qsum[COLS][Lay<D>::NG];
   uint4 qf[NT][Lay<D>::NG][32];
   int fail;   // a wait gave up
 };
 
-template <int D, int NT, bool CAP>
+// Weight of a part (base, sum) against a base m: 0 for one without keys; one whose logits were all NaN (its base
+// never moved) passes its NaN on.
+FAK_DEV float part_weight(float base, float sum, float m) {
+  return base == -INFINITY ? (sum != sum ? 1.f : 0.f) : ex2(base - m);
+}
+// One split's (weight f, sum ls, N outputs z) into the running sums.
+template <int N>
+FAK_DEV void merge_split(float f, float ls, const float* z, float& l, float (&acc)[N]) {
+  if (f == 0.f) return;   // (a split without keys: nothing of it is defined)
+  l = fmaf(f, ls, l);
+#pragma unroll
+  for (int i = 0; i < N; i++) acc[i] = fmaf(f, z[i], acc[i]);
+}
+
+FAK_DEV float2 remote_f2(const float* p, int rank) {   // *p of the cluster's CTA `rank`
+  uint32_t at;
+  float2 v;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(tc::smem_addr(p)), "r"(rank));
+  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(at) : "memory");
+  return v;
+}
+FAK_DEV void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+// CLUSTER: the splits of a block are one thread-block cluster and merge through shared memory; else they
+// leave partial results for k_kv4_combine.  The sums are the same, in the same order.
+template <int D, int NT, bool CAP, bool CLUSTER>
 __global__ void __launch_bounds__(W * 32, 4)
-k_kv4_attn(const __grid_constant__ Kv4Attn a, int n_split, int pps) {
+k_kv4_attn(const __grid_constant__ Kv4Attn a, int n_split) {
   using L = Lay<D>;
   constexpr int NG = L::NG;
   constexpr int COLS = 8 * NT;
@@ -105,8 +133,9 @@ k_kv4_attn(const __grid_constant__ Kv4Attn a, int n_split, int pps) {
   pdl_wait();
 
   const int* row = a.table + (int64_t)b * a.table_stride;
-  const int ahead = split * pps + warp + W * lane;   // without a window a split's first page is known: its table
-  const int early = a.window <= 0 && lane * W < pps && ahead < a.width ? row[ahead] : -1;   // entries travel with ctx
+  // table entries travel with ctx: those of a sequence that fills its table (others are fetched again)
+  const int pps_full = a.window <= 0 ? spread(a.width, n_split, W) : -1, ahead = split * pps_full + warp + W * lane;
+  const int early = lane * W < pps_full && ahead < a.width ? row[ahead] : -1;
   const int ctx = min(a.ctx[b], a.width * PAGE);
   int tok0 = b, n = 1;
   if (a.q_off) {
@@ -119,9 +148,9 @@ k_kv4_attn(const __grid_constant__ Kv4Attn a, int n_split, int pps) {
   }
   const int R = n * G, r0 = rc * COLS;
   if (R <= r0) return;
-  const Span sp = span_of(ctx, n, a.query_of(r0), a.query_of(min(R - 1, r0 + COLS - 1)), a.window, pps, a.width);
-  const int p_begin = sp.p0 + split * pps, p_end = min(sp.p1, p_begin + pps);
-  if (p_begin >= p_end && !(split == 0 && sp.live == 0)) return;
+  const Span sp = span_of(ctx, n, a.query_of(r0), a.query_of(min(R - 1, r0 + COLS - 1)), a.window, n_split, W, a.width);
+  const int p_begin = sp.p0 + split * sp.pps, p_end = min(sp.p1, p_begin + sp.pps);
+  if (!CLUSTER && p_begin >= p_end && !(split == 0 && sp.live == 0)) return;
 
   // pages of this warp: p_begin + warp, + W, ..; 32 table entries at a time, one a lane
   const int np = max(0, (p_end - p_begin - warp + W - 1) / W);
@@ -129,7 +158,7 @@ k_kv4_attn(const __grid_constant__ Kv4Attn a, int n_split, int pps) {
   const uint8_t* page = nullptr;   // lane l: address of page 32 j + l, refreshed every 32 pages
   auto issue = [&](int i) {
     if ((i & 31) == 0 && i + lane < np) {
-      int pid = i == 0 && a.window <= 0 ? early : table[(int64_t)W * (i + lane)];
+      int pid = i == 0 && sp.pps == pps_full ? early : table[(int64_t)W * (i + lane)];
       if ((unsigned)pid >= (uint64_t)a.n_pages) {
         report_error(a.err, 2);
         pid = 0;
@@ -432,13 +461,12 @@ k_kv4_attn(const __grid_constant__ Kv4Attn a, int n_split, int pps) {
     float m = -INFINITY;
 #pragma unroll
     for (int w = 0; w < W; w++) m = fmaxf(m, sm.base[w][c]);
-    const float sink = alone && a.sinks ? a.sinks[h] * LOG2E : -INFINITY;
+    const float sink = !CLUSTER && alone && a.sinks ? a.sinks[h] * LOG2E : -INFINITY;
     const float mt_ = fmaxf(m, sink), bs = mt_ == -INFINITY ? 0.f : mt_;
     float f[W], l = 0.f;
 #pragma unroll
     for (int w = 0; w < W; w++) {
-      f[w] = ex2(sm.base[w][c] - bs);
-      if (sm.base[w][c] == -INFINITY) f[w] = 0.f;
+      f[w] = part_weight(sm.base[w][c], sm.sum[w][c], bs);
       l += f[w] * sm.sum[w][c];
     }
     if (sink > -INFINITY) l += ex2(sink - bs + LIFT);
@@ -452,7 +480,9 @@ k_kv4_attn(const __grid_constant__ Kv4Attn a, int n_split, int pps) {
         v.x += f[w] * y.x;
         v.y += f[w] * y.y;
       }
-      if (alone) {
+      if constexpr (CLUSTER) {
+        *reinterpret_cast<float2*>(&sm.o[0][c][d]) = v;   // (this thread read the element last)
+      } else if (alone) {
         const float inv = l != 0.f ? 1.f / l : 0.f;
         const int64_t at = (int64_t)(tok0 + qi) * a.o_tok + (int64_t)h * a.o_head + d;
         store_elt(a.out, a.o_type, at, v.x * inv);
@@ -461,17 +491,42 @@ k_kv4_attn(const __grid_constant__ Kv4Attn a, int n_split, int pps) {
         *reinterpret_cast<float2*>(a.part + ((part_col + c) * n_split + split) * D + d) = v;
       }
     }
-    if (!alone && lane == 0) {
-      float* ml = part_ml + ((part_col + c) * n_split + split) * 2;
+    if (CLUSTER ? lane == 0 : !alone && lane == 0) {
+      float* ml = CLUSTER ? sm.ml[c] : part_ml + ((part_col + c) * n_split + split) * 2;
       ml[0] = mt_;
       ml[1] = l;
     }
+  }
+  if constexpr (CLUSTER) {
+    cluster_sync();
+    // 32 pairs of dims of a column are one warp's job; the jobs go round the cluster's CTAs
+    for (int job = split + n_split * warp; job < COLS * D / 64; job += n_split * W) {
+      const int c = job / (D / 64), d = job % (D / 64) * 64 + 2 * lane, r = r0 + c;
+      if (r >= R) continue;
+      const int qi = a.query_of(r), h = kvh * G + r - qi * G;
+      const float sink = a.sinks ? a.sinks[h] * LOG2E : -INFINITY;
+      const float2 y = lane < n_split ? remote_f2(sm.ml[c], lane) : make_float2(-INFINITY, 0.f);
+      const float m = fmaxf(sink, warp_max(y.x));
+      const float f = part_weight(y.x, y.y, m);
+      float l = 0.f, acc[2] = {0.f, 0.f};
+#pragma unroll 8
+      for (int s = 0; s < n_split; s++) {
+        const float2 z = remote_f2(&sm.o[0][c][d], s);
+        merge_split(__shfl_sync(0xffffffffu, f, s), __shfl_sync(0xffffffffu, y.y, s), &z.x, l, acc);
+      }
+      if (sink > -INFINITY) l += ex2(sink - m + LIFT);
+      const float inv = l != 0.f ? 1.f / l : 0.f;
+      const int64_t at = (int64_t)(tok0 + qi) * a.o_tok + (int64_t)h * a.o_head + d;
+      store_elt(a.out, a.o_type, at, acc[0] * inv);
+      store_elt(a.out, a.o_type, at + 1, acc[1] * inv);
+    }
+    cluster_sync();   // shared memory stays until every CTA has read it
   }
 }
 
 // One warp merges the live splits of one query row: D / 32 dims a lane, up to 16 splits' loads in flight.
 template <int D>
-__global__ void __launch_bounds__(256) k_kv4_combine(const __grid_constant__ Kv4Attn a, int n_split, int pps, int cols, int row_chunks, float lift) {
+__global__ void __launch_bounds__(256) k_kv4_combine(const __grid_constant__ Kv4Attn a, int n_split, int grain, int cols, int row_chunks, float lift) {
   constexpr int V = D / 32;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rc = blockIdx.x / (cols / 8), kvh = blockIdx.y, b = blockIdx.z;
@@ -490,7 +545,7 @@ __global__ void __launch_bounds__(256) k_kv4_combine(const __grid_constant__ Kv4
   }
   const int R = n * G, r0 = rc * cols;
   if (R <= r0) return;
-  const Span sp = span_of(ctx, n, a.query_of(r0), a.query_of(min(R - 1, r0 + cols - 1)), a.window, pps, a.width);
+  const Span sp = span_of(ctx, n, a.query_of(r0), a.query_of(min(R - 1, r0 + cols - 1)), a.window, n_split, grain, a.width);
   const int live = max(1, sp.live);   // an empty block's split 0 wrote zeros
   if (r0 + c < R) {
     const int r = r0 + c, qi = a.query_of(r), h = kvh * G + r - qi * G;
@@ -502,23 +557,24 @@ __global__ void __launch_bounds__(256) k_kv4_combine(const __grid_constant__ Kv4
       const float2 y = s0 == 0 ? first : s0 + lane < live ? __ldcg(&ml[s0 + lane]) : make_float2(-INFINITY, 0.f);
       const float yb = s0 + lane < live ? y.x : -INFINITY;
       const float mn = fmaxf(m, warp_max(yb));
-      const float keep = m == -INFINITY ? 0.f : ex2(m - mn), f = yb == -INFINITY ? 0.f : ex2(yb - mn);
+      const float keep = m == -INFINITY ? 0.f : ex2(m - mn), f = s0 + lane < live ? part_weight(y.x, y.y, mn) : 0.f;
       m = mn;
-      l = l * keep + warp_sum(f == 0.f ? 0.f : f * y.y);
+      l *= keep;
 #pragma unroll
       for (int i = 0; i < V; i++) acc[i] *= keep;
       const int e = min(32, live - s0);
 #pragma unroll 16
       for (int s = 0; s < e; s++) {
-        const float fs = __shfl_sync(0xffffffffu, f, s);
         const float* p = po + (int64_t)(s0 + s) * D;
+        float z[V];
         if constexpr (V == 4) {
-          const float4 z = __ldcg(reinterpret_cast<const float4*>(p));
-          acc[0] += fs * z.x; acc[1] += fs * z.y; acc[2] += fs * z.z; acc[3] += fs * z.w;
+          const float4 x = __ldcg(reinterpret_cast<const float4*>(p));
+          z[0] = x.x; z[1] = x.y; z[2] = x.z; z[3] = x.w;
         } else {
-          const float2 z = __ldcg(reinterpret_cast<const float2*>(p));
-          acc[0] += fs * z.x; acc[1] += fs * z.y;
+          const float2 x = __ldcg(reinterpret_cast<const float2*>(p));
+          z[0] = x.x; z[1] = x.y;
         }
+        merge_split(__shfl_sync(0xffffffffu, f, s), __shfl_sync(0xffffffffu, y.y, s), z, l, acc);
       }
     }
     if (sink > -INFINITY) l += ex2(sink - m + lift);
@@ -547,11 +603,7 @@ Kv4AttnPlan kv4_attn_plan(const Kv4Attn& a, int n_sm) {
     // 256 rows a CTA, one CTA a SM: with fewer CTAs than SMs the keys are split, eight steps a split at least
     p.row_chunks = (int)((rows + 255) / 256);
     const int64_t ctas = (int64_t)a.B * a.Hkv * p.row_chunks;
-    const int64_t want = a.n_split > 0 ? a.n_split : std::min<int64_t>(n_sm / ctas, a.width / 64);
-    int64_t pps = (a.width + std::max<int64_t>(want, 1) - 1) / std::max<int64_t>(want, 1);
-    pps = (pps + 7) / 8 * 8;
-    p.pps = (int)pps;
-    p.n_split = (int)((a.width + pps - 1) / pps);
+    p.n_split = a.n_split > 0 ? a.n_split : (int)std::max<int64_t>(1, std::min<int64_t>(n_sm / ctas, a.width / 64));
     p.part_floats = p.n_split > 1 ? ctas * 256 * p.n_split * (a.D + 2) : 0;
     return p;
   }
@@ -562,16 +614,27 @@ Kv4AttnPlan kv4_attn_plan(const Kv4Attn& a, int n_sm) {
   // at 4 x 64 rows over 8000.
   p.nt = a.D == 64 && rows > 8 ? 2 : 1;
   p.row_chunks = (int)((rows + 8 * p.nt - 1) / (8 * p.nt));
-  // Splits of pps pages each, the same for every sequence, so that CTAs are alike whatever the lengths: if
-  // every sequence filled its table, 2 1/4 CTAs a SM, between W and 128 pages a split.  (5 x 9000 tokens over 4
-  // KV heads: 16 splits, 320 CTAs, 16.4 us; 29 splits, 580 CTAs, one wave of four a SM, 19.4; 8 splits 21.4.
-  // 32 lanes up to 32768 over 8: 128 pages a split 164 us, 64 184, 256 164.)
-  const int64_t ctas = (int64_t)a.B * a.Hkv * p.row_chunks, room = 9 * (int64_t)n_sm / 4;
-  int64_t pps = a.n_split > 0 ? (a.width + a.n_split - 1) / a.n_split : std::min<int64_t>(128, (a.width * ctas + room - 1) / room);
-  pps = std::max<int64_t>((pps + W - 1) / W * W, W);
-  p.pps = (int)pps;
-  p.n_split = std::max(1, (int)((a.width + pps - 1) / pps));
-  p.part_floats = p.n_split > 1 ? ctas * 8 * p.nt * p.n_split * (a.D + 2) : 0;
+  // Splits: 2 1/4 CTAs a SM, though no more than 40, and 192 pages each at most where every sequence fills its
+  // table.  (us by splits: 16 x 8000 tokens over 4 KV heads 1: 67, 4: 32, 8: 25, 16: 31; 1 x 32000 over 4 8: 37,
+  // 16: 22, 32: 18, 64: 22; 64 lanes up to 4000 over 4 1: 42, 2: 35, 4: 36, 8: 39; 32 lanes up to 32768 over 8
+  // 2: 195, 8: 165, 16: 170, 32: 193.)
+  const int64_t ctas = (int64_t)a.B * a.Hkv * p.row_chunks, most = (a.width + W - 1) / W;
+  int64_t n = a.n_split;
+  if (n <= 0)
+    n = std::min(std::max<int64_t>({1, (a.width + 191) / 192, std::min<int64_t>(40, 9 * (int64_t)n_sm / (4 * ctas))}),
+                 std::max<int64_t>(most, 1));
+  // Up to 16 splits that are resident at once merge inside a cluster, without partial results in memory and a
+  // second launch (1 x 2048 9.8 -> 5.8 us); a warp may have nine pages then before more splits pay for them.
+  int64_t c = 1;
+  while (c < 16 && 2 * c * ctas <= 4 * n_sm && c < most) c *= 2;
+  if (a.n_split > 0) {
+    p.cluster = n > 1 && n <= c && (n & (n - 1)) == 0;
+  } else if (c > 1 && n > 1 && (n <= c || a.width <= 9 * W * c)) {
+    p.cluster = true;
+    n = c;
+  }
+  p.n_split = (int)n;
+  p.part_floats = p.n_split > 1 && !p.cluster ? ctas * 8 * p.nt * p.n_split * (a.D + 2) : 0;
   return p;
 }
 
@@ -580,18 +643,26 @@ static void split_launch(const Kv4Attn& a, const Kv4AttnPlan& p, cudaStream_t st
   cfg.gridDim = dim3((unsigned)(p.n_split * p.row_chunks), (unsigned)a.Hkv, (unsigned)a.B);
   cfg.blockDim = dim3(W * 32);
   cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   pdl(cfg, attr);
+  if (p.cluster) {
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim = {(unsigned)p.n_split, 1, 1};
+    cfg.numAttrs = 2;
+  }
   auto go = [&](auto kern, size_t smem) {
     cfg.dynamicSmemBytes = smem;
     FAK_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-    FAK_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kern, a, p.n_split, p.pps));
+    if (p.cluster) FAK_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+    FAK_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kern, a, p.n_split));
   };
   const bool cap = a.softcap > 0.f;
-#define FAK_KV4(DV, NTV)                                                    \
-  {                                                                         \
-    if (cap) go(k_kv4_attn<DV, NTV, true>, sizeof(Smem<DV, NTV>));          \
-    else go(k_kv4_attn<DV, NTV, false>, sizeof(Smem<DV, NTV>));             \
+#define FAK_KV4(DV, NTV)                                                                  \
+  {                                                                                       \
+    if (cap && p.cluster) go(k_kv4_attn<DV, NTV, true, true>, sizeof(Smem<DV, NTV>));     \
+    else if (cap) go(k_kv4_attn<DV, NTV, true, false>, sizeof(Smem<DV, NTV>));            \
+    else if (p.cluster) go(k_kv4_attn<DV, NTV, false, true>, sizeof(Smem<DV, NTV>));      \
+    else go(k_kv4_attn<DV, NTV, false, false>, sizeof(Smem<DV, NTV>));                    \
   }
   if (a.D == 128) FAK_KV4(128, 1)
   else if (p.nt == 1) FAK_KV4(64, 1)
@@ -603,15 +674,15 @@ void kv4_attn_launch(const Kv4Attn& a, const Kv4AttnPlan& p, cudaStream_t stream
   if (p.tc) kv4_prefill_launch(a, p, stream);
   else split_launch(a, p, stream);
   cudaLaunchAttribute attr[1];
-  if (p.n_split > 1) {
+  if (p.n_split > 1 && !p.cluster) {
     cudaLaunchConfig_t c2 = {};
     const int cols = p.tc ? 256 : 8 * p.nt;
     c2.gridDim = dim3((unsigned)(p.row_chunks * cols / 8), (unsigned)a.Hkv, (unsigned)a.B);
     c2.blockDim = dim3(256);
     c2.stream = stream;
     pdl(c2, attr);
-    if (a.D == 128) FAK_CUDA_CHECK(cudaLaunchKernelEx(&c2, k_kv4_combine<128>, a, p.n_split, p.pps, cols, p.row_chunks, p.tc ? kPrefillLift : LIFT));
-    else FAK_CUDA_CHECK(cudaLaunchKernelEx(&c2, k_kv4_combine<64>, a, p.n_split, p.pps, cols, p.row_chunks, p.tc ? kPrefillLift : LIFT));
+    if (a.D == 128) FAK_CUDA_CHECK(cudaLaunchKernelEx(&c2, k_kv4_combine<128>, a, p.n_split, p.tc ? kTilesGrain : kRowsGrain, cols, p.row_chunks, p.tc ? kPrefillLift : LIFT));
+    else FAK_CUDA_CHECK(cudaLaunchKernelEx(&c2, k_kv4_combine<64>, a, p.n_split, p.tc ? kTilesGrain : kRowsGrain, cols, p.row_chunks, p.tc ? kPrefillLift : LIFT));
   }
 }
 

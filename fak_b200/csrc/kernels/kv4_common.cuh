@@ -5,8 +5,12 @@
 
 #include "../serve_ops.h"
 
+#define FAK_HD __host__ __device__
+
 namespace fak {
 namespace kv4 {
+
+constexpr int kRowsGrain = 4, kTilesGrain = 8;   // pages: a warp's one of the streaming CTA's four; a step of 128 keys
 
 FAK_DEV uint32_t pack_f16(float lo, float hi) {
   const __half2 h = __floats2half2_rn(lo, hi);
@@ -46,19 +50,25 @@ FAK_DEV void lds(const uint8_t* p, uint32_t (&r)[N]) {
   }
 }
 
-// The pages one CTA column block needs, and how the splits share them: the same arithmetic in the
-// attention kernel and in the combine.
+// The pages one CTA column block needs and how n_split splits share them, `grain` pages at least: the same
+// arithmetic in the attention kernels and in the combine.  It depends on the sequence alone.
+FAK_HD inline int spread(int pages, int n_split, int grain) {
+  const int each = (pages + n_split - 1) / n_split;
+  return each <= grain ? grain : (each + grain - 1) / grain * grain;
+}
 struct Span {
-  int p0, p1, live;   // pages [p0, p1), splits of pps pages that hold any
+  int p0, p1, pps, live;   // pages [p0, p1), pages a split, splits that hold any
 };
-FAK_DEV Span span_of(int ctx, int n, int i_lo, int i_hi, int window, int pps, int width) {
+FAK_DEV Span span_of(int ctx, int n, int i_lo, int i_hi, int window, int n_split, int grain, int width) {
   Span s;
   const int last = min(ctx - n + i_hi, ctx - 1);               // the last key any row of the block sees
   const int first = window > 0 ? max(0, ctx - n + i_lo + 1 - window) : 0;
   s.p0 = first / PAGE;
   s.p1 = min(width, last / PAGE + 1);
   if (last < 0) s.p1 = s.p0;
-  s.live = (max(0, s.p1 - s.p0) + pps - 1) / pps;
+  const int pages = max(0, s.p1 - s.p0);
+  s.pps = spread(pages, n_split, grain);
+  s.live = (pages + s.pps - 1) / s.pps;
   return s;
 }
 

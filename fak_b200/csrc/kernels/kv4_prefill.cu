@@ -38,6 +38,7 @@ using kv4::Span;
 constexpr int ROWS = 128;          // query rows per tile, two tiles a CTA
 constexpr int KEYS = 128;          // keys per step
 constexpr int PPT = KEYS / PAGE;   // pages per step
+static_assert(PPT == kv4::kTilesGrain, "splits of whole steps");
 constexpr int SLOTS = 12;          // ring slots of page halves
 constexpr int THREADS = 512;
 constexpr float LIFT = 4.f, HEADROOM = 8.f;
@@ -136,7 +137,7 @@ FAK_DEV uint32_t dup_hi(uint32_t x) { return __byte_perm(x, x, 0x3232); }
 
 template <int D, bool CAP>
 __global__ void __launch_bounds__(THREADS, 1)
-k_kv4_prefill(const __grid_constant__ Kv4Attn a, int n_split, int pps) {
+k_kv4_prefill(const __grid_constant__ Kv4Attn a, int n_split) {
   using L = Lay<D>;
   constexpr int NG = L::NG;
   extern __shared__ uint8_t smem_raw[];
@@ -160,8 +161,8 @@ k_kv4_prefill(const __grid_constant__ Kv4Attn a, int n_split, int pps) {
   const int R = n * G, r0 = blk * 2 * ROWS;
   if (R <= r0) return;
   const int i_first = a.query_of(r0), i_last = a.query_of(min(R - 1, r0 + 2 * ROWS - 1));
-  const Span sp = kv4::span_of(ctx, n, i_first, i_last, a.window, pps, a.width);
-  const int p_begin = sp.p0 + split * pps, p_end = min(sp.p1, p_begin + pps);
+  const Span sp = kv4::span_of(ctx, n, i_first, i_last, a.window, n_split, kv4::kTilesGrain, a.width);
+  const int p_begin = sp.p0 + split * sp.pps, p_end = min(sp.p1, p_begin + sp.pps);
   if (p_begin >= p_end && !(split == 0 && sp.live == 0)) return;
   const int n_pages = max(0, p_end - p_begin);
   const int NJ = (n_pages + PPT - 1) / PPT;
@@ -588,7 +589,7 @@ void kv4_prefill_launch(const Kv4Attn& a, const Kv4AttnPlan& p, cudaStream_t str
   auto go = [&](auto kern, size_t smem) {
     cfg.dynamicSmemBytes = smem + 1024;
     FAK_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)cfg.dynamicSmemBytes));
-    FAK_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kern, a, p.n_split, p.pps));
+    FAK_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kern, a, p.n_split));
   };
   const bool cap = a.softcap > 0.f;
   if (a.D == 128 && cap) go(k_kv4_prefill<128, true>, sizeof(Smem<128>));

@@ -52,8 +52,8 @@ struct Kv4Attn {
   int* err;
 };
 struct Kv4AttnPlan {
-  bool tc;
-  int nt, row_chunks, n_split, pps;
+  bool tc, cluster;   // tiles of query rows on tcgen05; the splits merge inside thread-block clusters
+  int nt, row_chunks, n_split;
   int64_t part_floats;
 };
 Kv4AttnPlan kv4_attn_plan(const Kv4Attn& a, int n_sm);

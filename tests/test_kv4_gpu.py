@@ -237,6 +237,39 @@ def test_decode_nan_value_beyond_the_window_is_not_read(K):
     assert torch.isnan(out).all()
 
 
+@pytest.mark.parametrize("lens,n_split", [([1], 1), ([17], 4), ([200], 16), ([200], 20)])
+def test_decode_all_keys_nan(K, lens, n_split):
+    """No finite logit anywhere is not the same as no key."""
+    g = gen(1)
+    pages, table, ks, vs = cache_of(K, g, lens, 1, 64)
+    j = torch.arange(lens[0], device="cuda")
+    bad = torch.full((lens[0], 1, 64), math.nan, device="cuda")
+    K.kv4_append(bad, bad, (table[0, j // 16] * 16 + j % 16).to(torch.int32), pages)
+    out = torch.zeros(1, 2, 64, device="cuda")
+    K.kv4_decode_attention(torch.randn(1, 2, 64, device="cuda"), pages, table,
+                           torch.tensor(lens, dtype=torch.int32, device="cuda"), out, n_split=n_split)
+    assert torch.isnan(out).all()
+
+
+@pytest.mark.parametrize("H,Hkv,D", [(28, 4, 128), (16, 2, 64), (24, 1, 128)])
+@pytest.mark.parametrize("sink", [False, True])
+def test_decode_splits_merge_alike_in_clusters_and_in_memory(K, H, Hkv, D, sink):
+    """2 to 16 splits merge in a cluster while their CTAs are all resident, else through memory: a sequence's
+    bits are the same, alone (clusters) and in a batch of 40 (memory)."""
+    g = gen(8)
+    lens = [700, 33, 1, 250] * 10
+    pages, table, ks, vs = cache_of(K, g, lens, Hkv, D)
+    ctx = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    q = torch.randn(40, H, D, generator=g, device="cuda").to(torch.bfloat16)
+    sinks = torch.randn(H, generator=g, device="cuda") if sink else None
+    for n_split in (2, 8, 16):
+        every, one = torch.empty(40, H, D, device="cuda"), torch.empty(1, H, D, device="cuda")
+        K.kv4_decode_attention(q, pages, table, ctx, every, n_split=n_split, sinks=sinks)
+        for b in range(5):
+            K.kv4_decode_attention(q[b:b + 1], pages, table[b:b + 1], ctx[b:b + 1], one, n_split=n_split, sinks=sinks)
+            assert torch.equal(one[0], every[b])
+
+
 def test_decode_strides_and_streams(K):
     lens, H, Hkv, D = [50, 20], 8, 2, 64
     g = gen(2)
@@ -313,7 +346,7 @@ def test_refusals(K):
     with pytest.raises(RuntimeError, match="int32"):
         K.kv4_decode_attention(q, pages, table.long(), ctx, out)
     with pytest.raises(RuntimeError, match="workspace"):
-        K.kv4_decode_attention(q, pages, torch.zeros(1, 64, dtype=torch.int32, device="cuda"), ctx, out, n_split=4,
+        K.kv4_decode_attention(q, pages, torch.zeros(1, 64, dtype=torch.int32, device="cuda"), ctx, out, n_split=20,
                                workspace=torch.zeros(8, device="cuda"))
     with pytest.raises(RuntimeError, match="max_new"):
         K.kv4_prefill_attention(q, pages, table, torch.zeros(2, dtype=torch.int32, device="cuda"), ctx, out, 2)
