@@ -137,6 +137,7 @@ k_kv4_attn(const __grid_constant__ Kv4Attn a, int n_split) {
   const int pps_full = a.window <= 0 ? spread(a.width, n_split, W) : -1, ahead = split * pps_full + warp + W * lane;
   const int early = lane * W < pps_full && ahead < a.width ? row[ahead] : -1;
   const int ctx = min(a.ctx[b], a.width * PAGE);
+  if (tid == 0 && a.ctx[b] > ctx) report_error(a.err, 2);   // more keys than the table has pages for
   int tok0 = b, n = 1;
   if (a.q_off) {
     tok0 = max(a.q_off[b], 0);

@@ -49,6 +49,18 @@ FAK_DEV void lds(const uint8_t* p, uint32_t (&r)[N]) {
     r[0] = *reinterpret_cast<const uint32_t*>(p);
   }
 }
+template <int N>
+FAK_DEV void ldg(const uint8_t* p, uint32_t (&r)[N]) {
+  if constexpr (N == 4) {
+    const uint4 v = __ldg(reinterpret_cast<const uint4*>(p));
+    r[0] = v.x; r[1] = v.y; r[2] = v.z; r[3] = v.w;
+  } else if constexpr (N == 2) {
+    const uint2 v = __ldg(reinterpret_cast<const uint2*>(p));
+    r[0] = v.x; r[1] = v.y;
+  } else {
+    r[0] = __ldg(reinterpret_cast<const uint32_t*>(p));
+  }
+}
 
 // The pages one CTA column block needs and how n_split splits share them, `grain` pages at least: the same
 // arithmetic in the attention kernels and in the combine.  It depends on the sequence alone.

@@ -5,17 +5,19 @@
 // 256 rows whatever the group size.  Warp roles:
 //   warps 0-3, 4-7  softmax of tile 0 / 1, one row a thread: S from TMEM, P = 2^(S c - base) back into
 //                   TMEM as f16 over the first half of S's columns (the A operand of P V is read there);
-//   warps 8-11      dequantization: codes of 128 keys to f16 K [keys][dims] and V^T [dims][keys] in the
-//                   128-byte swizzle, two buffers each;
-//   warps 12, 15    issue the matrix products of tile 0 / 1, S = Q K^T and O += P V, so that one tile's softmax
-//                   runs under the other's products (one warp for both, polling, took 0.7k cycles to notice);
-//   warps 13, 14    bulk copies of the pages' K and V halves into rings of 12 slots (one warp for both made
-//                   K wait for V's slots: 7.3k cycles a step even without softmax and dequantization).
-// A step's 128 keys are taken in halves: P of the first 64 is multiplied while the softmax of the others
-// runs.  A row's exponent base moves only when a half's maximum outgrows it by 2^8 (then O is scaled, after
-// the first half's product where there is one), so P <= 2^12 and S is read once.  Steps that need a mask or a soft-cap are rewritten in TMEM by a small loop first: the main
-// loop then has one form, which matters because four roles' code shares the instruction caches (with the
-// mask inside the unrolled loops, waits for instructions were the first stall and a step took 12.6k cycles).
+//   warps 8-11      dequantization: codes of 128 keys, fetched a step ahead into registers, to f16 K
+//                   [keys][dims] and V^T [dims][keys] in the 128-byte swizzle, two buffers each (bulk copies
+//                   into rings of 12 page halves held 4.0k cycles a step on their own);
+//   warps 12, 13    issue the matrix products of tile 0 / 1, S = Q K^T and O += P V, so that one tile's softmax
+//                   runs under the other's products (one warp for both, polling, took 0.7k cycles to notice).
+// The work of a tile goes in halves of 64 keys with two buffers of S: S of half u + 1 is multiplied while the
+// softmax of half u runs, once the P in its columns (of half u - 1) is used up.  (128 x 64 products take 48
+// cycles for every 16 dims, three quarters of the rate of 128 x 128 ones; whole steps with one buffer of S left
+// the softmax waiting for its own products.)  A row's exponent base moves only when a half's maximum outgrows
+// it by 2^8 (then O is scaled, after the product of the half before), so P <= 2^12 and S is read once.  Halves
+// that need a mask or a soft-cap are rewritten in TMEM by a small loop first: the main loop then has one form,
+// which matters because three roles' code shares the instruction caches (with the mask inside the unrolled
+// loops, waits for instructions were the first stall and a step took 12.6k cycles).
 // Orders: a K chunk of 8 dims keeps its nibble pairs (0,4) (1,5) (2,6) (3,7) and Q is stored in the same
 // order; within a page's upper half the pairs of keys are swapped (key ^ 2), which keeps the V reads of a
 // warp on distinct banks, and the masks follow.
@@ -39,23 +41,17 @@ constexpr int ROWS = 128;          // query rows per tile, two tiles a CTA
 constexpr int KEYS = 128;          // keys per step
 constexpr int PPT = KEYS / PAGE;   // pages per step
 static_assert(PPT == kv4::kTilesGrain, "splits of whole steps");
-constexpr int SLOTS = 12;          // ring slots of page halves
-constexpr int THREADS = 512;
+constexpr int THREADS = 448;
 constexpr float LIFT = 4.f, HEADROOM = 8.f;
 constexpr float LOG2E = 1.4426950408889634f;
 
 template <int D>
 struct Smem {
-  static constexpr int HALF = Lay<D>::VC;          // bytes of a page's K part, and of its V part
-  static constexpr int SLOT_V = HALF + 64;         // (an odd multiple of 64 spreads two pages over the banks)
   alignas(1024) __half q[2][D / 64][ROWS * 64];    // [tile][64-dim half][row][64]
   alignas(1024) __half k[2][D / 64][KEYS * 64];    // [buffer][64-dim half][key][64]
   alignas(1024) __half v[2][2][D * 64];            // [buffer][64-key half][dim][64]
-  alignas(128) uint8_t raw_k[SLOTS][HALF];
-  alignas(128) uint8_t raw_v[SLOTS][SLOT_V];
   uint64_t q_full, k_full[2], k_empty[2], v_full[2], v_empty[2];
-  uint64_t s_full[2], p_full[2][2], pv_half[2], pv_done[2], turn[2];   // p_full: [tile][64-key half]
-  uint64_t rk_full[SLOTS], rk_empty[SLOTS], rv_full[SLOTS], rv_empty[SLOTS];
+  uint64_t s_full[2][2], p_full[2][2], pv_done[2][2];   // [tile][64-key half]
   uint32_t tmem;
   int fail;
 };
@@ -149,6 +145,7 @@ k_kv4_prefill(const __grid_constant__ Kv4Attn a, int n_split) {
   const int G = a.G;
   pdl_wait();
   const int ctx = min(a.ctx[b], a.width * PAGE);
+  if (threadIdx.x == 0 && a.ctx[b] > ctx) report_error(a.err, 2);   // more keys than the table has pages for
   int tok0 = b, n = 1;
   if (a.q_off) {
     tok0 = max(a.q_off[b], 0);
@@ -165,7 +162,7 @@ k_kv4_prefill(const __grid_constant__ Kv4Attn a, int n_split) {
   const int p_begin = sp.p0 + split * sp.pps, p_end = min(sp.p1, p_begin + sp.pps);
   if (p_begin >= p_end && !(split == 0 && sp.live == 0)) return;
   const int n_pages = max(0, p_end - p_begin);
-  const int NJ = (n_pages + PPT - 1) / PPT;
+  const int NJ = (n_pages + PPT - 1) / PPT, NU = (n_pages + PPT / 2 - 1) / (PPT / 2);   // steps; halves of 64 keys
   const int tiles = R - r0 > ROWS ? 2 : 1;
   const int lim_any = ctx - n + i_last + 1;                                            // keys some row sees: below
   const int low_any = a.window > 0 ? max(0, ctx - n + i_first + 1 - a.window) : 0;     // and from here
@@ -177,18 +174,11 @@ k_kv4_prefill(const __grid_constant__ Kv4Attn a, int n_split) {
       tc::mbar_init(&sm.k_empty[i], tiles);
       tc::mbar_init(&sm.v_full[i], 4);
       tc::mbar_init(&sm.v_empty[i], tiles);
-      tc::mbar_init(&sm.s_full[i], 1);
-      tc::mbar_init(&sm.p_full[i][0], 4);
-      tc::mbar_init(&sm.p_full[i][1], 4);
-      tc::mbar_init(&sm.pv_half[i], 1);
-      tc::mbar_init(&sm.turn[i], 4);
-      tc::mbar_init(&sm.pv_done[i], 1);
-    }
-    for (int i = 0; i < SLOTS; i++) {
-      tc::mbar_init(&sm.rk_full[i], 1);
-      tc::mbar_init(&sm.rk_empty[i], 1);
-      tc::mbar_init(&sm.rv_full[i], 1);
-      tc::mbar_init(&sm.rv_empty[i], 1);
+      for (int h = 0; h < 2; h++) {
+        tc::mbar_init(&sm.s_full[i][h], 1);
+        tc::mbar_init(&sm.p_full[i][h], 4);
+        tc::mbar_init(&sm.pv_done[i][h], 1);
+      }
     }
     sm.fail = 0;
     tc::fence_mbar_init();
@@ -204,38 +194,12 @@ k_kv4_prefill(const __grid_constant__ Kv4Attn a, int n_split) {
   int* fail = &sm.fail;
 
   if (warp >= 12) {
-    if (warp == 13 || warp == 14) {
-      // ---- page loaders: lane l holds the address of page 32 i + l
-      const bool is_v = warp == 14;
-      const int* table = a.table + (int64_t)b * a.table_stride + p_begin;
-      uint64_t* full = is_v ? sm.rv_full : sm.rk_full;
-      uint64_t* empty = is_v ? sm.rv_empty : sm.rk_empty;
-      uint8_t* ring = is_v ? sm.raw_v[0] : sm.raw_k[0];
-      const int pitch = is_v ? Smem<D>::SLOT_V : Smem<D>::HALF;
-      const uint8_t* src = nullptr;
-#pragma unroll 1
-      for (int i = 0; i < n_pages; i++) {
-        if ((i & 31) == 0 && i + lane < n_pages) {
-          int pid = table[i + lane];
-          if ((unsigned)pid >= (uint64_t)a.n_pages) {
-            report_error(a.err, 2);
-            pid = 0;
-          }
-          src = a.pages + ((int64_t)pid * a.Hkv + kvh) * L::BYTES + (is_v ? L::VC : 0);
-        }
-        const int s = i % SLOTS;
-        if (lane == (i & 31)) {
-          tc::mbar_wait(&empty[s], (uint32_t)((i / SLOTS) & 1) ^ 1u, fail);
-          tc::mbar_arrive_expect_tx(&full[s], Smem<D>::HALF);
-          kv4::bulk_load(ring + s * pitch, src, Smem<D>::HALF, &full[s]);
-        }
-        __syncwarp();
-      }
-    } else if (const int t = warp == 12 ? 0 : 1; t < tiles && NJ > 0) {
+    if (const int t = warp - 12; t < tiles && NJ > 0) {
       // ---- matrix products of tile t.  The whole warp walks the loop, so that descriptors stay warp-uniform; one
       // lane's instructions take effect.
-      constexpr uint32_t id_s = idesc_f16(ROWS, KEYS), id_o = idesc_f16(ROWS, D);
-      constexpr uint32_t HALF_Q = ROWS * 128 / 16, HALF_V = D * 128 / 16;   // 64-dim / 64-key halves, 16-byte units
+      constexpr uint32_t id_s = idesc_f16(ROWS, KEYS / 2), id_o = idesc_f16(ROWS, D);
+      // 64-dim halves of Q and K, 64-key halves of K and V, in units of 16 bytes
+      constexpr uint32_t HALF_Q = ROWS * 128 / 16, KEYS_K = KEYS / 2 * 128 / 16, HALF_V = D * 128 / 16;
       const uint32_t leader = elect_one();
       const uint32_t hi = (uint32_t)(tc::smem_desc_sw128(sm.q) >> 32);      // (the same for every operand)
       const uint32_t lq = (uint32_t)tc::smem_desc_sw128(sm.q) + t * (D / 64) * HALF_Q;
@@ -243,90 +207,107 @@ k_kv4_prefill(const __grid_constant__ Kv4Attn a, int n_split) {
       const uint32_t ts = tmem + t * 128, to = tmem + 256 + t * D;
       tc::mbar_wait(&sm.q_full, 0, fail);
 #pragma unroll 1
-      for (int j = 0; j < NJ; j++) {
-        const uint32_t buf = j & 1, par = j & 1, par2 = (j >> 1) & 1;
-        tc::mbar_wait(&sm.k_full[buf], par2, fail);
-        if (j > 0) tc::mbar_wait(&sm.pv_done[t], par ^ 1u, fail);   // P sits in S's columns until its product is done
-        // the tiles keep half a step apart: each waits until a quarter of the other's softmax is through
-        if (t == 1) tc::mbar_wait(&sm.turn[0], par, fail);
-        else if (j > 0 && tiles == 2) tc::mbar_wait(&sm.turn[1], par ^ 1u, fail);
-        __syncwarp();
-        tc::tc_fence_after();
-        const uint32_t k = lk + buf * (D / 64) * HALF_Q;
+      for (int u = 0; u <= NU; u++) {   // S of half u, then O += P V of half u - 1
+        if (u < NU) {
+          const int j = u >> 1, h = u & 1;
+          const uint32_t buf = j & 1;
+          if (h == 0) tc::mbar_wait(&sm.k_full[buf], (uint32_t)(j >> 1) & 1, fail);
+          if (u > 1) tc::mbar_wait(&sm.pv_done[t][h], (uint32_t)(j - 1) & 1, fail);   // P of half u - 2 sits in these columns
+          __syncwarp();
+          tc::tc_fence_after();
+          const uint32_t k = lk + buf * (D / 64) * HALF_Q + h * KEYS_K;
 #pragma unroll
-        for (int kk = 0; kk < D / 16; kk++)
-          mma_ss(ts, lq + (kk >> 2) * HALF_Q + 2 * (kk & 3), k + (kk >> 2) * HALF_Q + 2 * (kk & 3), hi, id_s, kk != 0, leader);
-        commit(&sm.s_full[t], leader);
-        commit(&sm.k_empty[buf], leader);
-        tc::mbar_wait(&sm.v_full[buf], par2, fail);
-#pragma unroll
-        for (int h = 0; h < 2; h++) {   // each half of P V once that half of P is there
-          tc::mbar_wait(&sm.p_full[t][h], par, fail);
+          for (int kk = 0; kk < D / 16; kk++)
+            mma_ss(ts + h * 64, lq + (kk >> 2) * HALF_Q + 2 * (kk & 3), k + (kk >> 2) * HALF_Q + 2 * (kk & 3), hi, id_s, kk != 0, leader);
+          commit(&sm.s_full[t][h], leader);
+          if (h == 1) commit(&sm.k_empty[buf], leader);
+        }
+        if (u > 0) {
+          const int j = (u - 1) >> 1, h = (u - 1) & 1;
+          const uint32_t buf = j & 1;
+          if (h == 0) tc::mbar_wait(&sm.v_full[buf], (uint32_t)(j >> 1) & 1, fail);
+          tc::mbar_wait(&sm.p_full[t][h], (uint32_t)j & 1, fail);
           __syncwarp();
           tc::tc_fence_after();
           const uint32_t v = lv + (buf * 2 + h) * HALF_V;
 #pragma unroll
-          for (int ks = 0; ks < 4; ks++) mma_ts(to, ts + h * 32 + ks * 8, v + 2 * ks, hi, id_o, ks != 0 || h > 0 || j > 0, leader);
-          commit(h == 0 ? &sm.pv_half[t] : &sm.pv_done[t], leader);
+          for (int ks = 0; ks < 4; ks++) mma_ts(to, ts + h * 64 + ks * 8, v + 2 * ks, hi, id_o, ks != 0 || u > 1, leader);
+          commit(&sm.pv_done[t][h], leader);
+          if (h == 1) commit(&sm.v_empty[buf], leader);
         }
-        commit(&sm.v_empty[buf], leader);
       }
     }
   } else if (warp >= 8) {
-    // ---- dequantization: this warp's two pages of every step
+    // ---- dequantization: this warp's two pages of every step, fetched a step ahead into registers
     const int w = warp - 8;
     // K lanes: (token bits 0, 1, 2; t); V lanes: (g, half of the page, page of the pair)
     const int kt = lane & 3, ktok = ((lane >> 2) & 1) * 4 + (lane >> 3);
     const int vg = (lane & 1) | (lane >> 3) << 1, vh = (lane >> 1) & 1, vp = (lane >> 2) & 1;
+    const int* table = a.table + (int64_t)b * a.table_stride + p_begin;
+    uint32_t kc[4][NG], ks[4][NG / 2], km[4][NG / 2], vc[4][NG], vs[4][NG], vm[4][NG];
+    auto entries = [&](int j) {   // 16 steps of the table: lane 2 i + u holds page u of step j + i
+      const int i = (j + (lane >> 1)) * PPT + 2 * w + (lane & 1);
+      int pid = i < n_pages ? table[i] : 0;
+      if ((unsigned)pid >= (uint64_t)a.n_pages) {
+        report_error(a.err, 2);
+        pid = 0;
+      }
+      return pid;
+    };
+    int ids = NJ > 0 ? entries(0) : 0, ids_next = 0;
+    auto fetch_k = [&](int j) {
+      if (j >= NJ) return;
+      if ((j & 15) == 0) {
+        if (j > 0) ids = ids_next;
+        ids_next = entries(j + 16);
+      }
+#pragma unroll
+      for (int u = 0; u < 2; u++) {
+        const uint8_t* pg = a.pages + ((int64_t)__shfl_sync(0xffffffffu, ids, 2 * (j & 15) + u) * a.Hkv + kvh) * L::BYTES;
+#pragma unroll
+        for (int hf = 0; hf < 2; hf++) {
+          const int tok = hf * 8 + ktok;
+          kv4::ldg(pg + L::KC + tok * (D / 2) + kt * 4 * NG, kc[2 * u + hf]);
+          kv4::ldg(pg + L::KS + tok * 2 * NG, ks[2 * u + hf]);
+          kv4::ldg(pg + L::KM + tok * 2 * NG, km[2 * u + hf]);
+        }
+      }
+    };
+    auto fetch_v = [&](int j) {
+      if (j >= NJ) return;
+      const uint8_t* pg = a.pages + ((int64_t)__shfl_sync(0xffffffffu, ids, 2 * (j & 15) + vp) * a.Hkv + kvh) * L::BYTES;
+#pragma unroll
+      for (int e = 0; e < 4; e++) {
+        const int p = vh * 4 + (e ^ vh);
+        kv4::ldg(pg + L::VC + ((p * 8 + (vg ^ (2 * (p & 3)))) * NG) * 4, vc[e]);
+        kv4::ldg(pg + L::VS + p * NG * 4, vs[e]);
+        kv4::ldg(pg + L::VM + p * NG * 4, vm[e]);
+      }
+    };
+    fetch_k(0);
+    fetch_v(0);
+#pragma unroll 1
     for (int j = 0; j < NJ; j++) {
       const int buf = j & 1;
       const uint32_t free_parity = (uint32_t)((j >> 1) & 1) ^ 1u;
       tc::mbar_wait(&sm.k_empty[buf], free_parity, fail);
-#pragma unroll 1
-      for (int u = 0; u < 2; u++) {
-        const int i = j * PPT + 2 * w + u, s = i % SLOTS;
-        if (i < n_pages) {   // (rows of pages that do not exist are masked in S)
-          tc::mbar_wait(&sm.rk_full[s], (uint32_t)((i / SLOTS) & 1), fail);
-          const uint8_t* pg = sm.raw_k[s];
-#pragma unroll 1
-          for (int hf = 0; hf < 2; hf++) {
-            const int tok = hf * 8 + ktok;
-            uint32_t c[NG], sc[NG / 2], mn[NG / 2];
-            kv4::lds(pg + L::KC + tok * (D / 2) + kt * 4 * NG, c);
-            kv4::lds(pg + L::KS + tok * 2 * NG, sc);
-            kv4::lds(pg + L::KM + tok * 2 * NG, mn);
-            const int row = (2 * w + u) * PAGE + (tok ^ (hf * 2));
+      // (rows of pages that do not exist hold whatever page 0 does; they are masked in S)
 #pragma unroll
-            for (int gr = 0; gr < NG; gr++) {
-              uint32_t o[4];
-              dequant_word(c[gr], gr & 1 ? dup_hi(sc[gr / 2]) : dup_lo(sc[gr / 2]), gr & 1 ? dup_hi(mn[gr / 2]) : dup_lo(mn[gr / 2]), o);
-              uint8_t* dst = reinterpret_cast<uint8_t*>(sm.k[buf][gr >> 1]) + row * 128 + ((((gr & 1) * 4 + kt) ^ (row & 7)) << 4);
-              *reinterpret_cast<uint4*>(dst) = make_uint4(o[0], o[1], o[2], o[3]);
-            }
-          }
-          __syncwarp();
-          if (lane == 0) tc::mbar_arrive(&sm.rk_empty[s]);
+      for (int x = 0; x < 4; x++) {
+        const int row = (2 * w + (x >> 1)) * PAGE + (((x & 1) * 8 + ktok) ^ ((x & 1) * 2));
+#pragma unroll
+        for (int gr = 0; gr < NG; gr++) {
+          uint32_t o[4];
+          dequant_word(kc[x][gr], gr & 1 ? dup_hi(ks[x][gr / 2]) : dup_lo(ks[x][gr / 2]), gr & 1 ? dup_hi(km[x][gr / 2]) : dup_lo(km[x][gr / 2]), o);
+          uint8_t* dst = reinterpret_cast<uint8_t*>(sm.k[buf][gr >> 1]) + row * 128 + ((((gr & 1) * 4 + kt) ^ (row & 7)) << 4);
+          *reinterpret_cast<uint4*>(dst) = make_uint4(o[0], o[1], o[2], o[3]);
         }
       }
       tc::fence_proxy_async();
       __syncwarp();
       if (lane == 0) tc::mbar_arrive(&sm.k_full[buf]);
 
-      tc::mbar_wait(&sm.v_empty[buf], free_parity, fail);
-      const int i0 = j * PPT + 2 * w, i = i0 + vp, s = i % SLOTS;
-      if (i0 < n_pages) tc::mbar_wait(&sm.rv_full[i0 % SLOTS], (uint32_t)((i0 / SLOTS) & 1), fail);
-      if (i0 + 1 < n_pages) tc::mbar_wait(&sm.rv_full[(i0 + 1) % SLOTS], (uint32_t)(((i0 + 1) / SLOTS) & 1), fail);
-      uint32_t c[4][NG], sc[4][NG], mn[4][NG];
-      const uint8_t* pg = sm.raw_v[s];   // (offsets of the layout count from the page's start)
-      const int key0 = (p_begin + i) * PAGE;
-#pragma unroll
-      for (int e = 0; e < 4; e++) {
-        const int p = vh * 4 + (e ^ vh);
-        kv4::lds(pg + ((p * 8 + (vg ^ (2 * (p & 3)))) * NG) * 4, c[e]);
-        kv4::lds(pg + L::VS - L::VC + p * NG * 4, sc[e]);
-        kv4::lds(pg + L::VM - L::VC + p * NG * 4, mn[e]);
-      }
-      const int step0 = (p_begin + j * PPT) * PAGE;
+      const int i = j * PPT + 2 * w + vp, key0 = (p_begin + i) * PAGE, step0 = (p_begin + j * PPT) * PAGE;
       if (step0 < low_any || step0 + KEYS > min(lim_any, p_end * PAGE)) {
         // tokens no row sees (memory nobody wrote, pages that do not exist): zero
 #pragma unroll
@@ -336,17 +317,19 @@ k_kv4_prefill(const __grid_constant__ Kv4Attn a, int n_split) {
                                 (i < n_pages && key + 1 >= low_any && key + 1 < lim_any ? 0xffff0000u : 0u);
 #pragma unroll
           for (int gr = 0; gr < NG; gr++) {
-            sc[e][gr] &= keep;
-            mn[e][gr] &= keep;
+            vs[e][gr] &= keep;
+            vm[e][gr] &= keep;
           }
         }
       }
+      fetch_k(j + 1);
+      tc::mbar_wait(&sm.v_empty[buf], free_parity, fail);
       const int pos = 2 * w + vp, chunk = (pos & 3) * 2 + vh;
 #pragma unroll
       for (int gr = 0; gr < NG; gr++) {
         uint32_t o[4][4];
 #pragma unroll
-        for (int e = 0; e < 4; e++) dequant_word(c[e][gr], sc[e][gr], mn[e][gr], o[e]);
+        for (int e = 0; e < 4; e++) dequant_word(vc[e][gr], vs[e][gr], vm[e][gr], o[e]);
 #pragma unroll
         for (int e = 0; e < 4; e++) {
           const int d = gr * 32 + 4 * vg + e;
@@ -356,11 +339,8 @@ k_kv4_prefill(const __grid_constant__ Kv4Attn a, int n_split) {
       }
       tc::fence_proxy_async();
       __syncwarp();
-      if (lane == 0) {
-        if (i0 < n_pages) tc::mbar_arrive(&sm.rv_empty[i0 % SLOTS]);
-        if (i0 + 1 < n_pages) tc::mbar_arrive(&sm.rv_empty[(i0 + 1) % SLOTS]);
-        tc::mbar_arrive(&sm.v_full[buf]);
-      }
+      if (lane == 0) tc::mbar_arrive(&sm.v_full[buf]);
+      fetch_v(j + 1);
     }
   } else if ((warp >> 2) < tiles) {
     // ---- softmax of tile t, one row a thread
@@ -427,15 +407,17 @@ k_kv4_prefill(const __grid_constant__ Kv4Attn a, int n_split) {
     const uint32_t ts = tmem + ((uint32_t)(quarter * 32) << 16) + t * 128;
     const uint32_t to = tmem + ((uint32_t)(quarter * 32) << 16) + 256 + t * D;
     float base = -INFINITY, l = 0.f;
-    for (int j = 0; j < NJ; j++) {
-      const int key0 = (p_begin + j * PPT) * PAGE;
-      tc::mbar_wait(&sm.s_full[t], (uint32_t)(j & 1), fail);
-      tc::tc_fence_after();
-      if (CAP || key0 < low_max || key0 + KEYS > lim_min) {
 #pragma unroll 1
-        for (int c = 0; c < 8; c++) {
+    for (int u = 0; u < NU; u++) {   // 64 keys
+      const int key0 = p_begin * PAGE + u * (KEYS / 2);
+      const uint32_t par = (uint32_t)(u >> 1) & 1, su = ts + (u & 1) * 64;
+      tc::mbar_wait(&sm.s_full[t][u & 1], par, fail);
+      tc::tc_fence_after();
+      if (CAP || key0 < low_max || key0 + KEYS / 2 > lim_min) {
+#pragma unroll 1
+        for (int c = 0; c < 4; c++) {
           uint32_t x[16];
-          tc::tmem_ld16(ts + c * 16, x);
+          tc::tmem_ld16(su + c * 16, x);
           ld_wait(x);
 #pragma unroll
           for (int e = 0; e < 16; e++) {
@@ -444,73 +426,63 @@ k_kv4_prefill(const __grid_constant__ Kv4Attn a, int n_split) {
             if constexpr (CAP) y = cap_out * tanhf(y * cf * cap_in);
             x[e] = __float_as_uint(key >= low && key < lim ? y : -INFINITY);
           }
-          tc::tmem_st16(ts + c * 16, x);
+          tc::tmem_st16(su + c * 16, x);
         }
         tc::tmem_st_wait();
       }
       const float mul = CAP ? 1.f : cf;
+      uint32_t x[2][32];
+      ld32(su, x[0]);
+      ld32(su + 32, x[1]);
+      ld_wait(x[0]);
+      ld_wait(x[1]);
+      float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+      for (int e = 0; e < 64; e += 2)
+        m4[(e >> 1) & 3] = fmaxf(m4[(e >> 1) & 3], fmaxf(__uint_as_float(x[e >> 5][e & 31]), __uint_as_float(x[e >> 5][(e & 31) + 1])));
+      const float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * mul;
+      if (__any_sync(0xffffffffu, mx > base + HEADROOM)) {
+        // some row outgrew its base: every row of the warp moves to its maximum, once the half before is multiplied
+        const float nw = fmaxf(base, mx), f = nw == -INFINITY ? 1.f : kv4::ex2(base - nw);
+        if (u > 0) {
+          tc::mbar_wait(&sm.pv_done[t][(u - 1) & 1], (uint32_t)((u - 1) >> 1) & 1, fail);
+          tc::tc_fence_after();
 #pragma unroll 1
-      for (int hf = 0; hf < 2; hf++) {   // 64 keys
-        uint32_t x[2][32];
-        ld32(ts + hf * 64, x[0]);
-        ld32(ts + hf * 64 + 32, x[1]);
-        ld_wait(x[0]);
-        ld_wait(x[1]);
-        float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+          for (int c = 0; c < D / 16; c++) {
+            uint32_t y[16];
+            tc::tmem_ld16(to + c * 16, y);
+            ld_wait(y);
 #pragma unroll
-        for (int e = 0; e < 64; e += 2)
-          m4[(e >> 1) & 3] = fmaxf(m4[(e >> 1) & 3], fmaxf(__uint_as_float(x[e >> 5][e & 31]), __uint_as_float(x[e >> 5][(e & 31) + 1])));
-        const float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * mul;
-        if (__any_sync(0xffffffffu, mx > base + HEADROOM)) {
-          // some row outgrew its base: every row of the warp moves to its maximum.  The product of the step
-          // before is done (S of this one was issued after it); the first half's is waited for.
-          const float nw = fmaxf(base, mx), f = nw == -INFINITY ? 1.f : kv4::ex2(base - nw);
-          if (hf == 1) {
-            tc::mbar_wait(&sm.pv_half[t], (uint32_t)(j & 1), fail);
-            tc::tc_fence_after();
-          }
-          if (j > 0 || hf == 1) {
-#pragma unroll 1
-            for (int c = 0; c < D / 16; c++) {
-              uint32_t y[16];
-              tc::tmem_ld16(to + c * 16, y);
-              ld_wait(y);
-#pragma unroll
-              for (int e = 0; e < 16; e++) y[e] = __float_as_uint(__uint_as_float(y[e]) * f);
-              tc::tmem_st16(to + c * 16, y);
-            }
-          }
-          l *= f;
-          base = nw;
-        }
-        const float nb = base == -INFINITY ? 0.f : LIFT - base;
-        float s4[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int c = 0; c < 2; c++) {
-          uint32_t pk[16];
-#pragma unroll
-          for (int e = 0; e < 32; e += 2) {
-            const float p0 = kv4::ex2(fmaf(__uint_as_float(x[c][e]), mul, nb)), p1 = kv4::ex2(fmaf(__uint_as_float(x[c][e + 1]), mul, nb));
-            s4[(e >> 1) & 3] += p0 + p1;
-            pk[e >> 1] = kv4::pack_f16(p0, p1);
-          }
-          tc::tmem_st16(ts + hf * 32 + c * 16, pk);   // (columns of S that have been read)
-          if (c == 0 && hf == 0) {
-            __syncwarp();
-            if (lane == 0) tc::mbar_arrive(&sm.turn[t]);
+            for (int e = 0; e < 16; e++) y[e] = __float_as_uint(__uint_as_float(y[e]) * f);
+            tc::tmem_st16(to + c * 16, y);
           }
         }
-        l += (s4[0] + s4[1]) + (s4[2] + s4[3]);
-        tc::tmem_st_wait();
-        tc::tc_fence_before();
-        __syncwarp();
-        if (lane == 0) tc::mbar_arrive(&sm.p_full[t][hf]);
+        l *= f;
+        base = nw;
       }
+      const float nb = base == -INFINITY ? 0.f : LIFT - base;
+      float s4[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int c = 0; c < 2; c++) {
+        uint32_t pk[16];
+#pragma unroll
+        for (int e = 0; e < 32; e += 2) {
+          const float p0 = kv4::ex2(fmaf(__uint_as_float(x[c][e]), mul, nb)), p1 = kv4::ex2(fmaf(__uint_as_float(x[c][e + 1]), mul, nb));
+          s4[(e >> 1) & 3] += p0 + p1;
+          pk[e >> 1] = kv4::pack_f16(p0, p1);
+        }
+        tc::tmem_st16(su + c * 16, pk);   // (columns of S that have been read)
+      }
+      l += (s4[0] + s4[1]) + (s4[2] + s4[3]);
+      tc::tmem_st_wait();
+      tc::tc_fence_before();
+      __syncwarp();
+      if (lane == 0) tc::mbar_arrive(&sm.p_full[t][u & 1]);
     }
     // ---- output
     const bool alone = n_split == 1;
-    if (NJ > 0) {
-      tc::mbar_wait(&sm.pv_done[t], (uint32_t)((NJ - 1) & 1), fail);
+    if (NU > 0) {
+      tc::mbar_wait(&sm.pv_done[t][(NU - 1) & 1], (uint32_t)((NU - 1) >> 1) & 1, fail);
       tc::tc_fence_after();
     }
     const float sink = alone && a.sinks ? a.sinks[h] * LOG2E : -INFINITY;
@@ -528,7 +500,7 @@ k_kv4_prefill(const __grid_constant__ Kv4Attn a, int n_split) {
 #pragma unroll 1
     for (int c = 0; c < D / 16; c++) {
       uint32_t o[16];
-      if (NJ > 0) {
+      if (NU > 0) {
         tc::tmem_ld16(to + c * 16, o);
         ld_wait(o);
       } else {
