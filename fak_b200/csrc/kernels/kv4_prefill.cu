@@ -128,6 +128,27 @@ FAK_DEV void dequant_word(uint32_t w, uint32_t s, uint32_t m, uint32_t (&o)[4]) 
   o[2] = h2_fma(h2_add((u & 0x000f000fu) | BIAS, 0xe400e400u), s, m);
   o[3] = h2_fma(h2_fma((u & 0x00f000f0u) | BIAS, 0x2c002c00u, 0xd400d400u), s, m);
 }
+// two f32 at a time
+FAK_DEV uint64_t pair(float lo, float hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+FAK_DEV float2 unpair(uint64_t v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+FAK_DEV uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+FAK_DEV uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
 FAK_DEV uint32_t dup_lo(uint32_t x) { return __byte_perm(x, x, 0x1010); }
 FAK_DEV uint32_t dup_hi(uint32_t x) { return __byte_perm(x, x, 0x3232); }
 
@@ -461,19 +482,22 @@ k_kv4_prefill(const __grid_constant__ Kv4Attn a, int n_split) {
         base = nw;
       }
       const float nb = base == -INFINITY ? 0.f : LIFT - base;
-      float s4[4] = {0.f, 0.f, 0.f, 0.f};
+      const uint64_t mul2 = pair(mul, mul), nb2 = pair(nb, nb);
+      uint64_t s2[2] = {0, 0};
 #pragma unroll
       for (int c = 0; c < 2; c++) {
         uint32_t pk[16];
 #pragma unroll
         for (int e = 0; e < 32; e += 2) {
-          const float p0 = kv4::ex2(fmaf(__uint_as_float(x[c][e]), mul, nb)), p1 = kv4::ex2(fmaf(__uint_as_float(x[c][e + 1]), mul, nb));
-          s4[(e >> 1) & 3] += p0 + p1;
+          const float2 z = unpair(fma2(pair(__uint_as_float(x[c][e]), __uint_as_float(x[c][e + 1])), mul2, nb2));
+          const float p0 = kv4::ex2(z.x), p1 = kv4::ex2(z.y);
+          s2[(e >> 1) & 1] = add2(s2[(e >> 1) & 1], pair(p0, p1));
           pk[e >> 1] = kv4::pack_f16(p0, p1);
         }
         tc::tmem_st16(su + c * 16, pk);   // (columns of S that have been read)
       }
-      l += (s4[0] + s4[1]) + (s4[2] + s4[3]);
+      const float2 sum = unpair(add2(s2[0], s2[1]));
+      l += sum.x + sum.y;
       tc::tmem_st_wait();
       tc::tc_fence_before();
       __syncwarp();
