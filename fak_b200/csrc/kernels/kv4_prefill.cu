@@ -18,9 +18,7 @@
 // that need a mask or a soft-cap are rewritten in TMEM by a small loop first: the main loop then has one form,
 // which matters because three roles' code shares the instruction caches (with the mask inside the unrolled
 // loops, waits for instructions were the first stall and a step took 12.6k cycles).
-// Orders: a K chunk of 8 dims keeps its nibble pairs (0,4) (1,5) (2,6) (3,7) and Q is stored in the same
-// order; within a page's upper half the pairs of keys are swapped (key ^ 2), which keeps the V reads of a
-// warp on distinct banks, and the masks follow.
+// Orders: a K chunk of 8 dims keeps its nibble pairs (0,4) (1,5) (2,6) (3,7) and Q is stored in the same order.
 // Rounding: Q to f16 after a power-of-two scaling of its row (exact for f16, and for bf16 down to 2^-21
 // of the row's largest), K and V to f16, P to f16; sums in f32.
 // Every wait is bounded (tc::mbar_wait); no load uses multicast.
@@ -149,8 +147,14 @@ FAK_DEV uint64_t add2(uint64_t a, uint64_t b) {
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
 }
-FAK_DEV uint32_t dup_lo(uint32_t x) { return __byte_perm(x, x, 0x1010); }
-FAK_DEV uint32_t dup_hi(uint32_t x) { return __byte_perm(x, x, 0x3232); }
+FAK_DEV uint32_t dup_lo(uint32_t x) {
+  const __half2 r = __low2half2(*reinterpret_cast<__half2*>(&x));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+FAK_DEV uint32_t dup_hi(uint32_t x) {
+  const __half2 r = __high2half2(*reinterpret_cast<__half2*>(&x));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
 
 template <int D, bool CAP>
 __global__ void __launch_bounds__(THREADS, 1)
@@ -299,8 +303,8 @@ k_kv4_prefill(const __grid_constant__ Kv4Attn a, int n_split) {
       const uint8_t* pg = a.pages + ((int64_t)__shfl_sync(0xffffffffu, ids, 2 * (j & 15) + vp) * a.Hkv + kvh) * L::BYTES;
 #pragma unroll
       for (int e = 0; e < 4; e++) {
-        const int p = vh * 4 + (e ^ vh);
-        kv4::ldg(pg + L::VC + ((p * 8 + (vg ^ (2 * (p & 3)))) * NG) * 4, vc[e]);
+        const int p = vh * 4 + e;
+        kv4::ldg(pg + L::VC + ((p * 8 + (vg ^ (2 * e))) * NG) * 4, vc[e]);
         kv4::ldg(pg + L::VS + p * NG * 4, vs[e]);
         kv4::ldg(pg + L::VM + p * NG * 4, vm[e]);
       }
@@ -315,7 +319,7 @@ k_kv4_prefill(const __grid_constant__ Kv4Attn a, int n_split) {
       // (rows of pages that do not exist hold whatever page 0 does; they are masked in S)
 #pragma unroll
       for (int x = 0; x < 4; x++) {
-        const int row = (2 * w + (x >> 1)) * PAGE + (((x & 1) * 8 + ktok) ^ ((x & 1) * 2));
+        const int row = (2 * w + (x >> 1)) * PAGE + (x & 1) * 8 + ktok;
 #pragma unroll
         for (int gr = 0; gr < NG; gr++) {
           uint32_t o[4];
@@ -333,7 +337,7 @@ k_kv4_prefill(const __grid_constant__ Kv4Attn a, int n_split) {
         // tokens no row sees (memory nobody wrote, pages that do not exist): zero
 #pragma unroll
         for (int e = 0; e < 4; e++) {
-          const int key = key0 + 2 * (vh * 4 + (e ^ vh));
+          const int key = key0 + 2 * (vh * 4 + e);
           const uint32_t keep = (i < n_pages && key >= low_any && key < lim_any ? 0x0000ffffu : 0u) |
                                 (i < n_pages && key + 1 >= low_any && key + 1 < lim_any ? 0xffff0000u : 0u);
 #pragma unroll
@@ -442,7 +446,7 @@ k_kv4_prefill(const __grid_constant__ Kv4Attn a, int n_split) {
           ld_wait(x);
 #pragma unroll
           for (int e = 0; e < 16; e++) {
-            const int key = key0 + c * 16 + (e ^ ((e & 8) >> 2));
+            const int key = key0 + c * 16 + e;
             float y = __uint_as_float(x[e]);
             if constexpr (CAP) y = cap_out * tanhf(y * cf * cap_in);
             x[e] = __float_as_uint(key >= low && key < lim ? y : -INFINITY);
