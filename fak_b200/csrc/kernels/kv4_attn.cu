@@ -453,7 +453,7 @@ k_kv4_attn(const __grid_constant__ Kv4Attn a, int n_split) {
   __syncthreads();
   pdl_launch_dependents();
   const bool alone = n_split == 1;
-  const int64_t part_col = (((int64_t)b * a.Hkv + kvh) * (gridDim.x / n_split) + rc) * COLS;
+  const int64_t part_col = block_no(b, rc, kvh, gridDim.x / n_split, a.Hkv) * COLS;
   float* part_ml = a.part + (int64_t)gridDim.z * gridDim.y * (gridDim.x / n_split) * COLS * n_split * D;
   for (int c = warp; c < COLS; c += W) {
     const int r = r0 + c;
@@ -527,15 +527,16 @@ k_kv4_attn(const __grid_constant__ Kv4Attn a, int n_split) {
 
 // One warp merges the live splits of one query row: D / 32 dims a lane, up to 16 splits' loads in flight.
 template <int D>
-__global__ void __launch_bounds__(256) k_kv4_combine(const __grid_constant__ Kv4Attn a, int n_split, int grain, int cols, int row_chunks, float lift) {
+__global__ void __launch_bounds__(256) k_kv4_combine(const __grid_constant__ Kv4Attn a, int n_split, int whole, int grain, int cols, int row_chunks, float lift) {
   constexpr int V = D / 32;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int rc = blockIdx.x / (cols / 8), kvh = blockIdx.y, b = blockIdx.z;
-  const int c = blockIdx.x % (cols / 8) * 8 + warp;
+  const int no = blockIdx.x / (cols / 8), c = blockIdx.x % (cols / 8) * 8 + warp;   // of the row blocks that were split
+  int b, rc, kvh;
+  block_at((int64_t)whole + no, row_chunks, a.Hkv, b, rc, kvh);
   const int G = a.G;
   pdl_wait();
-  const int64_t part_col = (((int64_t)b * a.Hkv + kvh) * row_chunks + rc) * cols;
-  const float* part_ml = a.part + (int64_t)gridDim.z * gridDim.y * row_chunks * cols * n_split * D;
+  const int64_t part_col = (int64_t)no * cols;
+  const float* part_ml = a.part + (int64_t)gridDim.x * 8 * n_split * D;
   const float2* ml = reinterpret_cast<const float2*>(part_ml) + (part_col + c) * n_split;
   const float2 first = lane < n_split ? __ldcg(&ml[lane]) : make_float2(-INFINITY, 0.f);   // (travels with ctx)
   const int ctx = min(a.ctx[b], a.width * PAGE);
@@ -601,11 +602,13 @@ Kv4AttnPlan kv4_attn_plan(const Kv4Attn& a, int n_sm) {
   const int64_t rows = (int64_t)a.max_new * (a.H / a.Hkv);
   p.tc = a.tiles < 0 ? rows > kPrefillRows : a.tiles > 0;
   if (p.tc) {
-    // 256 rows a CTA, one CTA a SM: with fewer CTAs than SMs the keys are split, eight steps a split at least
+    // 256 rows a CTA, one CTA a SM: the blocks that would fill less than half of a last wave have their keys
+    // split, eight steps a split at least (448 blocks of 64 to 96 steps: @@ us whole, @@ with the last four split)
     p.row_chunks = (int)((rows + 255) / 256);
-    const int64_t ctas = (int64_t)a.B * a.Hkv * p.row_chunks;
-    p.n_split = a.n_split > 0 ? a.n_split : (int)std::max<int64_t>(1, std::min<int64_t>(n_sm / ctas, a.width / 64));
-    p.part_floats = p.n_split > 1 ? ctas * 256 * p.n_split * (a.D + 2) : 0;
+    const int64_t ctas = (int64_t)a.B * a.Hkv * p.row_chunks, last = ctas % n_sm;
+    p.n_split = a.n_split > 0 ? a.n_split : (int)std::max<int64_t>(1, std::min<int64_t>(last ? n_sm / last : 1, a.width / 64));
+    p.whole = p.n_split == 1 ? ctas : a.n_split > 0 ? 0 : ctas - last;
+    p.part_floats = (ctas - p.whole) * 256 * p.n_split * (a.D + 2);
     return p;
   }
   // Columns a CTA: 16 at head dim 64 where there are that many rows, else 8.  More columns save unpacking but
@@ -678,12 +681,12 @@ void kv4_attn_launch(const Kv4Attn& a, const Kv4AttnPlan& p, cudaStream_t stream
   if (p.n_split > 1 && !p.cluster) {
     cudaLaunchConfig_t c2 = {};
     const int cols = p.tc ? 256 : 8 * p.nt;
-    c2.gridDim = dim3((unsigned)(p.row_chunks * cols / 8), (unsigned)a.Hkv, (unsigned)a.B);
+    c2.gridDim = dim3((unsigned)(((int64_t)a.B * a.Hkv * p.row_chunks - p.whole) * (cols / 8)));
     c2.blockDim = dim3(256);
     c2.stream = stream;
     pdl(c2, attr);
-    if (a.D == 128) FAK_CUDA_CHECK(cudaLaunchKernelEx(&c2, k_kv4_combine<128>, a, p.n_split, p.tc ? kTilesGrain : kRowsGrain, cols, p.row_chunks, p.tc ? kPrefillLift : LIFT));
-    else FAK_CUDA_CHECK(cudaLaunchKernelEx(&c2, k_kv4_combine<64>, a, p.n_split, p.tc ? kTilesGrain : kRowsGrain, cols, p.row_chunks, p.tc ? kPrefillLift : LIFT));
+    if (a.D == 128) FAK_CUDA_CHECK(cudaLaunchKernelEx(&c2, k_kv4_combine<128>, a, p.n_split, (int)p.whole, p.tc ? kTilesGrain : kRowsGrain, cols, p.row_chunks, p.tc ? kPrefillLift : LIFT));
+    else FAK_CUDA_CHECK(cudaLaunchKernelEx(&c2, k_kv4_combine<64>, a, p.n_split, (int)p.whole, p.tc ? kTilesGrain : kRowsGrain, cols, p.row_chunks, p.tc ? kPrefillLift : LIFT));
   }
 }
 

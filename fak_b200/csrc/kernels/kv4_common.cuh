@@ -84,6 +84,16 @@ FAK_DEV Span span_of(int ctx, int n, int i_lo, int i_hi, int window, int n_split
   return s;
 }
 
+// Row blocks are numbered in the order of their launch: a sequence's last chunks, with the longest causal
+// ranges, first.
+FAK_DEV int64_t block_no(int b, int chunk, int kvh, int chunks, int Hkv) { return ((int64_t)b * chunks + chunks - 1 - chunk) * Hkv + kvh; }
+FAK_DEV void block_at(int64_t no, int chunks, int Hkv, int& b, int& chunk, int& kvh) {
+  const uint32_t rest = (uint32_t)no / (uint32_t)Hkv;
+  kvh = (int)((uint32_t)no - rest * Hkv);
+  b = (int)(rest / (uint32_t)chunks);
+  chunk = chunks - 1 - (int)(rest - (uint32_t)b * chunks);
+}
+
 FAK_DEV float load_elt(const void* p, Elt t, int64_t i) {
   if (t == Elt::F32) return ((const float*)p)[i];
   if (t == Elt::F16) return __half2float(((const __half*)p)[i]);

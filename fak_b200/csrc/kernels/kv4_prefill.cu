@@ -158,15 +158,17 @@ FAK_DEV uint32_t dup_hi(uint32_t x) {
 
 template <int D, bool CAP>
 __global__ void __launch_bounds__(THREADS, 1)
-k_kv4_prefill(const __grid_constant__ Kv4Attn a, int n_split) {
+k_kv4_prefill(const __grid_constant__ Kv4Attn a, int splits, int whole, int n_blk) {
   using L = Lay<D>;
   constexpr int NG = L::NG;
   extern __shared__ uint8_t smem_raw[];
   Smem<D>& sm = *reinterpret_cast<Smem<D>*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int n_blk = gridDim.y;
-  // blocks with the longest causal range first
-  const int split = blockIdx.x % n_split, kvh = blockIdx.x / n_split, blk = n_blk - 1 - (int)blockIdx.y, b = blockIdx.z;
+  // the first `whole` row blocks have a CTA each, the others `splits`
+  const int n_split = blockIdx.x < whole ? 1 : splits, past = max(0, (int)blockIdx.x - whole);
+  const int split = past % n_split, no = past / n_split;   // (number among the blocks that are split)
+  int b, blk, kvh;
+  kv4::block_at(blockIdx.x < whole ? blockIdx.x : whole + no, n_blk, a.Hkv, b, blk, kvh);
   const int G = a.G;
   pdl_wait();
   const int ctx = min(a.ctx[b], a.width * PAGE);
@@ -523,7 +525,7 @@ k_kv4_prefill(const __grid_constant__ Kv4Attn a, int n_split) {
       }
       f = l != 0.f ? f / l : 0.f;
     }
-    const int64_t part_row = ((((int64_t)b * a.Hkv + kvh) * n_blk + blk) * (2 * ROWS) + t * ROWS + row) * n_split + split;
+    const int64_t part_row = ((int64_t)no * (2 * ROWS) + t * ROWS + row) * n_split + split;
     const int64_t at = (int64_t)(tok0 + qi) * a.o_tok + (int64_t)h * a.o_head;
 #pragma unroll 1
     for (int c = 0; c < D / 16; c++) {
@@ -559,7 +561,7 @@ k_kv4_prefill(const __grid_constant__ Kv4Attn a, int n_split) {
       __syncwarp();
     }
     if (!alone && live) {
-      float* ml = a.part + (int64_t)gridDim.z * a.Hkv * n_blk * (2 * ROWS) * n_split * D + part_row * 2;
+      float* ml = a.part + (int64_t)(gridDim.x - whole) * (2 * ROWS) * D + part_row * 2;
       ml[0] = base;
       ml[1] = l;
     }
@@ -578,7 +580,7 @@ k_kv4_prefill(const __grid_constant__ Kv4Attn a, int n_split) {
 
 void kv4_prefill_launch(const Kv4Attn& a, const Kv4AttnPlan& p, cudaStream_t stream) {
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(p.n_split * a.Hkv), (unsigned)p.row_chunks, (unsigned)a.B);
+  cfg.gridDim = dim3((unsigned)(p.whole + ((int64_t)a.B * a.Hkv * p.row_chunks - p.whole) * p.n_split));
   cfg.blockDim = dim3(THREADS);
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
@@ -589,7 +591,7 @@ void kv4_prefill_launch(const Kv4Attn& a, const Kv4AttnPlan& p, cudaStream_t str
   auto go = [&](auto kern, size_t smem) {
     cfg.dynamicSmemBytes = smem + 1024;
     FAK_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)cfg.dynamicSmemBytes));
-    FAK_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kern, a, p.n_split));
+    FAK_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kern, a, p.n_split, (int)p.whole, p.row_chunks));
   };
   const bool cap = a.softcap > 0.f;
   if (a.D == 128 && cap) go(k_kv4_prefill<128, true>, sizeof(Smem<128>));

@@ -188,6 +188,7 @@ void kv4_attention(Tensor q, Tensor pages, Tensor table, OptTensor q_off, Tensor
   if (a.B == 0 || a.n_tokens == 0 || a.max_new == 0) return;
   c10::cuda::CUDAGuard guard(q.device());
   const fak::Kv4AttnPlan p = fak::kv4_attn_plan(a, sms(q));
+  TORCH_CHECK((int64_t)a.B * a.Hkv * p.row_chunks * std::max(p.n_split, 32) < (int64_t(1) << 31), "kv4_attention: too many query rows");
   Tensor ws;
   if (p.part_floats > 0) {
     if (workspace.has_value()) {

@@ -54,6 +54,7 @@ struct Kv4Attn {
 struct Kv4AttnPlan {
   bool tc, cluster;   // tiles of query rows on tcgen05; the splits merge inside thread-block clusters
   int nt, row_chunks, n_split;
+  int64_t whole;      // row blocks (of B * Hkv * row_chunks, in block_no's order) whose keys are not split
   int64_t part_floats;
 };
 Kv4AttnPlan kv4_attn_plan(const Kv4Attn& a, int n_sm);

@@ -328,6 +328,44 @@ def test_prefill(K, old, new, H, Hkv, D, dtype, window):
     assert (out[T:] == 7).all()
 
 
+def test_prefill_splits_the_blocks_of_a_short_last_wave(K):
+    """Two blocks more than multiprocessors: the last two sequences' keys are split, the others' are not."""
+    g = gen(77)
+    B = torch.cuda.get_device_properties(0).multi_processor_count + 2
+    lens = [66 + b % 40 for b in range(B - 2)] + [2190, 1500]
+    pages, table, ks, vs = cache_of(K, g, lens, 1, 64)
+    new = [66] * B
+    q = torch.randn(sum(new), 1, 64, generator=g, device="cuda").to(torch.bfloat16)
+    off = torch.arange(0, sum(new) + 1, 66, dtype=torch.int32, device="cuda")
+    ctx = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    out, one = torch.full_like(q, 7), torch.full_like(q, 7)
+    K.kv4_prefill_attention(q, pages, table, off, ctx, out, 66)
+    K.kv4_prefill_attention(q, pages, table, off, ctx, one, 66, n_split=1)
+    assert torch.equal(out[:66 * (B - 2)], one[:66 * (B - 2)])
+    for b in (0, 1, B - 3, B - 2, B - 1):
+        want = plain.attention([q[66 * b:66 * b + 66].double().cpu()], ks[b:b + 1], vs[b:b + 1], lens[b:b + 1])[0]
+        tol = 4 * UBF * vs[b].abs().max() + OUT_U[torch.bfloat16] * want.abs()
+        for o in (out, one):
+            assert ((o[66 * b:66 * b + 66].double().cpu() - want).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("tiles", [False, True])
+def test_context_past_the_table_is_reported(K, tiles):
+    g = gen(5)
+    pages, table, ks, vs = cache_of(K, g, [30], 1, 64)          # three table columns, the last a page of zeros' id
+    err = torch.zeros(1, dtype=torch.int32, device="cuda")
+    K.register_error_word(err.device, err)
+    try:
+        q = torch.randn(1, 1, 64, generator=g, device="cuda").to(torch.bfloat16)
+        off = torch.tensor([0, 1], dtype=torch.int32, device="cuda")
+        K.kv4_prefill_attention(q, pages, table, off, torch.tensor([48], dtype=torch.int32, device="cuda"), torch.empty_like(q), 1, tiles=tiles)
+        assert err.item() == 0
+        K.kv4_prefill_attention(q, pages, table, off, torch.tensor([49], dtype=torch.int32, device="cuda"), torch.empty_like(q), 1, tiles=tiles)
+        assert err.item() == 2
+    finally:
+        K.register_error_word(err.device, None)
+
+
 def test_refusals(K):
     pages = torch.zeros(4, 2, K.kv4_page_bytes(64), dtype=torch.uint8, device="cuda")
     q = torch.zeros(1, 4, 64, device="cuda")
