@@ -6,7 +6,8 @@
 // base is the exclusive sum of the counts over requests from *head on; q_off is the exclusive sum of new.
 // Every CTA scans the lengths of all requests itself (a few KB out of L2) and then fills its own range of
 // tokens, so one launch does it all and no CTA waits for another.  Latency-bound: two dependent reads
-// (lengths, then the page) and the scan.
+// (lengths, then the page) and the scan.  Measured: 48 requests with one token each 2.8 us, 333 requests with
+// 42 thousand new tokens 6.0 us.
 #include "common.cuh"
 
 #include <stdexcept>

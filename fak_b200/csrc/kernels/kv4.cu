@@ -1,6 +1,7 @@
 // Append into and read from the 4-bit KV cache (layout in kv4.cuh).
 //
-// Quantization of a group x[32], after clamping to +-65504:  m = f16(min x),  s = f16((max x - m) / 15),
+// Quantization of a group x[32], after clamping to +-65504:  m = f16(min x),  s = f16((max x - m) / 15), one
+// f16 step less where m + 15 s would pass f16's range (its readers round values to f16),
 // code = rint((x - m) / s) clamped to [0, 15], all codes 0 where s = 0 (a constant group).  f16 holds the
 // minimum to 11 bits, more than the bf16 values that come in; the subtraction and the division are done
 // in f32.  A group that holds a not-a-number stores m = NaN and reads back as NaN.
@@ -10,6 +11,8 @@
 // instructions decide: the per-element divide is q = d r corrected by one remainder step with r = 1 / s
 // correctly rounded (Markstein 1990: the result is the correctly rounded quotient), the four codes of a
 // half word are summed as floats (c0 + 16 c1 + 256 c2 + 4096 c3 is exact), and heads are a grid dimension.
+// Measured at 8191 tokens x 8 heads of 128, bf16: append 18.5 us (44 MB, 2.4 TB/s; bound by instructions),
+// read 10.3 us (4.3 TB/s, its output stays in L2).
 #include "kv4.cuh"
 
 #include <cuda_fp16.h>

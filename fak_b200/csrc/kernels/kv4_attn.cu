@@ -20,7 +20,13 @@
 //
 // A warp streams its own pages through a ring of shared memory filled by one bulk copy a page and walks
 // them with an online softmax whose base moves only when a row outgrows it; the CTA's warps, then the
-// splits of a sequence (k_kv4_combine), are merged at the end.
+// splits of a sequence, are merged at the end: through distributed shared memory where the splits of a
+// sequence form a cluster, by k_kv4_combine where there are more of them.
+//
+// Measured (graph of calls, us): single tokens of 28 heads over 4 KV heads of 128, 32 lanes up to 32768 keys
+// 167 (834 MB, 5.0 TB/s; bound by the copies), 5 up to 9000 15.3 and 1 x 2048 5.8 (both bound by latency: the
+// longest chain is lengths, table entry, page, softmax, merge); 16 x 5 tokens of 64 heads over 8 KV heads of 64
+// at 4097 keys 49 (bound by instructions: three column blocks unpack the same pages).
 #include "kv4_common.cuh"
 
 #include <algorithm>
@@ -37,10 +43,10 @@ constexpr int STAGES = 4;     // pages in flight per warp
 constexpr float HEADROOM = 0.875f;   // log2 growth of a row's max before its base moves
 constexpr float LIFT = 2.f;          // P = 2^(z - base + LIFT) <= 2^2.875 < 7.5
 constexpr float LOG2E = 1.4426950408889634f;
-// More query rows than this per (sequence, KV head) go to kv4_prefill.cu.  Measured (us, here / there): 63 rows
-// 8 x 8000 61.5 / 57.3, 1 x 16000 25.7 / 41.0; 128 rows 8 x 8000 124.8 / 60.2, 1 x 32000 64.0 / 45.7 (head dim
-// 128); 64 rows 4 x 8000 38.3 / 48.7 (head dim 64).
-constexpr int kPrefillRows = 64;
+// More query rows than this per (sequence, KV head) go to kv4_prefill.cu.  Measured over 4 KV heads (us, here /
+// there): head dim 128, 48 rows 8 x 8000 50.8 / 49.6, 16 x 1000 18.3 / 25.6, 64 rows 73.8 / 49.9, 21.9 / 25.6;
+// head dim 64, 64 rows 39.4 / 38.0, 18.7 / 19.5, 80 rows 51.3 / 38.5, 19.2 / 19.8.
+constexpr int prefill_rows(int D) { return D == 128 ? 48 : 64; }
 constexpr float kPrefillLift = 4.f;   // LIFT of that kernel
 
 FAK_DEV void mma_f16_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -600,10 +606,10 @@ void pdl(cudaLaunchConfig_t& cfg, cudaLaunchAttribute* attr) {
 Kv4AttnPlan kv4_attn_plan(const Kv4Attn& a, int n_sm) {
   Kv4AttnPlan p{};
   const int64_t rows = (int64_t)a.max_new * (a.H / a.Hkv);
-  p.tc = a.tiles < 0 ? rows > kPrefillRows : a.tiles > 0;
+  p.tc = a.tiles < 0 ? rows > prefill_rows(a.D) : a.tiles > 0;
   if (p.tc) {
     // 256 rows a CTA, one CTA a SM: the blocks that would fill less than half of a last wave have their keys
-    // split, eight steps a split at least (448 blocks of 64 to 96 steps: @@ us whole, @@ with the last four split)
+    // split, eight steps a split at least (448 blocks of 64 to 96 steps: 726 us whole, 649 with the last four split)
     p.row_chunks = (int)((rows + 255) / 256);
     const int64_t ctas = (int64_t)a.B * a.Hkv * p.row_chunks, last = ctas % n_sm;
     p.n_split = a.n_split > 0 ? a.n_split : (int)std::max<int64_t>(1, std::min<int64_t>(last ? n_sm / last : 1, a.width / 64));

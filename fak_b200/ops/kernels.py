@@ -329,7 +329,8 @@ def kv4_append(k: torch.Tensor, v: torch.Tensor, slot: torch.Tensor, pages: torc
     meant.  slot [T] int32: page * 16 + offset of each row, -1 for rows to skip.  A slot past the pages
     is skipped and reported as code 2 in the device's error word.  Groups of 32 dims get
     minimum = f16(min x), scale = f16((max x - minimum) / 15), code = rint((x - minimum) / scale);
-    values are clamped to +-65504, a group with a NaN reads back as NaN."""
+    values are clamped to +-65504 (the scale is one f16 step lower where minimum + 15 scale would pass that),
+    a group with a NaN reads back as NaN.  Rows with the same slot leave one of them, not a defined one."""
     ext().kv4_append(k, v, slot, pages, _err_word.get(pages.device))
     count()
 
@@ -365,9 +366,11 @@ def kv4_prefill_attention(q: torch.Tensor, pages: torch.Tensor, block_table: tor
     """Causal attention of packed new tokens (their K / V already appended) over the 4-bit cache: q, out
     [T, H, D]; q_off [B + 1] int32 packed offsets of the sequences' tokens (``BatchPlan.q_off``), ctx_len
     [B] int32 keys with the new ones (``BatchPlan.ctx``); max_new: an upper bound of the new tokens of one
-    sequence.  Sequences without new tokens are skipped.  tiles: True takes the tensor-core kernel over tiles of 256
-    query rows, False the one whose warps stream pages, None the faster one for max_new (a fixed choice with
-    n_split = 1 makes a sequence's result independent of its batch).  The other arguments as kv4_decode_attention."""
+    sequence.  Sequences without new tokens are skipped.  tiles: True takes the tensor-core kernel over tiles of
+    256 query rows (keys and values rounded to f16), False the one whose warps stream pages, None the faster one
+    for max_new (a fixed choice with n_split = 1 makes a sequence's result independent of its batch).  A value
+    that is not a number reaches every row of a tile in which some row sees it.  The other arguments as
+    kv4_decode_attention."""
     ext().kv4_attention(q, pages, block_table, q_off, ctx_len, out, max_new, scale, softcap, window, sinks, n_split,
                         workspace, _err_word.get(q.device), -1 if tiles is None else int(tiles))
     count()
