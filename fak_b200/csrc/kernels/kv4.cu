@@ -12,7 +12,7 @@
 // correctly rounded (Markstein 1990: the result is the correctly rounded quotient), the four codes of a
 // half word are summed as floats (c0 + 16 c1 + 256 c2 + 4096 c3 is exact), and heads are a grid dimension.
 // Measured at 8191 tokens x 8 heads of 128, bf16: append 18.5 us (44 MB, 2.4 TB/s; bound by instructions),
-// read 10.3 us (4.3 TB/s, its output stays in L2).
+// read 10.3 us (4.3 TB/s).
 #include "kv4.cuh"
 
 #include <cuda_fp16.h>

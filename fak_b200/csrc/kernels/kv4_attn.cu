@@ -635,8 +635,12 @@ Kv4AttnPlan kv4_attn_plan(const Kv4Attn& a, int n_sm) {
                  std::max<int64_t>(most, 1));
   // Up to 16 splits that are resident at once merge inside a cluster, without partial results in memory and a
   // second launch (1 x 2048 9.8 -> 5.8 us); a warp may have nine pages then before more splits pay for them.
+  // Clusters do not span the groups of SMs, so up to c - 1 of a group's slots stay empty: at 2000 keys 28 blocks of
+  // 16 take 8.8 us, 32 take 13.1; 140 of 4 15.2, 144 21.3.  (Sizes between the powers of two lose more slots than
+  // they gain: 96 blocks over 4000 keys 21.7 us in fours, 26.6 in sixes.)
+  const int resident = a.D == 64 && p.nt == 1 ? 5 : 4;   // CTAs a SM (36 blocks of 16 at head dim 64: 7.8 us, 28 7.8)
   int64_t c = 1;
-  while (c < 16 && 2 * c * ctas <= 4 * n_sm && c < most) c *= 2;
+  while (c < 16 && 2 * c * (ctas + 9) <= resident * n_sm && c < most) c *= 2;
   if (a.n_split > 0) {
     p.cluster = n > 1 && n <= c && (n & (n - 1)) == 0;
   } else if (c > 1 && n > 1 && (n <= c || a.width <= 9 * W * c)) {
