@@ -8,16 +8,19 @@
 //
 // Four lanes hold one group, eight consecutive dims each: two rows a warp at head dim 128, four at 64, K
 // and V of a row in the same lanes.  The bytes (2 D each of K and V per row in, 20 D / 16 out) are few, so
-// instructions decide: the per-element divide is q = d r corrected by one remainder step with r = 1 / s
-// correctly rounded (Markstein 1990: the result is the correctly rounded quotient), the four codes of a
-// half word are summed as floats (c0 + 16 c1 + 256 c2 + 4096 c3 is exact), and heads are a grid dimension.
-// Measured at 8191 tokens x 8 heads of 128, bf16: append 18.5 us (44 MB, 2.4 TB/s; bound by instructions),
-// read 10.3 us (4.3 TB/s).
+// instructions decide: the extremes of 16-bit types are taken two values at a time, of K and V in one word
+// across lanes; half of a group's lanes work out the scale of K, half that of V; quotients are q = d r
+// corrected by one remainder step with r = 1 / s correctly rounded (Markstein 1990: the result is the
+// correctly rounded quotient), two at a time; the four codes of a half word are summed as floats (c0 + 16 c1
+// + 256 c2 + 4096 c3 is exact); heads are a grid dimension.
+// Measured at 8191 tokens x 8 heads of 128, bf16: append 15.6 us (44 MB, 2.8 TB/s; bound by instructions; 18.5
+// with every lane on both scales and one quotient at a time), read 10.3 us (4.3 TB/s).
 #include "kv4.cuh"
 
 #include <cuda_fp16.h>
 #include <stdexcept>
 #include <string>
+#include <type_traits>
 
 #include "../serve_ops.h"
 
@@ -25,31 +28,6 @@ namespace fak {
 namespace {
 
 constexpr int THREADS = 256;
-
-template <typename T>
-FAK_DEV void load8(const T* p, bool vec, float (&x)[8]) {
-  if (vec) {
-    if constexpr (sizeof(T) == 4) {
-      const float4 f = *reinterpret_cast<const float4*>(p), h = *reinterpret_cast<const float4*>(p + 4);
-      x[0] = f.x; x[1] = f.y; x[2] = f.z; x[3] = f.w;
-      x[4] = h.x; x[5] = h.y; x[6] = h.z; x[7] = h.w;
-    } else {
-      const uint4 u = *reinterpret_cast<const uint4*>(p);
-      T h[8];
-      memcpy(h, &u, 16);
-#pragma unroll
-      for (int i = 0; i < 8; i++) x[i] = (float)h[i];
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; i++) x[i] = (float)p[i];
-  }
-}
-
-struct Group {
-  uint32_t lo, hi;   // codes of the lane's dims 0-3 and 4-7, 16 bits each
-  __half s, m;
-};
 
 FAK_DEV float min_nan(float a, float b) {   // as fminf, but a NaN stays
   float r;
@@ -61,67 +39,170 @@ FAK_DEV float max_nan(float a, float b) {
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
   return r;
 }
+template <typename T, bool MAX>
+FAK_DEV uint32_t pick2(uint32_t a, uint32_t b) {   // the same for pairs of 16-bit values
+  uint32_t r;
+  if constexpr (std::is_same_v<T, __half>) {
+    if constexpr (MAX) asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    else asm("min.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  } else {
+    if constexpr (MAX) asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    else asm("min.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  }
+  return r;
+}
+template <typename T>
+FAK_DEV float half_of(uint32_t u, int i) {
+  const uint16_t h = (uint16_t)(i ? u >> 16 : u);
+  if constexpr (std::is_same_v<T, __half>) return __half2float(__ushort_as_half(h));
+  else return __uint_as_float((uint32_t)h << 16);
+}
 
-// Eight values of a group held by 4 lanes.  In ordinary groups no clamp can act: all values are within
-// +-65504, the rounding of the minimum moves no quotient below -1/2 (s > 2^-10 |m|) nor that of a normal
-// scale one above 15 1/2.  Other groups send their warp through the clamping loop.
-FAK_DEV Group quant8(float (&x)[8]) {
-  constexpr float LIM = 65504.f, MAGIC = 12582912.f;   // adding 1.5 * 2^23 rounds to whole numbers, ties to even
-  float lo = x[0], hi = x[0];
+// A lane's eight dims of K and of V: as floats, and 16-bit types also as they are.
+template <typename T>
+struct Rows8 {
+  float k[8] = {}, v[8] = {};
+  uint32_t kp[4] = {}, vp[4] = {};
+  FAK_DEV static void load(const T* p, bool vec, float (&x)[8], uint32_t (&w)[4]) {
+    if constexpr (sizeof(T) == 4) {
+      if (vec) {
+        const float4 f = *reinterpret_cast<const float4*>(p), h = *reinterpret_cast<const float4*>(p + 4);
+        x[0] = f.x; x[1] = f.y; x[2] = f.z; x[3] = f.w;
+        x[4] = h.x; x[5] = h.y; x[6] = h.z; x[7] = h.w;
+      } else {
 #pragma unroll
-  for (int i = 1; i < 8; i++) {
-    lo = min_nan(lo, x[i]);
-    hi = max_nan(hi, x[i]);
-  }
+        for (int i = 0; i < 8; i++) x[i] = p[i];
+      }
+    } else {
+      const uint16_t* u = reinterpret_cast<const uint16_t*>(p);
+      if (vec) {
+        const uint4 q = *reinterpret_cast<const uint4*>(u);
+        w[0] = q.x; w[1] = q.y; w[2] = q.z; w[3] = q.w;
+      } else {
 #pragma unroll
-  for (int o = 2; o > 0; o >>= 1) {
-    lo = min_nan(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-    hi = max_nan(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+        for (int i = 0; i < 4; i++) w[i] = u[2 * i] | (uint32_t)u[2 * i + 1] << 16;
+      }
+#pragma unroll
+      for (int i = 0; i < 8; i++) x[i] = half_of<T>(w[i >> 1], i & 1);
+    }
   }
+  // smallest and largest of the group (four lanes), of K for mine = 0, of V for 1
+  FAK_DEV void range(int mine, float& lo, float& hi) const {
+    if constexpr (sizeof(T) == 4) {
+      float l[2] = {k[0], v[0]}, h[2] = {k[0], v[0]};
+#pragma unroll
+      for (int i = 1; i < 8; i++) {
+        l[0] = min_nan(l[0], k[i]);
+        h[0] = max_nan(h[0], k[i]);
+        l[1] = min_nan(l[1], v[i]);
+        h[1] = max_nan(h[1], v[i]);
+      }
+#pragma unroll
+      for (int o = 2; o > 0; o >>= 1)
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+          l[e] = min_nan(l[e], __shfl_xor_sync(0xffffffffu, l[e], o));
+          h[e] = max_nan(h[e], __shfl_xor_sync(0xffffffffu, h[e], o));
+        }
+      lo = mine ? l[1] : l[0];
+      hi = mine ? h[1] : h[0];
+    } else {
+      auto both = [](const uint32_t (&a)[4], const uint32_t (&b)[4], auto pick) {   // {K, V} in one word
+        const uint32_t x = pick(pick(a[0], a[1]), pick(a[2], a[3])), y = pick(pick(b[0], b[1]), pick(b[2], b[3]));
+        uint32_t r = pick(__byte_perm(x, y, 0x5410), __byte_perm(x, y, 0x7632));
+        r = pick(r, __shfl_xor_sync(0xffffffffu, r, 2));
+        return pick(r, __shfl_xor_sync(0xffffffffu, r, 1));
+      };
+      lo = half_of<T>(both(kp, vp, pick2<T, false>), mine);
+      hi = half_of<T>(both(kp, vp, pick2<T, true>), mine);
+    }
+  }
+};
+
+struct Scale {
+  __half2 sm;   // scale, minimum
+  float r;      // 1 / scale, 0 for a constant group
+  bool plain;   // no clamp can act
+};
+// Ordinary groups: all values are within +-65504, the rounding of the minimum moves no quotient below -1/2
+// (s > 2^-10 |m|) nor that of a normal scale one above 15 1/2.
+FAK_DEV Scale scale_of(float lo, float hi) {
+  constexpr float LIM = 65504.f;
   const bool nan = hi != hi;
   lo = fminf(fmaxf(lo, -LIM), LIM);
   hi = fminf(fmaxf(hi, -LIM), LIM);
-  Group g;
-  g.m = __float2half_rn(lo);
-  const float m = __half2float(g.m);
-  g.s = __float2half_rn(__fdiv_rn(hi - m, 15.f));
+  __half hm = __float2half_rn(lo);
+  const float m = __half2float(hm), d = hi - m, r15 = 1.f / 15.f;
+  const float q = d * r15;   // (below f32's normal range the corrected quotient may be off: f16 has 0 there)
+  __half hs = __float2half_rn(fmaf(fmaf(-q, 15.f, d), r15, q));
   // code 15 of the largest values may round past f16's range, where the readers compute in f16
-  if (m + 15.f * __half2float(g.s) > LIM) g.s = __ushort_as_half(__half_as_ushort(g.s) - 1);
-  const float s = __half2float(g.s);
-  const float r = s > 0.f ? __frcp_rn(s) : 0.f;   // a constant group: all codes 0
-  const bool plain = s > fabsf(m) * 0.0009765625f && s >= 6.103515625e-5f && lo > -LIM && hi < LIM && !nan;
+  if (m + 15.f * __half2float(hs) > LIM) hs = __ushort_as_half(__half_as_ushort(hs) - 1);
+  const float s = __half2float(hs);
+  Scale g;
+  g.r = s > 0.f && !nan ? __frcp_rn(s) : 0.f;
+  g.plain = s > fabsf(m) * 0.0009765625f && s >= 6.103515625e-5f && lo > -LIM && hi < LIM && !nan;
+  if (nan) {
+    hm = __ushort_as_half(0x7fff);
+    hs = __ushort_as_half(0);
+  }
+  g.sm = __halves2half2(hs, hm);
+  return g;
+}
+
+// two f32 at a time
+FAK_DEV uint64_t pair(float lo, float hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+FAK_DEV uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+FAK_DEV uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+FAK_DEV uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
+struct Codes {
+  uint32_t lo, hi;   // of the lane's dims 0-3 and 4-7, 16 bits each
+};
+FAK_DEV Codes codes_of(float (&x)[8], __half2 sm, float r, bool plain) {
+  constexpr float LIM = 65504.f, MAGIC = 12582912.f;   // adding 1.5 * 2^23 rounds to whole numbers, ties to even
+  const float s = __low2float(sm), m = __high2float(sm);
   float c[2] = {0.f, 0.f};
-  if (__all_sync(0xffffffffu, plain)) {
-    asm volatile("");
+  if (plain) {
+    const uint64_t r2 = pair(r, r), s2 = pair(-s, -s), m2 = pair(-m, -m), up = pair(MAGIC, MAGIC), down = pair(-MAGIC, -MAGIC);
+    uint64_t c2 = 0;
 #pragma unroll
-    for (int i = 7; i >= 0; i--) {
-      const float d = x[i] - m;
-      float q = d * r;
-      q = (fmaf(fmaf(-q, s, d), r, q) + MAGIC) - MAGIC;
-      c[i >> 2] = fmaf(c[i >> 2], 16.f, q);
+    for (int i = 3; i >= 0; i--) {
+      const uint64_t d = add2(pair(x[i], x[i + 4]), m2);
+      uint64_t q = mul2(d, r2);
+      q = add2(add2(fma2(fma2(q, s2, d), r2, q), up), down);
+      c2 = fma2(c2, pair(16.f, 16.f), q);
     }
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(c[0]), "=f"(c[1]) : "l"(c2));
   } else {
-    asm volatile("");
 #pragma unroll 1
     for (int i = 7; i >= 0; i--) {
       const float d = fminf(fmaxf(x[7], -LIM), LIM) - m;   // (rotated below: no indexed registers)
       float q = d * r;
       q = fmaf(fmaf(-q, s, d), r, q);
-      q = (fminf(fmaxf(q, 0.f), 15.f) + MAGIC) - MAGIC;
+      q = (fminf(fmaxf(q, 0.f), 15.f) + MAGIC) - MAGIC;   // (0 in a group with a NaN)
       if (i >= 4) c[1] = fmaf(c[1], 16.f, q);
       else c[0] = fmaf(c[0], 16.f, q);
 #pragma unroll
       for (int e = 7; e > 0; e--) x[e] = x[e - 1];
     }
-    if (nan) {
-      g.m = __ushort_as_half(0x7fff);
-      g.s = __ushort_as_half(0);
-      c[0] = c[1] = 0.f;
-    }
   }
-  g.lo = (uint32_t)__float_as_int(c[0] + 8388608.f) & 0xffffu;
-  g.hi = (uint32_t)__float_as_int(c[1] + 8388608.f) & 0xffffu;
-  return g;
+  return {(uint32_t)__float_as_int(c[0] + 8388608.f) & 0xffffu, (uint32_t)__float_as_int(c[1] + 8388608.f) & 0xffffu};
 }
 
 // The row (token, head) of a lane: heads along the grid's x, tokens along its y.
@@ -149,14 +230,24 @@ k_kv4_append(const __grid_constant__ Kv4Rows r, const int* __restrict__ slot, in
   const int sl = w.tok < n_tok ? slot[w.tok] : -1;
   const bool in = sl >= 0 && (sl >> 4) < n_pages;
   if (sl >= 0 && !in) report_error(err, 2);
-  float k[8] = {}, v[8] = {};
+  Rows8<T> x;
   if (in) {
     const int d = w.grp * 32 + 8 * w.j;
     const int64_t pg = w.tok >> 4, row = w.tok & 15;
-    load8((const T*)r.k + pg * r.ks_page + row * r.ks_row + w.h * r.ks_head + d, r.vec, k);
-    load8((const T*)r.v + pg * r.vs_page + row * r.vs_row + w.h * r.vs_head + d, r.vec, v);
+    x.load((const T*)r.k + pg * r.ks_page + row * r.ks_row + w.h * r.ks_head + d, r.vec, x.k, x.kp);
+    x.load((const T*)r.v + pg * r.vs_page + row * r.vs_row + w.h * r.vs_head + d, r.vec, x.v, x.vp);
   }
-  const Group gk = quant8(k), gv = quant8(v);
+  // lanes 0 and 1 of a group work out the scale of K, 2 and 3 that of V
+  const bool of_v = w.j & 2;
+  float lo, hi;
+  x.range(of_v, lo, hi);
+  const Scale mine = scale_of(lo, hi);
+  const uint32_t sm = *reinterpret_cast<const uint32_t*>(&mine.sm), osm = __shfl_xor_sync(0xffffffffu, sm, 2);
+  const float orr = __shfl_xor_sync(0xffffffffu, mine.r, 2);
+  const uint32_t smk = of_v ? osm : sm, smv = of_v ? sm : osm;
+  const bool plain = __all_sync(0xffffffffu, mine.plain);
+  const Codes gk = codes_of(x.k, *reinterpret_cast<const __half2*>(&smk), of_v ? orr : mine.r, plain);
+  const Codes gv = codes_of(x.v, *reinterpret_cast<const __half2*>(&smv), of_v ? mine.r : orr, plain);
   if (in) {
     uint8_t* pg = pages + ((int64_t)(sl >> 4) * Hkv + w.h) * L::BYTES;
     const int t = sl & 15;
@@ -164,9 +255,8 @@ k_kv4_append(const __grid_constant__ Kv4Rows r, const int* __restrict__ slot, in
     *reinterpret_cast<uint16_t*>(pg + L::v_u16(t, w.grp, 2 * w.j)) = (uint16_t)gv.lo;
     *reinterpret_cast<uint16_t*>(pg + L::v_u16(t, w.grp, 2 * w.j + 1)) = (uint16_t)gv.hi;
     // lane j of the group stores one of its four halves
-    const __half x = w.j == 0 ? gk.s : w.j == 1 ? gk.m : w.j == 2 ? gv.s : gv.m;
     const int at = w.j < 2 ? L::KS + 32 * L::NG * w.j + L::k_meta(t, w.grp) : L::VS + 32 * L::NG * (w.j - 2) + L::v_meta(t, w.grp);
-    *reinterpret_cast<__half*>(pg + at) = x;
+    *reinterpret_cast<uint16_t*>(pg + at) = (uint16_t)(w.j & 1 ? sm >> 16 : sm);
   }
   pdl_launch_dependents();
 }
