@@ -16,7 +16,10 @@
 //                                                         sum is one m16n8k16 whose fifth row, all ones,
 //                                                         gives the softmax denominator
 // Queries are rounded to f16 after a power-of-two scaling of their row (exact for bf16 and f16 inputs up
-// to 28 binades below the row's largest); P is f16: at most 7.5, so that P s stays below 65504.
+// to 28 binades below the row's largest); P is f16: at most 7.5, so that P s stays below 65504.  Rounding P
+// alone moves numerator and denominator alike; what P s loses meets codes around 8, and for outputs finer than
+// bf16 the loss times 8 is added back over up to 1024 keys (f16, 3 to 12 keys: error 3.4e-4 -> 2.4e-4 of the
+// output, 2.0e-4 being that of its rounding; over 8000 keys 2.04e-4 -> 2.02e-4, for 9 to 14% more time).
 //
 // A warp streams its own pages through a ring of shared memory filled by one bulk copy a page and walks
 // them with an online softmax whose base moves only when a row outgrows it; the CTA's warps, then the
@@ -26,12 +29,13 @@
 // Measured (graph of calls, us): single tokens of 28 heads over 4 KV heads of 128, 32 lanes up to 32768 keys
 // 167 (834 MB, 5.0 TB/s; bound by the copies), 5 up to 9000 15.3 and 1 x 2048 5.8 (both bound by latency: the
 // longest chain is lengths, table entry, page, softmax, merge); 16 x 5 tokens of 64 heads over 8 KV heads of 64
-// at 4097 keys 49 (bound by instructions: three column blocks unpack the same pages).
+// at 4097 keys, f16, 51 (bound by instructions: three column blocks unpack the same pages).
 #include "kv4_common.cuh"
 
 #include <algorithm>
 #include <stdexcept>
 #include <string>
+#include <type_traits>
 
 namespace fak {
 namespace {
@@ -42,6 +46,9 @@ constexpr int W = kRowsGrain;   // warps per CTA
 constexpr int STAGES = 4;     // pages in flight per warp
 constexpr float HEADROOM = 0.875f;   // log2 growth of a row's max before its base moves
 constexpr float LIFT = 2.f;          // P = 2^(z - base + LIFT) <= 2^2.875 < 7.5
+template <int D, int NT>
+constexpr int kResident = D == 64 && NT == 1 ? 5 : 4;   // CTAs a SM
+constexpr int FEW = 1024;            // keys up to which f16 and f32 outputs take the finer sums
 constexpr float LOG2E = 1.4426950408889634f;
 // More query rows than this per (sequence, KV head) go to kv4_prefill.cu.  Measured over 4 KV heads (us, here /
 // there): head dim 128, 48 rows 8 x 8000 50.8 / 49.6, 16 x 1000 18.3 / 25.6, 64 rows 73.8 / 49.9, 21.9 / 25.6;
@@ -66,6 +73,20 @@ FAK_DEV void mma_f16_1688_z(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t b0
   asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5}, {%6}, {%7,%7,%7,%7};"
                : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
                : "r"(a0), "r"(a1), "r"(b0), "f"(0.f));
+}
+FAK_DEV void mma_f16_1688(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t b0) {
+  asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5}, {%6}, {%0,%1,%2,%3};"
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+               : "r"(a0), "r"(a1), "r"(b0));
+}
+// a b - c, exact for c = a b rounded
+FAK_DEV uint32_t left_h2(uint32_t a, uint32_t b, uint32_t c) {
+  const __half2 r = __hfma2(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b), __hneg2(*reinterpret_cast<__half2*>(&c)));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+FAK_DEV uint32_t add_h2(uint32_t a, uint32_t b) {
+  const __half2 r = __hadd2(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&r);
 }
 FAK_DEV uint32_t movmatrix(uint32_t a) {
   uint32_t r;
@@ -116,8 +137,8 @@ FAK_DEV void cluster_sync() {
 
 // CLUSTER: the splits of a block are one thread-block cluster and merge through shared memory; else they
 // leave partial results for k_kv4_combine.  The sums are the same, in the same order.
-template <int D, int NT, bool CAP, bool CLUSTER>
-__global__ void __launch_bounds__(W * 32, 4)
+template <int D, int NT, bool CAP, bool CLUSTER, bool FINE>
+__global__ void __launch_bounds__(W * 32, kResident<D, NT>)
 k_kv4_attn(const __grid_constant__ Kv4Attn a, int n_split) {
   using L = Lay<D>;
   constexpr int NG = L::NG;
@@ -144,6 +165,7 @@ k_kv4_attn(const __grid_constant__ Kv4Attn a, int n_split) {
   const int early = lane * W < pps_full && ahead < a.width ? row[ahead] : -1;
   const int ctx = min(a.ctx[b], a.width * PAGE);
   if (tid == 0 && a.ctx[b] > ctx) report_error(a.err, 2);   // more keys than the table has pages for
+  const bool few = ctx <= FEW;
   int tok0 = b, n = 1;
   if (a.q_off) {
     tok0 = max(a.q_off[b], 0);
@@ -426,6 +448,11 @@ k_kv4_attn(const __grid_constant__ Kv4Attn a, int n_split) {
           const uint32_t b0 = mul_h2(p0[nt], s0[gr]), b1 = mul_h2(p1[nt], s1[gr]);
           mma_f16_16816(o[nt][gr][0], w0 & M0, w0 & M4, w1 & M0, w1 & M4, b0, b1);   // dims 4 g, 4 g + 1
           mma_f16_16816(o[nt][gr][1], u0 & M0, u0 & M4, u1 & M0, u1 & M4, b0, b1);   // dims 4 g + 2, 4 g + 3
+          if (FINE && few) {   // what the products p s lost, times the middle code 8
+            const uint32_t e = add_h2(left_h2(p0[nt], s0[gr], b0), left_h2(p1[nt], s1[gr], b1));
+            mma_f16_1688(o[nt][gr][0], 0x00080008u, 0x00800080u, e);
+            mma_f16_1688(o[nt][gr][1], 0x00080008u, 0x00800080u, e);
+          }
         }
       }
     }
@@ -638,7 +665,7 @@ Kv4AttnPlan kv4_attn_plan(const Kv4Attn& a, int n_sm) {
   // Clusters do not span the groups of SMs, so up to c - 1 of a group's slots stay empty: at 2000 keys 28 blocks of
   // 16 take 8.8 us, 32 take 13.1; 140 of 4 15.2, 144 21.3.  (Sizes between the powers of two lose more slots than
   // they gain: 96 blocks over 4000 keys 21.7 us in fours, 26.6 in sixes.)
-  const int resident = a.D == 64 && p.nt == 1 ? 5 : 4;   // CTAs a SM (36 blocks of 16 at head dim 64: 7.8 us, 28 7.8)
+  const int resident = a.D == 64 && p.nt == 1 ? kResident<64, 1> : 4;   // (36 blocks of 16 at head dim 64: 7.8 us, as 28)
   int64_t c = 1;
   while (c < 16 && 2 * c * (ctas + 9) <= resident * n_sm && c < most) c *= 2;
   if (a.n_split > 0) {
@@ -670,18 +697,24 @@ static void split_launch(const Kv4Attn& a, const Kv4AttnPlan& p, cudaStream_t st
     if (p.cluster) FAK_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
     FAK_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kern, a, p.n_split));
   };
-  const bool cap = a.softcap > 0.f;
-#define FAK_KV4(DV, NTV)                                                                  \
-  {                                                                                       \
-    if (cap && p.cluster) go(k_kv4_attn<DV, NTV, true, true>, sizeof(Smem<DV, NTV>));     \
-    else if (cap) go(k_kv4_attn<DV, NTV, true, false>, sizeof(Smem<DV, NTV>));            \
-    else if (p.cluster) go(k_kv4_attn<DV, NTV, false, true>, sizeof(Smem<DV, NTV>));      \
-    else go(k_kv4_attn<DV, NTV, false, false>, sizeof(Smem<DV, NTV>));                    \
-  }
-  if (a.D == 128) FAK_KV4(128, 1)
-  else if (p.nt == 1) FAK_KV4(64, 1)
-  else FAK_KV4(64, 2)
-#undef FAK_KV4
+  auto pick = [&](auto d, auto nt, auto cap, auto fine) {
+    constexpr int DV = decltype(d)::value, NTV = decltype(nt)::value;
+    constexpr bool CAP = decltype(cap)::value, FINE = decltype(fine)::value;
+    if (p.cluster) go(k_kv4_attn<DV, NTV, CAP, true, FINE>, sizeof(Smem<DV, NTV>));
+    else go(k_kv4_attn<DV, NTV, CAP, false, FINE>, sizeof(Smem<DV, NTV>));
+  };
+  auto by_type = [&](auto d, auto nt, auto cap) {
+    if (a.o_type == Elt::BF16) pick(d, nt, cap, std::false_type{});
+    else pick(d, nt, cap, std::true_type{});
+  };
+  auto by_cap = [&](auto d, auto nt) {
+    if (a.softcap > 0.f) by_type(d, nt, std::true_type{});
+    else by_type(d, nt, std::false_type{});
+  };
+  using std::integral_constant;
+  if (a.D == 128) by_cap(integral_constant<int, 128>{}, integral_constant<int, 1>{});
+  else if (p.nt == 1) by_cap(integral_constant<int, 64>{}, integral_constant<int, 1>{});
+  else by_cap(integral_constant<int, 64>{}, integral_constant<int, 2>{});
 }
 
 void kv4_attn_launch(const Kv4Attn& a, const Kv4AttnPlan& p, cudaStream_t stream) {
