@@ -28,6 +28,7 @@ namespace fak {
 namespace {
 
 constexpr int THREADS = 256;
+static_assert(sizeof(uint4) == kKv4LoadBytes && sizeof(float4) == kKv4LoadBytes, "the vector loads of Rows8");
 
 FAK_DEV float min_nan(float a, float b) {   // as fminf, but a NaN stays
   float r;

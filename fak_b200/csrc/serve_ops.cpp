@@ -103,7 +103,8 @@ void kv4_append(Tensor k, Tensor v, Tensor slot, Tensor pages, OptTensor err) {
       s_page = 16 * s_row;
       s_head = x.stride(1);
     }
-    r.vec = r.vec && aligned(x, 4) && s_page % 4 == 0 && s_row % 4 == 0 && s_head % 4 == 0;
+    const int64_t per = fak::kKv4LoadBytes / x.element_size();
+    r.vec = r.vec && aligned(x, per) && s_page % per == 0 && s_row % per == 0 && s_head % per == 0;
   };
   rows(k, "k", r.ks_page, r.ks_row, r.ks_head);
   rows(v, "v", r.vs_page, r.vs_row, r.vs_head);

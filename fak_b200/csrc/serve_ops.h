@@ -8,12 +8,14 @@ namespace fak {
 
 enum class Elt : int { F32 = 0, F16 = 1, BF16 = 2 };
 
+constexpr int kKv4LoadBytes = 16;   // what one vector load of the append takes of a row
+
 struct Kv4Rows {   // k / v rows: element (token, head, d) at ptr + (tok / 16) * s_page + (tok % 16) * s_row + head * s_head + d
   const void* k;
   const void* v;
   int64_t ks_page, ks_row, ks_head, vs_page, vs_row, vs_head;
   Elt type;
-  bool vec;   // every row 4-element aligned
+  bool vec;   // every row of every page and head starts on kKv4LoadBytes
 };
 void kv4_append_launch(const Kv4Rows& r, const int* slot, int T, int Hkv, int D, uint8_t* pages, int64_t n_pages,
                        int* err, cudaStream_t stream);
