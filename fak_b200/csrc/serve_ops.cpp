@@ -284,6 +284,7 @@ std::vector<Tensor> token_logprobs(Tensor logits, int64_t V, Tensor target, int6
   a.rank = rank.data_ptr<int>();
   a.top_ids = ids.data_ptr<int>();
   a.top_logprobs = top.data_ptr<float>();
+  if (T == 0) return {lp, en, rank, ids, top};
   a.n_seg = fak::logprob_segments(a.T, a.V, sms(logits));
   Tensor part, tickets;
   if (a.n_seg > 1) {
