@@ -228,7 +228,7 @@ __global__ void __launch_bounds__(THREADS, 4) k_logprobs(LogprobArgs a, int seg_
   const int rounds = (i_end - i_begin + STEP - 1) / STEP, first = i_begin + warp * TILE, lane0 = VEC<T> * lane;
   if (first < i_end) even.load(x, first + lane0, i_end, whole(first));
   if (given) xt = cap((float)x[tgt]);
-  xt_above = nextafterf(xt, INFINITY);
+  xt_above = xt == INFINITY ? __int_as_float(0x7fffffff) : nextafterf(xt, INFINITY);   // (a NaN: nothing reaches it)
 #pragma unroll 1
   for (int r2 = 0, base = first; base < i_end; r2 += 2, base += 2 * STEP) {
     const bool more = base + STEP < i_end;
