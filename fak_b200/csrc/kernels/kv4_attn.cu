@@ -16,7 +16,9 @@
 //                                                         sum is one m16n8k16 whose fifth row, all ones,
 //                                                         gives the softmax denominator
 // Queries are rounded to f16 after a power-of-two scaling of their row (exact for bf16 and f16 inputs up
-// to 28 binades below the row's largest); P is f16: at most 7.5, so that P s stays below 65504.  Rounding P
+// to 28 binades below the row's largest); P is f16, raised by a power of two that the warp's largest scale so far
+// allows, so that P s is neither above 65504 nor subnormal where a key of little weight meets a small scale (values
+// around 1e-4, 8000 keys 7 below the largest logit, one split: error 5e-2 -> 7e-4 of the largest output).  Rounding P
 // alone moves numerator and denominator alike; what P s loses meets codes around 8, and for outputs finer than
 // bf16 the loss times 8 is added back over up to 1024 keys (f16, 3 to 12 keys: error 3.4e-4 -> 2.4e-4 of the
 // output, 2.0e-4 being that of its rounding; over 8000 keys 2.04e-4 -> 2.02e-4, for 9 to 14% more time).
@@ -45,7 +47,11 @@ using namespace kv4;
 constexpr int W = kRowsGrain;   // warps per CTA
 constexpr int STAGES = 4;     // pages in flight per warp
 constexpr float HEADROOM = 0.875f;   // log2 growth of a row's max before its base moves
-constexpr float LIFT = 2.f;          // P = 2^(z - base + LIFT) <= 2^2.875 < 7.5
+constexpr float LIFT = 2.f;          // P = 2^(z - base + LIFT + raise) <= 7.34 * 2^raise
+// P s must fit f16 from its largest (P 7.34 * 2^raise, scales up to 8736 from the append) down to keys of little
+// weight under small scales, whose products would be subnormal: a warp raises P by the most its scales allow,
+// 2^raise with all of them below 2^(MOST_RAISE - raise).
+constexpr int MOST_RAISE = 13;
 template <int D, int NT>
 constexpr int kResident = D == 64 && NT == 1 ? 5 : 4;   // CTAs a SM
 constexpr int FEW = 1024;            // keys up to which f16 and f32 outputs take the finer sums
@@ -87,6 +93,14 @@ FAK_DEV uint32_t left_h2(uint32_t a, uint32_t b, uint32_t c) {
 FAK_DEV uint32_t add_h2(uint32_t a, uint32_t b) {
   const __half2 r = __hadd2(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b));
   return *reinterpret_cast<const uint32_t*>(&r);
+}
+FAK_DEV uint32_t max_h2(uint32_t a, uint32_t b) {
+  const __half2 r = __hmax2(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+FAK_DEV uint32_t pow2_h2(int n) { return (uint32_t)(n + 15) * 0x04000400u; }   // 2^n, -14 <= n <= 15
+FAK_DEV bool reaches(uint32_t a, uint32_t b) {   // either half of a is at least b's
+  return __hge2_mask(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b)) != 0;
 }
 FAK_DEV uint32_t movmatrix(uint32_t a) {
   uint32_t r;
@@ -298,7 +312,9 @@ k_kv4_attn(const __grid_constant__ Kv4Attn a, int n_split) {
   const int low_max = a.window > 0 ? max(0, lim_any - a.window) : 0;
 
   float o[NT][NG][2][4], mt[NT][4], base[NT][2];
-  float lift[NT][2];   // LIFT - base (0 while the base is -inf: then every z is -inf too)
+  float lift[NT][2];   // LIFT + raise - base (0 while the base is -inf: then every z is -inf too)
+  int raise = MOST_RAISE;
+  uint32_t s_most = pow2_h2(0);   // 2^(MOST_RAISE - raise), twice; infinity once raise is 0
 #pragma unroll
   for (int nt = 0; nt < NT; nt++) {
     base[nt][0] = base[nt][1] = -INFINITY;
@@ -387,7 +403,7 @@ k_kv4_attn(const __grid_constant__ Kv4Attn a, int n_split) {
           m = fmaxf(m, base[nt][e]);
           const float f = m == -INFINITY ? 1.f : ex2(base[nt][e] - m);
           base[nt][e] = m;
-          lift[nt][e] = m == -INFINITY ? 0.f : LIFT - m;
+          lift[nt][e] = m == -INFINITY ? 0.f : LIFT + raise - m;
           mt[nt][e] *= f;
 #pragma unroll
           for (int gr = 0; gr < NG; gr++)
@@ -438,6 +454,35 @@ k_kv4_attn(const __grid_constant__ Kv4Attn a, int n_split) {
         m0 &= keep0;
         m1 &= keep1;
       }
+      uint32_t s_top = max_h2(s0[0], s1[0]);
+#pragma unroll
+      for (int gr = 1; gr < NG; gr++) s_top = max_h2(s_top, max_h2(s0[gr], s1[gr]));
+      if (__any_sync(0xffffffffu, reaches(s_top, s_most))) {   // scales that do not allow this raise
+        asm volatile("");
+        const float2 y = unpack_h2(s_top);
+        const float top = warp_max(fmaxf(y.x, y.y));
+        const int drop = min(raise, (int)(__float_as_uint(top) >> 23) - 126 - (MOST_RAISE - raise));
+        const float f = __uint_as_float((uint32_t)(127 - drop) << 23);
+        const uint32_t f2 = pack_f16(f, f);
+        raise -= drop;
+        s_most = raise == 0 ? 0x7c007c00u : pow2_h2(MOST_RAISE - raise);
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++) {
+          p0[nt] = mul_h2(p0[nt], f2);
+          p1[nt] = mul_h2(p1[nt], f2);
+#pragma unroll
+          for (int e = 0; e < 2; e++) lift[nt][e] -= base[nt][e] == -INFINITY ? 0 : drop;
+#pragma unroll
+          for (int e = 0; e < 4; e++) {
+            mt[nt][e] *= f;
+#pragma unroll
+            for (int gr = 0; gr < NG; gr++) {
+              o[nt][gr][0][e] *= f;
+              o[nt][gr][1][e] *= f;
+            }
+          }
+        }
+      }
 #pragma unroll
       for (int nt = 0; nt < NT; nt++) mma_f16_16816(mt[nt], m0, 0u, m1, 0u, p0[nt], p1[nt]);
 #pragma unroll
@@ -478,7 +523,7 @@ k_kv4_attn(const __grid_constant__ Kv4Attn a, int n_split) {
             make_float4(fmaf(o[nt][gr][0][e], 16777216.f, ml[gr][e]), fmaf(o[nt][gr][0][e + 2], 1048576.f, ml[gr][e]),
                         fmaf(o[nt][gr][1][e], 16777216.f, ml[gr][e]), fmaf(o[nt][gr][1][e + 2], 1048576.f, ml[gr][e]));
       if (g == 4) {
-        sm.base[warp][col] = base[nt][e];
+        sm.base[warp][col] = base[nt][e] - raise;   // what the sums are against, without raise
         sm.sum[warp][col] = mt[nt][e];
       }
     }

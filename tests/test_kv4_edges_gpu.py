@@ -60,3 +60,81 @@ def test_append_rows_between_vector_boundaries(K, D, dtype, odd, by):
     for got, src in zip(K.kv4_read(pages, slot, D, torch.float32), x):
         want, _ = plain.quantized(src[:T].double().cpu().numpy())
         np.testing.assert_array_equal(got.double().cpu().numpy(), want.astype(np.float32).astype(np.float64))
+
+
+# ------------------------------------------------------------------------------------ attention
+U16 = 2.0 ** -11
+OUT_U = {torch.float32: 2.0 ** -24, torch.float16: 2.0 ** -11, torch.bfloat16: 2.0 ** -8}
+
+
+def cache(K, ks, vs):
+    """A cache of the rows ks, vs (lists of [c, Hkv, D]): pages, table, and the values it stands for (64 bits)."""
+    n = [max(1, -(-k.shape[0] // 16)) for k in ks]
+    Hkv, D = ks[0].shape[1:]
+    pages = torch.full((sum(n) + 1, Hkv, K.kv4_page_bytes(D)), 255, dtype=torch.uint8, device="cuda")   # NaN scales
+    table = torch.zeros(len(ks), max(n), dtype=torch.int32, device="cuda")
+    at, rk, rv = 1, [], []
+    for b, (k, v) in enumerate(zip(ks, vs)):
+        table[b, :n[b]] = torch.arange(at, at + n[b], device="cuda").flip(0)
+        at += n[b]
+        j = torch.arange(k.shape[0], device="cuda")
+        slot = (table[b, j // 16] * 16 + j % 16).to(torch.int32)
+        K.kv4_append(k, v, slot, pages)
+        for out, r in zip((rk, rv), K.kv4_read(pages, slot, D, torch.float32)):
+            out.append(r.double().cpu())
+    return pages, table, rk, rv
+
+
+def product_step(c):
+    """What the products of probabilities and scales may lose to f16's smallest step, over c keys: half a step
+    each, times the largest code, against a sum that holds a probability of 2^15 (scales below 1)."""
+    return c * 15 * 2.0 ** -25 / 2.0 ** 15
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("size", [1.0, 1e-2, 1e-3, 1e-4, 1e-5])
+@pytest.mark.parametrize("logit", [0.0, 7.0, 10.0])
+def test_small_values_under_a_key_that_stands_out(K, D, size, logit):
+    """One key's logit lies ``logit`` above thousands of equal ones, values of every magnitude: the others' share
+    must survive their products with small scales.  Tolerance as for decode (4 roundings of the largest value),
+    plus f16's smallest step."""
+    c, H = 4000, 3
+    g = gen(7)
+    k, v = torch.randn(c, 1, D, generator=g, device="cuda"), torch.randn(c, 1, D, generator=g, device="cuda") * size
+    k[:, :, 0] = 0
+    k[0, :, 0] = 8
+    pages, table, ks, vs = cache(K, [k], [v])
+    q = (torch.randn(2, H, D, generator=g, device="cuda") * 0.01).half().float()
+    q[:, :, 0] = round(logit * math.sqrt(D) * 16) / 128
+    want = plain.attention([q.double().cpu()[1:]], ks, vs, [c])[0]
+    for dtype in (torch.float32, torch.bfloat16):
+        tol = 4 * U16 * vs[0].abs().max() + OUT_U[dtype] * want.abs() + product_step(c)
+        for n_split in (0, 1, 3, 16, 20):
+            out = torch.empty(1, H, D, dtype=dtype, device="cuda")
+            K.kv4_decode_attention(q[1:], pages, table, dev([c]), out, n_split=n_split)
+            assert ((out.double().cpu() - want).abs() <= tol).all()
+            out = torch.empty(2, H, D, dtype=dtype, device="cuda")      # several rows
+            K.kv4_prefill_attention(q, pages, table, dev([0, 2]), dev([c]), out, 2, n_split=n_split, tiles=False)
+            assert ((out[1:].double().cpu() - want).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("D,H", [(64, 1), (64, 12), (128, 4)])
+@pytest.mark.parametrize("order", ["up", "down", "mixed"])
+@pytest.mark.parametrize("window", [0, 150])
+def test_scales_that_change_along_the_keys(K, D, H, order, window):
+    """Values from 1e-4 up to f16's largest: what a warp allows its probabilities has to follow the pages."""
+    c, n = 400, 3
+    g = gen(H)
+    size = torch.logspace(-4, math.log10(15000), c, device="cuda")
+    size = {"up": size, "down": size.flip(0), "mixed": size[torch.randperm(c, generator=g, device="cuda")]}[order]
+    k, v = torch.randn(c, 1, D, generator=g, device="cuda"), torch.randn(c, 1, D, generator=g, device="cuda") * size[:, None, None]
+    v[c // 2, 0, :32] = torch.linspace(-65504, 65504, 32, device="cuda")      # the largest scale
+    pages, table, ks, vs = cache(K, [k], [v])
+    q = torch.randn(n, H, D, generator=g, device="cuda").half().float()
+    sinks = torch.randn(H, generator=g, device="cuda") * 2
+    for sk in (None, sinks):
+        want = plain.attention([q.double().cpu()], ks, vs, [c], window=window, sinks=None if sk is None else sk.double().cpu())[0]
+        for n_split in (1, 2, 5, 16):
+            out = torch.empty(n, H, D, device="cuda")
+            K.kv4_prefill_attention(q, pages, table, dev([0, n]), dev([c]), out, n, n_split=n_split, window=window, sinks=sk, tiles=False)
+            assert ((out.double().cpu() - want).abs() <= 4 * U16 * vs[0].abs().max()).all()
