@@ -29,6 +29,7 @@
 #include "kv4_common.cuh"
 
 #include <algorithm>
+#include <cfloat>
 #include <stdexcept>
 #include <string>
 
@@ -428,7 +429,8 @@ k_kv4_prefill(const __grid_constant__ Kv4Attn a, int splits, int whole, int n_bl
         *reinterpret_cast<uint4*>(dst) = make_uint4(kv4::pack_f16(x[0] * f, x[4] * f), kv4::pack_f16(x[1] * f, x[5] * f),
                                                     kv4::pack_f16(x[2] * f, x[6] * f), kv4::pack_f16(x[3] * f, x[7] * f));
       }
-      cf = a.scale / f * (CAP ? 1.f : LOG2E);
+      // (never 0: a masked logit, -inf, is multiplied by it; |S| is at most 2^31, so that logits stay below 2^-94 there)
+      cf = fmaxf(a.scale / f * (CAP ? 1.f : LOG2E), FLT_MIN);
       tc::fence_proxy_async();
       __syncwarp();
       if (lane == 0) tc::mbar_arrive(&sm.q_full);

@@ -138,3 +138,19 @@ def test_scales_that_change_along_the_keys(K, D, H, order, window):
             out = torch.empty(n, H, D, device="cuda")
             K.kv4_prefill_attention(q, pages, table, dev([0, n]), dev([c]), out, n, n_split=n_split, window=window, sinks=sk, tiles=False)
             assert ((out.double().cpu() - want).abs() <= 4 * U16 * vs[0].abs().max()).all()
+
+
+@pytest.mark.parametrize("tiles", [False, True])
+@pytest.mark.parametrize("size,scale", [(0.0, 0.0), (0.0, 1e-8), (0.0, 1e-30), (1e-30, 1e-12), (1e-37, 1e-6), (1e-38, 0.125)])
+@pytest.mark.parametrize("softcap", [0.0, 20.0])
+def test_logits_that_vanish(K, tiles, size, scale, softcap):
+    """Queries and scales so small that every logit is 0: means over the keys each row sees."""
+    c, n, D = 200, 150, 64
+    g = gen(2)
+    pages, table, ks, vs = cache(K, [torch.randn(c, 1, D, generator=g, device="cuda")], [torch.randn(c, 1, D, generator=g, device="cuda")])
+    q = torch.randn(n, 1, D, generator=g, device="cuda") * size
+    out = torch.empty_like(q)
+    K.kv4_prefill_attention(q, pages, table, dev([0, n]), dev([c]), out, n, tiles=tiles, scale=scale, softcap=softcap)
+    hi = torch.arange(c - n + 1, c + 1)
+    want = (vs[0][:, 0].cumsum(0) / torch.arange(1, c + 1)[:, None])[hi - 1]
+    assert ((out[:, 0].double().cpu() - want).abs() <= 4 * U16 * vs[0].abs().max()).all()
