@@ -548,7 +548,7 @@ k_kv4_attn(const __grid_constant__ Kv4Attn a, int n_split) {
       f[w] = part_weight(sm.base[w][c], sm.sum[w][c], bs);
       l += f[w] * sm.sum[w][c];
     }
-    if (sink > -INFINITY) l += ex2(sink - bs + LIFT);
+    if (sink != -INFINITY) l += ex2(sink - bs + LIFT);
 #pragma unroll
     for (int d0 = 0; d0 < D; d0 += 64) {
       const int d = d0 + 2 * lane;
@@ -593,7 +593,7 @@ k_kv4_attn(const __grid_constant__ Kv4Attn a, int n_split) {
         const float2 z = remote_f2(&sm.o[0][c][d], s);
         merge_split(__shfl_sync(0xffffffffu, f, s), __shfl_sync(0xffffffffu, y.y, s), &z.x, l, acc);
       }
-      if (sink > -INFINITY) l += ex2(sink - m + LIFT);
+      if (sink != -INFINITY) l += ex2(sink - m + LIFT);
       const float inv = l != 0.f ? 1.f / l : 0.f;
       const int64_t at = (int64_t)(tok0 + qi) * a.o_tok + (int64_t)h * a.o_head + d;
       store_elt(a.out, a.o_type, at, acc[0] * inv);
@@ -657,7 +657,7 @@ __global__ void __launch_bounds__(256) k_kv4_combine(const __grid_constant__ Kv4
         merge_split(__shfl_sync(0xffffffffu, f, s), __shfl_sync(0xffffffffu, y.y, s), z, l, acc);
       }
     }
-    if (sink > -INFINITY) l += ex2(sink - m + lift);
+    if (sink != -INFINITY) l += ex2(sink - m + lift);
     const float inv = l != 0.f ? 1.f / l : 0.f;
     const int64_t at = (int64_t)(tok0 + qi) * a.o_tok + (int64_t)h * a.o_head + V * lane;
 #pragma unroll

@@ -533,7 +533,7 @@ k_kv4_prefill(const __grid_constant__ Kv4Attn a, int splits, int whole, int n_bl
     float f = 1.f;
     if (alone) {
       const float top = fmaxf(base, sink);
-      if (sink > -INFINITY) {
+      if (sink != -INFINITY) {
         f = base == -INFINITY ? 0.f : kv4::ex2(base - top);
         l = l * f + kv4::ex2(sink - top + LIFT);
       }

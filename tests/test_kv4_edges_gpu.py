@@ -154,3 +154,19 @@ def test_logits_that_vanish(K, tiles, size, scale, softcap):
     hi = torch.arange(c - n + 1, c + 1)
     want = (vs[0][:, 0].cumsum(0) / torch.arange(1, c + 1)[:, None])[hi - 1]
     assert ((out[:, 0].double().cpu() - want).abs() <= 4 * U16 * vs[0].abs().max()).all()
+
+
+@pytest.mark.parametrize("tiles,n_split", [(False, 1), (False, 4), (False, 20), (True, 1), (True, 3)])
+def test_sinks_that_are_no_numbers_or_none(K, tiles, n_split):
+    """A NaN sink makes its head NaN however the splits merge, with keys and without; one of -inf is no sink."""
+    D, lens = 64, [600, 0]
+    g = gen(3)
+    pages, table, ks, vs = cache(K, *([torch.randn(c, 2, D, generator=g, device="cuda") for c in lens] for _ in "kv"))
+    q = torch.randn(2, 4, D, generator=g, device="cuda")
+    sinks = torch.tensor([math.nan, -math.inf, 0.5, math.nan], device="cuda")
+    out, none = torch.empty_like(q), torch.empty_like(q)
+    for o, sk in ((out, sinks), (none, None)):
+        K.kv4_prefill_attention(q, pages, table, dev([0, 1, 2]), dev(lens), o, 1, tiles=tiles, n_split=n_split, sinks=sk)
+    assert torch.isnan(out[:, [0, 3]]).all() and torch.equal(out[:, 1], none[:, 1])
+    assert (none[1] == 0).all() and (out[1, 1:3] == 0).all()
+    assert not torch.equal(out[0, 2], none[0, 2]) and torch.isfinite(out[0, 2]).all()
