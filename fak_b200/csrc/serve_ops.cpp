@@ -71,6 +71,13 @@ Tensor tickets_for(const Tensor& like, int64_t n) {
   if (!t.defined() || t.numel() < n) t = torch::zeros({std::max<int64_t>(n, 4096)}, opt);
   return t;
 }
+// Some of v's first n elements lie among `rows` rows of `width` elements, `stride` apart, at t (4-byte elements).
+bool meets(const Tensor& v, int64_t n, const Tensor& t, int64_t rows, int64_t width, int64_t stride) {
+  if (n == 0 || rows == 0 || width == 0) return false;
+  const int64_t at = ((intptr_t)v.data_ptr() - (intptr_t)t.data_ptr()) / 4;
+  const int64_t row = stride > 0 && at >= width ? (at - width) / stride + 1 : 0;   // the first that ends past v's start
+  return row < rows && row * stride < at + n && row * stride + width > at;
+}
 bool aligned(const Tensor& t, int64_t elems) {
   return reinterpret_cast<uintptr_t>(t.data_ptr()) % (elems * t.element_size()) == 0;
 }
@@ -234,6 +241,13 @@ std::vector<Tensor> plan_batch(Tensor old_len, Tensor new_len, Tensor table, Ten
     const int64_t n[7] = {max_tokens, max_tokens, max_tokens, B + 1, B, B, 1};
     for (int i = 0; i < 7; i++) i32(o[i], n[i], old_len, "plan_batch: plan tensor");
     TORCH_CHECK(o[6].data_ptr() != free_head.data_ptr(), "plan_batch: the new free head needs a word of its own");
+    // CTAs read the lengths, the table and the free pages while others write the plan
+    for (int i = 0; i < 7; i++) {
+      for (const Tensor* in : {&old_len, &new_len, &free_pages, &free_head})
+        TORCH_CHECK(!meets(o[i], n[i], *in, 1, in->numel(), 0), "plan_batch: a plan tensor shares memory with the lengths or free pages");
+      TORCH_CHECK(!meets(o[i], n[i], table, table.size(0), table.size(1), table.stride(0)), "plan_batch: a plan tensor shares memory with the block table");
+      for (int j = 0; j < i; j++) TORCH_CHECK(!meets(o[i], n[i], o[j], 1, n[j], 0), "plan_batch: plan tensors share memory");
+    }
   } else {
     const int64_t n[7] = {max_tokens, max_tokens, max_tokens, B + 1, B, B, 1};
     int64_t at = 0, all = 0;

@@ -400,7 +400,8 @@ def plan_batch(cached: torch.Tensor, new: torch.Tensor, block_table: torch.Tenso
     cached, new [B] int32: tokens each request has in the cache and brings now.  block_table [B, W] int32
     holds the pages of the cached tokens; the entries of the pages that new tokens open are written from
     free_pages (int32), consumed in request order from index free_head[0] on.  max_tokens bounds the sum
-    of ``new``.  ``plan``: tensors to fill (BatchPlan.allocate; CUDA graphs), else new ones.  When the
+    of ``new``.  ``plan``: tensors to fill (BatchPlan.allocate; CUDA graphs), else new ones; they share no
+    memory with the inputs or with one another (``cached`` of the next step: a copy of ``plan.ctx``).  When the
     table is too narrow, the free pages run out, tokens pass max_tokens or a length is negative, the
     tokens concerned get slot -1 and code 2 goes to the device's error word."""
     p = BatchPlan(*ext().plan_batch(cached, new, block_table, free_pages, free_head, max_tokens, plan,
