@@ -10,6 +10,7 @@
 // 42 thousand new tokens 6.0 us.
 #include "common.cuh"
 
+#include <climits>
 #include <stdexcept>
 #include <string>
 
@@ -112,8 +113,8 @@ __global__ void __launch_bounds__(THREADS) k_batch_plan(BatchPlanArgs a) {
           }
         }
       }
-      if (page >= 0) slot = page * PAGE + pos % PAGE;
-      else report_error(a.err, 2);   // the table is too narrow or the free pages ran out: no slot
+      if (page >= 0 && page <= INT_MAX / PAGE) slot = page * PAGE + pos % PAGE;
+      else report_error(a.err, 2);   // the table is too narrow, the free pages ran out or hold no page: no slot
     }
     a.slot[i] = slot;
     a.pos[i] = pos;

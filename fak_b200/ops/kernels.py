@@ -402,8 +402,8 @@ def plan_batch(cached: torch.Tensor, new: torch.Tensor, block_table: torch.Tenso
     free_pages (int32), consumed in request order from index free_head[0] on.  max_tokens bounds the sum
     of ``new``.  ``plan``: tensors to fill (BatchPlan.allocate; CUDA graphs), else new ones; they share no
     memory with the inputs or with one another (``cached`` of the next step: a copy of ``plan.ctx``).  When the
-    table is too narrow, the free pages run out, tokens pass max_tokens or a length is negative, the
-    tokens concerned get slot -1 and code 2 goes to the device's error word."""
+    table is too narrow, the free pages run out, tokens pass max_tokens, a length is negative or
+    a page has no 32-bit slots, the tokens concerned get slot -1 and code 2 goes to the device's error word."""
     p = BatchPlan(*ext().plan_batch(cached, new, block_table, free_pages, free_head, max_tokens, plan,
                                     _err_word.get(cached.device)))
     count()

@@ -48,3 +48,24 @@ def test_a_plan_between_the_rows_of_its_table(K):
     r = K.plan_batch(dev([1, 2, 16]), dev([1, 2, 1]), table, dev([9]), dev([0]), 8, p)
     assert r.q_off[:4].tolist() == [0, 1, 3, 4] and r.ctx[:3].tolist() == [2, 4, 17] and r.last.tolist() == [0, 2, 3]
     assert r.slot.tolist() == [65, 82, 83, 144, -1, -1, -1, -1] and table.tolist() == [[4, 0, 0, 0], [5, 0, 0, 0], [6, 9, 0, 0]]
+
+
+@pytest.fixture
+def err(K):
+    word = torch.zeros(1, dtype=torch.int32, device="cuda")
+    K.register_error_word(word.device, word)
+    yield word
+    K.register_error_word(word.device, None)
+
+
+@pytest.mark.parametrize("where", ["table", "free pages"])
+def test_pages_at_the_end_of_32_bit_slots(K, err, where):
+    last = (2 ** 31 - 1) // 16
+    for page, slots, code in ((last, [2 ** 31 - 15], 0), (last + 1, [-1], 2), (2 ** 28, [-1], 2), (-1, [-1], 2)):
+        err.zero_()
+        if where == "table":
+            p = K.plan_batch(dev([1]), dev([1]), dev([[page]]), dev([0]), dev([0]), 1)
+        else:
+            p = K.plan_batch(dev([0]), dev([2]), dev([[0]]), dev([page]), dev([0]), 2)
+            slots = [slots[0] - 1 if slots[0] > 0 else -1, slots[0]]
+        assert p.slot.tolist() == slots and err.item() == code
