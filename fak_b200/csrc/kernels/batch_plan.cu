@@ -23,6 +23,10 @@ constexpr int PAGE = 16;
 constexpr int THREADS = 512;
 constexpr int PER_CTA = 2048;   // tokens filled by one CTA
 
+// Sums of tokens stay at MANY once they reach it: more than any capacity (checked below 2^30), and reported.
+constexpr int MANY = 1 << 30;
+FAK_DEV int add_tokens(int a, int b) { return (int)min((uint32_t)a + (uint32_t)b, (uint32_t)MANY); }   // a <= MANY
+
 __global__ void __launch_bounds__(THREADS) k_batch_plan(BatchPlanArgs a) {
   extern __shared__ int sm[];
   int* q_off = sm;               // [B + 1]
@@ -44,25 +48,26 @@ __global__ void __launch_bounds__(THREADS) k_batch_plan(BatchPlanArgs a) {
   for (int b = b0; b < b1; b++) {
     int o, n;
     lens(b, o, n);
-    mine.x += n;
+    mine.x = add_tokens(mine.x, n);
     mine.y += opened(o, n);
   }
   int2 inc = mine;
 #pragma unroll
   for (int d = 1; d < 32; d <<= 1) {
     const int x = __shfl_up_sync(0xffffffffu, inc.x, d), y = __shfl_up_sync(0xffffffffu, inc.y, d);
-    if (lane >= d) { inc.x += x; inc.y += y; }
+    if (lane >= d) { inc.x = add_tokens(inc.x, x); inc.y += y; }
   }
   if (lane == 31) sums[warp] = inc;
   __syncthreads();
-  int2 off = make_int2(inc.x - mine.x, inc.y - mine.y);
-  for (int w = 0; w < warp; w++) { off.x += sums[w].x; off.y += sums[w].y; }
+  int2 off = make_int2(__shfl_up_sync(0xffffffffu, inc.x, 1), __shfl_up_sync(0xffffffffu, inc.y, 1));
+  if (lane == 0) off = make_int2(0, 0);
+  for (int w = 0; w < warp; w++) { off.x = add_tokens(off.x, sums[w].x); off.y += sums[w].y; }
   for (int b = b0; b < b1; b++) {
     int o, n;
     lens(b, o, n);
     q_off[b] = off.x;
     base[b] = head + off.y;
-    off.x += n;
+    off.x = add_tokens(off.x, n);
     off.y += opened(o, n);
     if (b == B - 1) {
       q_off[B] = off.x;
@@ -73,7 +78,7 @@ __global__ void __launch_bounds__(THREADS) k_batch_plan(BatchPlanArgs a) {
     }
     if (blockIdx.x == 0) {
       // offsets never pass the capacity, so that what reads them stays inside the packed rows
-      a.q_off[b] = min(off.x - n, a.max_tokens);
+      a.q_off[b] = min(q_off[b], a.max_tokens);
       if (b == B - 1) a.q_off[B] = min(off.x, a.max_tokens);
       a.ctx[b] = o + n;
       a.last[b] = n > 0 && off.x <= a.max_tokens ? off.x - 1 : -1;
@@ -102,7 +107,7 @@ __global__ void __launch_bounds__(THREADS) k_batch_plan(BatchPlanArgs a) {
       pos = o + (i - q_off[seq]);
       const int pg = pos / PAGE, have = (o + PAGE - 1) / PAGE;
       int page = -1;
-      if (pos >= 0 && pg < a.width) {   // (sums that passed 32 bits would be negative)
+      if (pos >= 0 && pg < a.width) {   // (a position that passed 32 bits is negative)
         if (pg < have) {
           page = a.table[(int64_t)seq * a.table_stride + pg];
         } else {

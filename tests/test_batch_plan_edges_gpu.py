@@ -69,3 +69,18 @@ def test_pages_at_the_end_of_32_bit_slots(K, err, where):
             p = K.plan_batch(dev([0]), dev([2]), dev([[0]]), dev([page]), dev([0]), 2)
             slots = [slots[0] - 1 if slots[0] > 0 else -1, slots[0]]
         assert p.slot.tolist() == slots and err.item() == code
+
+
+@pytest.mark.parametrize("new", [[2 ** 31 - 1, 2 ** 31 - 1], [3] + [2 ** 30] * 4 + [5], [2 ** 30] * 600, [1, 2 ** 31 - 1, 1, 1]])
+def test_tokens_past_32_bits_are_reported(K, err, new):
+    """Sums that would come back to a small or negative number are tokens past the capacity like others."""
+    B, cap = len(new), 16
+    table = torch.arange(B, dtype=torch.int32, device="cuda")[:, None].contiguous()
+    p = K.plan_batch(dev([0] * B), dev(new), table, dev(list(range(B))), dev([0]), cap)
+    assert err.item() == 2
+    want = [0]
+    for n in new:
+        want.append(min(cap, want[-1] + n))
+    assert p.q_off.tolist() == want and p.ctx.tolist() == new
+    assert p.last.tolist() == [sum(new[:b + 1]) - 1 if sum(new[:b + 1]) <= cap else -1 for b in range(B)]
+    assert p.seq.tolist() == [next(b for b in range(B) if i < sum(new[:b + 1])) for i in range(cap)]
