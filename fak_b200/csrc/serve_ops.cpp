@@ -6,6 +6,7 @@
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGraphsC10Utils.h>
 
+#include <cmath>
 #include <map>
 #include <mutex>
 
@@ -185,6 +186,7 @@ void kv4_attention(Tensor q, Tensor pages, Tensor table, OptTensor q_off, Tensor
     a.sinks = sinks->data_ptr<float>();
   }
   TORCH_CHECK(softcap >= 0 && n_split >= 0 && n_split <= 4096, "kv4_attention: softcap >= 0, n_split in [0, 4096]");
+  TORCH_CHECK(scale >= 0 && std::isfinite((float)scale), "kv4_attention: scale ", std::to_string(scale), " (0: 1 / sqrt of the head dim)");
   a.scale = scale > 0 ? (float)scale : 1.0f / std::sqrt((float)a.D);
   a.softcap = (float)softcap;
   a.window = (int)window;

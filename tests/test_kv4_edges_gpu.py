@@ -170,3 +170,21 @@ def test_sinks_that_are_no_numbers_or_none(K, tiles, n_split):
     assert torch.isnan(out[:, [0, 3]]).all() and torch.equal(out[:, 1], none[:, 1])
     assert (none[1] == 0).all() and (out[1, 1:3] == 0).all()
     assert not torch.equal(out[0, 2], none[0, 2]) and torch.isfinite(out[0, 2]).all()
+
+
+# ------------------------------------------------------------------------------------ arguments
+@pytest.fixture(scope="module")
+def small(K):
+    g = gen(1)
+    x = [torch.randn(40, 2, 64, generator=g, device="cuda")]
+    pages, table, ks, vs = cache(K, x, x)
+    return torch.randn(1, 4, 64, generator=g, device="cuda"), pages, table, dev([40]), ks, vs
+
+
+@pytest.mark.parametrize("scale", [-0.125, math.nan, math.inf, 1e39])
+def test_scales_that_are_none_are_refused(K, small, scale):
+    q, pages, table, ctx, _, _ = small
+    with pytest.raises(RuntimeError, match="scale"):
+        K.kv4_decode_attention(q, pages, table, ctx, torch.empty_like(q), scale=scale)
+    with pytest.raises(RuntimeError, match="scale"):
+        K.kv4_prefill_attention(q, pages, table, dev([0, 1]), ctx, torch.empty_like(q), 1, scale=scale)
