@@ -189,7 +189,7 @@ void kv4_attention(Tensor q, Tensor pages, Tensor table, OptTensor q_off, Tensor
   TORCH_CHECK(scale >= 0 && std::isfinite((float)scale), "kv4_attention: scale ", std::to_string(scale), " (0: 1 / sqrt of the head dim)");
   a.scale = scale > 0 ? (float)scale : 1.0f / std::sqrt((float)a.D);
   a.softcap = (float)softcap;
-  a.window = (int)window;
+  a.window = (int)std::min<int64_t>(std::max<int64_t>(window, 0), INT32_MAX);   // (contexts are 32-bit)
   a.n_split = (int)n_split;
   a.tiles = (int)tiles;
   a.err = err_ptr(err, q);

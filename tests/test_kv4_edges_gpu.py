@@ -188,3 +188,14 @@ def test_scales_that_are_none_are_refused(K, small, scale):
         K.kv4_decode_attention(q, pages, table, ctx, torch.empty_like(q), scale=scale)
     with pytest.raises(RuntimeError, match="scale"):
         K.kv4_prefill_attention(q, pages, table, dev([0, 1]), ctx, torch.empty_like(q), 1, scale=scale)
+
+
+@pytest.mark.parametrize("tiles", [False, True])
+def test_windows_beyond_32_bits(K, small, tiles):
+    q, pages, table, ctx, _, _ = small
+    none, some = torch.empty_like(q), torch.empty_like(q)
+    K.kv4_prefill_attention(q, pages, table, dev([0, 1]), ctx, none, 1, tiles=tiles)
+    for window in (-5, -2 ** 40, 2 ** 31 - 1, 2 ** 31, 2 ** 32 + 5, 2 ** 62):
+        K.kv4_prefill_attention(q, pages, table, dev([0, 1]), ctx, some, 1, tiles=tiles, window=window)
+        # (a window may change how the keys are shared out, and with it the last bits)
+        assert ((some - none).abs() <= 1e-5).all()
