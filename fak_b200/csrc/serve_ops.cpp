@@ -185,7 +185,8 @@ void kv4_attention(Tensor q, Tensor pages, Tensor table, OptTensor q_off, Tensor
                     sinks->numel() >= a.H, "kv4_attention: sinks [H] float32");
     a.sinks = sinks->data_ptr<float>();
   }
-  TORCH_CHECK(softcap >= 0 && n_split >= 0 && n_split <= 4096, "kv4_attention: softcap >= 0, n_split in [0, 4096]");
+  TORCH_CHECK(softcap >= 0 && std::isfinite((float)softcap), "kv4_attention: softcap ", std::to_string(softcap), " (0: none)");
+  TORCH_CHECK(n_split >= 0 && n_split <= 4096, "kv4_attention: n_split in [0, 4096]");
   TORCH_CHECK(scale >= 0 && std::isfinite((float)scale), "kv4_attention: scale ", std::to_string(scale), " (0: 1 / sqrt of the head dim)");
   a.scale = scale > 0 ? (float)scale : 1.0f / std::sqrt((float)a.D);
   a.softcap = (float)softcap;
@@ -277,7 +278,7 @@ std::vector<Tensor> token_logprobs(Tensor logits, int64_t V, Tensor target, int6
               "token_logprobs: logits [T, >= V] on the GPU, last dimension contiguous");
   TORCH_CHECK(V > 0 && V <= logits.size(1) && V < (int64_t(1) << 30), "token_logprobs: V ", S(V), " of ", S(logits.size(1)), " columns");
   TORCH_CHECK(k >= 0 && k <= 32, "token_logprobs: 0 to 32 alternatives, got ", S(k));
-  TORCH_CHECK(softcap >= 0, "token_logprobs: softcap >= 0");
+  TORCH_CHECK(softcap >= 0 && std::isfinite((float)softcap), "token_logprobs: softcap ", std::to_string(softcap), " (0: none)");
   fak::LogprobArgs a{};
   a.type = elt(logits, "token_logprobs: logits");
   a.T = (int)logits.size(0);

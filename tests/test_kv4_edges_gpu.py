@@ -199,3 +199,12 @@ def test_windows_beyond_32_bits(K, small, tiles):
         K.kv4_prefill_attention(q, pages, table, dev([0, 1]), ctx, some, 1, tiles=tiles, window=window)
         # (a window may change how the keys are shared out, and with it the last bits)
         assert ((some - none).abs() <= 1e-5).all()
+
+
+@pytest.mark.parametrize("softcap", [-1.0, math.nan, math.inf, 1e39])
+def test_softcaps_that_are_none_are_refused(K, small, softcap):
+    q, pages, table, ctx, _, _ = small
+    with pytest.raises(RuntimeError, match="softcap"):
+        K.kv4_decode_attention(q, pages, table, ctx, torch.empty_like(q), softcap=softcap)
+    with pytest.raises(RuntimeError, match="softcap"):
+        K.token_logprobs(q[0], 64, dev([0] * 4), 0, softcap)
