@@ -317,7 +317,7 @@ k_kv4_read(const uint8_t* __restrict__ pages, int64_t n_pages, const int* __rest
 template <typename... P, typename... A>
 void launch_rows(void (*kern)(P...), int T, int Hkv, int D, cudaStream_t stream, A... args) {
   const int per_cta = THREADS / (D / 8);
-  const int n = (T + per_cta - 1) / per_cta, y = n < 32768 ? n : 32768;
+  const int n = (int)(((int64_t)T + per_cta - 1) / per_cta), y = n < 32768 ? n : 32768;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)Hkv, (unsigned)y, (unsigned)((n + y - 1) / y));
   cfg.blockDim = dim3(THREADS);

@@ -447,7 +447,7 @@ __global__ void __launch_bounds__(THREADS, 4) k_logprobs(LogprobArgs a, int seg_
 // 20.7 us, in 16 26.5; 148 rows in 1 / 2 / 4 52.4 / 42.2 / 38.8; 300 rows in 1 58.5, in 2 73.8.)
 int logprob_segments(int T, int V, int n_sm) {
   const int tiles = (V + WARPS * TILE - 1) / (WARPS * TILE);
-  const int want = std::max(1, std::min(9 * n_sm / (4 * T), std::min(tiles, 64)));
+  const int want = std::max(1, (int)std::min<int64_t>(9 * n_sm / ((int64_t)4 * T), std::min(tiles, 64)));
   return std::max(want, (tiles + MOST_TILES - 1) / MOST_TILES);
 }
 int64_t logprob_part_words(int T, int n_seg) { return n_seg > 1 ? (int64_t)T * n_seg * REC : 0; }
@@ -458,7 +458,7 @@ void logprob_launch(const LogprobArgs& a, cudaStream_t stream) {
   seg = (seg + TILE - 1) / TILE * TILE;
   const int tiles = (seg + WARPS * TILE - 1) / (WARPS * TILE);
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)a.n_seg, (unsigned)(a.T < 32768 ? a.T : 32768), (unsigned)((a.T + 32767) / 32768));
+  cfg.gridDim = dim3((unsigned)a.n_seg, (unsigned)(a.T < 32768 ? a.T : 32768), (unsigned)(((int64_t)a.T + 32767) / 32768));
   cfg.blockDim = dim3(THREADS);
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];

@@ -79,6 +79,11 @@ bool meets(const Tensor& v, int64_t n, const Tensor& t, int64_t rows, int64_t wi
   const int64_t row = stride > 0 && at >= width ? (at - width) / stride + 1 : 0;   // the first that ends past v's start
   return row < rows && row * stride < at + n && row * stride + width > at;
 }
+// rows (of a tensor that may be expanded) as the kernels count them
+int rows32(int64_t n, const char* what) {
+  TORCH_CHECK(n <= INT32_MAX, what, ": ", S(n), " rows are too many");
+  return (int)n;
+}
 bool aligned(const Tensor& t, int64_t elems) {
   return reinterpret_cast<uintptr_t>(t.data_ptr()) % (elems * t.element_size()) == 0;
 }
@@ -91,7 +96,7 @@ void kv4_append(Tensor k, Tensor v, Tensor slot, Tensor pages, OptTensor err) {
   fak::Kv4Rows r{};
   r.type = elt(k, "kv4_append: k");
   TORCH_CHECK(v.scalar_type() == k.scalar_type(), "kv4_append: k and v differ in type");
-  const int64_t T = slot.numel();
+  const int64_t T = rows32(slot.numel(), "kv4_append");
   r.vec = true;
   auto rows = [&](const Tensor& x, const char* what, int64_t& s_page, int64_t& s_row, int64_t& s_head) {
     TORCH_CHECK(x.device() == pages.device(), "kv4_append: ", what, " is not on the pages' device");
@@ -128,7 +133,7 @@ void kv4_append(Tensor k, Tensor v, Tensor slot, Tensor pages, OptTensor err) {
 std::vector<Tensor> kv4_read(Tensor pages, Tensor slot, int64_t head_dim, c10::ScalarType dtype, OptTensor err) {
   const int D = check_pages(pages, "kv4_read");
   TORCH_CHECK(D == head_dim, "kv4_read: the pages hold heads of ", S(D), ", not ", S(head_dim));
-  const int64_t T = slot.numel(), Hkv = pages.size(1);
+  const int64_t T = rows32(slot.numel(), "kv4_read"), Hkv = pages.size(1);
   const int* sl = i32(slot, T, pages, "kv4_read: slot");
   c10::cuda::CUDAGuard guard(pages.device());
   auto opt = pages.options().dtype(dtype);
@@ -166,12 +171,12 @@ void kv4_attention(Tensor q, Tensor pages, Tensor table, OptTensor q_off, Tensor
   a.table = table.data_ptr<int>();
   a.table_stride = table.stride(0);
   a.width = (int)std::min<int64_t>(table.size(1), INT32_MAX / 16);
+  a.n_tokens = rows32(q.size(0), "kv4_attention");
   a.ctx = i32(ctx, 0, q, "kv4_attention: ctx_len");
-  a.n_tokens = (int)q.size(0);
   a.H = (int)q.size(1);
   a.G = a.H / a.Hkv;
   a.g_inv = a.G > 1 ? (uint32_t)(((uint64_t(1) << 32) + a.G - 1) / a.G) : 0;
-  a.B = (int)ctx.numel();
+  a.B = rows32(ctx.numel(), "kv4_attention");
   a.max_new = (int)max_new;
   TORCH_CHECK(table.size(0) >= a.B, "kv4_attention: block table has ", S(table.size(0)), " rows for ", S(a.B), " sequences");
   if (q_off.has_value()) {
@@ -230,9 +235,9 @@ std::vector<Tensor> plan_batch(Tensor old_len, Tensor new_len, Tensor table, Ten
   a.B = (int)B;
   a.table = table.data_ptr<int>();
   a.table_stride = table.stride(0);
-  a.width = (int)table.size(1);
+  a.width = (int)std::min<int64_t>(table.size(1), INT32_MAX / 16 + 1);
+  a.n_free = rows32(free_pages.numel(), "plan_batch: free pages");
   a.free_pages = i32(free_pages, 0, old_len, "plan_batch: free pages");
-  a.n_free = (int)free_pages.numel();
   a.head = i32(free_head, 1, old_len, "plan_batch: free head");
   a.max_tokens = (int)max_tokens;
   a.err = err_ptr(err, old_len);
@@ -281,7 +286,7 @@ std::vector<Tensor> token_logprobs(Tensor logits, int64_t V, Tensor target, int6
   TORCH_CHECK(softcap >= 0 && std::isfinite((float)softcap), "token_logprobs: softcap ", std::to_string(softcap), " (0: none)");
   fak::LogprobArgs a{};
   a.type = elt(logits, "token_logprobs: logits");
-  a.T = (int)logits.size(0);
+  a.T = rows32(logits.size(0), "token_logprobs");
   a.V = (int)V;
   a.k = (int)k;
   a.x = logits.data_ptr();

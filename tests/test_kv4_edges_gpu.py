@@ -208,3 +208,20 @@ def test_softcaps_that_are_none_are_refused(K, small, softcap):
         K.kv4_decode_attention(q, pages, table, ctx, torch.empty_like(q), softcap=softcap)
     with pytest.raises(RuntimeError, match="softcap"):
         K.token_logprobs(q[0], 64, dev([0] * 4), 0, softcap)
+
+
+@pytest.mark.parametrize("n", [2 ** 31, 2 ** 32 + 1])
+def test_rows_past_32_bits_are_refused(K, small, n):
+    """Expanded tensors reach such counts in little memory."""
+    q, pages, table, ctx, _, _ = small
+    x, slot = torch.zeros(1, 2, 64, device="cuda"), dev([-1])
+    with pytest.raises(RuntimeError, match="too many"):
+        K.kv4_append(x.expand(n, -1, -1), x.expand(n, -1, -1), slot.expand(n), pages)
+    with pytest.raises(RuntimeError, match="too many"):
+        K.kv4_read(pages, slot.expand(n), 64)
+    with pytest.raises(RuntimeError, match="too many"):
+        K.kv4_decode_attention(q.expand(n, -1, -1), pages, table, ctx, torch.empty_like(q).expand(n, -1, -1))
+    with pytest.raises(RuntimeError, match="too many"):
+        K.token_logprobs(q[0, :1].expand(n, -1), 64, slot.expand(n))
+    with pytest.raises(RuntimeError, match="too many"):
+        K.plan_batch(dev([0]), dev([1]), table, slot.expand(n), dev([0]), 1)
