@@ -51,10 +51,9 @@ int check_pages(const Tensor& pages, const char* what) {
   TORCH_CHECK(reinterpret_cast<uintptr_t>(pages.data_ptr()) % 16 == 0, what, ": pages must start on a 16-byte boundary");
   return (int)pages.size(2) / 20;
 }
-// A tensor of 4-byte elements inside one buffer of them: an operator's outputs share one allocation.
-Tensor carve(const Tensor& buf, int64_t at, at::IntArrayRef sizes, c10::ScalarType type) {
-  Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(buf.storage()), buf.key_set(),
-                                                      c10::scalarTypeToTypeMeta(type));
+// A tensor inside a buffer of its own type: the parts of a plan share one allocation.
+Tensor carve(const Tensor& buf, int64_t at, at::IntArrayRef sizes) {
+  Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(buf.storage()), buf.key_set(), buf.dtype());
   t.unsafeGetTensorImpl()->set_storage_offset(at);
   t.unsafeGetTensorImpl()->set_sizes_contiguous(sizes);
   return t;
@@ -263,7 +262,7 @@ std::vector<Tensor> plan_batch(Tensor old_len, Tensor new_len, Tensor table, Ten
     Tensor buf = torch::empty({all}, old_len.options());
     o.reserve(7);
     for (int64_t k : n) {
-      o.push_back(carve(buf, at, {k}, torch::kInt32));
+      o.push_back(carve(buf, at, {k}));
       at += up4(k);
     }
   }
@@ -296,11 +295,10 @@ std::vector<Tensor> token_logprobs(Tensor logits, int64_t V, Tensor target, int6
   const int64_t per = a.type == fak::Elt::F32 ? 4 : 8;
   a.vec = aligned(logits, per) && (a.stride % per == 0 || a.T <= 1);
   c10::cuda::CUDAGuard guard(logits.device());
-  const int64_t T = a.T, rows = up4(T);
-  Tensor buf = torch::empty({3 * rows + 2 * up4(T * k)}, logits.options().dtype(torch::kFloat32));
-  Tensor lp = carve(buf, 0, {T}, torch::kFloat32), en = carve(buf, rows, {T}, torch::kFloat32);
-  Tensor rank = carve(buf, 2 * rows, {T}, torch::kInt32), ids = carve(buf, 3 * rows, {T, k}, torch::kInt32);
-  Tensor top = carve(buf, 3 * rows + up4(T * k), {T, k}, torch::kFloat32);
+  const int64_t T = a.T;
+  const auto f32 = logits.options().dtype(torch::kFloat32), i32t = logits.options().dtype(torch::kInt32);
+  Tensor lp = torch::empty({T}, f32), en = torch::empty({T}, f32), rank = torch::empty({T}, i32t);
+  Tensor ids = torch::empty({T, k}, i32t), top = torch::empty({T, k}, f32);
   a.logprob = lp.data_ptr<float>();
   a.entropy = en.data_ptr<float>();
   a.rank = rank.data_ptr<int>();
@@ -312,7 +310,7 @@ std::vector<Tensor> token_logprobs(Tensor logits, int64_t V, Tensor target, int6
   if (a.n_seg > 1) {
     tickets = tickets_for(logits, T);
     a.tickets = tickets.data_ptr<int>();
-    part = torch::empty({fak::logprob_part_words(a.T, a.n_seg)}, buf.options());
+    part = torch::empty({fak::logprob_part_words(a.T, a.n_seg)}, f32);
     a.part = part.data_ptr<float>();
   }
   fak::logprob_launch(a, stream_of(logits));

@@ -84,3 +84,9 @@ def test_tokens_past_32_bits_are_reported(K, err, new):
     assert p.q_off.tolist() == want and p.ctx.tolist() == new
     assert p.last.tolist() == [sum(new[:b + 1]) - 1 if sum(new[:b + 1]) <= cap else -1 for b in range(B)]
     assert p.seq.tolist() == [next(b for b in range(B) if i < sum(new[:b + 1])) for i in range(cap)]
+
+
+def test_a_plan_is_saved(K, tmp_path):
+    p = K.plan_batch(dev([1]), dev([2]), dev([[3]]), dev([4]), dev([0]), 4)
+    torch.save(tuple(p), tmp_path / "p.pt")
+    assert all(torch.equal(a, b) for a, b in zip(p, torch.load(tmp_path / "p.pt")))

@@ -30,3 +30,13 @@ def test_rank_beside_infinities(K, V, dtype, softcap):
         x[:, i] = float("inf")
     r = K.token_logprobs(x, V, torch.tensor(at, dtype=torch.int32, device="cuda"), 4, softcap)
     assert r.rank.tolist() == [1, 2, 3] and r.top_ids[:, :3].tolist() == [at] * 3
+
+
+def test_outputs_are_saved_and_kept_by_themselves(K, tmp_path):
+    g = torch.Generator(device="cuda")
+    g.manual_seed(1)
+    x = torch.randn(3, 500, generator=g, device="cuda")
+    r = K.token_logprobs(x, 500, torch.tensor([1, 2, 3], dtype=torch.int32, device="cuda"), 4)
+    torch.save(tuple(r), tmp_path / "r.pt")
+    assert all(torch.equal(a, b) for a, b in zip(r, torch.load(tmp_path / "r.pt")))
+    assert all(t.untyped_storage().nbytes() == t.numel() * 4 for t in r)
