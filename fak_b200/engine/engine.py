@@ -278,6 +278,8 @@ class Engine:
             raise ValueError("score: empty prompt")
         if max(map(len, prompts)) > self.max_context:
             raise ValueError(f"score: a prompt exceeds context {self.max_context}")
+        if min(map(min, prompts)) < 0 or max(map(max, prompts)) >= self.cfg.vocab_size:
+            raise ValueError(f"score: a token outside the vocabulary of {self.cfg.vocab_size}")
         if not 0 <= top_k <= 32:
             raise ValueError("score: 0 to 32 alternatives")
         self._drain()

@@ -1,0 +1,49 @@
+"""Scoring and the engine on a 4-bit KV cache where they can go wrong."""
+import numpy as np
+import pytest
+import torch
+
+from fak_b200.config import EngineConfig, preset
+from fak_b200.gguf.synth import write_synthetic_gguf
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module", params=["tiny-qwen2", "tiny-llama", "tiny-gemma2"])
+def model_file(request, tmp_path_factory):
+    path = str(tmp_path_factory.mktemp("kv4e") / f"{request.param}.gguf")
+    write_synthetic_gguf(path, preset(request.param), "q8_0", seed=5, std=0.05)
+    return path
+
+
+def engine(path, precision="q4", graphs=False, **kw):
+    from fak_b200.engine import Engine
+    kw = {"max_batch": 4, "kv_pages": 256, **kw}
+    eng = Engine.from_gguf(path, EngineConfig(cuda_graph=graphs, graph_batch_buckets=(1, 2, 4), kv_precision=precision, **kw),
+                           "cuda", max_context=1024)
+    if graphs:
+        eng.warmup_graphs()
+    return eng
+
+
+def prompts(vocab, lens, seed=0):
+    rng = np.random.default_rng(seed)
+    return [rng.integers(0, vocab, n).tolist() for n in lens]
+
+
+@pytest.mark.parametrize("precision", ["bf16", "q4"])
+def test_score_refuses_tokens_outside_the_vocabulary(model_file, precision):
+    """Before they reach the device, whose error word would end every request that runs."""
+    eng = engine(model_file, precision)
+    V = eng.cfg.vocab_size
+    p = prompts(V, [30])[0]
+    alone = eng.generate([p], max_new_tokens=8)[0]
+    r = eng.add_request(p, 8)
+    eng.step()
+    for bad in ([[1, V]], [[1, 2], [3, -1, 4]]):
+        with pytest.raises(ValueError, match="vocabulary"):
+            eng.score(bad)
+    while eng.has_work():
+        eng.step()
+    assert r.finish_reason == "length" and r.output == alone
+    assert len(eng.score([[0, V - 1]])[0]["logprob"]) == 1
