@@ -289,14 +289,22 @@ class Engine:
         to = lambda a: torch.tensor(a, dtype=torch.int32).pin_memory().to(dev, non_blocking=True)
         queue = list(range(len(prompts)))
         while queue:
-            need, active = 0, []     # the group's pages are held until all of it is scored
-            while queue and len(active) < 4096:   # prompts whose pages fit together (one at least)
+            # prompts whose pages fit together (one at least); the group's pages are held until all of it is scored.
+            # Cached prefixes give way to one chunk's worth of prompts, as to any request.
+            need, active, room = 0, [], self.pool.n_free()
+            if self.radix is not None:
+                room = max(room, min(room + self.radix.stats()["cached_pages"], -(-cap // ps)))
+            while queue and len(active) < 4096:
                 n = -(-len(prompts[queue[0]]) // ps)
-                if active and need + n > self.pool.n_free():
+                if active and need + n > room:
                     break
                 need += n
                 active.append(queue.pop(0))
-            pages = self._alloc(need)
+            try:
+                pages = self._alloc(need)
+            except OutOfPages:      # cached pages that running requests hold as well
+                queue[:0], active = active[1:], active[:1]
+                pages = self._alloc(-(-len(prompts[active[0]]) // ps))
             try:
                 free, head = to(pages), to([0])
                 bt = torch.zeros(len(active), max(-(-len(prompts[i]) // ps) for i in active), dtype=torch.int32, device=dev)

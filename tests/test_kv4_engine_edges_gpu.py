@@ -47,3 +47,34 @@ def test_score_refuses_tokens_outside_the_vocabulary(model_file, precision):
         eng.step()
     assert r.finish_reason == "length" and r.output == alone
     assert len(eng.score([[0, V - 1]])[0]["logprob"]) == 1
+
+
+@pytest.mark.parametrize("held", [False, True])
+def test_score_groups_prompts_beside_a_full_prefix_cache(model_file, held):
+    """Cached prefixes that nobody uses give way to a chunk's prompts, so that a pool full of them does not mean
+    one prompt a pass; prefixes that a running request holds stay."""
+    ps = prompts(preset("tiny-llama").vocab_size, [40] * 8, 1)
+    want = engine(model_file).score(ps)
+    eng = engine(model_file, kv_pages=64, max_prefill_tokens=512)
+    seen = prompts(eng.cfg.vocab_size, [200] * 4, 2)
+    for p in seen:
+        eng.generate([p], max_new_tokens=4)
+    assert eng.pool.n_free() < 24       # the prompts take 24 pages
+    if held:
+        reqs = [eng.add_request(p + [1], 40) for p in seen]
+        while any(not r.output for r in reqs):
+            eng.step()
+    calls, plain = [], eng.runner.score
+
+    def score(*a, **kw):
+        calls.append(1)
+        return plain(*a, **kw)
+    eng.runner.score = score
+    got = eng.score(ps)
+    assert (len(calls) > 1) if held else (len(calls) == 1)
+    for a, b in zip(want, got):     # the same values through other tiles, as in chunks
+        np.testing.assert_allclose(a["logprob"], b["logprob"], atol=0.1)
+    if held:
+        while eng.has_work():
+            eng.step()
+        assert all(r.finish_reason == "length" for r in reqs)
