@@ -484,8 +484,15 @@ class Engine:
         part, _ = K.tgemv_workspace(self.device)
         part.fill_(nan)
         if self._kv_type is KV4Cache:
-            # code 15 with scale 2048 and minimum 0: the largest finite values of the layout's f16 parts
-            self.kv.pages.fill_(0x68)
+            # every code 15, every scale and minimum 2048: values of 32768, finite in f16
+            D, pages = self.cfg.head_dim, self.kv.pages
+            for at in (0, 10 * D):      # K, then V: 8 D bytes of codes, 2 D of f16 scales and minima
+                pages[..., at:at + 8 * D].fill_(0xFF)
+                meta = pages[..., at + 8 * D:at + 10 * D]
+                meta[..., 0::2].fill_(0x00)
+                meta[..., 1::2].fill_(0x68)
+            for t in (rn.stage.k, rn.stage.v, rn.attn_out, rn.kv4_ws):
+                t.fill_(nan)
         else:
             self.kv.k.fill_(3.0e4)
             self.kv.v.fill_(3.0e4)

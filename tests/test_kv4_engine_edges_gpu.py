@@ -78,3 +78,19 @@ def test_score_groups_prompts_beside_a_full_prefix_cache(model_file, held):
         while eng.has_work():
             eng.step()
         assert all(r.finish_reason == "length" for r in reqs)
+
+
+@pytest.mark.parametrize("graphs", [False, True])
+def test_poisoned_scratch_and_pages_change_nothing(model_file, graphs):
+    """The debug fill: NaN in the scratch of the 4-bit path too, 32768 wherever a page was not written."""
+    from fak_b200.ops import kernels as K
+    eng = engine(model_file, graphs=graphs, debug_poison=True)
+    ps = prompts(eng.cfg.vocab_size, [40, 7, 100, 16], 2)
+    rn = eng.runner
+    k, v = K.kv4_read(rn.kv.pages[0], torch.arange(64, dtype=torch.int32, device="cuda") + 160, rn.D, torch.float32)
+    assert (k == 32768).all() and (v == 32768).all()
+    if not graphs:      # (their capture runs steps)
+        assert all(torch.isnan(t).all() for t in (rn.stage.k, rn.stage.v, rn.attn_out, rn.kv4_ws))
+    clean = engine(model_file, graphs=graphs)
+    assert eng.generate(ps, max_new_tokens=24) == clean.generate(ps, max_new_tokens=24)
+    assert eng.score(ps, top_k=2) == clean.score(ps, top_k=2)
