@@ -94,3 +94,27 @@ def test_poisoned_scratch_and_pages_change_nothing(model_file, graphs):
     clean = engine(model_file, graphs=graphs)
     assert eng.generate(ps, max_new_tokens=24) == clean.generate(ps, max_new_tokens=24)
     assert eng.score(ps, top_k=2) == clean.score(ps, top_k=2)
+
+
+@pytest.mark.parametrize("precision", ["bf16", "q4"])
+def test_score_in_chunks_of_either_cache(model_file, precision):
+    """Chunks in which some prompts have no token left, or none yet."""
+    ps = prompts(preset("tiny-llama").vocab_size, [100, 3, 61, 20, 1], 1)
+    whole = engine(model_file, precision).score(ps, top_k=3)
+    for cap in (17, 32):
+        for a, b in zip(whole, engine(model_file, precision, max_prefill_tokens=cap).score(ps, top_k=3)):
+            # the same values through other tiles: 16-bit roundings of the attention and GEMM inputs move
+            assert len(a["logprob"]) == len(b["logprob"])
+            np.testing.assert_allclose(a["logprob"], b["logprob"], atol=0.1)
+            np.testing.assert_allclose(a["entropy"], b["entropy"], atol=0.1)
+
+
+@pytest.mark.parametrize("drafter", ["self", "lookup", "multi"])
+def test_speculation_keeps_the_tokens(model_file, drafter):
+    """Verified tokens are those of one step after another, drafts and their rejected rows in the pages or not."""
+    p = prompts(preset("tiny-llama").vocab_size, [11, 40], 6)
+    ps = [p[0] * 4, p[1]]       # one that repeats itself
+    want = engine(model_file, graphs=True).generate(ps, max_new_tokens=24)
+    eng = engine(model_file, graphs=True, spec_k=3, spec_drafter=drafter, max_batch=16)    # 4 rows a request
+    assert eng.generate(ps, max_new_tokens=24) == want
+    assert eng.stats["spec_proposed"] > 0
