@@ -329,7 +329,7 @@ class EngineConfig:
     async_decode: bool = True           # device-resident lane state; tokens read back one step behind
     p2p_spin_limit: int = 0             # polls before a cross-rank wait gives up (0: kernel default, ~1 s)
     kv_precision: str = "bf16"          # paged KV cache: "bf16", or "q4" (4-bit codes, f16 scale and minimum per 32
-                                        # dims; 3.2x the tokens; one GPU, no span eviction / swap / hand-off / tree)
+                                        # dims; 3.2x the tokens; one GPU, no span eviction / swap / hand-off / tree / cascade)
     cpu_offload_experts: bool = False   # MoE experts in host memory, their FFNs on the CPU (no CUDA graphs)
 
     ENV_KEYS = {

@@ -13,8 +13,8 @@
 // corrected by one remainder step with r = 1 / s correctly rounded (Markstein 1990: the result is the
 // correctly rounded quotient), two at a time; the four codes of a half word are summed as floats (c0 + 16 c1
 // + 256 c2 + 4096 c3 is exact); heads are a grid dimension.
-// Measured at 8191 tokens x 8 heads of 128, bf16: append 14.9 us (44 MB, 3.0 TB/s; bound by instructions; 18.5
-// with every lane on both scales and one quotient at a time), read 9.5 us (4.6 TB/s).
+// Measured at 8191 tokens x 8 heads of 128, bf16: append 15.5 us (44 MB, 2.8 TB/s; bound by instructions; 18.5
+// with every lane on both scales and one quotient at a time), read 9.6 us (4.6 TB/s).
 #include "kv4.cuh"
 
 #include <cuda_fp16.h>

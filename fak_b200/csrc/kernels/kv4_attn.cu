@@ -15,11 +15,11 @@
 //   o_d = sum_j (p_j s_jg) c_jd + sum_j p_j m_jg          the scale multiplies P (f16) per group; the second
 //                                                         sum is one m16n8k16 whose fifth row, all ones,
 //                                                         gives the softmax denominator
-// Queries are rounded to f16 after a power-of-two scaling of their row (exact for bf16 and f16 inputs up
-// to 28 binades below the row's largest); P is f16, raised by a power of two that the warp's largest scale so far
-// allows, so that P s is neither above 65504 nor subnormal where a key of little weight meets a small scale (values
-// around 1e-4, 8000 keys 7 below the largest logit, one split: error 5e-2 -> 7e-4 of the largest output).  Rounding P
-// alone moves numerator and denominator alike; what P s loses meets codes around 8, and for outputs finer than
+// Queries are rounded to f16 after a power-of-two scaling of their row (exact for f16 inputs up to 23 binades below
+// the row's largest, for bf16 up to 26: every other dim is scaled down by 16 more); P is f16, raised by a power of
+// two that the warp's largest scale so far allows, so that P s is neither above 65504 nor subnormal where a key of
+// little weight meets a small scale (values around 1e-4, 8000 keys 7 below the largest logit, one split: error
+// 5e-2 -> 7e-4 of the largest output).  Rounding P alone moves numerator and denominator alike; what P s loses meets codes around 8, and for outputs finer than
 // bf16 the loss times 8 is added back over up to 1024 keys (f16, 3 to 12 keys: error 3.4e-4 -> 2.4e-4 of the
 // output, 2.0e-4 being that of its rounding; over 8000 keys 2.04e-4 -> 2.02e-4, for 9 to 14% more time).
 //
@@ -28,10 +28,11 @@
 // splits of a sequence, are merged at the end: through distributed shared memory where the splits of a
 // sequence form a cluster, by k_kv4_combine where there are more of them.
 //
-// Measured (graph of calls, us): single tokens of 28 heads over 4 KV heads of 128, 32 lanes up to 32768 keys
-// 167 (834 MB, 5.0 TB/s; bound by the copies), 5 up to 9000 15.3 and 1 x 2048 5.8 (both bound by latency: the
-// longest chain is lengths, table entry, page, softmax, merge); 16 x 5 tokens of 64 heads over 8 KV heads of 64
-// at 4097 keys, f16, 51 (bound by instructions: three column blocks unpack the same pages).
+// Measured (graph of calls, us): single tokens, 32 lanes up to 32768 keys of 40 heads over 8 KV heads of 128
+// 183 (834 MB, 4.6 TB/s; bound by the copies; f32 in and out in 16 splits 197), 28 heads over 4 KV heads of 128, 5 up
+// to 9000 16.4 and 1 x 2048 5.9 (both bound by latency: the longest chain is lengths, table entry, page, softmax,
+// merge); 16 x 5 tokens of 64 heads over 8 KV heads of 64 at 4097 keys, f16, 55 (bound by instructions: three
+// column blocks unpack the same pages).  The vote on the scales of every page takes 3 to 6% of these.
 #include "kv4_common.cuh"
 
 #include <algorithm>

@@ -19,12 +19,14 @@
 // which matters because three roles' code shares the instruction caches (with the mask inside the unrolled
 // loops, waits for instructions were the first stall and a step took 12.6k cycles).
 // Orders: a K chunk of 8 dims keeps its nibble pairs (0,4) (1,5) (2,6) (3,7) and Q is stored in the same order.
-// Rounding: Q to f16 after a power-of-two scaling of its row (exact for f16, and for bf16 down to 2^-21
-// of the row's largest), K and V to f16, P to f16; sums in f32.
+// Rounding, whatever the types of q and out: Q to f16 after a power-of-two scaling of its row (exact for f16 down to
+// 2^-21 of the row's largest, for bf16 to 2^-24), K and V to f16, P to f16; sums in f32.  (The 4 bits of a value are
+// coarser than any of these.  rms error of f32 outputs up to 2.3e-4 of their size, with f32 queries 5.5e-4; rounding
+// to f16 alone is 2.1e-4.)
 // Every wait is bounded (tc::mbar_wait); no load uses multicast.
-// Measured, 28 heads over 4 KV heads of 128 (us): 4096 tokens over 8192 644 (601 GFLOP, 934 TFLOP/s), 5 turns of
-// up to 256 tokens over 8448 189 (823 TFLOP/s), with cold pages.  A step of 2 x 128 rows and 128 keys takes 4.2k
-// cycles, of which products and their operands alone 3.1k (2.6k if nothing waited), with dequantization 3.7k: the
+// Measured, 28 heads over 4 KV heads of 128 (graph of calls, us): 4096 tokens over 8192 692 (601 GFLOP, 869 TFLOP/s;
+// without the split of the short last wave 782), 5 turns of up to 256 tokens over 8448 194 (802 TFLOP/s).  A step
+// of 2 x 128 rows and 128 keys takes 4.2k cycles, of which products and their operands alone 3.1k (2.6k if nothing waited), with dequantization 3.7k: the
 // schedulers issue in half of the cycles, 8.9k instructions a step, and the exponentials hold their unit for 2.1k.
 #include "kv4_common.cuh"
 

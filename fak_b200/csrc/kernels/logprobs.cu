@@ -13,9 +13,9 @@
 // bounds the k-th logit from below, the few groups that reach it are read again (about k of V / 32), and
 // their logits that reach it are merged as 64-bit keys (ordered value, complemented index), 32 sorted ones at
 // a time.  So selecting costs one store for two tiles and a few microseconds at the end of a row.
-// Measured at 5 x 152064 with 5 alternatives: 12.3 us, bound by latency (some ten dependent steps).
+// Measured at 5 x 152064 with 5 alternatives: 11.4 us, bound by latency (some ten dependent steps).
 // Measured at 2048 x 152064: f32 without alternatives 183 us (6.8 TB/s, above the copy rate it is compared
-// with), with 20 218 us (5.7 TB/s); bf16 138 and 175 us, bound by instructions.  Candidates sorted out during
+// with), with 20 226 us (5.5 TB/s); bf16 139 and 176 us, bound by instructions.  Candidates sorted out during
 // the walk instead cost 293 us, groups read again one after another 256 us.
 // Where the bound is -inf (a mask left fewer than k lanes a token) only larger logits and the first k indices
 // can be in the list.  More candidates than the pool holds (equal logits) go to a list of each warp's own.

@@ -90,7 +90,7 @@ struct LogprobArgs {
   int* top_ids;
   float* top_logprobs;
   int n_seg;
-  float* part;      // [T, n_seg, 36] words when n_seg > 1 (see logprobs.cu)
+  float* part;      // logprob_part_words(T, n_seg) when n_seg > 1: a record a segment
   int* tickets;     // [T] zeroed
   bool vec;
 };

@@ -330,7 +330,8 @@ def kv4_append(k: torch.Tensor, v: torch.Tensor, slot: torch.Tensor, pages: torc
     is skipped and reported as code 2 in the device's error word.  Groups of 32 dims get
     minimum = f16(min x), scale = f16((max x - minimum) / 15), code = rint((x - minimum) / scale);
     values are clamped to +-65504 (the scale is one f16 step lower where minimum + 15 scale would pass that),
-    a group with a NaN reads back as NaN.  Rows with the same slot leave one of them, not a defined one."""
+    a group with a NaN reads back as NaN.  Rows with the same slot leave a mixture of them: their codes, scales
+    and minima, heads and K and V are stored in no order."""
     ext().kv4_append(k, v, slot, pages, _err_word.get(pages.device))
     count()
 
@@ -353,7 +354,9 @@ def kv4_decode_attention(q: torch.Tensor, pages: torch.Tensor, block_table: torc
     softcap > 0: logits cap * tanh(logit / cap); window > 0: the last ``window`` keys; sinks [H] f32.
     n_split splits of each sequence's pages (0: chosen from B, heads and the table's width; a fixed count
     makes a sequence's result independent of its batch).  workspace: float32 scratch for the splits
-    (allocated when not given)."""
+    (allocated when not given).  Probabilities and their products with the values' scales are f16 and sums f32,
+    and f32 queries are rounded to f16 after a scaling of their row, whatever the type of out: f32 outputs carry an
+    rms error of up to 1.2e-4 of their size, with f32 queries 3.5e-4 (rounding to f16 alone is 2.1e-4)."""
     ext().kv4_attention(q, pages, block_table, None, ctx_len, out, 1, scale, softcap, window, sinks, n_split, workspace,
                         _err_word.get(q.device), 0)
     count()
@@ -367,8 +370,9 @@ def kv4_prefill_attention(q: torch.Tensor, pages: torch.Tensor, block_table: tor
     [T, H, D]; q_off [B + 1] int32 packed offsets of the sequences' tokens (``BatchPlan.q_off``), ctx_len
     [B] int32 keys with the new ones (``BatchPlan.ctx``); max_new: an upper bound of the new tokens of one
     sequence.  Sequences without new tokens are skipped.  tiles: True takes the tensor-core kernel over tiles of
-    256 query rows (keys and values rounded to f16), False the one whose warps stream pages, None the faster one
-    for max_new (a fixed choice with n_split = 1 makes a sequence's result independent of its batch).  A value
+    256 query rows (keys, values and probabilities rounded to f16: rms error of f32 outputs up to 2.3e-4 of
+    their size, with f32 queries 5.5e-4), False the one whose warps stream pages (as kv4_decode_attention), None the faster one for max_new,
+    whatever the types (a fixed choice with n_split = 1 makes a sequence's result independent of its batch).  A value
     that is not a number reaches every row of a tile in which some row sees it.  The other arguments as
     kv4_decode_attention."""
     ext().kv4_attention(q, pages, block_table, q_off, ctx_len, out, max_new, scale, softcap, window, sinks, n_split,
