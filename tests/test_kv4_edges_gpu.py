@@ -62,6 +62,24 @@ def test_append_rows_between_vector_boundaries(K, D, dtype, odd, by):
         np.testing.assert_array_equal(got.double().cpu().numpy(), want.astype(np.float32).astype(np.float64))
 
 
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
+def test_append_of_the_widest_groups(K, D, dtype):
+    """-65504 + 15 f16(131008 / 15) is 65536, past f16: the scale is one step less, 8728, and the largest value 65416.
+    Attention rounds values to f16, so it has to stay finite."""
+    x = torch.linspace(-65504, 65504, 32, device="cuda").repeat(D // 32).view(1, 1, D).to(dtype)
+    pages = torch.zeros(1, 1, K.kv4_page_bytes(D), dtype=torch.uint8, device="cuda")
+    K.kv4_append(x, x, dev([0]), pages)
+    want = torch.round((x.double() + 65504) / 8728).clamp(0, 15) * 8728 - 65504
+    for r in K.kv4_read(pages, dev([0]), D, torch.float32):
+        assert torch.equal(r.double(), want) and r.max() == 65416
+    q = torch.zeros(1, 1, D, device="cuda")
+    for tiles in (False, True):
+        out = torch.empty_like(q)
+        K.kv4_prefill_attention(q, pages, dev([[0]]), dev([0, 1]), dev([1]), out, 1, tiles=tiles)
+        assert ((out.double() - want).abs() <= 4 * U16 * 65504).all()
+
+
 # ------------------------------------------------------------------------------------ attention
 U16 = 2.0 ** -11
 OUT_U = {torch.float32: 2.0 ** -24, torch.float16: 2.0 ** -11, torch.bfloat16: 2.0 ** -8}
