@@ -237,7 +237,7 @@ def main():
             "arm": {"C": "shared radix prefix + batched decode", "B": "per-agent warm KV, one agent at a time",
                     "A": "no KV reuse: full re-prefill every turn"}[args.arm],
             "l2": "each decode step streams the 4.4 GB weight set (>> 126 MB L2); no explicit flush",
-            "kv_dtype": "bf16", "weight_format": "GGUF Q4_K/Q6_K blocks (decode), bf16 copy (prefill GEMM)",
+            "kv_dtype": ecfg.kv_precision, "weight_format": "GGUF Q4_K/Q6_K blocks (decode), bf16 copy (prefill GEMM)",
         },
         "ttft_p50_ms": round(ttfts_ms[len(ttfts_ms) // 2], 3),
         "ttft_p99_ms": round(ttfts_ms[min(len(ttfts_ms) - 1, int(0.99 * len(ttfts_ms)))], 3),

@@ -118,3 +118,20 @@ def test_speculation_keeps_the_tokens(model_file, drafter):
     eng = engine(model_file, graphs=True, spec_k=3, spec_drafter=drafter, max_batch=16)    # 4 rows a request
     assert eng.generate(ps, max_new_tokens=24) == want
     assert eng.stats["spec_proposed"] > 0
+
+
+@pytest.mark.parametrize("precision", [None, "q4"])
+def test_the_benchmark_names_the_cache_it_ran_on(precision):
+    import json
+    import os
+    import subprocess
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    env = {k: v for k, v in os.environ.items() if k != "FAK_KV_PRECISION"}
+    if precision:
+        env["FAK_KV_PRECISION"] = precision
+    r = subprocess.run([sys.executable, "bench.py", "--model", "tiny-qwen2", "--mix", "q8_0", "--steps", "1", "--warmup", "3", "--agents", "2",
+                        "--prefix", "64", "--user", "16", "--decode", "4"], cwd=root, env=env, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stderr[-2000:]
+    line = json.loads(r.stdout.strip().splitlines()[-1])
+    assert line["config"]["kv_dtype"] == (precision or "bf16") and line["value"] > 0
