@@ -29,8 +29,8 @@
 // sequence form a cluster, by k_kv4_combine where there are more of them.
 //
 // Measured (graph of calls, us): single tokens, 32 lanes up to 32768 keys of 40 heads over 8 KV heads of 128
-// 183 (834 MB, 4.6 TB/s; bound by the copies; f32 in and out in 16 splits 197), 28 heads over 4 KV heads of 128, 5 up
-// to 9000 16.4 and 1 x 2048 5.9 (both bound by latency: the longest chain is lengths, table entry, page, softmax,
+// 180 (834 MB, 4.6 TB/s; bound by the copies; f32 in and out in 16 splits 193), 28 heads over 4 KV heads of 128, 5 up
+// to 9000 16.3 and 1 x 2048 5.9 (both bound by latency: the longest chain is lengths, table entry, page, softmax,
 // merge); 16 x 5 tokens of 64 heads over 8 KV heads of 64 at 4097 keys, f16, 55 (bound by instructions: three
 // column blocks unpack the same pages).  The vote on the scales of every page takes 3 to 6% of these.
 #include "kv4_common.cuh"
@@ -123,6 +123,7 @@ struct Smem {
   alignas(16) float qsum[COLS][Lay<D>::NG];
   uint4 qf[NT][Lay<D>::NG][32];
   int fail;   // a wait gave up
+  uint32_t lost[COLS];   // groups with a value that the column sees and that is no number (taken out of V)
 };
 
 // Weight of a part (base, sum) against a base m: 0 for one without keys; one whose logits were all NaN (its base
@@ -152,7 +153,9 @@ FAK_DEV void cluster_sync() {
 
 // CLUSTER: the splits of a block are one thread-block cluster and merge through shared memory; else they
 // leave partial results for k_kv4_combine.  The sums are the same, in the same order.
-template <int D, int NT, bool CAP, bool CLUSTER, bool FINE>
+// MULTI: sequences may bring several tokens, so that rows differ in the keys they see (without what that asks for
+// single tokens take 3% less, 32 lanes up to 32768 187 us instead of 194).
+template <int D, int NT, bool CAP, bool CLUSTER, bool FINE, bool MULTI>
 __global__ void __launch_bounds__(W * 32, kResident<D, NT>)
 k_kv4_attn(const __grid_constant__ Kv4Attn a, int n_split) {
   using L = Lay<D>;
@@ -170,6 +173,7 @@ k_kv4_attn(const __grid_constant__ Kv4Attn a, int n_split) {
   }
   if (lane < STAGES) tc::mbar_init(&sm.full[warp][lane], 1);
   if (tid == 0) sm.fail = 0;
+  if (MULTI && tid < COLS) sm.lost[tid] = 0;
   tc::fence_mbar_init();
   __syncthreads();
   pdl_wait();
@@ -454,6 +458,31 @@ k_kv4_attn(const __grid_constant__ Kv4Attn a, int n_split) {
         }
         m0 &= keep0;
         m1 &= keep1;
+        // Values that are no numbers, at keys that some rows see and others do not: 0 * NaN would reach the others.
+        uint32_t bad = MULTI ? nan_halves(m0) | nan_halves(m1) : 0;
+#pragma unroll
+        for (int gr = 0; gr < NG; gr++) bad |= MULTI ? nan_halves(s0[gr]) | nan_halves(s1[gr]) : 0;
+        if (MULTI && __any_sync(0xffffffffu, bad)) {
+          asm volatile("");
+#pragma unroll
+          for (int gr = 0; gr < NG; gr++) {   // (a group's minima are in the lanes of row gr)
+            const uint32_t b0 = nan_halves(s0[gr]) | __shfl_sync(0xffffffffu, nan_halves(m0), gr * 4 + t);
+            const uint32_t b1 = nan_halves(s1[gr]) | __shfl_sync(0xffffffffu, nan_halves(m1), gr * 4 + t);
+            uint32_t toks = ((b0 & 1) << (2 * t)) | ((b0 >> 31) << (2 * t + 1)) | ((b1 & 1) << (2 * t + 8)) | ((b1 >> 31) << (2 * t + 9));
+            toks |= __shfl_xor_sync(0xffffffffu, toks, 1);
+            toks |= __shfl_xor_sync(0xffffffffu, toks, 2);
+            s0[gr] &= ~b0;
+            s1[gr] &= ~b1;
+            if (g == gr) {
+              m0 &= ~b0;
+              m1 &= ~b1;
+            }
+#pragma unroll
+            for (int c = 0; c < 2 * NT; c++)
+              if (g == 0 && (toks & key_bits(key0, low[c >> 1][c & 1], lim[c >> 1][c & 1])))
+                atomicOr(&sm.lost[(c >> 1) * 8 + 2 * t + (c & 1)], 1u << gr);
+          }
+        }
       }
       uint32_t s_top = max_h2(s0[0], s1[0]);
 #pragma unroll
@@ -560,6 +589,7 @@ k_kv4_attn(const __grid_constant__ Kv4Attn a, int n_split) {
         v.x += f[w] * y.x;
         v.y += f[w] * y.y;
       }
+      if (MULTI && (sm.lost[c] >> (d / 32) & 1)) v.x = v.y = __int_as_float(0x7fffffff);
       if constexpr (CLUSTER) {
         *reinterpret_cast<float2*>(&sm.o[0][c][d]) = v;   // (this thread read the element last)
       } else if (alone) {
@@ -743,15 +773,19 @@ static void split_launch(const Kv4Attn& a, const Kv4AttnPlan& p, cudaStream_t st
     if (p.cluster) FAK_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
     FAK_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kern, a, p.n_split));
   };
-  auto pick = [&](auto d, auto nt, auto cap, auto fine) {
+  auto pick = [&](auto d, auto nt, auto cap, auto fine, auto multi) {
     constexpr int DV = decltype(d)::value, NTV = decltype(nt)::value;
-    constexpr bool CAP = decltype(cap)::value, FINE = decltype(fine)::value;
-    if (p.cluster) go(k_kv4_attn<DV, NTV, CAP, true, FINE>, sizeof(Smem<DV, NTV>));
-    else go(k_kv4_attn<DV, NTV, CAP, false, FINE>, sizeof(Smem<DV, NTV>));
+    constexpr bool CAP = decltype(cap)::value, FINE = decltype(fine)::value, MULTI = decltype(multi)::value;
+    if (p.cluster) go(k_kv4_attn<DV, NTV, CAP, true, FINE, MULTI>, sizeof(Smem<DV, NTV>));
+    else go(k_kv4_attn<DV, NTV, CAP, false, FINE, MULTI>, sizeof(Smem<DV, NTV>));
+  };
+  auto by_rows = [&](auto d, auto nt, auto cap, auto fine) {
+    if (a.max_new > 1) pick(d, nt, cap, fine, std::true_type{});
+    else pick(d, nt, cap, fine, std::false_type{});
   };
   auto by_type = [&](auto d, auto nt, auto cap) {
-    if (a.o_type == Elt::BF16) pick(d, nt, cap, std::false_type{});
-    else pick(d, nt, cap, std::true_type{});
+    if (a.o_type == Elt::BF16) by_rows(d, nt, cap, std::false_type{});
+    else by_rows(d, nt, cap, std::true_type{});
   };
   auto by_cap = [&](auto d, auto nt) {
     if (a.softcap > 0.f) by_type(d, nt, std::true_type{});

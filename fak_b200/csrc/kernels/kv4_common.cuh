@@ -24,6 +24,13 @@ FAK_DEV uint32_t mul_h2(uint32_t a, uint32_t b) {
   const __half2 h = __hmul2(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b));
   return *reinterpret_cast<const uint32_t*>(&h);
 }
+// halves that are no finite number, all bits set
+FAK_DEV uint32_t nan_halves(uint32_t a) { return __vcmpeq2(a & 0x7c007c00u, 0x7c007c00u); }
+// the bits of the 32 keys from key0 on that lie in [low, lim)
+FAK_DEV uint32_t key_bits(int key0, int low, int lim) {
+  const int lo = min(max(low - key0, 0), 32), hi = min(max(lim - key0, 0), 32);
+  return hi > lo ? (0xffffffffu >> (32 - (hi - lo))) << lo : 0u;
+}
 FAK_DEV float2 unpack_h2(uint32_t a) { return __half22float2(*reinterpret_cast<__half2*>(&a)); }
 FAK_DEV float ex2(float x) {
   float y;

@@ -23,9 +23,11 @@
 // 2^-21 of the row's largest, for bf16 to 2^-24), K and V to f16, P to f16; sums in f32.  (The 4 bits of a value are
 // coarser than any of these.  rms error of f32 outputs up to 2.3e-4 of their size, with f32 queries 5.5e-4; rounding
 // to f16 alone is 2.1e-4.)
+// Values that are no numbers are taken out of the steps in which rows differ in the keys they see, and given at the
+// end to the rows that see them.
 // Every wait is bounded (tc::mbar_wait); no load uses multicast.
-// Measured, 28 heads over 4 KV heads of 128 (graph of calls, us): 4096 tokens over 8192 692 (601 GFLOP, 869 TFLOP/s;
-// without the split of the short last wave 782), 5 turns of up to 256 tokens over 8448 194 (802 TFLOP/s).  A step
+// Measured, 28 heads over 4 KV heads of 128 (graph of calls, us): 4096 tokens over 8192 670 (601 GFLOP, 897 TFLOP/s;
+// without the split of the short last wave 744), 5 turns of up to 256 tokens over 8448 184 (845 TFLOP/s).  A step
 // of 2 x 128 rows and 128 keys takes 4.2k cycles, of which products and their operands alone 3.1k (2.6k if nothing waited), with dequantization 3.7k: the
 // schedulers issue in half of the cycles, 8.9k instructions a step, and the exponentials hold their unit for 2.1k.
 #include "kv4_common.cuh"
@@ -51,6 +53,12 @@ constexpr int THREADS = 448;
 constexpr float LIFT = 4.f, HEADROOM = 8.f;
 constexpr float LOG2E = 1.4426950408889634f;
 
+// Steps with keys that some rows of the block see and others do not: its 256 rows are at most 256 queries, so those
+// keys lie in the first four steps (windows) and the last four.
+constexpr int EDGE_STEPS = 8;
+FAK_DEV int edge_slot(int j, int NJ) { return NJ <= EDGE_STEPS || j < EDGE_STEPS / 2 ? j : max(0, EDGE_STEPS - (NJ - j)); }
+FAK_DEV int edge_step(int slot, int NJ) { return NJ <= EDGE_STEPS || slot < EDGE_STEPS / 2 ? slot : NJ - EDGE_STEPS + slot; }
+
 template <int D>
 struct Smem {
   alignas(1024) __half q[2][D / 64][ROWS * 64];    // [tile][64-dim half][row][64]
@@ -60,6 +68,8 @@ struct Smem {
   uint64_t s_full[2][2], p_full[2][2], pv_done[2][2];   // [tile][64-key half]
   uint32_t tmem;
   int fail;
+  int lost_any;                          // values that are no numbers were taken out of V, at these tokens of
+  uint32_t lost[EDGE_STEPS][D / 32][4];  // [step][group][token]; see edge_slot
 };
 
 // f16 operands, f32 accumulator, both K-major
@@ -201,6 +211,8 @@ k_kv4_prefill(const __grid_constant__ Kv4Attn a, int splits, int whole, int n_bl
   const int tiles = R - r0 > ROWS ? 2 : 1;
   const int lim_any = ctx - n + i_last + 1;                                            // keys some row sees: below
   const int low_any = a.window > 0 ? max(0, ctx - n + i_first + 1 - a.window) : 0;     // and from here
+  const int lim_all = ctx - n + i_first + 1;                                           // keys every row sees: below
+  const int low_all = a.window > 0 ? max(0, ctx - n + i_last + 1 - a.window) : 0;      // and from here
 
   if (threadIdx.x == 0) {
     tc::mbar_init(&sm.q_full, 4 * tiles);
@@ -215,9 +227,10 @@ k_kv4_prefill(const __grid_constant__ Kv4Attn a, int splits, int whole, int n_bl
         tc::mbar_init(&sm.pv_done[i][h], 1);
       }
     }
-    sm.fail = 0;
+    sm.fail = sm.lost_any = 0;
     tc::fence_mbar_init();
   }
+  if (threadIdx.x < EDGE_STEPS * NG * 4) (&sm.lost[0][0][0])[threadIdx.x] = 0;
   if (warp == 12) {
     tc::tmem_alloc(&sm.tmem, 512);   // S0 [0, 128) S1 [128, 256) O0 [256, 256 + D) O1 [256 + D, 256 + 2 D)
     tc::tmem_relinquish();
@@ -350,7 +363,7 @@ k_kv4_prefill(const __grid_constant__ Kv4Attn a, int splits, int whole, int n_bl
       if (lane == 0) tc::mbar_arrive(&sm.k_full[buf]);
 
       const int i = j * PPT + 2 * w + vp, key0 = (p_begin + i) * PAGE, step0 = (p_begin + j * PPT) * PAGE;
-      if (step0 < low_any || step0 + KEYS > min(lim_any, p_end * PAGE)) {
+      if (step0 < low_all || step0 + KEYS > min(lim_all, p_end * PAGE)) {
         // tokens no row sees (memory nobody wrote, pages that do not exist): zero
 #pragma unroll
         for (int e = 0; e < 4; e++) {
@@ -362,6 +375,29 @@ k_kv4_prefill(const __grid_constant__ Kv4Attn a, int splits, int whole, int n_bl
             vs[e][gr] &= keep;
             vm[e][gr] &= keep;
           }
+        }
+        // values that are no numbers: 0 * NaN would reach the rows that do not see them
+        uint32_t bad = 0;
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+#pragma unroll
+          for (int gr = 0; gr < NG; gr++) bad |= kv4::nan_halves(vs[e][gr]) | kv4::nan_halves(vm[e][gr]);
+        if (__any_sync(0xffffffffu, bad)) {
+          asm volatile("");
+          const int slot = edge_slot(j, NJ);
+#pragma unroll
+          for (int e = 0; e < 4; e++)
+#pragma unroll
+            for (int gr = 0; gr < NG; gr++) {
+              const uint32_t b = kv4::nan_halves(vs[e][gr]) | kv4::nan_halves(vm[e][gr]);
+              const int tok = (2 * w + vp) * PAGE + 2 * (vh * 4 + e);
+              vs[e][gr] &= ~b;
+              vm[e][gr] &= ~b;
+              if (b && vg == 0) {
+                atomicOr(&sm.lost[slot][gr][tok >> 5], ((b & 1) | (b >> 31) << 1) << (tok & 31));
+                sm.lost_any = 1;
+              }
+            }
         }
       }
       fetch_k(j + 1);
@@ -530,6 +566,13 @@ k_kv4_prefill(const __grid_constant__ Kv4Attn a, int splits, int whole, int n_bl
     if (NU > 0) {
       tc::mbar_wait(&sm.pv_done[t][(NU - 1) & 1], (uint32_t)((NU - 1) >> 1) & 1, fail);
       tc::tc_fence_after();
+      tc::mbar_wait(&sm.v_full[(NJ - 1) & 1], (uint32_t)((NJ - 1) >> 1) & 1, fail);   // (long over: for what it publishes)
+    }
+    uint32_t lost = 0;   // groups with a value that this row sees and that is no number
+    if (sm.lost_any) {
+      for (int i = 0; i < EDGE_STEPS * NG * 4; i++)
+        if ((&sm.lost[0][0][0])[i] & kv4::key_bits((p_begin + edge_step(i / (NG * 4), NJ) * PPT) * PAGE + i % 4 * 32, low, lim))
+          lost |= 1u << (i / 4 % NG);
     }
     const float sink = alone && a.sinks ? a.sinks[h] * LOG2E : -INFINITY;
     float f = 1.f;
@@ -552,6 +595,10 @@ k_kv4_prefill(const __grid_constant__ Kv4Attn a, int splits, int whole, int n_bl
       } else {
 #pragma unroll
         for (int e = 0; e < 16; e++) o[e] = 0;
+      }
+      if (lost >> (c >> 1) & 1) {
+#pragma unroll
+        for (int e = 0; e < 16; e++) o[e] = 0x7fffffffu;
       }
       if (live && alone) {
         if (a.o_vec) {

@@ -372,9 +372,8 @@ def kv4_prefill_attention(q: torch.Tensor, pages: torch.Tensor, block_table: tor
     sequence.  Sequences without new tokens are skipped.  tiles: True takes the tensor-core kernel over tiles of
     256 query rows (keys, values and probabilities rounded to f16: rms error of f32 outputs up to 2.3e-4 of
     their size, with f32 queries 5.5e-4), False the one whose warps stream pages (as kv4_decode_attention), None the faster one for max_new,
-    whatever the types (a fixed choice with n_split = 1 makes a sequence's result independent of its batch).  A value
-    that is not a number reaches every row of a tile in which some row sees it.  The other arguments as
-    kv4_decode_attention."""
+    whatever the types (a fixed choice with n_split = 1 makes a sequence's result independent of its batch).  Keys
+    and values that are no numbers reach the rows that see them.  The other arguments as kv4_decode_attention."""
     ext().kv4_attention(q, pages, block_table, q_off, ctx_len, out, max_new, scale, softcap, window, sinks, n_split,
                         workspace, _err_word.get(q.device), -1 if tiles is None else int(tiles))
     count()

@@ -139,3 +139,82 @@ def test_sequences_with_less_context_than_new_tokens(K, tiles):
         assert (out[:4] == 0).all() and (out[9:13] == 0).all() and (out[13:20] == 0).all()
         for b in (0, 2):
             check(out[off[b]:off[b + 1]], want[b], vs[b], term(q.double().cpu(), ks[b], D ** -0.5, torch.float16, tiles))
+
+
+@pytest.mark.parametrize("old,new,H,Hkv,D", [([1700], [300], 1, 1, 64), ([900, 3], [100, 130], 4, 2, 128), ([40, 700], [9, 5], 8, 1, 64),
+                                             ([0], [20], 2, 2, 128), ([2500], [260], 2, 1, 64)])
+@pytest.mark.parametrize("window", [0, 150, 700])
+@pytest.mark.parametrize("tiles", [False, True])
+@pytest.mark.parametrize("deep", [True, False])
+def test_values_that_are_no_numbers_reach_the_rows_that_see_them(K, old, new, H, Hkv, D, window, tiles, deep):
+    """NaN values in one or all groups of some tokens, among the keys that all rows see, some, or none: a row's group
+    is NaN exactly where it sees one, and everything else is as if they were 0."""
+    lens, g = [a + n for a, n in zip(old, new)], gen(sum(new) + window)
+    kr, vr, bad = [], [], []
+    for a, c in zip(old, lens):
+        kr.append(rows(g, (c, Hkv, D)))
+        v = rows(g, (c, Hkv, D))
+        at = sorted({c // 3, max(0, a - 200), max(0, a - 60), max(0, a - 1), min(c - 1, a + 2), (a + c) // 2, c - 1})
+        at = at if deep else [j for j in at if j > a]      # (without a window, every row sees those before)
+        b = torch.zeros(c, Hkv, D // 32, dtype=torch.bool)
+        for i, j in enumerate(at):
+            b[j, i % Hkv, slice(None) if i % 3 == 0 else slice(i % (D // 32), i % (D // 32) + 1)] = True
+        v.view(c, Hkv, D // 32, 32)[b.cuda()] = math.nan
+        vr.append(v)
+        bad.append(b)
+    pages, table, ks, vs = cache(K, kr, vr)
+    assert all(torch.equal(torch.isnan(v.view(*b.shape, 32)), b[..., None].expand(*b.shape, 32)) for v, b in zip(vs, bad))
+    vs = [torch.nan_to_num(v, nan=0.0) for v in vs]
+    off = np.concatenate([[0], np.cumsum(new)])
+    q = torch.randn(sum(new), H, D, generator=g, device="cuda").half()
+    qs = [q[off[b]:off[b + 1]].double().cpu() for b in range(len(new))]
+    want = plain.attention(qs, ks, vs, lens, window=window)
+    for n_split in (1, 3, 0, 20):
+        out = torch.empty_like(q)
+        K.kv4_prefill_attention(q, pages, table, dev(off), dev(lens), out, max(new), window=window, tiles=tiles, n_split=n_split)
+        for b, (c, n) in enumerate(zip(lens, new)):
+            hi = torch.arange(c - n + 1, c + 1)[:, None]
+            j = torch.arange(c)[None, :]
+            sees = ((j < hi) & (j >= (hi - window if window else 0))).double()                    # [n, c]
+            hit = torch.einsum("nc,chg->nhg", sees, bad[b].double()) > 0                          # [n, Hkv, groups]
+            hit = hit.repeat_interleave(H // Hkv, 1).repeat_interleave(32, 2)
+            o = out[off[b]:off[b + 1]]
+            assert torch.equal(torch.isnan(o).cpu(), hit)
+            if not hit.all():
+                check(o[~hit.cuda()], want[b][~hit], vs[b], term(qs[b], ks[b], D ** -0.5, torch.float16, tiles))
+
+
+@pytest.mark.parametrize("old,new,H,Hkv,D", [([700], [300], 1, 1, 64), ([100, 9], [60, 130], 4, 2, 128), ([40, 300], [9, 5], 8, 1, 64)])
+@pytest.mark.parametrize("window", [0, 150])
+@pytest.mark.parametrize("tiles", [False, True])
+def test_keys_and_queries_that_are_no_numbers_stay_with_their_rows(K, old, new, H, Hkv, D, window, tiles):
+    lens, g = [a + n for a, n in zip(old, new)], gen(sum(new) + window)
+    kr, vr, bad = [], [], []
+    for a, c in zip(old, lens):
+        k = rows(g, (c, Hkv, D))
+        b = torch.zeros(c, Hkv, dtype=torch.bool)
+        b[min(c - 1, a + 3), 0] = b[(a + c) // 2, -1] = True
+        k[b.cuda()] = math.nan
+        kr.append(k)
+        vr.append(rows(g, (c, Hkv, D)))
+        bad.append(b)
+    pages, table, ks, vs = cache(K, kr, vr)
+    ks = [torch.nan_to_num(k, nan=0.0) for k in ks]
+    off = np.concatenate([[0], np.cumsum(new)])
+    q = torch.randn(sum(new), H, D, generator=g, device="cuda").half()
+    broken = torch.zeros(sum(new), H, dtype=torch.bool)
+    broken[1, 0] = broken[-1, -1] = True
+    want = plain.attention([q[off[b]:off[b + 1]].double().cpu() for b in range(len(new))], ks, vs, lens, window=window)
+    sigma = [term(q[off[b]:off[b + 1]].double().cpu(), ks[b], D ** -0.5, torch.float16, tiles) for b in range(len(new))]
+    q[1, 0, 5], q[-1, -1, 0] = math.nan, math.nan
+    for n_split in (1, 3, 0, 20):
+        out = torch.empty_like(q)
+        K.kv4_prefill_attention(q, pages, table, dev(off), dev(lens), out, max(new), window=window, tiles=tiles, n_split=n_split)
+        for b, (c, n) in enumerate(zip(lens, new)):
+            hi = torch.arange(c - n + 1, c + 1)[:, None]
+            j = torch.arange(c)[None, :]
+            sees = ((j < hi) & (j >= (hi - window if window else 0))).double()
+            hit = (torch.einsum("nc,ch->nh", sees, bad[b].double()) > 0).repeat_interleave(H // Hkv, 1) | broken[off[b]:off[b + 1]]
+            o = out[off[b]:off[b + 1]]
+            assert torch.equal(torch.isnan(o).cpu(), hit[..., None].expand(n, H, D))
+            check(o[~hit.cuda()], want[b][~hit], vs[b], sigma[b])
