@@ -19,9 +19,10 @@
 // the row's largest, for bf16 up to 26: every other dim is scaled down by 16 more); P is f16, raised by a power of
 // two that the warp's largest scale so far allows, so that P s is neither above 65504 nor subnormal where a key of
 // little weight meets a small scale (values around 1e-4, 8000 keys 7 below the largest logit, one split: error
-// 5e-2 -> 7e-4 of the largest output).  Rounding P alone moves numerator and denominator alike; what P s loses meets codes around 8, and for outputs finer than
-// bf16 the loss times 8 is added back over up to 1024 keys (f16, 3 to 12 keys: error 3.4e-4 -> 2.4e-4 of the
-// output, 2.0e-4 being that of its rounding; over 8000 keys 2.04e-4 -> 2.02e-4, for 9 to 14% more time).
+// 5e-2 -> 7e-4 of the largest output).  Rounding P alone moves numerator and denominator alike; what P s loses
+// meets codes around 8, and for outputs finer than bf16 the loss times 8 is added back over up to 1024 keys (f16,
+// 3 to 12 keys: error 3.4e-4 -> 2.4e-4 of the output, 2.0e-4 being that of its rounding; over 8000 keys 2.04e-4 ->
+// 2.02e-4, for 9 to 14% more time).
 //
 // A warp streams its own pages through a ring of shared memory filled by one bulk copy a page and walks
 // them with an online softmax whose base moves only when a row outgrows it; the CTA's warps, then the
